@@ -18,6 +18,7 @@
 
 #include "pa_device.hpp"
 #include "pa_mi355x.h"
+#include "pa_mi355x_ext.h"
 
 namespace {
 
@@ -782,6 +783,9 @@ struct RunOpts {
   int bias_b = 0, bias_h = 0, bias_rows = 0, bias_cols = 0;
   const int32_t* bias_col_off = nullptr;  // per-sequence bias column offsets (sliding rings)
   bool smooth_softmax = false;
+  // pa_masked_attention: its mask, and every key and value, the new rows included, from the pages
+  bool masked = false;
+  const pa_mask* mask = nullptr;
   bool images = true;  // operand images allowed (see make_plan)
   HostLens host;       // host metadata lengths (LATENT chunk sizing)
 };
@@ -864,7 +868,13 @@ pa::AttnParams attn_params(const pa_cache* c, const pa_batch* b, const pa_attn* 
   p.softcap = a->softcap;
   p.window = a->local_window_size;
   p.causal = a->is_causal ? 1 : 0;
-  p.read_all_from_cache = quant ? 1 : 0;
+  p.read_all_from_cache = quant || opts.masked ? 1 : 0;
+  p.masked = opts.masked ? 1 : 0;
+  if (opts.mask) {
+    p.slopes = opts.mask->distance_slopes;
+    p.prefix_lens = opts.mask->prefix_lens;
+    p.doc_starts = opts.mask->document_starts;
+  }
   p.k_quant = c->k_quant_type;
   p.v_quant = c->v_quant_type;
   p.v_head_dim = a->v_head_size > 0 ? a->v_head_size : c->head_dim;
@@ -903,7 +913,7 @@ int run_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dty
     return fail(PA_ERR_INVALID_ARGUMENT, "SEPARATE layout requires equal key and value head sizes");
   if (vd > c->head_dim)
     return fail(PA_ERR_INVALID_ARGUMENT, "LATENT v_head_size must not exceed head_size");
-  if (!q || !out || (!quant && (!kn || (!vn && !latent))))
+  if (!q || !out || (!quant && !opts.masked && (!kn || (!vn && !latent))))
     return fail(PA_ERR_INVALID_ARGUMENT, "q/k_new/v_new/out pointers are NULL");
   if (kind < 0 || kind > 4) return fail(PA_ERR_INVALID_ARGUMENT, "unknown kernel kind %d", kind);
   if (latent && kind != 0 && kind != 3)
@@ -1228,6 +1238,187 @@ int pa_attention_ex(const pa_cache* cache, const pa_batch* batch, const pa_attn*
                     int32_t chunk_tokens, pa_stream_t stream) {
   return run_attention(cache, batch, attn, act_dtype, q, k_new, v_new, out, workspace,
                        workspace_bytes, kind, chunk_tokens, reinterpret_cast<hipStream_t>(stream));
+}
+
+// ------------------------------------------------------------------------------ masks, prefixes
+namespace {
+
+// Checks that the entries with masks and shared prefixes have in common beyond run_attention's.
+int check_masked(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dtype act) {
+  int rc = check_cache(c, act);
+  if (rc) return rc;
+  if ((rc = check_batch(b))) return rc;
+  if (!a) return fail(PA_ERR_INVALID_ARGUMENT, "attention descriptor is NULL");
+  if (!c->value_cache)
+    return fail(PA_ERR_UNSUPPORTED, "masked attention takes the SEPARATE cache layout");
+  if (b->slot_mapping)
+    return fail(PA_ERR_INVALID_ARGUMENT,
+                "masked attention reads the block-table pages: slot_mapping must be NULL");
+  if (!std::isfinite(a->scale))
+    return fail(PA_ERR_INVALID_ARGUMENT, "scale must be finite");
+  return PA_OK;
+}
+
+int check_share(const pa_shared_prefix* g) {
+  if (!g || g->groups < 1 || !g->group_cum || !g->prefix_lens || g->max_prefix_len < 0)
+    return fail(PA_ERR_INVALID_ARGUMENT,
+                "shared prefix: group_cum, prefix_lens and at least one group are required");
+  return PA_OK;
+}
+
+RunOpts masked_opts(const pa_mask* mask) {
+  RunOpts o;
+  o.mask = mask;
+  o.masked = o.new_rows_in_cache = true;
+  return o;
+}
+
+}  // namespace
+
+size_t pa_masked_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
+                                           const pa_attn* attn, const pa_mask*,
+                                           pa_dtype act_dtype) {
+  if (!cache || !batch || !attn || cache->kv_heads <= 0 || batch->batch <= 0) return 0;
+  return ws_need(cache, batch, attn, act_dtype, 3, 0).best;
+}
+
+int pa_masked_attention(const pa_cache* cache, const pa_batch* batch, const pa_attn* attn,
+                        const pa_mask* mask, pa_dtype act_dtype, const void* q, void* out,
+                        void* workspace, size_t workspace_bytes, pa_stream_t stream) {
+  const int rc = check_masked(cache, batch, attn, act_dtype);
+  if (rc) return rc;
+  return run_attention(cache, batch, attn, act_dtype, q, nullptr, nullptr, out, workspace,
+                       workspace_bytes, 3, 0, reinterpret_cast<hipStream_t>(stream),
+                       masked_opts(mask));
+}
+
+size_t pa_shared_prefix_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
+                                                  const pa_attn* attn,
+                                                  const pa_shared_prefix*, const pa_mask* mask,
+                                                  pa_dtype act_dtype) {
+  return pa_masked_attention_workspace_bytes(cache, batch, attn, mask, act_dtype);
+}
+
+int pa_shared_prefix_attention(const pa_cache* cache, const pa_batch* batch, const pa_attn* attn,
+                               const pa_shared_prefix* share, const pa_mask* mask,
+                               pa_dtype act_dtype, const void* q, void* out, void* workspace,
+                               size_t workspace_bytes, pa_stream_t stream) {
+  const int rc = check_share(share);
+  if (rc) return rc;
+  return pa_masked_attention(cache, batch, attn, mask, act_dtype, q, out, workspace,
+                             workspace_bytes, stream);
+}
+
+// ------------------------------------------------------------------------------ multi-axis append
+int pa_multi_axis_rotary_append(const pa_cache* c, const pa_batch* b, int32_t num_heads,
+                                pa_dtype act, const void* query, int64_t q_stride,
+                                const void* key, int64_t k_stride, const void* value,
+                                int64_t v_stride, const pa_axis_rotary* r, const void* qn,
+                                const void* kn, float eps, void* q_out, pa_stream_t stream) {
+  int rc = check_cache(c, act);
+  if (rc) return rc;
+  if ((rc = check_batch(b))) return rc;
+  if (!c->value_cache)
+    return fail(PA_ERR_UNSUPPORTED, "multi-axis rotary append takes the SEPARATE cache layout");
+  if (!r) return fail(PA_ERR_INVALID_ARGUMENT, "rotary descriptor is NULL");
+  if (r->axes < 1 || r->axes > PA_MAX_AXES)
+    return fail(PA_ERR_INVALID_ARGUMENT, "axes must be 1..%d, got %d", PA_MAX_AXES, r->axes);
+  if (r->rotary_half <= 0 || r->rotary_offset < 0 || r->rotary_positions <= 0 ||
+      (int64_t)r->rotary_offset + 2 * (int64_t)r->rotary_half > c->head_dim)
+    return fail(PA_ERR_INVALID_ARGUMENT,
+                "rotary_offset + rotary_dim must not exceed head_size");
+  if (r->table_dtype != act && r->table_dtype != PA_DTYPE_FLOAT32)
+    return fail(PA_ERR_INVALID_ARGUMENT,
+                "cos/sin tables must be in the activation dtype or fp32");
+  int64_t sum = 0;
+  for (int i = 0; i < r->axes; ++i) {
+    if (r->sections[i] < 0)
+      return fail(PA_ERR_INVALID_ARGUMENT, "axis sections must not be negative");
+    sum += r->sections[i];
+  }
+  if (sum != r->rotary_half)
+    return fail(PA_ERR_INVALID_ARGUMENT, "axis sections sum to %lld, rotary_half is %d",
+                (long long)sum, r->rotary_half);
+  if ((qn == nullptr) != (kn == nullptr))
+    return fail(PA_ERR_INVALID_ARGUMENT,
+                "q_norm_weight and k_norm_weight must be provided together");
+  if ((query == nullptr) != (q_out == nullptr))
+    return fail(PA_ERR_INVALID_ARGUMENT, "query and q_out must be provided together");
+  if (query && num_heads <= 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "num_heads must be positive");
+  const int64_t D = c->head_dim, qw = (int64_t)num_heads * D, kw = (int64_t)c->kv_heads * D;
+  const int64_t ql = q_stride ? q_stride : qw, kl = k_stride ? k_stride : kw,
+                vl = v_stride ? v_stride : kw;
+  if ((query && ql < qw) || kl < kw || vl < kw)
+    return fail(PA_ERR_INVALID_ARGUMENT, "row strides must cover a token's heads");
+  if (r->position_stride != 0 && r->position_stride < b->num_tokens)
+    return fail(PA_ERR_INVALID_ARGUMENT, "position_stride must cover num_tokens");
+  if (b->num_tokens == 0) return PA_OK;
+  if (!key || !value || !r->positions || !r->cos_cache || !r->sin_cache)
+    return fail(PA_ERR_INVALID_ARGUMENT, "key/value/positions/cos/sin pointers are NULL");
+  if (query) {
+    const int64_t es = (int64_t)elem_size(act), n = b->num_tokens;
+    auto meets = [&](const void* x, int64_t ld, int64_t w) {
+      const uintptr_t a0 = reinterpret_cast<uintptr_t>(q_out), a1 = a0 + (uintptr_t)(n * qw * es);
+      const uintptr_t b0 = reinterpret_cast<uintptr_t>(x);
+      return a0 < b0 + (uintptr_t)(((n - 1) * ld + w) * es) && b0 < a1;
+    };
+    const bool own = q_out == query && ql == qw;
+    if ((!own && meets(query, ql, qw)) || meets(key, kl, kw) || meets(value, vl, kw))
+      return fail(PA_ERR_INVALID_ARGUMENT,
+                  "q_out must be the dense query buffer or apart from every input");
+  }
+  pa::AppendParams p{};
+  p.query = query;
+  p.key = key;
+  p.value = value;
+  p.q_out = q_out;
+  p.key_cache = c->key_cache;
+  p.value_cache = c->value_cache;
+  p.k_scale = c->k_scale;
+  p.v_scale = c->v_scale;
+  p.cos_cache = r->cos_cache;
+  p.sin_cache = r->sin_cache;
+  p.q_norm = qn;
+  p.k_norm = kn;
+  p.cum = b->cumulative_sequence_length;
+  p.past = b->past_seqlens;
+  p.block_table = b->block_table;
+  p.slot_mapping = b->slot_mapping;
+  p.num_blocks = c->num_blocks;
+  p.rotary_positions = r->rotary_positions;
+  p.block_size = c->block_size;
+  p.kv_heads = c->kv_heads;
+  p.head_dim = c->head_dim;
+  p.num_heads = query ? num_heads : 0;
+  p.batch = b->batch;
+  p.max_blocks = b->max_blocks;
+  p.num_tokens = b->num_tokens;
+  p.rotary_half = r->rotary_half;
+  p.rotary_offset = r->rotary_offset;
+  p.rotary_interleaved = r->rotary_interleaved ? 1 : 0;
+  p.do_q = query ? 1 : 0;
+  p.norm_eps = eps;
+  p.slots_distinct = (b->flags & PA_BATCH_SLOTS_DISTINCT) ? 1 : 0;
+  p.q_ld = ql;
+  p.k_ld = kl;
+  p.v_ld = vl;
+  p.k_quant = c->k_quant_type;
+  p.v_quant = c->v_quant_type;
+  pa::AxisParams ax{};
+  ax.positions = r->positions;
+  ax.ld = r->position_stride ? r->position_stride : b->num_tokens;
+  ax.axes = r->axes;
+  ax.interleaved = r->axes_interleaved ? 1 : 0;
+  for (int i = 0, end = 0; i < r->axes; ++i) {
+    end += r->sections[i];
+    ax.bound[i] = ax.interleaved ? r->axes * r->sections[i] : end;
+  }
+  ax.table_f32 = r->table_dtype == PA_DTYPE_FLOAT32 ? 1 : 0;
+  const hipError_t e =
+      pa::launch_axes_append(p, ax, act, c->dtype, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "multi-axis rotary append launch");
+  return PA_OK;
 }
 
 // ------------------------------------------------------------------------------ operator level

@@ -105,6 +105,7 @@ __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams 
   const int b = seq_of_token(p.cum, p.batch, t);
   const int s0 = p.cum[b];
   const int nq = p.cum[b + 1] - s0;
+  if (p.masked && (t < s0 || t - s0 >= nq)) return;
   const int64_t pastb = max(p.past[b], 0);
   const int64_t total = seq_keys(p, b, pastb, nq);
   const int64_t start = (int64_t)split * p.chunk;
@@ -114,7 +115,9 @@ __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams 
   const int kh = h / g;
   const int64_t rp = pastb + (t - s0);
   int64_t lo = start, hi = end;
-  if (p.causal) hi = min(hi, rp + 1);
+  if (p.causal)
+    hi = min(hi, p.prefix_lens ? max(rp + 1, (int64_t)p.prefix_lens[b]) : rp + 1);
+  if (p.doc_starts) lo = max(lo, (int64_t)p.doc_starts[t]);
   // window end point: the row's position, or the last key for rows past it (a right-padded
   // first prompt, causal_window_mask attention.rs:328-353)
   if (p.window > 0) lo = max(lo, min(rp, total - 1) - p.window + 1);
@@ -209,6 +212,7 @@ __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams 
         const int64_t pos = p0 + NW * u;
         float s = part[u] * p.scale;
         if (cap > 0.0f) s = cap * tanhf(s / cap);
+        if (p.slopes) s -= p.slopes[h] * fabsf((float)(rp - pos));
         if (bias_row)
           s += TT::to_f32(
               bias_row[min(max(min(pos, hi - 1) + bias_off, (int64_t)0), (int64_t)p.bias_cols - 1)]);
@@ -303,6 +307,7 @@ __global__ __launch_bounds__(NT) void split_reduce_kernel(const AttnParams p) {
   const int VD = p.v_head_dim;
   const int b = seq_of_token(p.cum, p.batch, t);
   const int nq = p.cum[b + 1] - p.cum[b];
+  if (p.masked && (t < p.cum[b] || t - p.cum[b] >= nq)) return;
   const int64_t total = seq_keys(p, b, max(p.past[b], 0), nq);
   if (nq <= 0 || nq <= p.short_tokens) return;  // (short: a row of the streaming decode)
   const int nsplit = (int)min((total + p.chunk - 1) / p.chunk, (int64_t)p.max_splits);

@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "pa_mi355x.h"
+#include "pa_mi355x_ext.h"
 
 namespace pa {
 
@@ -378,6 +379,13 @@ struct AttnParams {
   // the staged view's rows are not absolute positions); NULL: pos
   const int32_t* bias_col_off;
   int32_t smooth_softmax;
+  // Masks of pa_masked_attention (VALU kernel; the others take none): a bias -slopes[h] * |distance|
+  // after the softcap, keys below prefix_lens[b] visible past the causal limit, none below
+  // doc_starts[t]; masked: tokens outside every sequence are left alone.
+  int32_t masked;
+  const float* slopes;
+  const int32_t* prefix_lens;
+  const int32_t* doc_starts;
   int32_t* plan;
   int32_t* plan_info;
   int32_t* plan_split;
@@ -536,6 +544,27 @@ struct RingParams {
 hipError_t launch_ring_move(const RingParams& r, hipStream_t s);
 hipError_t launch_rotary_append(const AppendParams& p, pa_dtype act, pa_dtype cache_dtype,
                                 hipStream_t s);
+// Multi-axis rotary append (pa_axes.hip): the axis of every frequency and the axes' positions, the
+// tables and the rest as AppendParams has them.
+struct AxisParams {
+  const int64_t* positions;  // [axes][ld]
+  int64_t ld;
+  int32_t axes, interleaved;
+  int32_t bound[PA_MAX_AXES];  // sections one after the other: end of axis a's; in turns: axes * section
+  int32_t table_f32;           // tables in fp32 instead of the activation dtype
+  __device__ __forceinline__ int axis_of(int i) const {
+    if (interleaved) {
+      const int a = i % axes;
+      return i < bound[a] ? a : 0;
+    }
+    int a = 0;
+#pragma unroll
+    for (int k = 0; k < PA_MAX_AXES - 1; ++k) a += (k + 1 < axes && i >= bound[k]) ? 1 : 0;
+    return a;
+  }
+};
+hipError_t launch_axes_append(const AppendParams& p, const AxisParams& ax, pa_dtype act,
+                              pa_dtype cache_dtype, hipStream_t s);
 hipError_t launch_attn_generic(const AttnParams& p, pa_dtype act, pa_dtype cache_dtype,
                                hipStream_t s);
 hipError_t launch_decode_mfma(const AttnParams& p, pa_dtype act, pa_dtype cache_dtype,

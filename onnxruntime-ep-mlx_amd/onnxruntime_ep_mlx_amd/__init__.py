@@ -7,14 +7,14 @@ importing it loads the library and fails loudly if it has not been built.
 from . import _capi
 from ._capi import PagedAttentionError, load
 from .ops import (PagePool, attention, group_query_attention, group_query_attention_claim,
-                  paged_attention, pa_dtype,
-                  reshape_and_cache, rotary_append)
+                  masked_attention, multi_axis_rotary_append, paged_attention, pa_dtype,
+                  reshape_and_cache, rotary_append, shared_prefix_attention)
 
 load()
 
 __all__ = [
     "PagePool", "PagedAttentionError", "attention", "group_query_attention",
-    "group_query_attention_claim", "load", "pa_dtype",
-    "paged_attention",
-    "reshape_and_cache", "rotary_append", "_capi",
+    "group_query_attention_claim", "load", "masked_attention", "multi_axis_rotary_append",
+    "pa_dtype", "paged_attention",
+    "reshape_and_cache", "rotary_append", "shared_prefix_attention", "_capi",
 ]

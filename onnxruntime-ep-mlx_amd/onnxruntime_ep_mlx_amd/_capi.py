@@ -178,6 +178,29 @@ class PaNodeInfo(C.Structure):
     ]
 
 
+PA_MAX_AXES = 4  # include/pa_mi355x_ext.h
+
+
+class PaAxisRotary(C.Structure):
+    _fields_ = [
+        ("positions", C.c_void_p), ("position_stride", C.c_int64), ("axes", C.c_int32),
+        ("sections", C.c_int32 * PA_MAX_AXES), ("axes_interleaved", C.c_int32),
+        ("cos_cache", C.c_void_p), ("sin_cache", C.c_void_p), ("table_dtype", C.c_int),
+        ("rotary_positions", C.c_int64), ("rotary_half", C.c_int32),
+        ("rotary_offset", C.c_int32), ("rotary_interleaved", C.c_int32),
+    ]
+
+
+class PaMask(C.Structure):
+    _fields_ = [("distance_slopes", C.c_void_p), ("prefix_lens", C.c_void_p),
+                ("document_starts", C.c_void_p)]
+
+
+class PaSharedPrefix(C.Structure):
+    _fields_ = [("group_cum", C.c_void_p), ("prefix_lens", C.c_void_p), ("groups", C.c_int32),
+                ("max_prefix_len", C.c_int32)]
+
+
 class PagedAttentionError(RuntimeError):
     """Raised when a C-ABI call returns a non-zero status; the message is pa_last_error()."""
 
@@ -220,6 +243,23 @@ def load() -> C.CDLL:
                                    C.c_int, P, P, P, P, P, SZ, P]),
         "pa_attention_ex": (C.c_int, [C.POINTER(PaCache), C.POINTER(PaBatch), C.POINTER(PaAttn),
                                       C.c_int, P, P, P, P, P, SZ, I32, I32, P]),
+        "pa_multi_axis_rotary_append": (C.c_int, [C.POINTER(PaCache), C.POINTER(PaBatch), I32,
+                                                  C.c_int, P, I64, P, I64, P, I64,
+                                                  C.POINTER(PaAxisRotary), P, P, C.c_float, P,
+                                                  P]),
+        "pa_masked_attention_workspace_bytes": (SZ, [C.POINTER(PaCache), C.POINTER(PaBatch),
+                                                     C.POINTER(PaAttn), C.POINTER(PaMask),
+                                                     C.c_int]),
+        "pa_masked_attention": (C.c_int, [C.POINTER(PaCache), C.POINTER(PaBatch),
+                                          C.POINTER(PaAttn), C.POINTER(PaMask), C.c_int, P, P, P,
+                                          SZ, P]),
+        "pa_shared_prefix_attention_workspace_bytes": (SZ, [C.POINTER(PaCache),
+                                                            C.POINTER(PaBatch), C.POINTER(PaAttn),
+                                                            C.POINTER(PaSharedPrefix),
+                                                            C.POINTER(PaMask), C.c_int]),
+        "pa_shared_prefix_attention": (C.c_int, [C.POINTER(PaCache), C.POINTER(PaBatch),
+                                                 C.POINTER(PaAttn), C.POINTER(PaSharedPrefix),
+                                                 C.POINTER(PaMask), C.c_int, P, P, P, SZ, P]),
         "pa_paged_attention_workspace_bytes": (SZ, [C.POINTER(PaNode), C.POINTER(PaIO)]),
         "pa_paged_attention": (C.c_int, [C.POINTER(PaNode), C.POINTER(PaIO), P, SZ, P]),
         "pa_paged_attention_static": (C.c_int, [C.POINTER(PaNode), C.POINTER(PaIO), P]),

@@ -264,6 +264,213 @@ def attention(q, k_new, v_new, key_cache, value_cache, cum, past, block_table, *
     return out
 
 
+def _same_device(ref: torch.Tensor, tensors: dict, contiguous: bool = True) -> None:
+    """Device tensors on ref's device (contiguous ones unless said otherwise); None is left out."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        _need_cuda(name, t)
+        if t.device != ref.device:
+            raise ValueError(f"PagedAttention: {name} is on {t.device}, query/key on {ref.device}")
+        if contiguous:
+            _contig(name, t)
+
+
+def _rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> int:
+    """Row stride of a [num_tokens, width] tensor whose rows are dense (a view of wider rows, too)."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"PagedAttention: {name} must be [num_tokens, width] with dense rows")
+    if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0]):
+        raise ValueError(f"PagedAttention: {name} must match the other rows' dtype and tokens")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def multi_axis_rotary_append(query, key, value, key_cache, value_cache, cum, past, block_table,
+                             positions, cos_cache, sin_cache, *, num_heads, axis_sections,
+                             axes_interleaved=False, rotary_interleaved=0, rotary_offset=0,
+                             q_norm_weight=None, k_norm_weight=None, qk_norm_epsilon=1e-6,
+                             slot_mapping=None, slots_distinct=False, k_scale=None, v_scale=None,
+                             k_quant_type="NONE", v_quant_type="NONE", q_out=None):
+    """Fused RMSNorm + rotary positions of several axes + append (pa_multi_axis_rotary_append).
+
+    ``positions`` int64 [axes, num_tokens] (time, height, width); frequency i turns at the position
+    of its axis: ``axis_sections`` frequencies per axis one section after the other, or in turns
+    with ``axes_interleaved``.  cos / sin tables [positions, sum(axis_sections)] in the activation
+    dtype or float32.  ``query``, ``key`` and ``value`` are [num_tokens, width] with dense rows
+    (slices of packed QKV rows, too).  Keys and values go to their pages; returns the query rows
+    (``q_out`` when given, which may be ``query`` itself).  All arithmetic in float32, one rounding.
+    ``query`` None: keys and values alone."""
+    lib = capi.load()
+    ref = key
+    _need_cuda("key", key)
+    ql = 0 if query is None else _rows("query", query, key)
+    kl, vl = _rows("key", key), _rows("value", value, key)
+    _same_device(ref, {"query": query, "value": value}, contiguous=False)
+    _same_device(ref, {"key_cache": key_cache, "value_cache": value_cache, "cum": cum, "past": past,
+                       "block_table": block_table, "cos_cache": cos_cache, "sin_cache": sin_cache,
+                       "q_norm_weight": q_norm_weight, "k_norm_weight": k_norm_weight,
+                       "slot_mapping": slot_mapping, "q_out": q_out})
+    _same_device(ref, {"positions": positions}, contiguous=False)
+    sections = [int(n) for n in axis_sections]
+    if not 1 <= len(sections) <= capi.PA_MAX_AXES:
+        raise ValueError(f"PagedAttention: axis_sections must name 1..{capi.PA_MAX_AXES} axes")
+    T = key.shape[0]
+    if (positions.dtype != torch.int64 or tuple(positions.shape) != (len(sections), T)
+            or (T > 1 and positions.stride(1) != 1)):
+        raise ValueError("PagedAttention: positions must be int64 [axes, num_tokens] with dense rows")
+    if cos_cache.dim() != 2 or cos_cache.shape != sin_cache.shape or cos_cache.dtype != sin_cache.dtype:
+        raise ValueError("PagedAttention: cos_cache and sin_cache must be [positions, rotary_dim / 2] alike")
+    kv = key_cache.shape[2]
+    if key.shape[1] % kv or value.shape[1] != key.shape[1]:
+        raise ValueError("PagedAttention: key and value rows must hold kv_num_heads heads")
+    head = key.shape[1] // kv
+    for name, w in (("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight)):
+        if w is not None and (w.dtype != key.dtype or w.numel() != head):
+            raise ValueError(f"PagedAttention: {name} must be [head_size] in the activation dtype")
+    if query is not None:
+        if query.shape[1] != num_heads * head:
+            raise ValueError("PagedAttention: query rows must hold num_heads heads")
+        if q_out is None:
+            q_out = query.new_empty((T, num_heads * head))
+        elif q_out.dtype != query.dtype or tuple(q_out.shape) != (T, num_heads * head):
+            raise ValueError("PagedAttention: q_out must be [num_tokens, num_heads * head_size] in the activation dtype")
+    elif q_out is not None:
+        raise ValueError("PagedAttention: q_out without query")
+    cache = cache_desc(key_cache, value_cache, k_scale, v_scale, head_dim=head,
+                       k_quant_type=k_quant_type, v_quant_type=v_quant_type)
+    batch = batch_desc(cum, past, block_table, T, slot_mapping, 0,
+                       capi.PA_BATCH_SLOTS_DISTINCT if slots_distinct else 0)
+    rot = capi.PaAxisRotary(_ptr(positions), positions.stride(0) if len(sections) > 1 else 0,
+                            len(sections),
+                            (C.c_int32 * capi.PA_MAX_AXES)(*sections), int(bool(axes_interleaved)),
+                            _ptr(cos_cache), _ptr(sin_cache), pa_dtype(cos_cache.dtype),
+                            cos_cache.shape[0], cos_cache.shape[1], rotary_offset,
+                            rotary_interleaved)
+    with torch.cuda.device(ref.device):
+        capi.check(lib.pa_multi_axis_rotary_append(
+            C.byref(cache), C.byref(batch), num_heads, pa_dtype(key.dtype), _ptr(query), ql,
+            _ptr(key), kl, _ptr(value), vl, C.byref(rot), _ptr(q_norm_weight),
+            _ptr(k_norm_weight), qk_norm_epsilon, _ptr(q_out), _stream(ref.device)))
+    return q_out
+
+
+def _mask_desc(q, cum, num_heads, distance_slopes, prefix_lens, document_starts):
+    batch, T = cum.numel() - 1, q.shape[0]
+    for name, t, dt, n in (("distance_slopes", distance_slopes, torch.float32, num_heads),
+                           ("prefix_lens", prefix_lens, torch.int32, batch),
+                           ("document_starts", document_starts, torch.int32, T)):
+        if t is not None and (t.dtype != dt or t.numel() != n):
+            raise ValueError(f"PagedAttention: {name} must be {dt} with {n} elements")
+    _same_device(q, {"distance_slopes": distance_slopes, "prefix_lens": prefix_lens,
+                     "document_starts": document_starts})
+    return capi.PaMask(_ptr(distance_slopes), _ptr(prefix_lens), _ptr(document_starts))
+
+
+def _masked_call(q, key_cache, value_cache, cum, past, block_table, share, *, num_heads, scale,
+                 softcap, local_window_size, is_causal, head_sink, distance_slopes, prefix_lens,
+                 document_starts, k_scale, v_scale, k_quant_type, v_quant_type, max_query_len,
+                 max_context_len, out, workspace):
+    lib = capi.load()
+    _need_cuda("query", q)
+    _contig("query", q)
+    if q.dim() != 2 or num_heads <= 0 or q.shape[1] % num_heads:
+        raise ValueError("PagedAttention: query must be [num_tokens, num_heads * head_size]")
+    if value_cache is None:
+        raise ValueError("PagedAttention: masked attention takes the SEPARATE cache layout")
+    _same_device(q, {"key_cache": key_cache, "value_cache": value_cache, "cum": cum, "past": past,
+                     "block_table": block_table, "head_sink": head_sink, "out": out,
+                     "k_scale": k_scale, "v_scale": v_scale, "workspace": workspace})
+    if past.numel() != cum.numel() - 1 or block_table.dim() != 2 or block_table.shape[0] != past.numel():
+        raise ValueError("PagedAttention: inconsistent cumulative lengths, past lengths or block table")
+    if head_sink is not None and (head_sink.dtype != q.dtype or head_sink.numel() != num_heads):
+        raise ValueError("PagedAttention: head_sink must be [num_heads] in the activation dtype")
+    mask = _mask_desc(q, cum, num_heads, distance_slopes, prefix_lens, document_starts)
+    cache = cache_desc(key_cache, value_cache, k_scale, v_scale, head_dim=q.shape[1] // num_heads,
+                       k_quant_type=k_quant_type, v_quant_type=v_quant_type)
+    batch = batch_desc(cum, past, block_table, q.shape[0], None, max_query_len,
+                       capi.PA_BATCH_NEW_ROWS_IN_CACHE, max_context_len)
+    attn = attn_desc(num_heads, scale, softcap, local_window_size, is_causal, head_sink)
+    act = pa_dtype(q.dtype)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("PagedAttention: out must match query's shape and dtype")
+    head = (C.byref(cache), C.byref(batch), C.byref(attn))
+    tail = (C.byref(mask), act)
+    if share is not None:
+        head += (C.byref(share),)
+        size, call = (lib.pa_shared_prefix_attention_workspace_bytes, lib.pa_shared_prefix_attention)
+    else:
+        size, call = lib.pa_masked_attention_workspace_bytes, lib.pa_masked_attention
+    with torch.cuda.device(q.device):
+        nbytes = size(*head, *tail)
+        # A workspace of the call's own: torch's allocator keeps it apart from work on other streams
+        # and in other captured graphs.
+        if workspace is None:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        have = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        capi.check(call(*head, *tail, _ptr(q), _ptr(out), _ptr(workspace), have,
+                        _stream(q.device)))
+    return out
+
+
+def masked_attention(q, key_cache, value_cache, cum, past, block_table, *, num_heads, scale=0.0,
+                     softcap=0.0, local_window_size=-1, is_causal=1, head_sink=None,
+                     distance_slopes=None, prefix_lens=None, document_starts=None, k_scale=None,
+                     v_scale=None, k_quant_type="NONE", v_quant_type="NONE", max_query_len=0,
+                     max_context_len=0, out=None, workspace=None):
+    """Attention over the pages, the new tokens' keys and values among them, under masks and a bias
+    by distance (pa_masked_attention).
+
+    A token at position i of its sequence sees key j iff max(its document's start,
+    i - local_window_size + 1) <= j < max(i + 1, the sequence's prefix length), and its score is
+    softcap(scale * q.k) - distance_slopes[h] * |i - j|.  ``document_starts`` int32 [num_tokens],
+    ``prefix_lens`` int32 [batch], ``distance_slopes`` float32 [num_heads]; each may be None.  Rows
+    that see no key are zero.  ``max_query_len`` / ``max_context_len`` bound every sequence's new
+    tokens / past + new tokens (0 = unknown).  ``workspace``: a uint8 tensor of at least the queried
+    size, for callers that keep their own."""
+    return _masked_call(q, key_cache, value_cache, cum, past, block_table, None,
+                        num_heads=num_heads, scale=scale, softcap=softcap,
+                        local_window_size=local_window_size, is_causal=is_causal,
+                        head_sink=head_sink, distance_slopes=distance_slopes,
+                        prefix_lens=prefix_lens, document_starts=document_starts,
+                        k_scale=k_scale, v_scale=v_scale, k_quant_type=k_quant_type,
+                        v_quant_type=v_quant_type, max_query_len=max_query_len,
+                        max_context_len=max_context_len, out=out, workspace=workspace)
+
+
+def shared_prefix_attention(q, key_cache, value_cache, cum, past, block_table, group_cum,
+                            shared_lens, *, num_heads, scale=0.0, softcap=0.0,
+                            local_window_size=-1, is_causal=1, head_sink=None,
+                            distance_slopes=None, prefix_lens=None, document_starts=None,
+                            k_scale=None, v_scale=None, k_quant_type="NONE", v_quant_type="NONE",
+                            max_query_len=0, max_context_len=0, max_prefix_len=0, out=None,
+                            workspace=None):
+    """masked_attention for groups of consecutive sequences whose first keys lie in the same pages
+    (pa_shared_prefix_attention): sequences [group_cum[i], group_cum[i + 1]) share their first
+    ``shared_lens[i]`` keys, which are read once for all of them.  ``group_cum`` int32 [groups + 1],
+    ``shared_lens`` int32 [groups]; the block tables of a group name the same pages for those keys.
+    ``max_prefix_len`` bounds ``shared_lens`` (0 = unknown).  ``prefix_lens`` are masked_attention's:
+    leading keys that every row of a sequence sees."""
+    for name, t in (("group_cum", group_cum), ("shared_lens", shared_lens)):
+        if t.dtype != torch.int32:
+            raise ValueError(f"input {name} must be int32")
+    if group_cum.numel() != shared_lens.numel() + 1:
+        raise ValueError("PagedAttention: group_cum must have one element more than shared_lens")
+    _need_cuda("query", q)
+    _same_device(q, {"group_cum": group_cum, "shared_lens": shared_lens})
+    share = capi.PaSharedPrefix(_ptr(group_cum), _ptr(shared_lens), shared_lens.numel(),
+                                max_prefix_len)
+    return _masked_call(q, key_cache, value_cache, cum, past, block_table, share,
+                        num_heads=num_heads, scale=scale, softcap=softcap,
+                        local_window_size=local_window_size, is_causal=is_causal,
+                        head_sink=head_sink, distance_slopes=distance_slopes,
+                        prefix_lens=prefix_lens, document_starts=document_starts,
+                        k_scale=k_scale, v_scale=v_scale, k_quant_type=k_quant_type,
+                        v_quant_type=v_quant_type, max_query_len=max_query_len,
+                        max_context_len=max_context_len, out=out, workspace=workspace)
+
+
 def paged_attention(query, key, value, key_cache, value_cache, cumulative_sequence_length,
                     past_seqlens, block_table, cos_cache=None, sin_cache=None,
                     slot_mapping=None, head_sink=None, q_norm_weight=None, k_norm_weight=None,
