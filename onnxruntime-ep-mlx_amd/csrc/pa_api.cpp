@@ -1273,30 +1273,142 @@ RunOpts masked_opts(const pa_mask* mask) {
   return o;
 }
 
+// Launch shape and workspace of the matrix-core kernel over key ranges (pa_ranged.hip).
+struct RangedPlan {
+  bool on = false;
+  int slots = 0, slot_rows = 0, grid = 0;
+  bool merge = false;
+  int64_t part_slots = 0;
+  size_t o_bytes = 0, ml_bytes = 0, table_bytes = 0;
+  size_t bytes() const { return o_bytes + ml_bytes + table_bytes; }
+};
+RangedPlan ranged_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a,
+                       const pa_shared_prefix* share, pa_dtype act) {
+  RangedPlan r;
+  if (!c->value_cache || !pa::ranged_supported(c->head_dim, act, c->dtype) || a->num_heads <= 0 ||
+      a->num_heads % c->kv_heads != 0 || b->num_tokens <= 0)
+    return r;
+  const int64_t g = a->num_heads / c->kv_heads, T = b->num_tokens;
+  const int64_t groups = share ? share->groups : 0;
+  // blocks of at most 128 rows of every sequence, and of every group's rows
+  const int64_t blocks = T * g / 128 + b->batch + (groups ? T * g / 128 + groups : 0);
+  const int64_t items = blocks * c->kv_heads;
+  if (items >= ((int64_t)1 << 24) || T * g > INT32_MAX) return r;
+  const int mq = b->max_query_len > 0 ? b->max_query_len : b->num_tokens;
+  r.on = true;
+  r.slots = (c->head_dim > 128 ? 1 : 2) * device_cus();
+  const bool split = items < 2 * (int64_t)r.slots;  // (else the device decides)
+  r.grid = (int)(split ? r.slots : std::max<int64_t>(items, r.slots));
+  // an item meets a workgroup at place workgroup + item; whole items leave parts for shared prefixes only
+  r.part_slots = r.slots + std::min<int64_t>(items, 2 * (int64_t)r.slots);
+  if (groups && !split) r.part_slots = std::max(r.part_slots, 2 * items);
+  r.slot_rows = !groups && mq * g <= 32 ? 32 : 128;
+  const int64_t ctx = b->max_context_len > 0 ? b->max_context_len
+                                             : (int64_t)b->max_blocks * c->block_size;
+  r.merge = groups > 0 || ctx > 64;
+  const size_t rows = (size_t)r.part_slots * r.slot_rows;
+  r.o_bytes = align256(rows * c->head_dim * sizeof(float));
+  r.ml_bytes = align256(rows * 2 * sizeof(float));
+  r.table_bytes = align256((size_t)(1 + groups + b->batch) * sizeof(pa::RTable));
+  return r;
+}
+
+size_t masked_workspace(const pa_cache* c, const pa_batch* b, const pa_attn* a,
+                        const pa_shared_prefix* share, pa_dtype act) {
+  if (!c || !b || !a || c->kv_heads <= 0 || b->batch <= 0) return 0;
+  const RangedPlan r = ranged_plan(c, b, a, share, act);
+  return r.on ? r.bytes() : ws_need(c, b, a, act, 3, 0).best;
+}
+
+int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, const pa_mask* mask,
+                     const pa_shared_prefix* share, pa_dtype act, const void* q, void* out,
+                     void* ws, size_t ws_bytes, hipStream_t s) {
+  const int rc = check_masked(c, b, a, act);
+  if (rc) return rc;
+  const RangedPlan r = ranged_plan(c, b, a, share, act);
+  // Other types and head sizes: the VALU kernel, which reads a shared prefix for every row
+  if (!r.on)
+    return run_attention(c, b, a, act, q, nullptr, nullptr, out, ws, ws_bytes, 3, 0, s,
+                         masked_opts(mask));
+  if (!q || !out) return fail(PA_ERR_INVALID_ARGUMENT, "q/out pointers are NULL");
+  if (a->v_head_size > 0 && a->v_head_size != c->head_dim)
+    return fail(PA_ERR_INVALID_ARGUMENT, "SEPARATE layout requires equal key and value head sizes");
+  if (!(a->softcap >= 0.0f) || !std::isfinite(a->softcap))
+    return fail(PA_ERR_INVALID_ARGUMENT, "softcap must be finite and non-negative");
+  if (!ws || ws_bytes < r.bytes())
+    return fail(PA_ERR_INVALID_ARGUMENT, "workspace too small: need %zu bytes, got %zu", r.bytes(),
+                ws_bytes);
+  pa::RangedParams p{};
+  p.q = q;
+  p.key_cache = c->key_cache;
+  p.value_cache = c->value_cache;
+  p.cum = b->cumulative_sequence_length;
+  p.past = b->past_seqlens;
+  p.block_table = b->block_table;
+  p.head_sink = a->head_sink;
+  p.out = out;
+  if (mask) {
+    p.slopes = mask->distance_slopes;
+    p.prefix_lens = mask->prefix_lens;
+    p.doc_starts = mask->document_starts;
+  }
+  if (share) {
+    p.group_cum = share->group_cum;
+    p.shared_lens = share->prefix_lens;
+    p.groups = share->groups;
+  }
+  char* base = reinterpret_cast<char*>(ws);
+  p.part_o = reinterpret_cast<float*>(base);
+  p.part_ml = reinterpret_cast<float2*>(base + r.o_bytes);
+  p.table = reinterpret_cast<pa::RTable*>(base + r.o_bytes + r.ml_bytes);
+  p.num_blocks = c->num_blocks;
+  p.part_slots = r.part_slots;
+  p.block_size = c->block_size;
+  const bool pow2 = (c->block_size & (c->block_size - 1)) == 0;
+  p.bs_shift = pow2 && c->block_size >= 16 ? __builtin_ctz((unsigned)c->block_size) : -1;
+  p.kv_heads = c->kv_heads;
+  p.head_dim = c->head_dim;
+  p.num_heads = a->num_heads;
+  p.batch = b->batch;
+  p.max_blocks = b->max_blocks;
+  p.num_tokens = b->num_tokens;
+  p.window = a->local_window_size;
+  p.causal = a->is_causal ? 1 : 0;
+  p.scale = a->scale != 0.0f ? a->scale : 1.0f / std::sqrt((float)c->head_dim);
+  p.scale_log2 = std::fabs(p.scale) * pa::kLog2e;
+  p.softcap = a->softcap;
+  p.qxor = p.scale < 0.0f ? 0x80008000u : 0u;
+  p.slots = r.slots;
+  p.least = 2;
+  p.slot_rows = r.slot_rows;
+  p.grid = r.grid;
+  p.merge = r.merge ? 1 : 0;
+  const hipError_t e = pa::launch_ranged(p, act, s);
+  if (e != hipSuccess) return hip_fail(e, "masked attention launch");
+  return PA_OK;
+}
+
 }  // namespace
 
 size_t pa_masked_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
                                            const pa_attn* attn, const pa_mask*,
                                            pa_dtype act_dtype) {
-  if (!cache || !batch || !attn || cache->kv_heads <= 0 || batch->batch <= 0) return 0;
-  return ws_need(cache, batch, attn, act_dtype, 3, 0).best;
+  return masked_workspace(cache, batch, attn, nullptr, act_dtype);
 }
 
 int pa_masked_attention(const pa_cache* cache, const pa_batch* batch, const pa_attn* attn,
                         const pa_mask* mask, pa_dtype act_dtype, const void* q, void* out,
                         void* workspace, size_t workspace_bytes, pa_stream_t stream) {
-  const int rc = check_masked(cache, batch, attn, act_dtype);
-  if (rc) return rc;
-  return run_attention(cache, batch, attn, act_dtype, q, nullptr, nullptr, out, workspace,
-                       workspace_bytes, 3, 0, reinterpret_cast<hipStream_t>(stream),
-                       masked_opts(mask));
+  return masked_attention(cache, batch, attn, mask, nullptr, act_dtype, q, out, workspace,
+                          workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
 
 size_t pa_shared_prefix_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
                                                   const pa_attn* attn,
-                                                  const pa_shared_prefix*, const pa_mask* mask,
+                                                  const pa_shared_prefix* share, const pa_mask*,
                                                   pa_dtype act_dtype) {
-  return pa_masked_attention_workspace_bytes(cache, batch, attn, mask, act_dtype);
+  if (!share || share->groups < 1) return 0;
+  return masked_workspace(cache, batch, attn, share, act_dtype);
 }
 
 int pa_shared_prefix_attention(const pa_cache* cache, const pa_batch* batch, const pa_attn* attn,
@@ -1305,8 +1417,8 @@ int pa_shared_prefix_attention(const pa_cache* cache, const pa_batch* batch, con
                                size_t workspace_bytes, pa_stream_t stream) {
   const int rc = check_share(share);
   if (rc) return rc;
-  return pa_masked_attention(cache, batch, attn, mask, act_dtype, q, out, workspace,
-                             workspace_bytes, stream);
+  return masked_attention(cache, batch, attn, mask, share, act_dtype, q, out, workspace,
+                          workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
 
 // ------------------------------------------------------------------------------ multi-axis append

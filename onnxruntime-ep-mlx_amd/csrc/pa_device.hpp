@@ -410,6 +410,49 @@ struct AttnParams {
   int32_t* plan_seq;
 };
 
+// Attention over key ranges per row, with shared prefixes (pa_ranged.hip).
+// A source's place in the flat list of 64-key tiles, for the merge (entry 0: all tiles, items, tiles per
+// workgroup; then groups and sequences).
+struct RTable {
+  int64_t first;
+  int32_t item, tiles, tok0, rows, ka, pad;
+};
+struct RangedParams {
+  const void* q;
+  const void* key_cache;
+  const void* value_cache;
+  const int32_t* cum;
+  const int32_t* past;
+  const int32_t* block_table;
+  const void* head_sink;
+  void* out;
+  // masks and shared prefixes (pa_mask, pa_shared_prefix); groups == 0: none shared
+  const float* slopes;
+  const int32_t* prefix_lens;
+  const int32_t* doc_starts;
+  const int32_t* group_cum;
+  const int32_t* shared_lens;
+  // Workspace: partial rows [part_slots][slot_rows][head_dim], their (m, l), and the table
+  float* part_o;
+  float2* part_ml;
+  RTable* table;
+  int64_t num_blocks, part_slots;
+  int32_t groups;
+  int32_t block_size, bs_shift;  // bs_shift: log2 of a power of two of at least 16, else -1
+  int32_t kv_heads, head_dim, num_heads;
+  int32_t batch, max_blocks, num_tokens;
+  int32_t window, causal;
+  float scale, scale_log2, softcap;  // scale_log2: |scale| log2(e)
+  uint32_t qxor;                     // 0x80008000 where scale is negative
+  int32_t slots;      // workgroups that share the tiles of few items
+  int32_t least;      // tiles per workgroup, at least
+  int32_t slot_rows;  // rows of a partial slot: 32 where every block is known to be that small, else 128
+  int32_t grid;       // workgroups
+  int32_t merge;      // some row may have several pieces
+};
+hipError_t launch_ranged(const RangedParams& p, pa_dtype act, hipStream_t s);
+bool ranged_supported(int head_dim, pa_dtype act, pa_dtype cache_dtype);
+
 // Parts of an item of a short planned prefill, at most, their keys in percent of an even share of
 // the workgroup slots (prefill_plan_kernel) and at least.
 constexpr int kFineParts = 16;

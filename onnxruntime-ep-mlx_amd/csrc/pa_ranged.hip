@@ -1,0 +1,1062 @@
+// pa_ranged.hip — paged attention whose rows each see a range of keys (documents, prefixes, windows,
+// causality), with a bias by distance, and prefixes that a group of sequences shares, on gfx950 matrix
+// cores.
+//
+// Row r of a sequence (or of a group, for its shared prefix) is query token r / g and head kh g + r % g
+// of kv-head kh.  It sees keys [lo, hi); with x = softcap(scale q.k) log2(e) - slope |i - j| the output
+// is sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m), m a maximum that moves only when a score exceeds it by
+// more than 2^8.
+//
+// Work.  Sources: every group (all its rows against the shared keys, read through its first
+// sequence's table) and every sequence (its rows against the keys behind the shared ones).  An item is a
+// block of rows of one source and kv-head; it costs one per 64 keys.  While the items are few (under two
+// per workgroup slot) the flat list of all items' 64-key tiles is cut into equal parts, one workgroup
+// each, whatever item borders lie inside: an item that meets several workgroups leaves (m, l, O) of each
+// in fp32 and ranged_merge_kernel joins them, as it joins a row's shared and own keys.  With more items
+// each workgroup takes a whole one.  The plan is a scan over the lengths that every workgroup makes for
+// itself, from the device's metadata.
+//
+// Both products run transposed on 32x32x16 tiles, so that a lane holds one query row:
+//   S^T[key][row] = K Q^T   (A: 32 keys x 16 dims from LDS, B: the queries in registers)
+//   O^T[dim][row] = V^T P^T (A: 32 dims x 16 keys by transposing LDS reads, B: the probabilities as the
+//                            score product leaves them)
+// A row's maximum and sum need one exchange between the lane halves, and its range, slope and position
+// are scalars of the lane.  Probabilities enter the second product rounded to the activation type (half
+// a step of it, the output's own rounding); scores, statistics and sums are fp32.
+//
+// Rows of more than 32 (prompts, shared prefixes): four wavefronts of 32 rows each on the same 64-key
+// tile (32 keys at head 256), staged by direct loads from the pages into two LDS buffers, one barrier
+// per tile.  At most 32 (decode): the wavefronts take 32-key tiles in turn, each with a tile of its own
+// in LDS, the next keys in flight while the values are multiplied, and meet in LDS at the end.
+//
+// Masked keys weigh exactly zero, but zero times an infinite value is NaN in the product: rows that come
+// out not finite are computed again one key at a time, which skips what they do not see.  Tiles read no
+// key outside [first visible, last visible] of their rows (such places repeat a visible one), so pages
+// behind a sequence's end or before its window may hold anything.
+#include <algorithm>
+
+#include "pa_tiles.hpp"
+
+namespace pa {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+constexpr int kRTile = 64;     // keys per unit of cost
+constexpr int kRWide = 128;    // rows of a block of four wavefronts
+constexpr int kRNarrow = 32;   // rows of a block whose wavefronts split the keys
+constexpr int kRChunk = 256;   // sources scanned at a time, one per thread
+constexpr int64_t kRMergeRows = 4096;  // rows up to which the merge gives each a workgroup
+
+template <typename TT>
+__device__ __forceinline__ f32x16 mfma_r(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (TT::code == PA_DTYPE_FLOAT16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float half_swap(float x) {  // lane l ^ 32's x
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x),
+                                                  __builtin_bit_cast(uint32_t, x), false, false);
+  return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// Eight probabilities in T, rounded to nearest even.
+template <typename TT>
+__device__ __forceinline__ u32x4 pack8(const float* x) {
+  typedef float f32x8 __attribute__((ext_vector_type(8)));
+  f32x8 v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = x[i];
+  return __builtin_bit_cast(u32x4, __builtin_convertvector(v, typename TT::vec8));
+}
+
+// Direct LDS loads of 16 bytes per lane to lds + 16 * lane, as inline assembly so that the compiler's
+// memory counters do not see them and nothing waits for them but the tile loops (wait_loads).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma_base(const char* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off), "s"(base), "s"(lds)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma_ptr(const char* ptr, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :
+               : "v"(ptr), "s"(lds)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // until at most N vector loads are outstanding
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(lds_char*)p;
+}
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)x) | ((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32));
+}
+// A table entry at a wave-uniform place, through the scalar cache (no kernel writes the tables).
+__device__ __forceinline__ int scalar_load(const int32_t* p) {
+  typedef const __attribute__((address_space(4))) int32_t* cptr;
+  return *(cptr)(uintptr_t)p;
+}
+
+// ------------------------------------------------------------------------------------ the plan
+struct RSeq {
+  int s0, nq, past, total;
+};
+__device__ __forceinline__ RSeq r_seq(const RangedParams& p, int b) {
+  RSeq q;
+  const int c0 = p.cum[b], c1 = p.cum[b + 1], pb = p.past[b];
+  const int cap = (int)min((int64_t)p.max_blocks * p.block_size, (int64_t)(INT32_MAX / 2));
+  q.s0 = min(max(c0, 0), p.num_tokens);
+  q.nq = min(min(max(c1, q.s0), p.num_tokens) - q.s0, cap);
+  q.past = min(max(pb, 0), cap - q.nq);
+  q.total = q.past + q.nq;
+  return q;
+}
+// Sequences of group gi and the keys that they share: none in a group of one sequence, at most the
+// keys of its first.
+struct RGroup {
+  int b0, b1, prefix;
+};
+__device__ __forceinline__ RGroup r_group(const RangedParams& p, int gi) {
+  RGroup q;
+  q.b0 = min(max(p.group_cum[gi], 0), p.batch);
+  q.b1 = min(max(p.group_cum[gi + 1], q.b0), p.batch);
+  q.prefix = q.b1 - q.b0 < 2 ? 0 : min(max(p.shared_lens[gi], 0), r_seq(p, q.b0).total);
+  return q;
+}
+// Group of sequence b, -1 if none.
+__device__ __forceinline__ int group_of(const RangedParams& p, int b) {
+  int lo = 0, hi = p.groups;  // the last group that begins at or before b
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (p.group_cum[mid] <= b) lo = mid + 1; else hi = mid;
+  }
+  return lo > 0 && b < p.group_cum[lo] ? lo - 1 : -1;
+}
+// Shared keys in front of sequence b's own.
+__device__ __forceinline__ int shared_of(const RangedParams& p, int b, int total) {
+  if (p.groups == 0) return 0;
+  const int gi = group_of(p, b);
+  return gi < 0 ? 0 : min(r_group(p, gi).prefix, total);
+}
+
+struct RSource {
+  int64_t first;  // its first tile in the flat list
+  int item;       // its first item
+  int tok0, rows; // first token, rows (tokens * g) of one kv-head
+  int b0, b1;     // its sequences; b0's table names the pages
+  int ka, kb;     // its keys
+  int tiles;      // tiles of one item
+};
+__device__ __forceinline__ int r_blocks(int rows) {
+  return rows <= kRNarrow ? (rows > 0) : (rows + kRWide - 1) / kRWide;
+}
+// Source i: groups, then sequences (first and item are the scan's).
+__device__ __forceinline__ RSource r_source(const RangedParams& p, int i) {
+  RSource s{};
+  const int g = p.num_heads / p.kv_heads;
+  if (i >= p.groups + p.batch) return s;
+  if (i < p.groups) {
+    const RGroup q = r_group(p, i);
+    if (q.prefix == 0) return s;
+    s.b0 = q.b0;
+    s.b1 = q.b1;
+    s.tok0 = r_seq(p, q.b0).s0;
+    const RSeq last = r_seq(p, q.b1 - 1);
+    s.rows = max(last.s0 + last.nq - s.tok0, 0) * g;
+    s.kb = q.prefix;
+  } else {
+    const int b = i - p.groups;
+    const RSeq q = r_seq(p, b);
+    s.b0 = b;
+    s.b1 = b + 1;
+    s.tok0 = q.s0;
+    s.rows = q.nq * g;
+    s.ka = shared_of(p, b, q.total);
+    if (p.window > 0) s.ka = max(s.ka, min(q.past - p.window + 1, q.total));
+    s.kb = q.total;
+  }
+  // (a sequence without keys of its own keeps a tile, whose workgroup writes its empty rows)
+  s.tiles = s.rows > 0 ? max((s.kb + kRTile - 1) / kRTile - s.ka / kRTile, 1) : 0;
+  return s;
+}
+
+// The scan's outcome: tiles and items of all sources and tiles per workgroup (0: an item each).
+struct RPlan {
+  int64_t tiles;
+  int items, per;
+};
+struct RScan {
+  RSource src[kRChunk];
+  int64_t wt[4];
+  int wi[4];
+};
+__device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+// Sources base .. base + 255 with their places in the flat list into sh.src; t0 / i0: tiles and items
+// before them, moved past them.  Called by all 256 threads.
+__device__ __forceinline__ void scan_chunk(const RangedParams& p, int base, RScan& sh, int64_t& t0,
+                                           int& i0) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  RSource s = r_source(p, base + tid);
+  const int items = r_blocks(s.rows) * p.kv_heads;
+  // items above, tiles below: a batch holds fewer than 2^24 items and 2^40 tiles (host)
+  const int64_t mine = ((int64_t)items << 40) + (int64_t)items * s.tiles;
+  const int64_t incl = scan64(mine, lane);
+  __syncthreads();  // the last chunk's readers are done
+  if (lane == 63) sh.wt[wave] = incl;
+  __syncthreads();
+  int64_t before = incl - mine, all = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) before += sh.wt[w];
+    all += sh.wt[w];
+  }
+  all = uniform64(all);
+  constexpr int64_t low = ((int64_t)1 << 40) - 1;
+  s.first = t0 + (before & low);
+  s.item = i0 + (int)(before >> 40);
+  sh.src[tid] = s;
+  t0 += all & low;
+  i0 += (int)(all >> 40);
+  __syncthreads();
+}
+__device__ __forceinline__ RPlan r_plan(const RangedParams& p, RScan& sh) {
+  RPlan r{0, 0, 0};
+  for (int base = 0; base < p.groups + p.batch; base += kRChunk)
+    scan_chunk(p, base, sh, r.tiles, r.items);
+  if (r.items < 2 * p.slots)
+    r.per = (int)max((r.tiles + p.slots - 1) / p.slots, (int64_t)p.least);
+  return r;
+}
+// Workgroup that takes tile x of an item (its first tile at `at`, its number `item`).
+__device__ __forceinline__ int64_t r_worker(int per, int64_t at, int item, int x) {
+  return per > 0 ? (at + x) / per : item;
+}
+
+// One row: its token, head, position and range.
+struct RRow {
+  int t, h, pos, lo, hi, shared;
+  bool valid;
+};
+__device__ __forceinline__ RRow r_row(const RangedParams& p, int t, int h, int b, bool valid) {
+  RRow r;
+  const RSeq q = r_seq(p, b);
+  r.t = t;
+  r.h = h;
+  r.pos = q.past + (t - q.s0);
+  r.valid = valid;
+  r.shared = shared_of(p, b, q.total);
+  int hi = p.causal ? r.pos + 1 : q.total;
+  if (p.causal && p.prefix_lens) hi = max(hi, p.prefix_lens[b]);
+  r.hi = valid ? min(hi, q.total) : 0;
+  int lo = p.window > 0 ? r.pos - p.window + 1 : 0;
+  if (p.doc_starts) lo = max(lo, p.doc_starts[t]);
+  r.lo = valid ? max(lo, 0) : 0;
+  return r;
+}
+
+// A workgroup's part of an item.
+struct RUnit {
+  RSource s;
+  bool group;
+  int kh, row0;    // first row of the block
+  int64_t at;      // the item's first tile in the flat list
+  int item, per;
+  int x0, x1;      // tiles of the item
+  int64_t worker;
+};
+// What a row needs of a unit: keys [lo, hi) of the unit that it sees, whether all that it sees lies in this
+// unit, whether this unit zeroes it (it sees nothing at all).
+struct RPart {
+  int lo, hi;
+  bool any, single, zero;
+};
+__device__ __forceinline__ RPart r_part(const RUnit& u, const RRow& r) {
+  RPart q;
+  const int sa = u.group ? 0 : r.shared, sb = u.group ? min(r.shared, u.s.kb) : u.s.kb;
+  const int a = max(r.lo, sa), z = min(r.hi, sb), kt = u.s.ka / kRTile;
+  q.lo = max(a, (kt + u.x0) * kRTile);
+  q.hi = min(z, (kt + u.x1) * kRTile);
+  q.any = r.valid && q.lo < q.hi;
+  const bool other = u.group ? r.hi > max(r.lo, r.shared) : r.lo < min(r.hi, r.shared);
+  q.single = q.any && !other &&
+             r_worker(u.per, u.at, u.item, a / kRTile - kt) ==
+                 r_worker(u.per, u.at, u.item, (z - 1) / kRTile - kt);
+  q.zero = r.valid && !u.group && r.lo >= r.hi && u.x0 == 0;
+  return q;
+}
+__device__ __forceinline__ int r_token_seq(const RangedParams& p, const RSource& s, int t) {
+  int lo = s.b0, hi = s.b1;  // the last sequence that begins at or before t
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.cum[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+__device__ __forceinline__ RRow r_unit_row(const RangedParams& p, const RUnit& u, int rl) {
+  const int g = p.num_heads / p.kv_heads, r = u.row0 + rl;
+  const bool valid = r < u.s.rows;
+  const int t = u.s.tok0 + (valid ? r / g : 0), h = u.kh * g + (valid ? r % g : 0);
+  return r_row(p, t, h, u.group ? r_token_seq(p, u.s, t) : u.s.b0, valid);
+}
+
+template <typename TT>
+__device__ __forceinline__ float r_sink(const RangedParams& p, int h) {
+  return p.head_sink ? TT::to_f32(reinterpret_cast<const typename TT::raw*>(p.head_sink)[h]) * kLog2e
+                     : kNegInf;
+}
+
+// Element offset of key / value row `pos` of kv-head kh in the pages that table row b names.
+__device__ __forceinline__ int64_t r_offset(const RangedParams& p, int b, int kh, int pos, int D) {
+  const int bi = min(pos / p.block_size, p.max_blocks - 1);
+  int64_t page = p.block_table[(int64_t)b * p.max_blocks + bi];
+  page = min(max(page, (int64_t)0), p.num_blocks - 1);
+  return ((page * p.block_size + pos % p.block_size) * p.kv_heads + kh) * D;
+}
+
+// One row of a unit one key at a time, by one wavefront, written like the others'.
+template <typename TT, int D>
+__device__ __forceinline__ void slow_row(const RangedParams& p, const RUnit& u, int rl) {
+  constexpr int NE = (D + 63) / 64;
+  const int lane = threadIdx.x & 63;
+  const RRow r = r_unit_row(p, u, rl);
+  const RPart q = r_part(u, r);
+  using raw = typename TT::raw;
+  float qv[NE], o[NE], m = kNegInf, l = 0.0f;
+  const float slope = p.slopes ? p.slopes[r.h] : 0.0f;
+#pragma unroll
+  for (int k = 0; k < NE; ++k) {
+    const int e = lane + 64 * k;
+    qv[k] = e < D ? TT::to_f32(reinterpret_cast<const raw*>(p.q)[((int64_t)r.t * p.num_heads + r.h) * D + e])
+                  : 0.0f;
+    o[k] = 0.0f;
+  }
+  for (int j = q.lo; j < q.hi; ++j) {
+    const int64_t at = r_offset(p, u.s.b0, u.kh, j, D);
+    float part = 0.0f, v[NE];
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+      const int e = lane + 64 * k;
+      v[k] = e < D ? TT::to_f32(reinterpret_cast<const raw*>(p.value_cache)[at + e]) : 0.0f;
+      if (e < D) part += qv[k] * TT::to_f32(reinterpret_cast<const raw*>(p.key_cache)[at + e]);
+    }
+    float x = wave_sum(part) * p.scale;
+    if (p.softcap > 0.0f) x = p.softcap * tanhf(x / p.softcap);
+    x = (x - slope * fabsf((float)(r.pos - j))) * kLog2e;
+    const float mn = fmaxf(m, x), ms = mn == kNegInf ? 0.0f : mn;
+    const float a = m == kNegInf ? 0.0f : exp2f(m - mn), w = exp2f(x - ms);
+    l = l * a + w;
+#pragma unroll
+    for (int k = 0; k < NE; ++k) o[k] = o[k] * a + w * v[k];
+    m = mn;
+  }
+  if (q.single) {
+    const float f = finalize_factor(m, l, r_sink<TT>(p, r.h));
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+      const int e = lane + 64 * k;
+      if (e < D)
+        reinterpret_cast<raw*>(p.out)[((int64_t)r.t * p.num_heads + r.h) * D + e] =
+            TT::from_f32(o[k] * (l == l ? f : l));
+    }
+  } else {
+    const int64_t slot = u.worker + u.item;
+    if (slot >= p.part_slots) return;
+    const int64_t row = slot * p.slot_rows + rl;
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+      const int e = lane + 64 * k;
+      if (e < D) p.part_o[row * D + e] = o[k];
+    }
+    if (lane == 0) p.part_ml[row] = float2{m, l};
+  }
+}
+
+// ------------------------------------------------------------------------------------ the tiles
+// LDS rows of one tile: PITCH bytes each, 16-byte pieces exchanged by an XOR with the row so that the
+// operand reads of 16 lanes meet 16 different bank groups.  Keys are read a row per lane: piece ^ row.
+// Values are read transposed, four rows of 32 dims at a time: pieces in fours, exchanged by row % 4.
+// Head 96 keeps rows of 256 bytes (its last four pieces are read twice and used once).
+template <int D>
+struct RGeom {
+  static constexpr int PITCH = D == 96 ? 256 : 2 * D;
+  static constexpr int CPR = PITCH / 16;     // pieces per row
+  static constexpr int RPI = 64 / CPR;       // rows per load instruction
+  static constexpr int KT = D > 128 ? 32 : 64;  // keys of a wide tile
+  static constexpr int WIDE = 2 * 2 * KT * PITCH;     // two buffers of keys and values
+  static constexpr int NARROW = 4 * 2 * 32 * PITCH;   // four wavefronts' tiles of 32 keys
+  static constexpr int LDS = WIDE > NARROW ? WIDE : NARROW;
+  __device__ static int kx(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
+  __device__ static int vx(int row) { return D == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3); }
+};
+
+// Loads of rows [R0, R0 + 16 or 8 * ..) of a tile by one wavefront: where its pieces come from.
+struct RFeed {
+  const char *kc, *vc;
+  const int32_t* bt;
+  int64_t rowb, hoff;  // bytes of a cache row, of the kv-head's place in it
+  int kmin, kmax;      // keys that may be read
+  int bs, sh;          // block size, its logarithm if it is a power of two of at least 16, else -1
+};
+
+// Tile rows [row0, row0 + ROWS) (row0 a multiple of ROWS, at most 32), keys t0 + row, into lds + PITCH row.  SIDE: 0 keys, 1 values.
+template <int D, int ROWS, int SIDE>
+__device__ __forceinline__ void feed_rows(const RangedParams& p, const RFeed& f, int t0, int row0,
+                                          uint32_t lds, int lane) {
+  using G = RGeom<D>;
+  constexpr int NI = ROWS / G::RPI;
+  const char* cache = SIDE ? f.vc : f.kc;
+  auto piece = [&](int row) {
+    int c = (lane % G::CPR) ^ (SIDE ? G::vx(row) : G::kx(row));
+    if (D == 96 && c >= 12) c -= 8;
+    return c;
+  };
+  const int lr = lane / G::CPR;
+  if (f.sh >= 0 && t0 + row0 >= f.kmin && t0 + row0 + ROWS <= f.kmax) {
+    // every 16 rows lie in one page
+    constexpr int GR = ROWS < 16 ? ROWS : 16;
+#pragma unroll
+    for (int gp = 0; gp < ROWS / GR; ++gp) {
+      const int pos = uniform(t0 + row0 + gp * GR);
+      int64_t page = scalar_load(f.bt + min(pos >> f.sh, p.max_blocks - 1));
+      page = min(max(page, (int64_t)0), p.num_blocks - 1);
+      const char* base = cache + ((page << f.sh) + (pos & (f.bs - 1))) * f.rowb + f.hoff;
+#pragma unroll
+      for (int i = 0; i < GR / G::RPI; ++i) {
+        const int rl = gp * GR + i * G::RPI;
+        dma_base(base + i * G::RPI * f.rowb, (uint32_t)(lr * (int)f.rowb + 16 * piece(row0 + rl + lr)),
+                 lds + (row0 + rl) * G::PITCH);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int row = row0 + i * G::RPI + lr;
+      const int pos = min(max(t0 + row, f.kmin), f.kmax - 1);
+      int64_t page = f.bt[min(pos / f.bs, p.max_blocks - 1)];
+      page = min(max(page, (int64_t)0), p.num_blocks - 1);
+      dma_ptr(cache + (page * f.bs + pos % f.bs) * f.rowb + f.hoff + 16 * piece(row),
+              lds + (row0 + i * G::RPI) * G::PITCH);
+    }
+  }
+}
+
+// A wavefront's 32 rows: lane l holds row l % 32, half h = l / 32 of the keys of a tile and of the dims.
+template <typename TT, int D>
+struct RState {
+  u32x4 q[D / 16];
+  f32x16 o[D / 32];
+  float m, l;
+  int lo, hi;  // keys that the row sees in this unit
+  int pos;
+  float slope;  // log2 units
+};
+
+// Scores of 32 KB keys at t0: raw products.
+template <typename TT, int D, int KB>
+__device__ __forceinline__ void r_scores(const RState<TT, D>& st, const char* kt, int lane,
+                                         f32x16 (&s)[KB]) {
+  using G = RGeom<D>;
+  const int c = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+  const char* row = kt + c * G::PITCH;
+  const int x = G::kx(c) ^ h;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) {
+    const char* a = row + (((2 * ks) ^ x) << 4);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+      s[kb] = mfma_r<TT>(*reinterpret_cast<const u32x4*>(a + kb * 32 * G::PITCH), st.q[ks], s[kb]);
+  }
+}
+
+// Bias, mask, the lazy maximum and the probabilities of 32 KB keys at t0, packed per 16 keys.
+template <typename TT, int D, int KB, bool EXTRA>
+__device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& st, f32x16 (&s)[KB],
+                                          int t0, bool masked, int lane, u32x4 (&pr)[2 * KB]) {
+  const int h = lane >> 5;
+  // EXTRA: scores become log2 units here; otherwise the scale enters each exponent's FMA
+  const float sl = EXTRA ? 1.0f : p.scale_log2;
+  if constexpr (EXTRA) {
+    const float ck = p.softcap > 0.0f ? fabsf(p.scale) / p.softcap : 0.0f, cl = p.softcap * kLog2e;
+    const float far = (float)(st.pos - t0 - 4 * h);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float x = p.softcap > 0.0f ? softcap_log2(s[kb][i], ck, cl) : s[kb][i] * p.scale_log2;
+        x -= st.slope * fabsf(far - (float)(32 * kb + 8 * (i >> 2) + (i & 3)));
+        s[kb][i] = x;
+      }
+  }
+  if (masked) {
+    const unsigned span = st.hi > st.lo ? (unsigned)(st.hi - st.lo) : 0u;
+    const unsigned rel = (unsigned)(t0 + 4 * h) - (unsigned)st.lo;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        s[kb][i] = rel + (unsigned)(32 * kb + 8 * (i >> 2) + (i & 3)) < span ? s[kb][i] : kNegInf;
+  }
+  float mx = kNegInf;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+  mx *= sl;
+  mx = fmaxf(mx, half_swap(mx));
+  if (__any(mx > st.m + 8.0f)) {
+    const float mn = fmaxf(st.m, mx);
+    const float a = mn == kNegInf ? 1.0f : exp2f(st.m - mn);
+    st.l *= a;
+    st.m = mn;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) st.o[n] *= a;
+  }
+  const float ms = st.m == kNegInf ? 0.0f : st.m;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    float e[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], sl, -ms));
+      st.l += e[i];
+    }
+    pr[2 * kb] = pack8<TT>(e);
+    pr[2 * kb + 1] = pack8<TT>(e + 8);
+  }
+}
+
+// O^T += V^T P^T over 32 KB keys.
+template <typename TT, int D, int KB>
+__device__ __forceinline__ void r_values(RState<TT, D>& st, const char* vt, int lane,
+                                         const u32x4 (&pr)[2 * KB]) {
+  using G = RGeom<D>;
+  const int h = lane >> 5, dh = (lane >> 4) & 1, i = lane & 15;
+  // rows 4 h + i / 4 (+ 8) of each 16 keys, dims 32 n + 16 dh + 4 (i % 4) .. + 3
+  const char* row = vt + (4 * h + (i >> 2)) * G::PITCH + 8 * (i & 1);
+  const int vx = G::vx(4 * h + (i >> 2)), sub = 2 * dh + ((i & 3) >> 1);
+#pragma unroll
+  for (int n = 0; n < D / 32; ++n) {
+    const char* a = row + ((((4 * n) ^ vx) + sub) << 4);
+#pragma unroll
+    for (int t = 0; t < 2 * KB; ++t) {
+      const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(a + t * 16 * G::PITCH));
+      const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(a + (t * 16 + 8) * G::PITCH));
+      const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
+      st.o[n] = mfma_r<TT>(u32x4{w0[0], w0[1], w1[0], w1[1]}, pr[t], st.o[n]);
+    }
+  }
+}
+
+template <typename TT, int D>
+__device__ __forceinline__ void r_init(const RangedParams& p, const RRow& r, const RPart& q, int lane,
+                                       RState<TT, D>& st) {
+  const char* src = reinterpret_cast<const char*>(p.q) + ((int64_t)r.t * p.num_heads + r.h) * D * 2 +
+                    16 * (lane >> 5);
+  // a negative scale goes into the queries' signs (p.scale_log2 has its magnitude)
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+    st.q[ks] = q.any ? (ld16(src + 32 * ks) ^ p.qxor) : u32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) st.o[n][i] = 0.0f;
+  st.m = kNegInf;
+  st.l = 0.0f;
+  st.lo = q.any ? q.lo : 0;
+  st.hi = q.any ? q.hi : 0;
+  st.pos = r.pos;
+  st.slope = p.slopes ? p.slopes[r.h] * kLog2e : 0.0f;
+}
+
+__device__ __forceinline__ int half_min(int v) {  // over the 32 rows of a wavefront (both halves alike)
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return uniform(v);
+}
+__device__ __forceinline__ int half_max(int v) { return -half_min(-v); }
+
+// ------------------------------------------------------------------------------------ a unit
+// 128 rows: wavefront w takes rows 32 w .. 32 w + 31 of every tile.
+template <typename TT, int D, bool EXTRA>
+__device__ __forceinline__ void wide_unit(const RangedParams& p, const RUnit& u, char* lds, int* red) {
+  using G = RGeom<D>;
+  constexpr int KB = G::KT / 32, SIDE = G::KT * G::PITCH;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int rl = 32 * wave + (lane & 31);
+  const RRow r = r_unit_row(p, u, rl);
+  const RPart q = r_part(u, r);
+  RState<TT, D> st;
+  r_init<TT, D>(p, r, q, lane, st);
+  // keys that some / every row of the wavefront sees, and some row of the workgroup
+  const int wlo = half_min(q.any ? q.lo : INT32_MAX), whi = half_max(q.any ? q.hi : 0);
+  const int flo = half_max(q.any ? q.lo : 0), fhi = half_min(q.any ? q.hi : INT32_MAX);
+  if (lane == 0) {
+    red[2 * wave] = wlo;
+    red[2 * wave + 1] = whi;
+  }
+  __syncthreads();
+  RFeed f;
+  f.kmin = uniform(min(min(red[0], red[2]), min(red[4], red[6])));
+  f.kmax = uniform(max(max(red[1], red[3]), max(red[5], red[7])));
+  f.kc = reinterpret_cast<const char*>(p.key_cache);
+  f.vc = reinterpret_cast<const char*>(p.value_cache);
+  f.bt = p.block_table + (int64_t)u.s.b0 * p.max_blocks;
+  f.rowb = (int64_t)p.kv_heads * D * 2;
+  f.hoff = (int64_t)u.kh * D * 2;
+  f.bs = p.block_size;
+  f.sh = p.bs_shift;
+  if (f.kmin < f.kmax) {
+    const int tb = f.kmin / G::KT, te = (f.kmax + G::KT - 1) / G::KT;
+    const uint32_t base = lds_address(lds);
+    auto issue = [&](int t) __attribute__((always_inline)) {
+      const uint32_t buf = base + ((t - tb) & 1) * 2 * SIDE;
+      feed_rows<D, G::KT / 4, 0>(p, f, t * G::KT, wave * (G::KT / 4), buf, lane);
+      feed_rows<D, G::KT / 4, 1>(p, f, t * G::KT, wave * (G::KT / 4), buf + SIDE, lane);
+    };
+    issue(tb);
+    for (int t = tb; t < te; ++t) {
+      wait_loads<0>();
+      __syncthreads();
+      if (t + 1 < te) issue(t + 1);
+      const int t0 = t * G::KT;
+      if (t0 >= whi || t0 + G::KT <= wlo) continue;
+      const char* buf = lds + ((t - tb) & 1) * 2 * SIDE;
+      f32x16 s[KB];
+      u32x4 pr[2 * KB];
+      r_scores<TT, D, KB>(st, buf, lane, s);
+      r_softmax<TT, D, KB, EXTRA>(p, st, s, t0, t0 < flo || t0 + G::KT > fhi, lane, pr);
+      r_values<TT, D, KB>(st, buf + SIDE, lane, pr);
+    }
+  }
+  const float l = st.l + half_swap(st.l);
+  const int h = lane >> 5;
+  float sum = 0.0f;  // NaN if an output is not finite
+#pragma unroll
+  for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(st.o[n][i], 0.0f, sum);
+  const bool odd = q.any && !(sum == 0.0f && l < __builtin_huge_valf());
+  const uint64_t odds = __ballot(odd);
+  uint32_t again = (uint32_t)(odds | (odds >> 32));
+  const bool skip = (again >> (lane & 31)) & 1;
+  if (q.zero || (q.any && q.single && !skip)) {
+    const float fct = q.zero ? 0.0f : finalize_factor(st.m, l, r_sink<TT>(p, r.h));
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((int64_t)r.t * p.num_heads + r.h) * D + 4 * h;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        u32x2 w;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          w[k] = (uint32_t)TT::from_f32(st.o[n][4 * i + 2 * k] * fct) |
+                 ((uint32_t)TT::from_f32(st.o[n][4 * i + 2 * k + 1] * fct) << 16);
+        *reinterpret_cast<u32x2*>(dst + 32 * n + 8 * i) = w;
+      }
+  } else if (q.any && !q.single && !skip) {
+    const int64_t slot = u.worker + u.item;
+    if (slot < p.part_slots) {
+      const int64_t row = slot * p.slot_rows + rl;
+#pragma unroll
+      for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f32x4*>(p.part_o + row * D + 32 * n + 8 * i + 4 * h) =
+              f32x4{st.o[n][4 * i], st.o[n][4 * i + 1], st.o[n][4 * i + 2], st.o[n][4 * i + 3]};
+      if (h == 0) p.part_ml[row] = float2{st.m, l};
+    }
+  }
+  for (; again; again &= again - 1) slow_row<TT, D>(p, u, 32 * wave + __builtin_ctz(again));
+  __syncthreads();  // the next unit reuses the buffers
+}
+
+// At most 32 rows: wavefront w takes 32-key tiles w, w + 4, ...
+template <typename TT, int D, bool EXTRA>
+__device__ __forceinline__ void narrow_unit(const RangedParams& p, const RUnit& u, char* lds, int* red) {
+  using G = RGeom<D>;
+  constexpr int SIDE = 32 * G::PITCH, NI = 32 / G::RPI;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int rl = lane & 31;
+  const RRow r = r_unit_row(p, u, rl);
+  const RPart q = r_part(u, r);
+  RState<TT, D> st;
+  r_init<TT, D>(p, r, q, lane, st);
+  RFeed f;
+  f.kmin = half_min(q.any ? q.lo : INT32_MAX);
+  f.kmax = half_max(q.any ? q.hi : 0);
+  const int flo = half_max(q.any ? q.lo : 0), fhi = half_min(q.any ? q.hi : INT32_MAX);
+  f.kc = reinterpret_cast<const char*>(p.key_cache);
+  f.vc = reinterpret_cast<const char*>(p.value_cache);
+  f.bt = p.block_table + (int64_t)u.s.b0 * p.max_blocks;
+  f.rowb = (int64_t)p.kv_heads * D * 2;
+  f.hoff = (int64_t)u.kh * D * 2;
+  f.bs = p.block_size;
+  f.sh = p.bs_shift;
+  char* mine = lds + wave * 2 * SIDE;
+  if (f.kmin < f.kmax) {
+    const int te = (f.kmax + 31) / 32;
+    const uint32_t base = lds_address(mine);
+    int t = f.kmin / 32 + wave;
+    if (t < te) {
+      feed_rows<D, 32, 0>(p, f, t * 32, 0, base, lane);
+      feed_rows<D, 32, 1>(p, f, t * 32, 0, base + SIDE, lane);
+    }
+    for (; t < te; t += 4) {
+      const int t0 = t * 32;
+      const bool more = t + 4 < te;
+      f32x16 s[1];
+      u32x4 pr[2];
+      wait_loads<NI>();  // the keys; the values are younger
+      r_scores<TT, D, 1>(st, mine, lane, s);
+      if (more) {
+        wait_lds_reads();
+        feed_rows<D, 32, 0>(p, f, t0 + 128, 0, base, lane);
+      }
+      r_softmax<TT, D, 1, EXTRA>(p, st, s, t0, t0 < flo || t0 + 32 > fhi, lane, pr);
+      if (more)
+        wait_loads<NI>();
+      else
+        wait_loads<0>();
+      r_values<TT, D, 1>(st, mine + SIDE, lane, pr);
+      if (more) {
+        wait_lds_reads();
+        feed_rows<D, 32, 1>(p, f, t0 + 128, 0, base + SIDE, lane);
+      }
+    }
+  }
+  // The four wavefronts' rows meet in LDS: O of wavefront w in its own tile's place, 16-byte pieces
+  // exchanged by the row.
+  constexpr int PC = D / 4;                      // pieces of a row
+  constexpr int PX = D == 96 ? 7 : PC - 1 < 31 ? PC - 1 : 31;
+  float* ml = reinterpret_cast<float*>(red);     // [wave][row][2]
+  const float l = st.l + half_swap(st.l);
+  {
+    const int h = lane >> 5;
+    f32x4* po = reinterpret_cast<f32x4*>(mine) + rl * PC;
+    wait_lds_reads();
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        po[(8 * n + 2 * i + h) ^ (rl & PX)] =
+            f32x4{st.o[n][4 * i], st.o[n][4 * i + 1], st.o[n][4 * i + 2], st.o[n][4 * i + 3]};
+    if (h == 0) {
+      ml[(wave * 32 + rl) * 2] = st.m;
+      ml[(wave * 32 + rl) * 2 + 1] = l;
+    }
+  }
+  __syncthreads();
+  // Eight threads per row; wavefront w holds rows 8 w .. 8 w + 7.
+  const int row = threadIdx.x >> 3, part = threadIdx.x & 7;
+  if (u.row0 + row < u.s.rows) {
+    const RRow rr = r_unit_row(p, u, row);
+    const RPart qq = r_part(u, rr);
+    float w[4], M = kNegInf, L = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) M = fmaxf(M, ml[(k * 32 + row) * 2]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float mk = ml[(k * 32 + row) * 2];
+      w[k] = mk == kNegInf ? 0.0f : exp2f(mk - M);
+      // (a wavefront whose scores were all NaN has no maximum, but a sum)
+      const float lk = ml[(k * 32 + row) * 2 + 1];
+      L += lk == lk ? lk * w[k] : lk;
+    }
+    f32x4 acc[PC / 8];
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < PC / 8; ++n) {
+      acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        acc[n] += reinterpret_cast<const f32x4*>(lds + k * 2 * SIDE)[row * PC + ((8 * n + part) ^ (row & PX))] * w[k];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(acc[n][e], 0.0f, sum);
+    }
+    bool odd = qq.any && !(sum == 0.0f && L < __builtin_huge_valf());
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) odd = __shfl_xor((int)odd, o, 64) || odd;
+    if (qq.zero || (qq.any && qq.single && !odd)) {
+      const float fct = qq.zero ? 0.0f : finalize_factor(M, L, r_sink<TT>(p, rr.h));
+      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((int64_t)rr.t * p.num_heads + rr.h) * D;
+#pragma unroll
+      for (int n = 0; n < PC / 8; ++n) {
+        u32x2 x;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          x[k] = (uint32_t)TT::from_f32(acc[n][2 * k] * fct) |
+                 ((uint32_t)TT::from_f32(acc[n][2 * k + 1] * fct) << 16);
+        *reinterpret_cast<u32x2*>(dst + 4 * (8 * n + part)) = x;
+      }
+    } else if (qq.any && !qq.single && !odd) {
+      const int64_t slot = u.worker + u.item;
+      if (slot < p.part_slots) {
+        const int64_t at = slot * p.slot_rows + row;
+#pragma unroll
+        for (int n = 0; n < PC / 8; ++n)
+          *reinterpret_cast<f32x4*>(p.part_o + at * D + 4 * (8 * n + part)) = acc[n];
+        if (part == 0) p.part_ml[at] = float2{M, L};
+      }
+    }
+    red[256 + row] = odd ? 1 : 0;
+  } else {
+    red[256 + row] = 0;
+  }
+  __syncthreads();
+  for (int k = wave; k < 32; k += 4)
+    if (uniform(red[256 + k])) slow_row<TT, D>(p, u, k);
+  __syncthreads();  // the next unit reuses the buffers
+}
+
+// Workgroups per CU: two by LDS (head 64: up to four) and registers, one at head 256.
+template <typename TT, int D, bool EXTRA>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2))) void
+ranged_kernel(const RangedParams p) {
+  __shared__ __attribute__((aligned(1024))) char lds[RGeom<D>::LDS];
+  __shared__ RScan sh;
+  __shared__ int red[256 + 32];
+  const RPlan plan = r_plan(p, sh);
+  const int64_t me = blockIdx.x;
+  if (me >= (plan.per > 0 ? p.slots : plan.items)) return;
+  // my stretch: tiles [me per, me per + per) of the flat list, or item number me
+  const int64_t a = me * plan.per, z = min(a + plan.per, plan.tiles);
+  if (plan.per > 0 && a >= plan.tiles) return;
+  const int n = p.groups + p.batch;
+  int64_t t0 = 0, at = a;
+  int i0 = 0;
+  if (me == 0) {  // the sources' places, for the merge
+    for (int base = 0; base < n; base += kRChunk) {
+      if (n > kRChunk) scan_chunk(p, base, sh, t0, i0);
+      const RSource s = sh.src[threadIdx.x];
+      if (base + (int)threadIdx.x < n)
+        p.table[1 + base + threadIdx.x] = RTable{s.first, s.item, s.tiles, s.tok0, s.rows, s.ka, 0};
+    }
+    if (threadIdx.x == 0) p.table[0] = RTable{plan.tiles, plan.items, plan.per, 0, 0, 0, 0};
+    t0 = 0;
+    i0 = 0;
+  }
+  for (int base = 0; base < n; base += kRChunk) {
+    const int64_t tb = t0;
+    const int ib = i0;
+    if (n > kRChunk)
+      scan_chunk(p, base, sh, t0, i0);
+    else {
+      t0 = plan.tiles;
+      i0 = plan.items;
+    }
+    for (;;) {
+      if (plan.per > 0 ? at >= min(z, t0) : (me < ib || me >= i0)) break;
+      if (plan.per > 0 && at < tb) break;
+      // the last source that begins at or before the place (sources without tiles begin where the next does)
+      int lo = 0, hi = min(kRChunk, n - base);
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        const bool before = plan.per > 0 ? sh.src[mid].first <= at : sh.src[mid].item <= (int)me;
+        if (before) lo = mid; else hi = mid;
+      }
+      RUnit u;
+      const RSource sl = sh.src[lo];
+      u.s = RSource{uniform64(sl.first), uniform(sl.item), uniform(sl.tok0), uniform(sl.rows), uniform(sl.b0),
+                    uniform(sl.b1), uniform(sl.ka), uniform(sl.kb), uniform(sl.tiles)};
+      u.group = base + lo < p.groups;
+      u.per = plan.per;
+      u.worker = me;
+      const int blocks = r_blocks(u.s.rows);
+      const int local = plan.per > 0 ? (int)((at - u.s.first) / u.s.tiles) : (int)me - u.s.item;
+      u.item = u.s.item + local;
+      u.at = u.s.first + (int64_t)local * u.s.tiles;
+      // the last rows, which see most keys, first
+      u.kh = local % p.kv_heads;
+      const int blk = blocks - 1 - local / p.kv_heads;
+      u.row0 = blk * kRWide;
+      u.x0 = plan.per > 0 ? (int)(at - u.at) : 0;
+      u.x1 = plan.per > 0 ? (int)min((int64_t)u.s.tiles, z - u.at) : u.s.tiles;
+      if (u.s.rows > kRNarrow)
+        wide_unit<TT, D, EXTRA>(p, u, lds, red);
+      else
+        narrow_unit<TT, D, EXTRA>(p, u, lds, red);
+      if (plan.per == 0) return;
+      at = u.at + u.x1;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------ the merge
+// Rows whose keys several workgroups took: their (m, l, O) joined.  A workgroup takes RM consecutive rows
+// (token, head of the group) of a kv-head; thread k < RM finds the pieces of row k -- the workgroups from
+// the one that holds the row's first key to the one that holds its last, for the shared keys and for its
+// own -- and groups of lanes, each lane 16 bytes of the row, sum them, several pieces in flight.
+struct RJoin {
+  int t, h, na, nb;          // pieces of the shared and of its own keys (na + nb < 2: nothing to join)
+  int64_t ra, rb;            // the first pieces' partial rows
+};
+constexpr int kRDepth = 4;
+template <typename TT, int D, int RM>
+__global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p) {
+  constexpr int LP = D == 96 ? 32 : D / 4, NG = 256 / LP;
+  constexpr int GPR = NG / (RM < NG ? RM : NG);  // groups of lanes per row
+  __shared__ RJoin join[RM];
+  __shared__ f32x4 sh_o[GPR > 1 ? NG : 1][LP];
+  __shared__ float2 sh_ml[GPR > 1 ? NG : 1];
+  const int per = p.table[0].tiles;
+  if (per == 0 && p.groups == 0) return;
+  const int tid = threadIdx.x, g = p.num_heads / p.kv_heads;
+  const int kh = blockIdx.x % p.kv_heads;
+  if (tid < RM) {
+    const int64_t gr = (int64_t)(blockIdx.x / p.kv_heads) * RM + tid;
+    const int t = (int)min(gr / g, (int64_t)p.num_tokens);
+    RJoin j{t, kh * g + (int)(gr % g), 0, 0, 0, 0};
+    if (t < p.num_tokens && t >= p.cum[0] && t < p.cum[p.batch]) {
+      RSource all{};
+      all.b1 = p.batch;
+      const int b = r_token_seq(p, all, t);
+      const RRow r = r_row(p, t, j.h, b, true);
+      auto pieces = [&](int i, int a, int z, int64_t& row) {
+        const RTable e = p.table[1 + i];
+        const int rr = (t - e.tok0) * g + j.h - kh * g, blocks = r_blocks(e.rows);
+        const int blk = e.rows > kRNarrow ? rr / kRWide : 0;
+        const int local = (blocks - 1 - blk) * p.kv_heads + kh, kt = e.ka / kRTile;
+        const int64_t at = e.first + (int64_t)local * e.tiles;
+        const int64_t w0 = r_worker(per, at, e.item + local, a / kRTile - kt);
+        row = (w0 + e.item + local) * p.slot_rows + rr - blk * kRWide;
+        return (int)(r_worker(per, at, e.item + local, (z - 1) / kRTile - kt) - w0) + 1;
+      };
+      const int sh_hi = min(r.hi, r.shared), own_lo = max(r.lo, r.shared);
+      if (r.lo < sh_hi) j.na = pieces(group_of(p, b), r.lo, sh_hi, j.ra);
+      if (own_lo < r.hi) j.nb = pieces(p.groups + b, own_lo, r.hi, j.rb);
+      const int64_t end = (int64_t)p.part_slots * p.slot_rows;
+      if (j.ra + (int64_t)(max(j.na, 1) - 1) * p.slot_rows >= end ||
+          j.rb + (int64_t)(max(j.nb, 1) - 1) * p.slot_rows >= end)
+        j.na = j.nb = 0;  // (metadata beyond its bounds)
+    }
+    join[tid] = j;
+  }
+  __syncthreads();
+  const int grp = tid / LP, d0 = 4 * min(tid % LP, D / 4 - 1);
+  for (int k = grp / GPR; k < RM; k += NG / GPR) {
+    const RJoin j = join[k];
+    const int n = j.na + j.nb;
+    if (n < 2) continue;  // (with several groups per row: RM == 1, and every thread goes)
+    float M = kNegInf, L = 0.0f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = grp % GPR; i0 < n; i0 += GPR * kRDepth) {
+      float2 ml[kRDepth];
+      f32x4 o[kRDepth];
+#pragma unroll
+      for (int i = 0; i < kRDepth; ++i) {
+        const int x = min(i0 + i * GPR, n - 1);
+        const int64_t row = x < j.na ? j.ra + (int64_t)x * p.slot_rows : j.rb + (int64_t)(x - j.na) * p.slot_rows;
+        ml[i] = p.part_ml[row];
+        o[i] = *reinterpret_cast<const f32x4*>(p.part_o + row * D + d0);
+      }
+      float mn = M;
+#pragma unroll
+      for (int i = 0; i < kRDepth; ++i)
+        if (i0 + i * GPR < n) mn = fmaxf(mn, ml[i].x);
+      const float a = M == kNegInf ? 0.0f : exp2f(M - mn);
+      L = L == L ? L * a : L;
+      acc *= a;
+#pragma unroll
+      for (int i = 0; i < kRDepth; ++i)
+        if (i0 + i * GPR < n) {
+          const float w = ml[i].x == kNegInf ? 0.0f : exp2f(ml[i].x - mn);
+          L += ml[i].y == ml[i].y ? ml[i].y * w : ml[i].y;
+          acc += o[i] * w;
+        }
+      M = mn;
+    }
+    if constexpr (GPR > 1) {
+      static_assert(RM == 1, "one row per workgroup");
+      sh_o[grp][tid % LP] = acc;
+      if (tid % LP == 0) sh_ml[grp] = float2{M, L};
+      __syncthreads();
+      if (grp > 0) return;
+#pragma unroll
+      for (int w = 1; w < NG; ++w) {
+        const float2 ml = sh_ml[w];
+        const float mn = fmaxf(M, ml.x);
+        const float wa = M == kNegInf ? 0.0f : exp2f(M - mn), wb = ml.x == kNegInf ? 0.0f : exp2f(ml.x - mn);
+        L = (L == L ? L * wa : L) + (ml.y == ml.y ? ml.y * wb : ml.y);
+        acc = acc * wa + sh_o[w][tid % LP] * wb;
+        M = mn;
+      }
+    }
+    if (tid % LP >= D / 4) continue;
+    const float f = L == L ? finalize_factor(M, L, r_sink<TT>(p, j.h)) : L;
+    u32x2 w;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+      w[m] = (uint32_t)TT::from_f32(acc[2 * m] * f) | ((uint32_t)TT::from_f32(acc[2 * m + 1] * f) << 16);
+    *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + ((int64_t)j.t * p.num_heads + j.h) * D + d0) = w;
+  }
+}
+
+template <typename TT, int D>
+hipError_t launch_d(const RangedParams& p, hipStream_t s) {
+  const dim3 grid(p.grid), block(256);
+  if (p.softcap > 0.0f || p.slopes)
+    hipLaunchKernelGGL((ranged_kernel<TT, D, true>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((ranged_kernel<TT, D, false>), grid, block, 0, s, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !p.merge) return e;
+  const int64_t rows = (int64_t)p.num_tokens * (p.num_heads / p.kv_heads);
+  if (rows * p.kv_heads <= kRMergeRows)
+    hipLaunchKernelGGL((ranged_merge_kernel<TT, D, 1>), dim3((unsigned)(rows * p.kv_heads)), block, 0, s, p);
+  else
+    hipLaunchKernelGGL((ranged_merge_kernel<TT, D, 32>), dim3((unsigned)((rows + 31) / 32 * p.kv_heads)), block, 0, s, p);
+  return hipGetLastError();
+}
+
+template <typename TT>
+hipError_t launch_t(const RangedParams& p, hipStream_t s) {
+  switch (p.head_dim) {
+    case 64: return launch_d<TT, 64>(p, s);
+    case 96: return launch_d<TT, 96>(p, s);
+    case 128: return launch_d<TT, 128>(p, s);
+    case 256: return launch_d<TT, 256>(p, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace
+
+bool ranged_supported(int head_dim, pa_dtype act, pa_dtype cache_dtype) {
+  return (act == PA_DTYPE_FLOAT16 || act == PA_DTYPE_BFLOAT16) && cache_dtype == act &&
+         (head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 256);
+}
+
+hipError_t launch_ranged(const RangedParams& p, pa_dtype act, hipStream_t s) {
+  if (p.num_tokens <= 0 || p.batch <= 0) return hipSuccess;
+  if (p.grid <= 0 || p.slots <= 0 || !p.table) return hipErrorInvalidValue;
+  return act == PA_DTYPE_FLOAT16 ? launch_t<TF16>(p, s) : launch_t<TBF16>(p, s);
+}
+
+}  // namespace pa
