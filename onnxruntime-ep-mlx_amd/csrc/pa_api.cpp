@@ -1293,7 +1293,7 @@ RangedPlan ranged_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a,
   // blocks of at most 128 rows of every sequence, and of every group's rows
   const int64_t blocks = T * g / 128 + b->batch + (groups ? T * g / 128 + groups : 0);
   const int64_t items = blocks * c->kv_heads;
-  if (items >= ((int64_t)1 << 24) || T * g > INT32_MAX) return r;
+  if (items >= ((int64_t)1 << 23) || T * g > INT32_MAX) return r;
   const int mq = b->max_query_len > 0 ? b->max_query_len : b->num_tokens;
   r.on = true;
   r.slots = (c->head_dim > 128 ? 1 : 2) * device_cus();
@@ -1383,6 +1383,7 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
   p.slot_rows = r.slot_rows;
   p.grid = r.grid;
   p.merge = r.merge ? 1 : 0;
+  p.wide = r.slot_rows > 32 ? 1 : 0;
   const hipError_t e = pa::launch_ranged(p, act, s);
   if (e != hipSuccess) return hip_fail(e, "masked attention launch");
   return PA_OK;

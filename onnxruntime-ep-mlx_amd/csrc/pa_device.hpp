@@ -415,7 +415,7 @@ struct AttnParams {
 // workgroup; then groups and sequences).
 struct RTable {
   int64_t first;
-  int32_t item, tiles, tok0, rows, ka, pad;
+  int32_t item, tiles, tok0, rows, ka, kb, shared, group;
 };
 struct RangedParams {
   const void* q;
@@ -449,6 +449,7 @@ struct RangedParams {
   int32_t slot_rows;  // rows of a partial slot: 32 where every block is known to be that small, else 128
   int32_t grid;       // workgroups
   int32_t merge;      // some row may have several pieces
+  int32_t wide;       // some block may hold more than 32 rows
 };
 hipError_t launch_ranged(const RangedParams& p, pa_dtype act, hipStream_t s);
 bool ranged_supported(int head_dim, pa_dtype act, pa_dtype cache_dtype);

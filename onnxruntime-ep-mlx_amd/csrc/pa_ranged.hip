@@ -80,11 +80,18 @@ __device__ __forceinline__ u32x4 pack8(const float* x) {
 // memory counters do not see them and nothing waits for them but the tile loops (wait_loads).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+template <bool NT>
 __device__ __forceinline__ void dma_base(const char* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-               :
-               : "v"(off), "s"(base), "s"(lds)
-               : "memory", "m0");
+  if constexpr (NT)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+                 :
+                 : "v"(off), "s"(base), "s"(lds)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(off), "s"(base), "s"(lds)
+                 : "memory", "m0");
 }
 __device__ __forceinline__ void dma_ptr(const char* ptr, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
@@ -137,22 +144,20 @@ __device__ __forceinline__ RGroup r_group(const RangedParams& p, int gi) {
   q.prefix = q.b1 - q.b0 < 2 ? 0 : min(max(p.shared_lens[gi], 0), r_seq(p, q.b0).total);
   return q;
 }
-// Group of sequence b, -1 if none.
+// Group of sequence b, -1 if none: the last one that begins at or before b.
 __device__ __forceinline__ int group_of(const RangedParams& p, int b) {
-  int lo = 0, hi = p.groups;  // the last group that begins at or before b
-  while (lo < hi) {
+  int lo = 0, hi = p.groups;
+  while (hi - lo > 4) {
     const int mid = (lo + hi) >> 1;
-    if (p.group_cum[mid] <= b) lo = mid + 1; else hi = mid;
+    if (p.group_cum[mid] <= b) lo = mid; else hi = mid;
   }
-  return lo > 0 && b < p.group_cum[lo] ? lo - 1 : -1;
-}
-// Shared keys in front of sequence b's own.
-__device__ __forceinline__ int shared_of(const RangedParams& p, int b, int total) {
-  if (p.groups == 0) return 0;
-  const int gi = group_of(p, b);
-  return gi < 0 ? 0 : min(r_group(p, gi).prefix, total);
+  int n = lo;  // (a few loads at once end the search in one round trip)
+#pragma unroll
+  for (int k = 0; k < 4; ++k) n += lo + k < hi && p.group_cum[lo + k] <= b ? 1 : 0;
+  return n > 0 && b < p.group_cum[n] ? n - 1 : -1;
 }
 
+// A group's rows against the keys it shares, or a sequence's against its own.
 struct RSource {
   int64_t first;  // its first tile in the flat list
   int item;       // its first item
@@ -160,6 +165,7 @@ struct RSource {
   int b0, b1;     // its sequences; b0's table names the pages
   int ka, kb;     // its keys
   int tiles;      // tiles of one item
+  int shared, group;  // keys that the sequence shares, and its group
 };
 __device__ __forceinline__ int r_blocks(int rows) {
   return rows <= kRNarrow ? (rows > 0) : (rows + kRWide - 1) / kRWide;
@@ -169,40 +175,44 @@ __device__ __forceinline__ RSource r_source(const RangedParams& p, int i) {
   RSource s{};
   const int g = p.num_heads / p.kv_heads;
   if (i >= p.groups + p.batch) return s;
-  if (i < p.groups) {
-    const RGroup q = r_group(p, i);
+  const bool seq = i >= p.groups;
+  const int b = i - p.groups, gi = seq ? (p.groups ? group_of(p, b) : -1) : i;
+  const RGroup q = gi >= 0 ? r_group(p, gi) : RGroup{0, 0, 0};
+  if (!seq) {
     if (q.prefix == 0) return s;
     s.b0 = q.b0;
     s.b1 = q.b1;
     s.tok0 = r_seq(p, q.b0).s0;
     const RSeq last = r_seq(p, q.b1 - 1);
     s.rows = max(last.s0 + last.nq - s.tok0, 0) * g;
-    s.kb = q.prefix;
+    s.kb = s.shared = q.prefix;
   } else {
-    const int b = i - p.groups;
-    const RSeq q = r_seq(p, b);
+    const RSeq e = r_seq(p, b);
     s.b0 = b;
     s.b1 = b + 1;
-    s.tok0 = q.s0;
-    s.rows = q.nq * g;
-    s.ka = shared_of(p, b, q.total);
-    if (p.window > 0) s.ka = max(s.ka, min(q.past - p.window + 1, q.total));
-    s.kb = q.total;
+    s.tok0 = e.s0;
+    s.rows = e.nq * g;
+    s.shared = s.ka = min(q.prefix, e.total);
+    if (p.window > 0) s.ka = max(s.ka, min(e.past - p.window + 1, e.total));
+    s.kb = e.total;
   }
+  s.group = gi;
   // (a sequence without keys of its own keeps a tile, whose workgroup writes its empty rows)
   s.tiles = s.rows > 0 ? max((s.kb + kRTile - 1) / kRTile - s.ka / kRTile, 1) : 0;
   return s;
 }
 
-// The scan's outcome: tiles and items of all sources and tiles per workgroup (0: an item each).
-struct RPlan {
-  int64_t tiles;
-  int items, per;
+// Rows of a unit, for the parts of the kernel that hold another row than their lane's.
+struct RInfo {
+  int t, h, pos, lo, hi, how;  // how: kRAny | kRSingle | kRZero | kROdd
 };
+constexpr int kRAny = 1, kRSingle = 2, kRZero = 4, kROdd = 8;
+
 struct RScan {
   RSource src[kRChunk];
+  RInfo row[kRWide];  // (a narrow unit keeps its wavefronts' (m, l) behind its 32 rows)
   int64_t wt[4];
-  int wi[4];
+  int red[8];
 };
 __device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
 #pragma unroll
@@ -219,7 +229,7 @@ __device__ __forceinline__ void scan_chunk(const RangedParams& p, int base, RSca
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   RSource s = r_source(p, base + tid);
   const int items = r_blocks(s.rows) * p.kv_heads;
-  // items above, tiles below: a batch holds fewer than 2^24 items and 2^40 tiles (host)
+  // items above, tiles below: a batch holds fewer than 2^23 items and 2^40 tiles (host)
   const int64_t mine = ((int64_t)items << 40) + (int64_t)items * s.tiles;
   const int64_t incl = scan64(mine, lane);
   __syncthreads();  // the last chunk's readers are done
@@ -240,39 +250,21 @@ __device__ __forceinline__ void scan_chunk(const RangedParams& p, int base, RSca
   i0 += (int)(all >> 40);
   __syncthreads();
 }
-__device__ __forceinline__ RPlan r_plan(const RangedParams& p, RScan& sh) {
-  RPlan r{0, 0, 0};
-  for (int base = 0; base < p.groups + p.batch; base += kRChunk)
-    scan_chunk(p, base, sh, r.tiles, r.items);
-  if (r.items < 2 * p.slots)
-    r.per = (int)max((r.tiles + p.slots - 1) / p.slots, (int64_t)p.least);
-  return r;
-}
 // Workgroup that takes tile x of an item (its first tile at `at`, its number `item`).
 __device__ __forceinline__ int64_t r_worker(int per, int64_t at, int item, int x) {
   return per > 0 ? (at + x) / per : item;
 }
 
-// One row: its token, head, position and range.
-struct RRow {
-  int t, h, pos, lo, hi, shared;
-  bool valid;
+// The range [lo, hi) of token t at position pos of sequence b (total keys).
+struct RRange {
+  int lo, hi;
 };
-__device__ __forceinline__ RRow r_row(const RangedParams& p, int t, int h, int b, bool valid) {
-  RRow r;
-  const RSeq q = r_seq(p, b);
-  r.t = t;
-  r.h = h;
-  r.pos = q.past + (t - q.s0);
-  r.valid = valid;
-  r.shared = shared_of(p, b, q.total);
-  int hi = p.causal ? r.pos + 1 : q.total;
+__device__ __forceinline__ RRange r_range(const RangedParams& p, int t, int pos, int b, int total) {
+  int hi = p.causal ? pos + 1 : total;
   if (p.causal && p.prefix_lens) hi = max(hi, p.prefix_lens[b]);
-  r.hi = valid ? min(hi, q.total) : 0;
-  int lo = p.window > 0 ? r.pos - p.window + 1 : 0;
+  int lo = p.window > 0 ? pos - p.window + 1 : 0;
   if (p.doc_starts) lo = max(lo, p.doc_starts[t]);
-  r.lo = valid ? max(lo, 0) : 0;
-  return r;
+  return RRange{max(lo, 0), min(hi, total)};
 }
 
 // A workgroup's part of an item.
@@ -285,39 +277,45 @@ struct RUnit {
   int x0, x1;      // tiles of the item
   int64_t worker;
 };
-// What a row needs of a unit: keys [lo, hi) of the unit that it sees, whether all that it sees lies in this
-// unit, whether this unit zeroes it (it sees nothing at all).
-struct RPart {
-  int lo, hi;
-  bool any, single, zero;
-};
-__device__ __forceinline__ RPart r_part(const RUnit& u, const RRow& r) {
-  RPart q;
-  const int sa = u.group ? 0 : r.shared, sb = u.group ? min(r.shared, u.s.kb) : u.s.kb;
-  const int a = max(r.lo, sa), z = min(r.hi, sb), kt = u.s.ka / kRTile;
-  q.lo = max(a, (kt + u.x0) * kRTile);
-  q.hi = min(z, (kt + u.x1) * kRTile);
-  q.any = r.valid && q.lo < q.hi;
-  const bool other = u.group ? r.hi > max(r.lo, r.shared) : r.lo < min(r.hi, r.shared);
-  q.single = q.any && !other &&
-             r_worker(u.per, u.at, u.item, a / kRTile - kt) ==
-                 r_worker(u.per, u.at, u.item, (z - 1) / kRTile - kt);
-  q.zero = r.valid && !u.group && r.lo >= r.hi && u.x0 == 0;
-  return q;
-}
-__device__ __forceinline__ int r_token_seq(const RangedParams& p, const RSource& s, int t) {
-  int lo = s.b0, hi = s.b1;  // the last sequence that begins at or before t
-  while (hi - lo > 1) {
+__device__ __forceinline__ int r_token_seq(const RangedParams& p, int lo, int hi, int t) {
+  while (hi - lo > 1) {  // the last of sequences lo .. hi - 1 that begins at or before t
     const int mid = (lo + hi) >> 1;
     if (p.cum[mid] <= t) lo = mid; else hi = mid;
   }
   return lo;
 }
-__device__ __forceinline__ RRow r_unit_row(const RangedParams& p, const RUnit& u, int rl) {
+// Row rl of a unit's block: the keys of the unit that it sees, whether all that it sees lies in this unit
+// (kRSingle), whether the unit zeroes it because it sees nothing at all (kRZero).
+__device__ __forceinline__ RInfo r_info(const RangedParams& p, const RUnit& u, int rl) {
   const int g = p.num_heads / p.kv_heads, r = u.row0 + rl;
   const bool valid = r < u.s.rows;
-  const int t = u.s.tok0 + (valid ? r / g : 0), h = u.kh * g + (valid ? r % g : 0);
-  return r_row(p, t, h, u.group ? r_token_seq(p, u.s, t) : u.s.b0, valid);
+  RInfo q;
+  q.t = u.s.tok0 + (valid ? r / g : 0);
+  q.h = u.kh * g + (valid ? r % g : 0);
+  int b = u.s.b0, total = u.s.kb, shared = u.s.shared;
+  if (u.group) {
+    b = r_token_seq(p, u.s.b0, u.s.b1, q.t);
+    const RSeq e = r_seq(p, b);
+    q.pos = e.past + (q.t - e.s0);
+    total = e.total;
+    shared = min(shared, total);
+  } else {
+    q.pos = total - u.s.rows / g + (q.t - u.s.tok0);
+  }
+  const RRange x = r_range(p, q.t, q.pos, b, total);
+  const int a = max(x.lo, u.group ? 0 : shared), z = min(x.hi, u.group ? shared : total);
+  const int kt = u.s.ka / kRTile;
+  q.lo = max(a, (kt + u.x0) * kRTile);
+  q.hi = min(z, (kt + u.x1) * kRTile);
+  q.how = 0;
+  if (valid && q.lo < q.hi) {
+    const bool other = u.group ? x.hi > max(x.lo, shared) : x.lo < min(x.hi, shared);
+    // (the unit's tiles end where a workgroup's do)
+    const bool here = a >= (kt + u.x0) * kRTile && z <= (kt + u.x1) * kRTile;
+    q.how = kRAny | (here && !other ? kRSingle : 0);
+  }
+  if (valid && !u.group && x.lo >= x.hi && u.x0 == 0) q.how |= kRZero;
+  return q;
 }
 
 template <typename TT>
@@ -336,21 +334,20 @@ __device__ __forceinline__ int64_t r_offset(const RangedParams& p, int b, int kh
 
 // One row of a unit one key at a time, by one wavefront, written like the others'.
 template <typename TT, int D>
-__device__ __forceinline__ void slow_row(const RangedParams& p, const RUnit& u, int rl) {
+__device__ __forceinline__ void slow_row(const RangedParams& p, const RUnit& u, const RInfo& q, int rl) {
   constexpr int NE = (D + 63) / 64;
   const int lane = threadIdx.x & 63;
-  const RRow r = r_unit_row(p, u, rl);
-  const RPart q = r_part(u, r);
   using raw = typename TT::raw;
   float qv[NE], o[NE], m = kNegInf, l = 0.0f;
-  const float slope = p.slopes ? p.slopes[r.h] : 0.0f;
+  const float slope = p.slopes ? p.slopes[q.h] : 0.0f;
 #pragma unroll
   for (int k = 0; k < NE; ++k) {
     const int e = lane + 64 * k;
-    qv[k] = e < D ? TT::to_f32(reinterpret_cast<const raw*>(p.q)[((int64_t)r.t * p.num_heads + r.h) * D + e])
+    qv[k] = e < D ? TT::to_f32(reinterpret_cast<const raw*>(p.q)[((int64_t)q.t * p.num_heads + q.h) * D + e])
                   : 0.0f;
     o[k] = 0.0f;
   }
+#pragma unroll 1
   for (int j = q.lo; j < q.hi; ++j) {
     const int64_t at = r_offset(p, u.s.b0, u.kh, j, D);
     float part = 0.0f, v[NE];
@@ -362,7 +359,7 @@ __device__ __forceinline__ void slow_row(const RangedParams& p, const RUnit& u, 
     }
     float x = wave_sum(part) * p.scale;
     if (p.softcap > 0.0f) x = p.softcap * tanhf(x / p.softcap);
-    x = (x - slope * fabsf((float)(r.pos - j))) * kLog2e;
+    x = (x - slope * fabsf((float)(q.pos - j))) * kLog2e;
     const float mn = fmaxf(m, x), ms = mn == kNegInf ? 0.0f : mn;
     const float a = m == kNegInf ? 0.0f : exp2f(m - mn), w = exp2f(x - ms);
     l = l * a + w;
@@ -370,26 +367,20 @@ __device__ __forceinline__ void slow_row(const RangedParams& p, const RUnit& u, 
     for (int k = 0; k < NE; ++k) o[k] = o[k] * a + w * v[k];
     m = mn;
   }
-  if (q.single) {
-    const float f = finalize_factor(m, l, r_sink<TT>(p, r.h));
+  const int64_t slot = u.worker + u.item, row = slot * p.slot_rows + rl;
+  const bool single = q.how & kRSingle;
+  if (!single && slot >= p.part_slots) return;
+  const float f = l == l ? finalize_factor(m, l, r_sink<TT>(p, q.h)) : l;
 #pragma unroll
-    for (int k = 0; k < NE; ++k) {
-      const int e = lane + 64 * k;
-      if (e < D)
-        reinterpret_cast<raw*>(p.out)[((int64_t)r.t * p.num_heads + r.h) * D + e] =
-            TT::from_f32(o[k] * (l == l ? f : l));
-    }
-  } else {
-    const int64_t slot = u.worker + u.item;
-    if (slot >= p.part_slots) return;
-    const int64_t row = slot * p.slot_rows + rl;
-#pragma unroll
-    for (int k = 0; k < NE; ++k) {
-      const int e = lane + 64 * k;
-      if (e < D) p.part_o[row * D + e] = o[k];
-    }
-    if (lane == 0) p.part_ml[row] = float2{m, l};
+  for (int k = 0; k < NE; ++k) {
+    const int e = lane + 64 * k;
+    if (e >= D) continue;
+    if (single)
+      reinterpret_cast<raw*>(p.out)[((int64_t)q.t * p.num_heads + q.h) * D + e] = TT::from_f32(o[k] * f);
+    else
+      p.part_o[row * D + e] = o[k];
   }
+  if (!single && lane == 0) p.part_ml[row] = float2{m, l};
 }
 
 // ------------------------------------------------------------------------------------ the tiles
@@ -420,7 +411,8 @@ struct RFeed {
 };
 
 // Tile rows [row0, row0 + ROWS) (row0 a multiple of ROWS, at most 32), keys t0 + row, into lds + PITCH row.  SIDE: 0 keys, 1 values.
-template <int D, int ROWS, int SIDE>
+// NT: streamed once (nt), else kept for the other workgroups that read the same keys.
+template <int D, int ROWS, int SIDE, bool NT>
 __device__ __forceinline__ void feed_rows(const RangedParams& p, const RFeed& f, int t0, int row0,
                                           uint32_t lds, int lane) {
   using G = RGeom<D>;
@@ -444,12 +436,12 @@ __device__ __forceinline__ void feed_rows(const RangedParams& p, const RFeed& f,
 #pragma unroll
       for (int i = 0; i < GR / G::RPI; ++i) {
         const int rl = gp * GR + i * G::RPI;
-        dma_base(base + i * G::RPI * f.rowb, (uint32_t)(lr * (int)f.rowb + 16 * piece(row0 + rl + lr)),
+        dma_base<NT>(base + i * G::RPI * f.rowb, (uint32_t)(lr * (int)f.rowb + 16 * piece(row0 + rl + lr)),
                  lds + (row0 + rl) * G::PITCH);
       }
     }
   } else {
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < NI; ++i) {
       const int row = row0 + i * G::RPI + lr;
       const int pos = min(max(t0 + row, f.kmin), f.kmax - 1);
@@ -575,24 +567,24 @@ __device__ __forceinline__ void r_values(RState<TT, D>& st, const char* vt, int 
 }
 
 template <typename TT, int D>
-__device__ __forceinline__ void r_init(const RangedParams& p, const RRow& r, const RPart& q, int lane,
-                                       RState<TT, D>& st) {
-  const char* src = reinterpret_cast<const char*>(p.q) + ((int64_t)r.t * p.num_heads + r.h) * D * 2 +
+__device__ __forceinline__ void r_init(const RangedParams& p, const RInfo& q, int lane, RState<TT, D>& st) {
+  const bool any = q.how & kRAny;
+  const char* src = reinterpret_cast<const char*>(p.q) + ((int64_t)q.t * p.num_heads + q.h) * D * 2 +
                     16 * (lane >> 5);
   // a negative scale goes into the queries' signs (p.scale_log2 has its magnitude)
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks)
-    st.q[ks] = q.any ? (ld16(src + 32 * ks) ^ p.qxor) : u32x4{0, 0, 0, 0};
+    st.q[ks] = any ? (ld16(src + 32 * ks) ^ p.qxor) : u32x4{0, 0, 0, 0};
 #pragma unroll
   for (int n = 0; n < D / 32; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) st.o[n][i] = 0.0f;
   st.m = kNegInf;
   st.l = 0.0f;
-  st.lo = q.any ? q.lo : 0;
-  st.hi = q.any ? q.hi : 0;
-  st.pos = r.pos;
-  st.slope = p.slopes ? p.slopes[r.h] * kLog2e : 0.0f;
+  st.lo = any ? q.lo : 0;
+  st.hi = any ? q.hi : 0;
+  st.pos = q.pos;
+  st.slope = p.slopes ? p.slopes[q.h] * kLog2e : 0.0f;
 }
 
 __device__ __forceinline__ int half_min(int v) {  // over the 32 rows of a wavefront (both halves alike)
@@ -602,51 +594,68 @@ __device__ __forceinline__ int half_min(int v) {  // over the 32 rows of a wavef
 }
 __device__ __forceinline__ int half_max(int v) { return -half_min(-v); }
 
-// ------------------------------------------------------------------------------------ a unit
-// 128 rows: wavefront w takes rows 32 w .. 32 w + 31 of every tile.
-template <typename TT, int D, bool EXTRA>
-__device__ __forceinline__ void wide_unit(const RangedParams& p, const RUnit& u, char* lds, int* red) {
-  using G = RGeom<D>;
-  constexpr int KB = G::KT / 32, SIDE = G::KT * G::PITCH;
-  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int rl = 32 * wave + (lane & 31);
-  const RRow r = r_unit_row(p, u, rl);
-  const RPart q = r_part(u, r);
-  RState<TT, D> st;
-  r_init<TT, D>(p, r, q, lane, st);
-  // keys that some / every row of the wavefront sees, and some row of the workgroup
-  const int wlo = half_min(q.any ? q.lo : INT32_MAX), whi = half_max(q.any ? q.hi : 0);
-  const int flo = half_max(q.any ? q.lo : 0), fhi = half_min(q.any ? q.hi : INT32_MAX);
-  if (lane == 0) {
-    red[2 * wave] = wlo;
-    red[2 * wave + 1] = whi;
-  }
-  __syncthreads();
+// The lane, hidden from the compiler once per unit: what follows from it would otherwise be computed at the
+// kernel's start for both kinds of unit, and spilled.
+__device__ __forceinline__ int unit_lane() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+__device__ __forceinline__ RFeed r_feed(const RangedParams& p, const RUnit& u, int D) {
   RFeed f;
-  f.kmin = uniform(min(min(red[0], red[2]), min(red[4], red[6])));
-  f.kmax = uniform(max(max(red[1], red[3]), max(red[5], red[7])));
   f.kc = reinterpret_cast<const char*>(p.key_cache);
   f.vc = reinterpret_cast<const char*>(p.value_cache);
   f.bt = p.block_table + (int64_t)u.s.b0 * p.max_blocks;
   f.rowb = (int64_t)p.kv_heads * D * 2;
   f.hoff = (int64_t)u.kh * D * 2;
+  f.kmin = f.kmax = 0;
   f.bs = p.block_size;
   f.sh = p.bs_shift;
+  return f;
+}
+
+// ------------------------------------------------------------------------------------ a unit
+// Both kinds leave the rows that came out not finite marked kROdd in sh.row and end at a barrier.
+//
+// 128 rows: wavefront w takes rows 32 w .. 32 w + 31 of every tile.
+template <typename TT, int D, bool EXTRA>
+__device__ __forceinline__ void wide_unit(const RangedParams& p, const RUnit& u, char* lds, RScan& sh) {
+  using G = RGeom<D>;
+  constexpr int KB = G::KT / 32, SIDE = G::KT * G::PITCH;
+  const int wave = uniform(threadIdx.x >> 6), lane = unit_lane(), h = lane >> 5;
+  const int rl = 32 * wave + (lane & 31);
+  const RInfo q = r_info(p, u, rl);
+  const bool any = q.how & kRAny;
+  RState<TT, D> st;
+  r_init<TT, D>(p, q, lane, st);
+  const float sink = r_sink<TT>(p, q.h);
+  // keys that some / every row of the wavefront sees, and some row of the workgroup
+  const int wlo = half_min(any ? q.lo : INT32_MAX), whi = half_max(any ? q.hi : 0);
+  const int flo = half_max(any ? q.lo : 0), fhi = half_min(any ? q.hi : INT32_MAX);
+  if (lane == 0) {
+    sh.red[2 * wave] = wlo;
+    sh.red[2 * wave + 1] = whi;
+  }
+  if (h == 0) sh.row[rl] = q;
+  __syncthreads();
+  RFeed f = r_feed(p, u, D);
+  f.kmin = uniform(min(min(sh.red[0], sh.red[2]), min(sh.red[4], sh.red[6])));
+  f.kmax = uniform(max(max(sh.red[1], sh.red[3]), max(sh.red[5], sh.red[7])));
   if (f.kmin < f.kmax) {
     const int tb = f.kmin / G::KT, te = (f.kmax + G::KT - 1) / G::KT;
     const uint32_t base = lds_address(lds);
-    auto issue = [&](int t) __attribute__((always_inline)) {
-      const uint32_t buf = base + ((t - tb) & 1) * 2 * SIDE;
-      feed_rows<D, G::KT / 4, 0>(p, f, t * G::KT, wave * (G::KT / 4), buf, lane);
-      feed_rows<D, G::KT / 4, 1>(p, f, t * G::KT, wave * (G::KT / 4), buf + SIDE, lane);
-    };
-    issue(tb);
-    for (int t = tb; t < te; ++t) {
+    // iteration t loads tile t + 1 and multiplies tile t (none in the first)
+    for (int t = tb - 1; t < te; ++t) {
       wait_loads<0>();
       __syncthreads();
-      if (t + 1 < te) issue(t + 1);
+      if (t + 1 < te) {
+        const uint32_t buf = base + ((t + 1 - tb) & 1) * 2 * SIDE;
+        feed_rows<D, G::KT / 4, 0, false>(p, f, (t + 1) * G::KT, wave * (G::KT / 4), buf, lane);
+        feed_rows<D, G::KT / 4, 1, false>(p, f, (t + 1) * G::KT, wave * (G::KT / 4), buf + SIDE, lane);
+      }
       const int t0 = t * G::KT;
-      if (t0 >= whi || t0 + G::KT <= wlo) continue;
+      if (t < tb || t0 >= whi || t0 + G::KT <= wlo) continue;
       const char* buf = lds + ((t - tb) & 1) * 2 * SIDE;
       f32x16 s[KB];
       u32x4 pr[2 * KB];
@@ -656,19 +665,17 @@ __device__ __forceinline__ void wide_unit(const RangedParams& p, const RUnit& u,
     }
   }
   const float l = st.l + half_swap(st.l);
-  const int h = lane >> 5;
   float sum = 0.0f;  // NaN if an output is not finite
 #pragma unroll
   for (int n = 0; n < D / 32; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(st.o[n][i], 0.0f, sum);
-  const bool odd = q.any && !(sum == 0.0f && l < __builtin_huge_valf());
-  const uint64_t odds = __ballot(odd);
-  uint32_t again = (uint32_t)(odds | (odds >> 32));
-  const bool skip = (again >> (lane & 31)) & 1;
-  if (q.zero || (q.any && q.single && !skip)) {
-    const float fct = q.zero ? 0.0f : finalize_factor(st.m, l, r_sink<TT>(p, r.h));
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((int64_t)r.t * p.num_heads + r.h) * D + 4 * h;
+  sum += half_swap(sum);
+  const bool odd = any && !(sum == 0.0f && l < __builtin_huge_valf());
+  if (odd && h == 0) sh.row[rl].how = q.how | kROdd;
+  if ((q.how & kRZero) || (any && (q.how & kRSingle))) {
+    const float fct = (q.how & kRZero) ? 0.0f : finalize_factor(st.m, l, sink);
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((int64_t)q.t * p.num_heads + q.h) * D + 4 * h;
 #pragma unroll
     for (int n = 0; n < D / 32; ++n)
 #pragma unroll
@@ -680,7 +687,7 @@ __device__ __forceinline__ void wide_unit(const RangedParams& p, const RUnit& u,
                  ((uint32_t)TT::from_f32(st.o[n][4 * i + 2 * k + 1] * fct) << 16);
         *reinterpret_cast<u32x2*>(dst + 32 * n + 8 * i) = w;
       }
-  } else if (q.any && !q.single && !skip) {
+  } else if (any) {
     const int64_t slot = u.worker + u.item;
     if (slot < p.part_slots) {
       const int64_t row = slot * p.slot_rows + rl;
@@ -693,74 +700,63 @@ __device__ __forceinline__ void wide_unit(const RangedParams& p, const RUnit& u,
       if (h == 0) p.part_ml[row] = float2{st.m, l};
     }
   }
-  for (; again; again &= again - 1) slow_row<TT, D>(p, u, 32 * wave + __builtin_ctz(again));
-  __syncthreads();  // the next unit reuses the buffers
+  __syncthreads();
 }
 
 // At most 32 rows: wavefront w takes 32-key tiles w, w + 4, ...
 template <typename TT, int D, bool EXTRA>
-__device__ __forceinline__ void narrow_unit(const RangedParams& p, const RUnit& u, char* lds, int* red) {
+__device__ __forceinline__ void narrow_unit(const RangedParams& p, const RUnit& u, char* lds, RScan& sh) {
   using G = RGeom<D>;
   constexpr int SIDE = 32 * G::PITCH, NI = 32 / G::RPI;
-  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wave = uniform(threadIdx.x >> 6), lane = unit_lane();
   const int rl = lane & 31;
-  const RRow r = r_unit_row(p, u, rl);
-  const RPart q = r_part(u, r);
+  const RInfo q = r_info(p, u, rl);
+  const bool any = q.how & kRAny;
   RState<TT, D> st;
-  r_init<TT, D>(p, r, q, lane, st);
-  RFeed f;
-  f.kmin = half_min(q.any ? q.lo : INT32_MAX);
-  f.kmax = half_max(q.any ? q.hi : 0);
-  const int flo = half_max(q.any ? q.lo : 0), fhi = half_min(q.any ? q.hi : INT32_MAX);
-  f.kc = reinterpret_cast<const char*>(p.key_cache);
-  f.vc = reinterpret_cast<const char*>(p.value_cache);
-  f.bt = p.block_table + (int64_t)u.s.b0 * p.max_blocks;
-  f.rowb = (int64_t)p.kv_heads * D * 2;
-  f.hoff = (int64_t)u.kh * D * 2;
-  f.bs = p.block_size;
-  f.sh = p.bs_shift;
+  r_init<TT, D>(p, q, lane, st);
+  const float sink = r_sink<TT>(p, q.h);
+  RFeed f = r_feed(p, u, D);
+  f.kmin = half_min(any ? q.lo : INT32_MAX);
+  f.kmax = half_max(any ? q.hi : 0);
+  const int flo = half_max(any ? q.lo : 0), fhi = half_min(any ? q.hi : INT32_MAX);
+  if (threadIdx.x < 32) sh.row[rl] = q;
   char* mine = lds + wave * 2 * SIDE;
   if (f.kmin < f.kmax) {
     const int te = (f.kmax + 31) / 32;
     const uint32_t base = lds_address(mine);
-    int t = f.kmin / 32 + wave;
-    if (t < te) {
-      feed_rows<D, 32, 0>(p, f, t * 32, 0, base, lane);
-      feed_rows<D, 32, 1>(p, f, t * 32, 0, base + SIDE, lane);
-    }
-    for (; t < te; t += 4) {
+    // iteration t loads tile t + 4 and multiplies tile t (none in the first)
+    for (int t = f.kmin / 32 + wave - 4; t < te; t += 4) {
+      const bool more = t + 4 < te, have = t >= f.kmin / 32;
       const int t0 = t * 32;
-      const bool more = t + 4 < te;
       f32x16 s[1];
       u32x4 pr[2];
-      wait_loads<NI>();  // the keys; the values are younger
-      r_scores<TT, D, 1>(st, mine, lane, s);
-      if (more) {
+      if (have) {
+        wait_loads<NI>();  // the keys; the values are younger
+        r_scores<TT, D, 1>(st, mine, lane, s);
         wait_lds_reads();
-        feed_rows<D, 32, 0>(p, f, t0 + 128, 0, base, lane);
       }
-      r_softmax<TT, D, 1, EXTRA>(p, st, s, t0, t0 < flo || t0 + 32 > fhi, lane, pr);
-      if (more)
-        wait_loads<NI>();
-      else
-        wait_loads<0>();
-      r_values<TT, D, 1>(st, mine + SIDE, lane, pr);
-      if (more) {
+      if (more) feed_rows<D, 32, 0, true>(p, f, t0 + 128, 0, base, lane);
+      if (have) {
+        r_softmax<TT, D, 1, EXTRA>(p, st, s, t0, t0 < flo || t0 + 32 > fhi, lane, pr);
+        if (more)
+          wait_loads<NI>();
+        else
+          wait_loads<0>();
+        r_values<TT, D, 1>(st, mine + SIDE, lane, pr);
         wait_lds_reads();
-        feed_rows<D, 32, 1>(p, f, t0 + 128, 0, base + SIDE, lane);
       }
+      if (more) feed_rows<D, 32, 1, true>(p, f, t0 + 128, 0, base + SIDE, lane);
     }
   }
   // The four wavefronts' rows meet in LDS: O of wavefront w in its own tile's place, 16-byte pieces
   // exchanged by the row.
   constexpr int PC = D / 4;                      // pieces of a row
   constexpr int PX = D == 96 ? 7 : PC - 1 < 31 ? PC - 1 : 31;
-  float* ml = reinterpret_cast<float*>(red);     // [wave][row][2]
+  float* ml = reinterpret_cast<float*>(sh.row + kRNarrow);  // [wave][row][2]
   const float l = st.l + half_swap(st.l);
   {
     const int h = lane >> 5;
     f32x4* po = reinterpret_cast<f32x4*>(mine) + rl * PC;
-    wait_lds_reads();
 #pragma unroll
     for (int n = 0; n < D / 32; ++n)
 #pragma unroll
@@ -773,11 +769,12 @@ __device__ __forceinline__ void narrow_unit(const RangedParams& p, const RUnit& 
     }
   }
   __syncthreads();
-  // Eight threads per row; wavefront w holds rows 8 w .. 8 w + 7.
+  // Eight threads per row; wavefront w holds rows 8 w .. 8 w + 7 (what it needs of them is in its lanes).
   const int row = threadIdx.x >> 3, part = threadIdx.x & 7;
-  if (u.row0 + row < u.s.rows) {
-    const RRow rr = r_unit_row(p, u, row);
-    const RPart qq = r_part(u, rr);
+  const int how = __shfl(q.how, row, 64);
+  const int64_t place = (int64_t)__shfl(q.t, row, 64) * p.num_heads + __shfl(q.h, row, 64);
+  const float rsink = __shfl(sink, row, 64);
+  if (how & (kRAny | kRZero)) {
     float w[4], M = kNegInf, L = 0.0f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) M = fmaxf(M, ml[(k * 32 + row) * 2]);
@@ -800,12 +797,10 @@ __device__ __forceinline__ void narrow_unit(const RangedParams& p, const RUnit& 
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(acc[n][e], 0.0f, sum);
     }
-    bool odd = qq.any && !(sum == 0.0f && L < __builtin_huge_valf());
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) odd = __shfl_xor((int)odd, o, 64) || odd;
-    if (qq.zero || (qq.any && qq.single && !odd)) {
-      const float fct = qq.zero ? 0.0f : finalize_factor(M, L, r_sink<TT>(p, rr.h));
-      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((int64_t)rr.t * p.num_heads + rr.h) * D;
+    if ((how & kRAny) && !(sum == 0.0f && L < __builtin_huge_valf())) sh.row[row].how = how | kROdd;
+    if ((how & kRZero) || (how & kRSingle)) {
+      const float fct = (how & kRZero) ? 0.0f : finalize_factor(M, L, rsink);
+      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + place * D;
 #pragma unroll
       for (int n = 0; n < PC / 8; ++n) {
         u32x2 x;
@@ -815,7 +810,7 @@ __device__ __forceinline__ void narrow_unit(const RangedParams& p, const RUnit& 
                  ((uint32_t)TT::from_f32(acc[n][2 * k + 1] * fct) << 16);
         *reinterpret_cast<u32x2*>(dst + 4 * (8 * n + part)) = x;
       }
-    } else if (qq.any && !qq.single && !odd) {
+    } else {
       const int64_t slot = u.worker + u.item;
       if (slot < p.part_slots) {
         const int64_t at = slot * p.slot_rows + row;
@@ -825,84 +820,89 @@ __device__ __forceinline__ void narrow_unit(const RangedParams& p, const RUnit& 
         if (part == 0) p.part_ml[at] = float2{M, L};
       }
     }
-    red[256 + row] = odd ? 1 : 0;
-  } else {
-    red[256 + row] = 0;
   }
   __syncthreads();
-  for (int k = wave; k < 32; k += 4)
-    if (uniform(red[256 + k])) slow_row<TT, D>(p, u, k);
-  __syncthreads();  // the next unit reuses the buffers
 }
 
-// Workgroups per CU: two by LDS (head 64: up to four) and registers, one at head 256.
-template <typename TT, int D, bool EXTRA>
+// WIDE: blocks of more than 32 rows may be among the batch's.
+// Workgroups per CU: two by LDS and registers, one at head 256.
+template <typename TT, int D, bool EXTRA, bool WIDE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2))) void
 ranged_kernel(const RangedParams p) {
-  __shared__ __attribute__((aligned(1024))) char lds[RGeom<D>::LDS];
+  __shared__ __attribute__((aligned(1024))) char
+      lds[WIDE && RGeom<D>::WIDE > RGeom<D>::NARROW ? RGeom<D>::WIDE : RGeom<D>::NARROW];
   __shared__ RScan sh;
-  __shared__ int red[256 + 32];
-  const RPlan plan = r_plan(p, sh);
   const int64_t me = blockIdx.x;
-  if (me >= (plan.per > 0 ? p.slots : plan.items)) return;
-  // my stretch: tiles [me per, me per + per) of the flat list, or item number me
-  const int64_t a = me * plan.per, z = min(a + plan.per, plan.tiles);
-  if (plan.per > 0 && a >= plan.tiles) return;
-  const int n = p.groups + p.batch;
-  int64_t t0 = 0, at = a;
-  int i0 = 0;
-  if (me == 0) {  // the sources' places, for the merge
-    for (int base = 0; base < n; base += kRChunk) {
-      if (n > kRChunk) scan_chunk(p, base, sh, t0, i0);
-      const RSource s = sh.src[threadIdx.x];
-      if (base + (int)threadIdx.x < n)
-        p.table[1 + base + threadIdx.x] = RTable{s.first, s.item, s.tiles, s.tok0, s.rows, s.ka, 0};
-    }
-    if (threadIdx.x == 0) p.table[0] = RTable{plan.tiles, plan.items, plan.per, 0, 0, 0, 0};
-    t0 = 0;
-    i0 = 0;
-  }
-  for (int base = 0; base < n; base += kRChunk) {
+  const int n = p.groups + p.batch, chunks = (n + kRChunk - 1) / kRChunk;
+  // Pass 0 adds up tiles and items of all sources, pass 1 walks them; both at once if one chunk has them all.
+  int64_t tiles = 0, t0 = 0, at = 0, z = 0;
+  int items = 0, i0 = 0, per = 0;
+  for (int c = chunks > 1 ? -chunks : 0; c < chunks; ++c) {
+    const int base = (c < 0 ? c + chunks : c) * kRChunk;
     const int64_t tb = t0;
     const int ib = i0;
-    if (n > kRChunk)
-      scan_chunk(p, base, sh, t0, i0);
-    else {
-      t0 = plan.tiles;
-      i0 = plan.items;
+    scan_chunk(p, base, sh, t0, i0);
+    if (c < -1) continue;
+    if (c == -1 || chunks == 1) {
+      tiles = t0;
+      items = i0;
+      // few items: their tiles in equal stretches, a workgroup each
+      if (items < 2 * p.slots) per = (int)max((tiles + p.slots - 1) / p.slots, (int64_t)p.least);
+      at = me * per;
+      z = min(at + per, tiles);
+      if (per > 0 ? at >= tiles && me > 0 : me >= items && me > 0) return;
+      if (c == -1) {
+        t0 = 0;
+        i0 = 0;
+        continue;
+      }
     }
-    for (;;) {
-      if (plan.per > 0 ? at >= min(z, t0) : (me < ib || me >= i0)) break;
-      if (plan.per > 0 && at < tb) break;
+    if (me == 0) {  // the sources' places, for the merge
+      const RSource s = sh.src[threadIdx.x];
+      if (base + (int)threadIdx.x < n)
+        p.table[1 + base + threadIdx.x] =
+            RTable{s.first, s.item, s.tiles, s.tok0, s.rows, s.ka, s.kb, s.shared, s.group};
+      if (base == 0 && threadIdx.x == 0) p.table[0] = RTable{tiles, items, per, 0, 0, 0, 0, 0, 0};
+    }
+    // my stretch of the flat list, or item number me
+    while (per > 0 ? at >= tb && at < min(z, t0) : me >= ib && me < i0) {
       // the last source that begins at or before the place (sources without tiles begin where the next does)
       int lo = 0, hi = min(kRChunk, n - base);
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        const bool before = plan.per > 0 ? sh.src[mid].first <= at : sh.src[mid].item <= (int)me;
+        const bool before = per > 0 ? sh.src[mid].first <= at : sh.src[mid].item <= (int)me;
         if (before) lo = mid; else hi = mid;
       }
       RUnit u;
       const RSource sl = sh.src[lo];
-      u.s = RSource{uniform64(sl.first), uniform(sl.item), uniform(sl.tok0), uniform(sl.rows), uniform(sl.b0),
-                    uniform(sl.b1), uniform(sl.ka), uniform(sl.kb), uniform(sl.tiles)};
+      u.s = RSource{uniform64(sl.first), uniform(sl.item), uniform(sl.tok0),  uniform(sl.rows),
+                    uniform(sl.b0),      uniform(sl.b1),   uniform(sl.ka),    uniform(sl.kb),
+                    uniform(sl.tiles),   uniform(sl.shared), 0};
       u.group = base + lo < p.groups;
-      u.per = plan.per;
+      u.per = per;
       u.worker = me;
-      const int blocks = r_blocks(u.s.rows);
-      const int local = plan.per > 0 ? (int)((at - u.s.first) / u.s.tiles) : (int)me - u.s.item;
+      const int local = per > 0 ? (int)((uint32_t)(at - u.s.first) / (uint32_t)u.s.tiles) : (int)me - u.s.item;
       u.item = u.s.item + local;
       u.at = u.s.first + (int64_t)local * u.s.tiles;
       // the last rows, which see most keys, first
       u.kh = local % p.kv_heads;
-      const int blk = blocks - 1 - local / p.kv_heads;
-      u.row0 = blk * kRWide;
-      u.x0 = plan.per > 0 ? (int)(at - u.at) : 0;
-      u.x1 = plan.per > 0 ? (int)min((int64_t)u.s.tiles, z - u.at) : u.s.tiles;
-      if (u.s.rows > kRNarrow)
-        wide_unit<TT, D, EXTRA>(p, u, lds, red);
+      u.row0 = (r_blocks(u.s.rows) - 1 - local / p.kv_heads) * kRWide;
+      u.x0 = per > 0 ? (int)(at - u.at) : 0;
+      u.x1 = per > 0 ? (int)min((int64_t)u.s.tiles, z - u.at) : u.s.tiles;
+      bool wide = false;
+      if constexpr (WIDE) wide = u.s.rows > kRNarrow;
+      if (wide)
+        wide_unit<TT, D, EXTRA>(p, u, lds, sh);
       else
-        narrow_unit<TT, D, EXTRA>(p, u, lds, red);
-      if (plan.per == 0) return;
+        narrow_unit<TT, D, EXTRA>(p, u, lds, sh);
+      // rows that came out not finite, again
+      const int wave = threadIdx.x >> 6;
+      for (int k = uniform(wave); k < (wide ? kRWide : kRNarrow); k += 4) {
+        const RInfo q = sh.row[k];
+        if (uniform(q.how) & kROdd) slow_row<TT, D>(p, u, q, k);
+      }
+      __syncthreads();  // the next unit reuses the buffers
+      if (per == 0) return;
       at = u.at + u.x1;
     }
   }
@@ -929,17 +929,18 @@ __global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p)
   if (per == 0 && p.groups == 0) return;
   const int tid = threadIdx.x, g = p.num_heads / p.kv_heads;
   const int kh = blockIdx.x % p.kv_heads;
+  int b1 = 0;  // one row: its sequence, searched by the whole wavefront
+  if constexpr (RM == 1)
+    if (tid < 64) b1 = seq_of_token(p.cum, p.batch, (int)min((int64_t)(blockIdx.x / p.kv_heads) / g, (int64_t)p.num_tokens));
   if (tid < RM) {
     const int64_t gr = (int64_t)(blockIdx.x / p.kv_heads) * RM + tid;
     const int t = (int)min(gr / g, (int64_t)p.num_tokens);
     RJoin j{t, kh * g + (int)(gr % g), 0, 0, 0, 0};
     if (t < p.num_tokens && t >= p.cum[0] && t < p.cum[p.batch]) {
-      RSource all{};
-      all.b1 = p.batch;
-      const int b = r_token_seq(p, all, t);
-      const RRow r = r_row(p, t, j.h, b, true);
-      auto pieces = [&](int i, int a, int z, int64_t& row) {
-        const RTable e = p.table[1 + i];
+      const int b = RM == 1 ? b1 : r_token_seq(p, 0, p.batch, t);
+      const RTable own = p.table[1 + p.groups + b];
+      const RRange r = r_range(p, t, own.kb - own.rows / g + (t - own.tok0), b, own.kb);
+      auto pieces = [&](const RTable& e, int a, int z, int64_t& row) {
         const int rr = (t - e.tok0) * g + j.h - kh * g, blocks = r_blocks(e.rows);
         const int blk = e.rows > kRNarrow ? rr / kRWide : 0;
         const int local = (blocks - 1 - blk) * p.kv_heads + kh, kt = e.ka / kRTile;
@@ -948,9 +949,9 @@ __global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p)
         row = (w0 + e.item + local) * p.slot_rows + rr - blk * kRWide;
         return (int)(r_worker(per, at, e.item + local, (z - 1) / kRTile - kt) - w0) + 1;
       };
-      const int sh_hi = min(r.hi, r.shared), own_lo = max(r.lo, r.shared);
-      if (r.lo < sh_hi) j.na = pieces(group_of(p, b), r.lo, sh_hi, j.ra);
-      if (own_lo < r.hi) j.nb = pieces(p.groups + b, own_lo, r.hi, j.rb);
+      const int sh_hi = min(r.hi, own.shared), own_lo = max(r.lo, own.shared);
+      if (r.lo < sh_hi) j.na = pieces(p.table[1 + own.group], r.lo, sh_hi, j.ra);
+      if (own_lo < r.hi) j.nb = pieces(own, own_lo, r.hi, j.rb);
       const int64_t end = (int64_t)p.part_slots * p.slot_rows;
       if (j.ra + (int64_t)(max(j.na, 1) - 1) * p.slot_rows >= end ||
           j.rb + (int64_t)(max(j.nb, 1) - 1) * p.slot_rows >= end)
@@ -1021,10 +1022,14 @@ __global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p)
 template <typename TT, int D>
 hipError_t launch_d(const RangedParams& p, hipStream_t s) {
   const dim3 grid(p.grid), block(256);
-  if (p.softcap > 0.0f || p.slopes)
-    hipLaunchKernelGGL((ranged_kernel<TT, D, true>), grid, block, 0, s, p);
-  else
-    hipLaunchKernelGGL((ranged_kernel<TT, D, false>), grid, block, 0, s, p);
+  const bool extra = p.softcap > 0.0f || p.slopes;
+  if (p.wide) {
+    if (extra) hipLaunchKernelGGL((ranged_kernel<TT, D, true, true>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((ranged_kernel<TT, D, false, true>), grid, block, 0, s, p);
+  } else {
+    if (extra) hipLaunchKernelGGL((ranged_kernel<TT, D, true, false>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((ranged_kernel<TT, D, false, false>), grid, block, 0, s, p);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.merge) return e;
   const int64_t rows = (int64_t)p.num_tokens * (p.num_heads / p.kv_heads);
