@@ -1275,40 +1275,52 @@ RunOpts masked_opts(const pa_mask* mask) {
 
 // Launch shape and workspace of the matrix-core kernel over key ranges (pa_ranged.hip).
 struct RangedPlan {
-  bool on = false;
-  int slots = 0, slot_rows = 0, grid = 0;
-  bool merge = false;
-  int64_t part_slots = 0;
+  bool on = false, whole = false, merge = false, wide = false;
+  int slots = 0, narrow_rows = 0;
+  int64_t part_rows = 0, part_narrow = 0;
   size_t o_bytes = 0, ml_bytes = 0, table_bytes = 0;
   size_t bytes() const { return o_bytes + ml_bytes + table_bytes; }
 };
+// Contexts of at most this many keys run as whole items, without a merge.
+constexpr int kRangedWhole = 512;
 RangedPlan ranged_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a,
                        const pa_shared_prefix* share, pa_dtype act) {
   RangedPlan r;
   if (!c->value_cache || !pa::ranged_supported(c->head_dim, act, c->dtype) || a->num_heads <= 0 ||
       a->num_heads % c->kv_heads != 0 || b->num_tokens <= 0)
     return r;
-  const int64_t g = a->num_heads / c->kv_heads, T = b->num_tokens;
+  // direct LDS loads want 16-byte rows
+  if (((reinterpret_cast<uintptr_t>(c->key_cache) | reinterpret_cast<uintptr_t>(c->value_cache)) & 15) != 0)
+    return r;
+  const int64_t g = a->num_heads / c->kv_heads, T = b->num_tokens, kv = c->kv_heads;
   const int64_t groups = share ? share->groups : 0;
-  // blocks of at most 128 rows of every sequence, and of every group's rows
-  const int64_t blocks = T * g / 128 + b->batch + (groups ? T * g / 128 + groups : 0);
-  const int64_t items = blocks * c->kv_heads;
-  if (items >= ((int64_t)1 << 23) || T * g > INT32_MAX) return r;
-  const int mq = b->max_query_len > 0 ? b->max_query_len : b->num_tokens;
+  const int64_t mq = std::min<int64_t>(b->max_query_len > 0 ? b->max_query_len : T, T);
+  const int64_t cap = (int64_t)b->max_blocks * c->block_size;
+  const int64_t ctx = b->max_context_len > 0 ? std::min<int64_t>(b->max_context_len, cap) : cap;
+  // wide items (blocks of up to 128 rows of the sequences and groups with more than 32), narrow ones
+  const int64_t wide = kv * ((mq * g > 32 ? T * g / 128 + std::min<int64_t>(b->batch, T * g / 33) : 0) +
+                             (groups ? T * g / 128 + std::min<int64_t>(groups, T * g / 33) : 0));
+  const int64_t narrow = kv * (b->batch + groups);
+  const int64_t tiles = std::min<int64_t>(cap, INT32_MAX / 2) / 64 + 2;
+  if (wide + narrow >= ((int64_t)1 << 23) || (wide + narrow) * tiles > INT32_MAX / 2 || T * g > INT32_MAX)
+    return r;
   r.on = true;
-  r.slots = (c->head_dim > 128 ? 1 : 2) * device_cus();
-  const bool split = items < 2 * (int64_t)r.slots;  // (else the device decides)
-  r.grid = (int)(split ? r.slots : std::max<int64_t>(items, r.slots));
-  // an item meets a workgroup at place workgroup + item; whole items leave parts for shared prefixes only
-  r.part_slots = r.slots + std::min<int64_t>(items, 2 * (int64_t)r.slots);
-  if (groups && !split) r.part_slots = std::max(r.part_slots, 2 * items);
-  r.slot_rows = !groups && mq * g <= 32 ? 32 : 128;
-  const int64_t ctx = b->max_context_len > 0 ? b->max_context_len
-                                             : (int64_t)b->max_blocks * c->block_size;
-  r.merge = groups > 0 || ctx > 64;
-  const size_t rows = (size_t)r.part_slots * r.slot_rows;
-  r.o_bytes = align256(rows * c->head_dim * sizeof(float));
-  r.ml_bytes = align256(rows * 2 * sizeof(float));
+  r.wide = wide > 0;
+  const int per_cu = c->head_dim > 128 ? 1 : c->head_dim == 64 ? 3 : 2;
+  r.whole = ctx <= kRangedWhole && groups == 0;
+  r.merge = !r.whole;
+  // no more workgroups than there are tiles for
+  const int64_t most = wide * ((ctx + 63) / 64 + 1) + (narrow * ((ctx + 63) / 64 + 1) + 3) / 4;
+  r.slots = (int)std::max<int64_t>(std::min<int64_t>((int64_t)per_cu * device_cus(), most), 2);
+  r.narrow_rows = (int)std::min<int64_t>(groups ? 32 : mq * g, 32);
+  if (r.merge) {
+    r.part_narrow = 128 * (wide == 0 ? 0 : groups ? std::max(r.slots + std::min(wide, 4 * (int64_t)r.slots), 2 * wide)
+                                                  : 2 * (int64_t)r.slots);
+    r.part_rows = r.part_narrow +
+                  (int64_t)r.narrow_rows * (groups ? 4 * r.slots + narrow : 8 * (int64_t)r.slots);
+  }
+  r.o_bytes = align256((size_t)r.part_rows * c->head_dim * sizeof(float));
+  r.ml_bytes = align256((size_t)r.part_rows * 2 * sizeof(float));
   r.table_bytes = align256((size_t)(1 + groups + b->batch) * sizeof(pa::RTable));
   return r;
 }
@@ -1338,6 +1350,9 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
   if (!ws || ws_bytes < r.bytes())
     return fail(PA_ERR_INVALID_ARGUMENT, "workspace too small: need %zu bytes, got %zu", r.bytes(),
                 ws_bytes);
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) ||
+      (reinterpret_cast<uintptr_t>(ws) & 15))
+    return fail(PA_ERR_INVALID_ARGUMENT, "q, out and workspace must be 16-byte aligned");
   pa::RangedParams p{};
   p.q = q;
   p.key_cache = c->key_cache;
@@ -1362,7 +1377,9 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
   p.part_ml = reinterpret_cast<float2*>(base + r.o_bytes);
   p.table = reinterpret_cast<pa::RTable*>(base + r.o_bytes + r.ml_bytes);
   p.num_blocks = c->num_blocks;
-  p.part_slots = r.part_slots;
+  p.part_rows = r.part_rows;
+  p.part_narrow = r.part_narrow;
+  p.narrow_rows = r.narrow_rows;
   p.block_size = c->block_size;
   const bool pow2 = (c->block_size & (c->block_size - 1)) == 0;
   p.bs_shift = pow2 && c->block_size >= 16 ? __builtin_ctz((unsigned)c->block_size) : -1;
@@ -1379,11 +1396,11 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
   p.softcap = a->softcap;
   p.qxor = p.scale < 0.0f ? 0x80008000u : 0u;
   p.slots = r.slots;
-  p.least = 2;
-  p.slot_rows = r.slot_rows;
-  p.grid = r.grid;
+  p.least[0] = 4;
+  p.least[1] = 3;
+  p.whole = r.whole ? 1 : 0;
   p.merge = r.merge ? 1 : 0;
-  p.wide = r.slot_rows > 32 ? 1 : 0;
+  p.wide = r.wide ? 1 : 0;
   const hipError_t e = pa::launch_ranged(p, act, s);
   if (e != hipSuccess) return hip_fail(e, "masked attention launch");
   return PA_OK;

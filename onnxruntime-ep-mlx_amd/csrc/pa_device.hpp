@@ -411,11 +411,10 @@ struct AttnParams {
 };
 
 // Attention over key ranges per row, with shared prefixes (pa_ranged.hip).
-// A source's place in the flat list of 64-key tiles, for the merge (entry 0: all tiles, items, tiles per
-// workgroup; then groups and sequences).
+// The plan as the merge reads it: entry 0 tiles per worker (wide, narrow), then the groups' and sequences'
+// places in the flat lists of 64-key tiles.
 struct RTable {
-  int64_t first;
-  int32_t item, tiles, tok0, rows, ka, kb, shared, group;
+  int32_t v[12];
 };
 struct RangedParams {
   const void* q;
@@ -432,11 +431,13 @@ struct RangedParams {
   const int32_t* doc_starts;
   const int32_t* group_cum;
   const int32_t* shared_lens;
-  // Workspace: partial rows [part_slots][slot_rows][head_dim], their (m, l), and the table
+  // Workspace: part_rows partial rows [head_dim] (those of wide blocks, then from part_narrow on those of
+  // narrow ones, narrow_rows each), their (m, l), and the table
   float* part_o;
   float2* part_ml;
   RTable* table;
-  int64_t num_blocks, part_slots;
+  int64_t num_blocks, part_rows, part_narrow;
+  int32_t narrow_rows;
   int32_t groups;
   int32_t block_size, bs_shift;  // bs_shift: log2 of a power of two of at least 16, else -1
   int32_t kv_heads, head_dim, num_heads;
@@ -444,12 +445,11 @@ struct RangedParams {
   int32_t window, causal;
   float scale, scale_log2, softcap;  // scale_log2: |scale| log2(e)
   uint32_t qxor;                     // 0x80008000 where scale is negative
-  int32_t slots;      // workgroups that share the tiles of few items
-  int32_t least;      // tiles per workgroup, at least
-  int32_t slot_rows;  // rows of a partial slot: 32 where every block is known to be that small, else 128
-  int32_t grid;       // workgroups
-  int32_t merge;      // some row may have several pieces
-  int32_t wide;       // some block may hold more than 32 rows
+  int32_t slots;     // workgroups
+  int32_t least[2];  // tiles per worker, at least (wide, narrow)
+  int32_t whole;     // every item whole (short contexts)
+  int32_t merge;     // some row may have several pieces
+  int32_t wide;      // some block may hold more than 32 rows
 };
 hipError_t launch_ranged(const RangedParams& p, pa_dtype act, hipStream_t s);
 bool ranged_supported(int head_dim, pa_dtype act, pa_dtype cache_dtype);

@@ -9,12 +9,14 @@
 //
 // Work.  Sources: every group (all its rows against the shared keys, read through its first
 // sequence's table) and every sequence (its rows against the keys behind the shared ones).  An item is a
-// block of rows of one source and kv-head; it costs one per 64 keys.  While the items are few (under two
-// per workgroup slot) the flat list of all items' 64-key tiles is cut into equal parts, one workgroup
-// each, whatever item borders lie inside: an item that meets several workgroups leaves (m, l, O) of each
-// in fp32 and ranged_merge_kernel joins them, as it joins a row's shared and own keys.  With more items
-// each workgroup takes a whole one.  The plan is a scan over the lengths that every workgroup makes for
-// itself, from the device's metadata.
+// block of rows of one source and kv-head, its cost the 64-key tiles that the block may see.  Sources of
+// more than 32 rows (prompts, shared prefixes) are wide: blocks of 128 rows, a workgroup each.  The others
+// (decode) are narrow: one block, a wavefront each.  Both kinds' tiles form a flat list which is cut into
+// equal stretches, whatever item borders lie inside, over workgroups and wavefronts in proportion to the
+// tiles: an item that meets several workers leaves (m, l, O) of each in fp32 and ranged_merge_kernel joins
+// them, as it joins a row's shared and own keys.  Where wide items are many, workgroups take whole ones in
+// turns, longest first, every other turn backwards.  The plan is a scan over the lengths that every
+// workgroup makes for itself, from the device's metadata.
 //
 // Both products run transposed on 32x32x16 tiles, so that a lane holds one query row:
 //   S^T[key][row] = K Q^T   (A: 32 keys x 16 dims from LDS, B: the queries in registers)
@@ -24,10 +26,9 @@
 // are scalars of the lane.  Probabilities enter the second product rounded to the activation type (half
 // a step of it, the output's own rounding); scores, statistics and sums are fp32.
 //
-// Rows of more than 32 (prompts, shared prefixes): four wavefronts of 32 rows each on the same 64-key
-// tile (32 keys at head 256), staged by direct loads from the pages into two LDS buffers, one barrier
-// per tile.  At most 32 (decode): the wavefronts take 32-key tiles in turn, each with a tile of its own
-// in LDS, the next keys in flight while the values are multiplied, and meet in LDS at the end.
+// Wide items: four wavefronts of 32 rows each on the same 64-key tile (32 keys at head 256), staged by
+// direct loads from the pages into two LDS buffers, one barrier per tile.  Narrow items: a wavefront with a
+// 32-key tile of its own in LDS, the next keys in flight while the values are multiplied, no barrier.
 //
 // Masked keys weigh exactly zero, but zero times an infinite value is NaN in the product: rows that come
 // out not finite are computed again one key at a time, which skips what they do not see.  Tiles read no
@@ -109,9 +110,6 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(lds_char*)p;
 }
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-  return (int64_t)((uint64_t)(uint32_t)uniform((int)x) | ((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32));
-}
 // A table entry at a wave-uniform place, through the scalar cache (no kernel writes the tables).
 __device__ __forceinline__ int scalar_load(const int32_t* p) {
   typedef const __attribute__((address_space(4))) int32_t* cptr;
@@ -159,61 +157,74 @@ __device__ __forceinline__ int group_of(const RangedParams& p, int b) {
 
 // A group's rows against the keys it shares, or a sequence's against its own.
 struct RSource {
-  int64_t first;  // its first tile in the flat list
-  int item;       // its first item
+  int first;      // its first tile in its kind's flat list
+  int item;       // its first item there
   int tok0, rows; // first token, rows (tokens * g) of one kv-head
   int b0, b1;     // its sequences; b0's table names the pages
   int ka, kb;     // its keys
-  int tiles;      // tiles of one item
-  int shared, group;  // keys that the sequence shares, and its group
+  int base;       // tiles of block 0 (see r_before)
+  int shared;     // keys that the sequence shares
+  int group;      // its group; -1 - group for the group's own source
 };
-__device__ __forceinline__ int r_blocks(int rows) {
-  return rows <= kRNarrow ? (rows > 0) : (rows + kRWide - 1) / kRWide;
+__device__ __forceinline__ bool r_wide(const RSource& s) { return s.rows > kRNarrow; }
+__device__ __forceinline__ int r_blocks(const RSource& s) {
+  return r_wide(s) ? (s.rows + kRWide - 1) / kRWide : s.rows > 0;
+}
+// Tiles of one kv-head before block i: all of the source's (constant), or growing with the rows' positions
+// under a causal mask -- base + 2 i / g each, close to what block i can see, in closed form.
+__device__ __forceinline__ int r_before(const RSource& s, int i, int g, bool grows) {
+  return i * s.base + (grows ? (int)((int64_t)i * (i - 1) / g) : 0);
+}
+__device__ __forceinline__ bool r_grows(const RangedParams& p, const RSource& s) {
+  return p.causal && !p.prefix_lens && s.group >= -1 && r_wide(s);
 }
 // Source i: groups, then sequences (first and item are the scan's).
 __device__ __forceinline__ RSource r_source(const RangedParams& p, int i) {
   RSource s{};
+  s.group = -1;
   const int g = p.num_heads / p.kv_heads;
   if (i >= p.groups + p.batch) return s;
   const bool seq = i >= p.groups;
   const int b = i - p.groups, gi = seq ? (p.groups ? group_of(p, b) : -1) : i;
   const RGroup q = gi >= 0 ? r_group(p, gi) : RGroup{0, 0, 0};
+  int end;
   if (!seq) {
+    s.group = -2 - gi;
     if (q.prefix == 0) return s;
     s.b0 = q.b0;
     s.b1 = q.b1;
     s.tok0 = r_seq(p, q.b0).s0;
     const RSeq last = r_seq(p, q.b1 - 1);
     s.rows = max(last.s0 + last.nq - s.tok0, 0) * g;
-    s.kb = s.shared = q.prefix;
+    end = s.kb = s.shared = q.prefix;
   } else {
     const RSeq e = r_seq(p, b);
+    s.group = gi;
     s.b0 = b;
     s.b1 = b + 1;
     s.tok0 = e.s0;
     s.rows = e.nq * g;
     s.shared = s.ka = min(q.prefix, e.total);
     if (p.window > 0) s.ka = max(s.ka, min(e.past - p.window + 1, e.total));
-    s.kb = e.total;
+    end = s.kb = e.total;
+    if (r_grows(p, s)) end = min(end, e.past + (kRWide + g - 1) / g);  // the last position of block 0
   }
-  s.group = gi;
-  // (a sequence without keys of its own keeps a tile, whose workgroup writes its empty rows)
-  s.tiles = s.rows > 0 ? max((s.kb + kRTile - 1) / kRTile - s.ka / kRTile, 1) : 0;
+  // (an item without keys keeps a tile, whose worker writes its empty rows)
+  s.base = max((end + kRTile - 1) / kRTile - s.ka / kRTile, 1);
   return s;
 }
 
-// Rows of a unit, for the parts of the kernel that hold another row than their lane's.
-struct RInfo {
-  int t, h, pos, lo, hi, how;  // how: kRAny | kRSingle | kRZero | kROdd
-};
-constexpr int kRAny = 1, kRSingle = 2, kRZero = 4, kROdd = 8;
-
+// Per kind (wide, narrow): items in the upper, tiles in the lower bits.
+constexpr int kRItemShift = 40;
 struct RScan {
   RSource src[kRChunk];
-  RInfo row[kRWide];  // (a narrow unit keeps its wavefronts' (m, l) behind its 32 rows)
-  int64_t wt[4];
+  int64_t wt[4][2];
   int red[8];
 };
+struct RTotals {
+  int tiles[2], items[2];  // wide, narrow
+};
+__device__ __forceinline__ int pick(const int (&x)[2], int kind) { return kind ? x[1] : x[0]; }
 __device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -222,37 +233,80 @@ __device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
   }
   return v;
 }
-// Sources base .. base + 255 with their places in the flat list into sh.src; t0 / i0: tiles and items
-// before them, moved past them.  Called by all 256 threads.
-__device__ __forceinline__ void scan_chunk(const RangedParams& p, int base, RScan& sh, int64_t& t0,
-                                           int& i0) {
+// Sources base .. base + 255 with their places in the flat lists into sh.src; t: tiles and items before
+// them, moved past them.  Called by all 256 threads.
+__device__ __forceinline__ void scan_chunk(const RangedParams& p, int base, RScan& sh, RTotals& t) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   RSource s = r_source(p, base + tid);
-  const int items = r_blocks(s.rows) * p.kv_heads;
-  // items above, tiles below: a batch holds fewer than 2^23 items and 2^40 tiles (host)
-  const int64_t mine = ((int64_t)items << 40) + (int64_t)items * s.tiles;
-  const int64_t incl = scan64(mine, lane);
-  __syncthreads();  // the last chunk's readers are done
-  if (lane == 63) sh.wt[wave] = incl;
-  __syncthreads();
-  int64_t before = incl - mine, all = 0;
+  const int blocks = r_blocks(s), kind = r_wide(s) ? 0 : 1;
+  const int64_t mine = ((int64_t)(blocks * p.kv_heads) << kRItemShift) +
+                       (int64_t)p.kv_heads * r_before(s, blocks, p.num_heads / p.kv_heads, r_grows(p, s));
+  int64_t before[2], all[2] = {0, 0};
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) before += sh.wt[w];
-    all += sh.wt[w];
+  for (int k = 0; k < 2; ++k) before[k] = scan64(kind == k ? mine : 0, lane);
+  __syncthreads();  // the last chunk's readers are done
+  if (lane == 63) {
+    sh.wt[wave][0] = before[0];
+    sh.wt[wave][1] = before[1];
   }
-  all = uniform64(all);
-  constexpr int64_t low = ((int64_t)1 << 40) - 1;
-  s.first = t0 + (before & low);
-  s.item = i0 + (int)(before >> 40);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (kind == k) before[k] -= mine;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before[k] += sh.wt[w][k];
+      all[k] += sh.wt[w][k];
+    }
+  }
+  constexpr int64_t low = ((int64_t)1 << kRItemShift) - 1;
+  const int64_t b = before[0] * (1 - kind) + before[1] * kind;
+  s.first = (kind ? t.tiles[1] : t.tiles[0]) + (int)(b & low);
+  s.item = (kind ? t.items[1] : t.items[0]) + (int)(b >> kRItemShift);
   sh.src[tid] = s;
-  t0 += all & low;
-  i0 += (int)(all >> 40);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    t.tiles[k] += uniform((int)(all[k] & low));
+    t.items[k] += uniform((int)(all[k] >> kRItemShift));
+  }
   __syncthreads();
 }
-// Workgroup that takes tile x of an item (its first tile at `at`, its number `item`).
-__device__ __forceinline__ int64_t r_worker(int per, int64_t at, int item, int x) {
-  return per > 0 ? (at + x) / per : item;
+// Who takes what: workgroups [0, wide) the wide items, the wavefronts of the others the narrow ones; tiles
+// per worker of each kind (0: whole items).
+struct RShare {
+  int wide, per[2];
+};
+__device__ __forceinline__ RShare r_share(const RangedParams& p, const RTotals& t) {
+  RShare r;
+  const int64_t all = (int64_t)t.tiles[0] + t.tiles[1];
+  r.wide = t.tiles[0] == 0 ? 0
+           : t.tiles[1] == 0
+               ? p.slots
+               : min(max((int)((float)p.slots * ((float)t.tiles[0] / (float)all)), 1), p.slots - 1);
+  const int waves = max((p.slots - r.wide) * 4, 1);
+  r.per[0] = p.whole || t.items[0] >= 4 * r.wide ? 0 : max((t.tiles[0] + r.wide - 1) / max(r.wide, 1), p.least[0]);
+  r.per[1] = p.whole ? 0 : max((t.tiles[1] + waves - 1) / waves, p.least[1]);
+  return r;
+}
+// One item: block blk of source s and kv-head kh, its place and tiles in the flat list.
+struct RItem {
+  int blk, kh, item, at, tiles;
+};
+__device__ __forceinline__ RItem r_item(const RangedParams& p, const RSource& s, int blk, int kh) {
+  const int g = p.num_heads / p.kv_heads;
+  const bool grows = r_grows(p, s);
+  RItem r;
+  r.blk = blk;
+  r.kh = kh;
+  r.item = s.item + blk * p.kv_heads + kh;
+  const int f = r_before(s, blk, g, grows);
+  r.tiles = r_before(s, blk + 1, g, grows) - f;
+  r.at = s.first + f * p.kv_heads + kh * r.tiles;
+  return r;
+}
+// Worker of tile x of an item; what lies behind its counted tiles belongs to its last worker.
+__device__ __forceinline__ int r_worker(int per, const RItem& q, int x) {
+  return per > 0 ? (q.at + min(x, q.tiles - 1)) / per : q.item;
 }
 
 // The range [lo, hi) of token t at position pos of sequence b (total keys).
@@ -267,15 +321,22 @@ __device__ __forceinline__ RRange r_range(const RangedParams& p, int t, int pos,
   return RRange{max(lo, 0), min(hi, total)};
 }
 
-// A workgroup's part of an item.
+// First partial row of a worker's part of an item.  With shared prefixes every part may be one of several of a
+// row: place worker + item (the parts of an item follow each other and the next begins with the worker where it
+// ends).  Otherwise only a worker's first and last items meet others: two places each.
+__device__ __forceinline__ int64_t r_slot(const RangedParams& p, int kind, int worker, int item, bool head) {
+  const int64_t slot = p.groups > 0 ? (int64_t)worker + item : 2 * (int64_t)worker + (head ? 1 : 0);
+  return kind == 0 ? slot * kRWide : p.part_narrow + slot * p.narrow_rows;
+}
+
+// A worker's part of an item: keys [k0, k1).
 struct RUnit {
   RSource s;
   bool group;
   int kh, row0;    // first row of the block
-  int64_t at;      // the item's first tile in the flat list
-  int item, per;
-  int x0, x1;      // tiles of the item
-  int64_t worker;
+  int k0, k1;
+  bool head;       // the item's first part
+  int64_t slot;    // its first partial row
 };
 __device__ __forceinline__ int r_token_seq(const RangedParams& p, int lo, int hi, int t) {
   while (hi - lo > 1) {  // the last of sequences lo .. hi - 1 that begins at or before t
@@ -284,8 +345,12 @@ __device__ __forceinline__ int r_token_seq(const RangedParams& p, int lo, int hi
   }
   return lo;
 }
-// Row rl of a unit's block: the keys of the unit that it sees, whether all that it sees lies in this unit
-// (kRSingle), whether the unit zeroes it because it sees nothing at all (kRZero).
+// A row of a unit's block: its token, head and position, the keys of the unit that it sees; how: kRAny (some),
+// kRSingle (all that it sees at all), kRZero (it sees nothing at all and this unit writes that).
+struct RInfo {
+  int t, h, pos, lo, hi, how;
+};
+constexpr int kRAny = 1, kRSingle = 2, kRZero = 4;
 __device__ __forceinline__ RInfo r_info(const RangedParams& p, const RUnit& u, int rl) {
   const int g = p.num_heads / p.kv_heads, r = u.row0 + rl;
   const bool valid = r < u.s.rows;
@@ -304,17 +369,14 @@ __device__ __forceinline__ RInfo r_info(const RangedParams& p, const RUnit& u, i
   }
   const RRange x = r_range(p, q.t, q.pos, b, total);
   const int a = max(x.lo, u.group ? 0 : shared), z = min(x.hi, u.group ? shared : total);
-  const int kt = u.s.ka / kRTile;
-  q.lo = max(a, (kt + u.x0) * kRTile);
-  q.hi = min(z, (kt + u.x1) * kRTile);
+  q.lo = max(a, u.k0);
+  q.hi = min(z, u.k1);
   q.how = 0;
   if (valid && q.lo < q.hi) {
     const bool other = u.group ? x.hi > max(x.lo, shared) : x.lo < min(x.hi, shared);
-    // (the unit's tiles end where a workgroup's do)
-    const bool here = a >= (kt + u.x0) * kRTile && z <= (kt + u.x1) * kRTile;
-    q.how = kRAny | (here && !other ? kRSingle : 0);
+    q.how = kRAny | (a >= u.k0 && z <= u.k1 && !other ? kRSingle : 0);
   }
-  if (valid && !u.group && x.lo >= x.hi && u.x0 == 0) q.how |= kRZero;
+  if (valid && !u.group && x.lo >= x.hi && u.head) q.how |= kRZero;
   return q;
 }
 
@@ -367,9 +429,9 @@ __device__ __forceinline__ void slow_row(const RangedParams& p, const RUnit& u, 
     for (int k = 0; k < NE; ++k) o[k] = o[k] * a + w * v[k];
     m = mn;
   }
-  const int64_t slot = u.worker + u.item, row = slot * p.slot_rows + rl;
   const bool single = q.how & kRSingle;
-  if (!single && slot >= p.part_slots) return;
+  const int64_t row = u.slot + rl;
+  if (!single && row >= p.part_rows) return;
   const float f = l == l ? finalize_factor(m, l, r_sink<TT>(p, q.h)) : l;
 #pragma unroll
   for (int k = 0; k < NE; ++k) {
@@ -616,16 +678,58 @@ __device__ __forceinline__ RFeed r_feed(const RangedParams& p, const RUnit& u, i
 }
 
 // ------------------------------------------------------------------------------------ a unit
-// Both kinds leave the rows that came out not finite marked kROdd in sh.row and end at a barrier.
-//
-// 128 rows: wavefront w takes rows 32 w .. 32 w + 31 of every tile.
+// The wavefront's rows, final where the unit has all their keys, else as partial rows; returns those that came
+// out not finite, which want slow_row.
+template <typename TT, int D>
+__device__ __forceinline__ uint32_t r_store(const RangedParams& p, const RUnit& u, const RInfo& q, int rl,
+                                            const RState<TT, D>& st, float sink, int lane) {
+  const int h = lane >> 5;
+  const bool any = q.how & kRAny;
+  const float l = st.l + half_swap(st.l);
+  float sum = 0.0f;  // NaN if an output is not finite
+#pragma unroll
+  for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(st.o[n][i], 0.0f, sum);
+  if ((q.how & kRZero) || (any && (q.how & kRSingle))) {
+    const float fct = (q.how & kRZero) ? 0.0f : finalize_factor(st.m, l, sink);
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((int64_t)q.t * p.num_heads + q.h) * D + 4 * h;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        u32x2 w;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          w[k] = (uint32_t)TT::from_f32(st.o[n][4 * i + 2 * k] * fct) |
+                 ((uint32_t)TT::from_f32(st.o[n][4 * i + 2 * k + 1] * fct) << 16);
+        *reinterpret_cast<u32x2*>(dst + 32 * n + 8 * i) = w;
+      }
+  } else if (any) {
+    const int64_t row = u.slot + rl;
+    if (row < p.part_rows) {
+#pragma unroll
+      for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f32x4*>(p.part_o + row * D + 32 * n + 8 * i + 4 * h) =
+              f32x4{st.o[n][4 * i], st.o[n][4 * i + 1], st.o[n][4 * i + 2], st.o[n][4 * i + 3]};
+      if (h == 0) p.part_ml[row] = float2{st.m, l};
+    }
+  }
+  const uint64_t odd = __ballot(any && !(sum == 0.0f && l < __builtin_huge_valf()));
+  return (uint32_t)(odd | (odd >> 32));
+}
+
+// A block of 128 rows, by the whole workgroup: wavefront w takes rows 32 w .. 32 w + 31 of every tile.
 template <typename TT, int D, bool EXTRA>
-__device__ __forceinline__ void wide_unit(const RangedParams& p, const RUnit& u, char* lds, RScan& sh) {
+__device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit& u, char* lds, RScan& sh,
+                                              RInfo& q) {
   using G = RGeom<D>;
   constexpr int KB = G::KT / 32, SIDE = G::KT * G::PITCH;
-  const int wave = uniform(threadIdx.x >> 6), lane = unit_lane(), h = lane >> 5;
+  const int wave = uniform(threadIdx.x >> 6), lane = unit_lane();
   const int rl = 32 * wave + (lane & 31);
-  const RInfo q = r_info(p, u, rl);
+  q = r_info(p, u, rl);
   const bool any = q.how & kRAny;
   RState<TT, D> st;
   r_init<TT, D>(p, q, lane, st);
@@ -633,11 +737,11 @@ __device__ __forceinline__ void wide_unit(const RangedParams& p, const RUnit& u,
   // keys that some / every row of the wavefront sees, and some row of the workgroup
   const int wlo = half_min(any ? q.lo : INT32_MAX), whi = half_max(any ? q.hi : 0);
   const int flo = half_max(any ? q.lo : 0), fhi = half_min(any ? q.hi : INT32_MAX);
+  __syncthreads();  // the last unit's readers are done
   if (lane == 0) {
     sh.red[2 * wave] = wlo;
     sh.red[2 * wave + 1] = whi;
   }
-  if (h == 0) sh.row[rl] = q;
   __syncthreads();
   RFeed f = r_feed(p, u, D);
   f.kmin = uniform(min(min(sh.red[0], sh.red[2]), min(sh.red[4], sh.red[6])));
@@ -664,69 +768,31 @@ __device__ __forceinline__ void wide_unit(const RangedParams& p, const RUnit& u,
       r_values<TT, D, KB>(st, buf + SIDE, lane, pr);
     }
   }
-  const float l = st.l + half_swap(st.l);
-  float sum = 0.0f;  // NaN if an output is not finite
-#pragma unroll
-  for (int n = 0; n < D / 32; ++n)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(st.o[n][i], 0.0f, sum);
-  sum += half_swap(sum);
-  const bool odd = any && !(sum == 0.0f && l < __builtin_huge_valf());
-  if (odd && h == 0) sh.row[rl].how = q.how | kROdd;
-  if ((q.how & kRZero) || (any && (q.how & kRSingle))) {
-    const float fct = (q.how & kRZero) ? 0.0f : finalize_factor(st.m, l, sink);
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((int64_t)q.t * p.num_heads + q.h) * D + 4 * h;
-#pragma unroll
-    for (int n = 0; n < D / 32; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u32x2 w;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          w[k] = (uint32_t)TT::from_f32(st.o[n][4 * i + 2 * k] * fct) |
-                 ((uint32_t)TT::from_f32(st.o[n][4 * i + 2 * k + 1] * fct) << 16);
-        *reinterpret_cast<u32x2*>(dst + 32 * n + 8 * i) = w;
-      }
-  } else if (any) {
-    const int64_t slot = u.worker + u.item;
-    if (slot < p.part_slots) {
-      const int64_t row = slot * p.slot_rows + rl;
-#pragma unroll
-      for (int n = 0; n < D / 32; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<f32x4*>(p.part_o + row * D + 32 * n + 8 * i + 4 * h) =
-              f32x4{st.o[n][4 * i], st.o[n][4 * i + 1], st.o[n][4 * i + 2], st.o[n][4 * i + 3]};
-      if (h == 0) p.part_ml[row] = float2{st.m, l};
-    }
-  }
-  __syncthreads();
+  return r_store<TT, D>(p, u, q, rl, st, sink, lane);
 }
 
-// At most 32 rows: wavefront w takes 32-key tiles w, w + 4, ...
+// At most 32 rows, by one wavefront on 32-key tiles in `mine`.
 template <typename TT, int D, bool EXTRA>
-__device__ __forceinline__ void narrow_unit(const RangedParams& p, const RUnit& u, char* lds, RScan& sh) {
+__device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUnit& u, char* mine, RInfo& q) {
   using G = RGeom<D>;
   constexpr int SIDE = 32 * G::PITCH, NI = 32 / G::RPI;
-  const int wave = uniform(threadIdx.x >> 6), lane = unit_lane();
-  const int rl = lane & 31;
-  const RInfo q = r_info(p, u, rl);
+  const int lane = unit_lane(), rl = lane & 31;
+  q = r_info(p, u, rl);
   const bool any = q.how & kRAny;
-  RState<TT, D> st;
-  r_init<TT, D>(p, q, lane, st);
-  const float sink = r_sink<TT>(p, q.h);
   RFeed f = r_feed(p, u, D);
   f.kmin = half_min(any ? q.lo : INT32_MAX);
   f.kmax = half_max(any ? q.hi : 0);
   const int flo = half_max(any ? q.lo : 0), fhi = half_min(any ? q.hi : INT32_MAX);
-  if (threadIdx.x < 32) sh.row[rl] = q;
-  char* mine = lds + wave * 2 * SIDE;
+  const float sink = r_sink<TT>(p, q.h);
+  RState<TT, D> st;
+  r_init<TT, D>(p, q, lane, st);
   if (f.kmin < f.kmax) {
-    const int te = (f.kmax + 31) / 32;
+    const int tb = f.kmin / 32, te = (f.kmax + 31) / 32;
     const uint32_t base = lds_address(mine);
-    // iteration t loads tile t + 4 and multiplies tile t (none in the first)
-    for (int t = f.kmin / 32 + wave - 4; t < te; t += 4) {
-      const bool more = t + 4 < te, have = t >= f.kmin / 32;
+    wait_lds_reads();
+    // iteration t loads tile t + 1 and multiplies tile t (none in the first)
+    for (int t = tb - 1; t < te; ++t) {
+      const bool more = t + 1 < te, have = t >= tb;
       const int t0 = t * 32;
       f32x16 s[1];
       u32x4 pr[2];
@@ -735,7 +801,7 @@ __device__ __forceinline__ void narrow_unit(const RangedParams& p, const RUnit& 
         r_scores<TT, D, 1>(st, mine, lane, s);
         wait_lds_reads();
       }
-      if (more) feed_rows<D, 32, 0, true>(p, f, t0 + 128, 0, base, lane);
+      if (more) feed_rows<D, 32, 0, true>(p, f, t0 + 32, 0, base, lane);
       if (have) {
         r_softmax<TT, D, 1, EXTRA>(p, st, s, t0, t0 < flo || t0 + 32 > fhi, lane, pr);
         if (more)
@@ -745,165 +811,136 @@ __device__ __forceinline__ void narrow_unit(const RangedParams& p, const RUnit& 
         r_values<TT, D, 1>(st, mine + SIDE, lane, pr);
         wait_lds_reads();
       }
-      if (more) feed_rows<D, 32, 1, true>(p, f, t0 + 128, 0, base + SIDE, lane);
+      if (more) feed_rows<D, 32, 1, true>(p, f, t0 + 32, 0, base + SIDE, lane);
     }
   }
-  // The four wavefronts' rows meet in LDS: O of wavefront w in its own tile's place, 16-byte pieces
-  // exchanged by the row.
-  constexpr int PC = D / 4;                      // pieces of a row
-  constexpr int PX = D == 96 ? 7 : PC - 1 < 31 ? PC - 1 : 31;
-  float* ml = reinterpret_cast<float*>(sh.row + kRNarrow);  // [wave][row][2]
-  const float l = st.l + half_swap(st.l);
-  {
-    const int h = lane >> 5;
-    f32x4* po = reinterpret_cast<f32x4*>(mine) + rl * PC;
-#pragma unroll
-    for (int n = 0; n < D / 32; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        po[(8 * n + 2 * i + h) ^ (rl & PX)] =
-            f32x4{st.o[n][4 * i], st.o[n][4 * i + 1], st.o[n][4 * i + 2], st.o[n][4 * i + 3]};
-    if (h == 0) {
-      ml[(wave * 32 + rl) * 2] = st.m;
-      ml[(wave * 32 + rl) * 2 + 1] = l;
-    }
-  }
-  __syncthreads();
-  // Eight threads per row; wavefront w holds rows 8 w .. 8 w + 7 (what it needs of them is in its lanes).
-  const int row = threadIdx.x >> 3, part = threadIdx.x & 7;
-  const int how = __shfl(q.how, row, 64);
-  const int64_t place = (int64_t)__shfl(q.t, row, 64) * p.num_heads + __shfl(q.h, row, 64);
-  const float rsink = __shfl(sink, row, 64);
-  if (how & (kRAny | kRZero)) {
-    float w[4], M = kNegInf, L = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) M = fmaxf(M, ml[(k * 32 + row) * 2]);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float mk = ml[(k * 32 + row) * 2];
-      w[k] = mk == kNegInf ? 0.0f : exp2f(mk - M);
-      // (a wavefront whose scores were all NaN has no maximum, but a sum)
-      const float lk = ml[(k * 32 + row) * 2 + 1];
-      L += lk == lk ? lk * w[k] : lk;
-    }
-    f32x4 acc[PC / 8];
-    float sum = 0.0f;
-#pragma unroll
-    for (int n = 0; n < PC / 8; ++n) {
-      acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        acc[n] += reinterpret_cast<const f32x4*>(lds + k * 2 * SIDE)[row * PC + ((8 * n + part) ^ (row & PX))] * w[k];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(acc[n][e], 0.0f, sum);
-    }
-    if ((how & kRAny) && !(sum == 0.0f && L < __builtin_huge_valf())) sh.row[row].how = how | kROdd;
-    if ((how & kRZero) || (how & kRSingle)) {
-      const float fct = (how & kRZero) ? 0.0f : finalize_factor(M, L, rsink);
-      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + place * D;
-#pragma unroll
-      for (int n = 0; n < PC / 8; ++n) {
-        u32x2 x;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          x[k] = (uint32_t)TT::from_f32(acc[n][2 * k] * fct) |
-                 ((uint32_t)TT::from_f32(acc[n][2 * k + 1] * fct) << 16);
-        *reinterpret_cast<u32x2*>(dst + 4 * (8 * n + part)) = x;
-      }
-    } else {
-      const int64_t slot = u.worker + u.item;
-      if (slot < p.part_slots) {
-        const int64_t at = slot * p.slot_rows + row;
-#pragma unroll
-        for (int n = 0; n < PC / 8; ++n)
-          *reinterpret_cast<f32x4*>(p.part_o + at * D + 4 * (8 * n + part)) = acc[n];
-        if (part == 0) p.part_ml[at] = float2{M, L};
-      }
-    }
-  }
-  __syncthreads();
+  return r_store<TT, D>(p, u, q, rl, st, sink, lane);
 }
 
-// WIDE: blocks of more than 32 rows may be among the batch's.
-// Workgroups per CU: two by LDS and registers, one at head 256.
+// WIDE: the batch may have wide items.
+// Workgroups per CU: two by LDS and registers, three at head 64, one at head 256.
 template <typename TT, int D, bool EXTRA, bool WIDE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2))) void
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : D == 64 ? 3 : 2))) void
 ranged_kernel(const RangedParams p) {
+  constexpr int kMine = 2 * 32 * RGeom<D>::PITCH;  // a wavefront's tile
   __shared__ __attribute__((aligned(1024))) char
-      lds[WIDE && RGeom<D>::WIDE > RGeom<D>::NARROW ? RGeom<D>::WIDE : RGeom<D>::NARROW];
+      lds[WIDE && RGeom<D>::WIDE > 4 * kMine ? RGeom<D>::WIDE : 4 * kMine];
   __shared__ RScan sh;
-  const int64_t me = blockIdx.x;
   const int n = p.groups + p.batch, chunks = (n + kRChunk - 1) / kRChunk;
+  const int wave = uniform(threadIdx.x >> 6);
   // Pass 0 adds up tiles and items of all sources, pass 1 walks them; both at once if one chunk has them all.
-  int64_t tiles = 0, t0 = 0, at = 0, z = 0;
-  int items = 0, i0 = 0, per = 0;
+  RTotals t{}, tb{};
+  RShare r{};
+  int me = 0, per = 0, kind = 0, at = 0, end = 0, stride = 0, turn = 0;
   for (int c = chunks > 1 ? -chunks : 0; c < chunks; ++c) {
     const int base = (c < 0 ? c + chunks : c) * kRChunk;
-    const int64_t tb = t0;
-    const int ib = i0;
-    scan_chunk(p, base, sh, t0, i0);
+    tb = t;
+    scan_chunk(p, base, sh, t);
     if (c < -1) continue;
     if (c == -1 || chunks == 1) {
-      tiles = t0;
-      items = i0;
-      // few items: their tiles in equal stretches, a workgroup each
-      if (items < 2 * p.slots) per = (int)max((tiles + p.slots - 1) / p.slots, (int64_t)p.least);
-      at = me * per;
-      z = min(at + per, tiles);
-      if (per > 0 ? at >= tiles && me > 0 : me >= items && me > 0) return;
+      r = r_share(p, t);
+      kind = (int)blockIdx.x < r.wide ? 0 : 1;
+      me = kind ? ((int)blockIdx.x - r.wide) * 4 + wave : (int)blockIdx.x;
+      per = kind ? r.per[1] : r.per[0];
+      // my stretch of tiles, or my first item
+      at = per > 0 ? me * per : me;
+      end = per > 0 ? min(at + per, pick(t.tiles, kind)) : pick(t.items, kind);
+      stride = kind ? (p.slots - r.wide) * 4 : r.wide;
+      // the sources' places, for the merge
+      if (blockIdx.x == 0 && threadIdx.x == 0) p.table[0] = RTable{{r.per[0], r.per[1], t.items[0], r.wide}};
       if (c == -1) {
-        t0 = 0;
-        i0 = 0;
+        t = RTotals{};
         continue;
       }
     }
-    if (me == 0) {  // the sources' places, for the merge
+    if (blockIdx.x == 0 && base + (int)threadIdx.x < n) {
       const RSource s = sh.src[threadIdx.x];
-      if (base + (int)threadIdx.x < n)
-        p.table[1 + base + threadIdx.x] =
-            RTable{s.first, s.item, s.tiles, s.tok0, s.rows, s.ka, s.kb, s.shared, s.group};
-      if (base == 0 && threadIdx.x == 0) p.table[0] = RTable{tiles, items, per, 0, 0, 0, 0, 0, 0};
+      p.table[1 + base + threadIdx.x] =
+          RTable{{s.first, s.item, s.tok0, s.rows, s.b0, s.b1, s.ka, s.kb, s.base, s.shared, s.group, 0}};
     }
-    // my stretch of the flat list, or item number me
-    while (per > 0 ? at >= tb && at < min(z, t0) : me >= ib && me < i0) {
-      // the last source that begins at or before the place (sources without tiles begin where the next does)
-      int lo = 0, hi = min(kRChunk, n - base);
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        const bool before = per > 0 ? sh.src[mid].first <= at : sh.src[mid].item <= (int)me;
-        if (before) lo = mid; else hi = mid;
+    // The parts of mine that this chunk's sources hold
+    for (;;) {
+      if (per > 0) {
+        if (at >= min(end, pick(t.tiles, kind))) break;
+      } else {
+        // whole items in turns; wide ones alternately up and down the list, in runs of eight (neighbours share
+        // keys, and runs keep them on their XCD)
+        bool found = false;
+        for (; turn * stride < end && !found; ++turn) {
+          const bool back = kind == 0 && (turn & 1) && (stride & 7) == 0;
+          at = turn * stride + (back ? (stride - 8 - (me & ~7)) + (me & 7) : me);
+          found = at >= pick(tb.items, kind) && at < pick(t.items, kind);
+        }
+        if (!found) {
+          turn = 0;  // (the next chunk looks from the first turn on)
+          break;
+        }
+      }
+      // its source: every lane looks at a few
+      int si = 0;
+      for (int b0 = 0; b0 < min(kRChunk, n - base); b0 += 64) {
+        const RSource& s = sh.src[b0 + (threadIdx.x & 63)];
+        const int blocks = r_blocks(s);
+        const int first = per > 0 ? s.first : s.item;
+        const int size = p.kv_heads * (per > 0 ? r_before(s, blocks, p.num_heads / p.kv_heads, r_grows(p, s)) : blocks);
+        const uint64_t hit = __ballot(b0 + (int)(threadIdx.x & 63) < n - base && r_wide(s) == (kind == 0) &&
+                                      at >= first && at - first < size);
+        if (hit) {
+          si = b0 + __builtin_ctzll(hit);
+          break;
+        }
       }
       RUnit u;
-      const RSource sl = sh.src[lo];
-      u.s = RSource{uniform64(sl.first), uniform(sl.item), uniform(sl.tok0),  uniform(sl.rows),
-                    uniform(sl.b0),      uniform(sl.b1),   uniform(sl.ka),    uniform(sl.kb),
-                    uniform(sl.tiles),   uniform(sl.shared), 0};
-      u.group = base + lo < p.groups;
-      u.per = per;
-      u.worker = me;
-      const int local = per > 0 ? (int)((uint32_t)(at - u.s.first) / (uint32_t)u.s.tiles) : (int)me - u.s.item;
-      u.item = u.s.item + local;
-      u.at = u.s.first + (int64_t)local * u.s.tiles;
-      // the last rows, which see most keys, first
-      u.kh = local % p.kv_heads;
-      u.row0 = (r_blocks(u.s.rows) - 1 - local / p.kv_heads) * kRWide;
-      u.x0 = per > 0 ? (int)(at - u.at) : 0;
-      u.x1 = per > 0 ? (int)min((int64_t)u.s.tiles, z - u.at) : u.s.tiles;
-      bool wide = false;
-      if constexpr (WIDE) wide = u.s.rows > kRNarrow;
-      if (wide)
-        wide_unit<TT, D, EXTRA>(p, u, lds, sh);
-      else
-        narrow_unit<TT, D, EXTRA>(p, u, lds, sh);
-      // rows that came out not finite, again
-      const int wave = threadIdx.x >> 6;
-      for (int k = uniform(wave); k < (wide ? kRWide : kRNarrow); k += 4) {
-        const RInfo q = sh.row[k];
-        if (uniform(q.how) & kROdd) slow_row<TT, D>(p, u, q, k);
+      const RSource sl = sh.src[si];
+      u.s = RSource{uniform(sl.first), uniform(sl.item), uniform(sl.tok0), uniform(sl.rows),
+                    uniform(sl.b0),    uniform(sl.b1),   uniform(sl.ka),   uniform(sl.kb),
+                    uniform(sl.base),  uniform(sl.shared), uniform(sl.group)};
+      u.group = u.s.group < -1;
+      const int g = p.num_heads / p.kv_heads;
+      int blk, kh;
+      if (per > 0) {
+        // the last block that begins at or before the place
+        const int rel = at - u.s.first;
+        const bool grows = r_grows(p, u.s);
+        int lo = 0, hi = r_blocks(u.s);
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (p.kv_heads * r_before(u.s, mid, g, grows) <= rel) lo = mid; else hi = mid;
+        }
+        blk = lo;
+        const int f = r_before(u.s, blk, g, grows);
+        kh = (rel - p.kv_heads * f) / (r_before(u.s, blk + 1, g, grows) - f);
+      } else {
+        blk = r_blocks(u.s) - 1 - (at - u.s.item) / p.kv_heads;  // the rows that see most keys first
+        kh = (at - u.s.item) % p.kv_heads;
       }
-      __syncthreads();  // the next unit reuses the buffers
-      if (per == 0) return;
-      at = u.at + u.x1;
+      blk = uniform(blk);
+      kh = uniform(kh);
+      const RItem it = r_item(p, u.s, blk, kh);
+      u.kh = kh;
+      u.row0 = blk * kRWide;
+      const int x0 = per > 0 ? at - it.at : 0, kt = u.s.ka / kRTile;
+      const int x1 = per > 0 ? min(it.tiles, end - it.at) : it.tiles;
+      u.head = x0 == 0;
+      u.k0 = u.head ? 0 : (kt + x0) * kRTile;
+      u.k1 = x1 == it.tiles ? INT32_MAX : (kt + x1) * kRTile;
+      u.slot = r_slot(p, kind, per > 0 ? me : it.item, it.item, u.head);
+      RInfo q;
+      uint32_t odd;
+      bool wide = false;
+      if constexpr (WIDE) wide = kind == 0;
+      if (wide)
+        odd = wide_unit<TT, D, EXTRA>(p, u, lds, sh, q);
+      else
+        odd = narrow_unit<TT, D, EXTRA>(p, u, lds + wave * kMine, q);
+      // rows that came out not finite, again
+      for (; odd; odd &= odd - 1) {
+        const int k = __builtin_ctz(odd);
+        const RInfo w{uniform(__shfl(q.t, k, 64)),  uniform(__shfl(q.h, k, 64)),  uniform(__shfl(q.pos, k, 64)),
+                      uniform(__shfl(q.lo, k, 64)), uniform(__shfl(q.hi, k, 64)), uniform(__shfl(q.how, k, 64))};
+        slow_row<TT, D>(p, u, w, (wide ? 32 * wave : 0) + k);
+      }
+      if (per > 0) at = it.at + x1;
     }
   }
 }
@@ -913,9 +950,14 @@ ranged_kernel(const RangedParams p) {
 // (token, head of the group) of a kv-head; thread k < RM finds the pieces of row k -- the workgroups from
 // the one that holds the row's first key to the one that holds its last, for the shared keys and for its
 // own -- and groups of lanes, each lane 16 bytes of the row, sum them, several pieces in flight.
+struct RPieces {
+  int n;             // pieces
+  int64_t first;     // the first one's partial row
+  int64_t next, step;  // piece k > 0: next + k * step
+};
 struct RJoin {
-  int t, h, na, nb;          // pieces of the shared and of its own keys (na + nb < 2: nothing to join)
-  int64_t ra, rb;            // the first pieces' partial rows
+  int t, h;
+  RPieces a, b;      // of the shared and of its own keys
 };
 constexpr int kRDepth = 4;
 template <typename TT, int D, int RM>
@@ -925,8 +967,8 @@ __global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p)
   __shared__ RJoin join[RM];
   __shared__ f32x4 sh_o[GPR > 1 ? NG : 1][LP];
   __shared__ float2 sh_ml[GPR > 1 ? NG : 1];
-  const int per = p.table[0].tiles;
-  if (per == 0 && p.groups == 0) return;
+  const int per0 = p.table[0].v[0], per1 = p.table[0].v[1];
+  if (per0 == 0 && per1 == 0 && p.groups == 0) return;
   const int tid = threadIdx.x, g = p.num_heads / p.kv_heads;
   const int kh = blockIdx.x % p.kv_heads;
   int b1 = 0;  // one row: its sequence, searched by the whole wavefront
@@ -935,27 +977,32 @@ __global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p)
   if (tid < RM) {
     const int64_t gr = (int64_t)(blockIdx.x / p.kv_heads) * RM + tid;
     const int t = (int)min(gr / g, (int64_t)p.num_tokens);
-    RJoin j{t, kh * g + (int)(gr % g), 0, 0, 0, 0};
+    RJoin j{t, kh * g + (int)(gr % g), RPieces{}, RPieces{}};
     if (t < p.num_tokens && t >= p.cum[0] && t < p.cum[p.batch]) {
       const int b = RM == 1 ? b1 : r_token_seq(p, 0, p.batch, t);
-      const RTable own = p.table[1 + p.groups + b];
+      auto source = [&](int i) {
+        const RTable e = p.table[1 + i];
+        return RSource{e.v[0], e.v[1], e.v[2], e.v[3], e.v[4], e.v[5], e.v[6], e.v[7], e.v[8], e.v[9], e.v[10]};
+      };
+      const RSource own = source(p.groups + b);
       const RRange r = r_range(p, t, own.kb - own.rows / g + (t - own.tok0), b, own.kb);
-      auto pieces = [&](const RTable& e, int a, int z, int64_t& row) {
-        const int rr = (t - e.tok0) * g + j.h - kh * g, blocks = r_blocks(e.rows);
-        const int blk = e.rows > kRNarrow ? rr / kRWide : 0;
-        const int local = (blocks - 1 - blk) * p.kv_heads + kh, kt = e.ka / kRTile;
-        const int64_t at = e.first + (int64_t)local * e.tiles;
-        const int64_t w0 = r_worker(per, at, e.item + local, a / kRTile - kt);
-        row = (w0 + e.item + local) * p.slot_rows + rr - blk * kRWide;
-        return (int)(r_worker(per, at, e.item + local, (z - 1) / kRTile - kt) - w0) + 1;
+      auto pieces = [&](const RSource& e, int a, int z) {
+        const int kind = r_wide(e) ? 0 : 1, per = kind ? per1 : per0;
+        const int rr = (t - e.tok0) * g + j.h - kh * g, blk = kind ? 0 : rr / kRWide, kt = e.ka / kRTile;
+        const RItem it = r_item(p, e, blk, kh);
+        const int w0 = r_worker(per, it, a / kRTile - kt), w1 = r_worker(per, it, (z - 1) / kRTile - kt);
+        const int rl = rr - blk * kRWide;
+        RPieces q;
+        q.n = w1 - w0 + 1;
+        q.first = r_slot(p, kind, w0, it.item, w0 == r_worker(per, it, 0)) + rl;
+        q.next = r_slot(p, kind, w0, it.item, false) + rl;
+        q.step = r_slot(p, kind, w0 + 1, it.item, false) + rl - q.next;
+        if (q.first >= p.part_rows || q.next + (q.n - 1) * q.step >= p.part_rows) q.n = 0;
+        return q;
       };
       const int sh_hi = min(r.hi, own.shared), own_lo = max(r.lo, own.shared);
-      if (r.lo < sh_hi) j.na = pieces(p.table[1 + own.group], r.lo, sh_hi, j.ra);
-      if (own_lo < r.hi) j.nb = pieces(own, own_lo, r.hi, j.rb);
-      const int64_t end = (int64_t)p.part_slots * p.slot_rows;
-      if (j.ra + (int64_t)(max(j.na, 1) - 1) * p.slot_rows >= end ||
-          j.rb + (int64_t)(max(j.nb, 1) - 1) * p.slot_rows >= end)
-        j.na = j.nb = 0;  // (metadata beyond its bounds)
+      if (r.lo < sh_hi) j.a = pieces(source(own.group), r.lo, sh_hi);
+      if (own_lo < r.hi) j.b = pieces(own, own_lo, r.hi);
     }
     join[tid] = j;
   }
@@ -963,7 +1010,7 @@ __global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p)
   const int grp = tid / LP, d0 = 4 * min(tid % LP, D / 4 - 1);
   for (int k = grp / GPR; k < RM; k += NG / GPR) {
     const RJoin j = join[k];
-    const int n = j.na + j.nb;
+    const int n = j.a.n + j.b.n;
     if (n < 2) continue;  // (with several groups per row: RM == 1, and every thread goes)
     float M = kNegInf, L = 0.0f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -973,7 +1020,9 @@ __global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p)
 #pragma unroll
       for (int i = 0; i < kRDepth; ++i) {
         const int x = min(i0 + i * GPR, n - 1);
-        const int64_t row = x < j.na ? j.ra + (int64_t)x * p.slot_rows : j.rb + (int64_t)(x - j.na) * p.slot_rows;
+        const RPieces& q = x < j.a.n ? j.a : j.b;
+        const int y = x < j.a.n ? x : x - j.a.n;
+        const int64_t row = y == 0 ? q.first : q.next + y * q.step;
         ml[i] = p.part_ml[row];
         o[i] = *reinterpret_cast<const f32x4*>(p.part_o + row * D + d0);
       }
@@ -1021,7 +1070,7 @@ __global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p)
 
 template <typename TT, int D>
 hipError_t launch_d(const RangedParams& p, hipStream_t s) {
-  const dim3 grid(p.grid), block(256);
+  const dim3 grid(p.slots), block(256);
   const bool extra = p.softcap > 0.0f || p.slopes;
   if (p.wide) {
     if (extra) hipLaunchKernelGGL((ranged_kernel<TT, D, true, true>), grid, block, 0, s, p);
@@ -1060,7 +1109,7 @@ bool ranged_supported(int head_dim, pa_dtype act, pa_dtype cache_dtype) {
 
 hipError_t launch_ranged(const RangedParams& p, pa_dtype act, hipStream_t s) {
   if (p.num_tokens <= 0 || p.batch <= 0) return hipSuccess;
-  if (p.grid <= 0 || p.slots <= 0 || !p.table) return hipErrorInvalidValue;
+  if (p.slots <= 0 || !p.table) return hipErrorInvalidValue;
   return act == PA_DTYPE_FLOAT16 ? launch_t<TF16>(p, s) : launch_t<TBF16>(p, s);
 }
 

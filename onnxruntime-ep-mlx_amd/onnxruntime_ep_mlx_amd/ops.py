@@ -264,16 +264,25 @@ def attention(q, k_new, v_new, key_cache, value_cache, cum, past, block_table, *
     return out
 
 
-def _same_device(ref: torch.Tensor, tensors: dict, contiguous: bool = True) -> None:
-    """Device tensors on ref's device (contiguous ones unless said otherwise); None is left out."""
-    for name, t in tensors.items():
+def _same_device(index: int, tensors: tuple, contiguous: bool = True) -> None:
+    """(name, tensor) pairs on device `index`, contiguous unless said otherwise; None is left out."""
+    for name, t in tensors:
         if t is None:
             continue
-        _need_cuda(name, t)
-        if t.device != ref.device:
-            raise ValueError(f"PagedAttention: {name} is on {t.device}, query/key on {ref.device}")
-        if contiguous:
+        if t.get_device() != index:
+            _need_cuda(name, t)
+            raise ValueError(f"PagedAttention: {name} is on {t.device}, not on cuda:{index}")
+        if contiguous and not t.is_contiguous():
             _contig(name, t)
+
+
+def _on_device(index: int, call, *args) -> int:
+    """The status of a library call on the current stream of device `index` (its last argument)."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        return call(*args, stream)
+    with torch.cuda.device(index):
+        return call(*args, stream)
 
 
 def _rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> int:
@@ -300,17 +309,15 @@ def multi_axis_rotary_append(query, key, value, key_cache, value_cache, cum, pas
     (slices of packed QKV rows, too).  Keys and values go to their pages; returns the query rows
     (``q_out`` when given, which may be ``query`` itself).  All arithmetic in float32, one rounding.
     ``query`` None: keys and values alone."""
-    lib = capi.load()
-    ref = key
     _need_cuda("key", key)
+    dev = key.get_device()
     ql = 0 if query is None else _rows("query", query, key)
     kl, vl = _rows("key", key), _rows("value", value, key)
-    _same_device(ref, {"query": query, "value": value}, contiguous=False)
-    _same_device(ref, {"key_cache": key_cache, "value_cache": value_cache, "cum": cum, "past": past,
-                       "block_table": block_table, "cos_cache": cos_cache, "sin_cache": sin_cache,
-                       "q_norm_weight": q_norm_weight, "k_norm_weight": k_norm_weight,
-                       "slot_mapping": slot_mapping, "q_out": q_out})
-    _same_device(ref, {"positions": positions}, contiguous=False)
+    _same_device(dev, (("query", query), ("value", value), ("positions", positions)), False)
+    _same_device(dev, (("key_cache", key_cache), ("value_cache", value_cache), ("cum", cum), ("past", past),
+                       ("block_table", block_table), ("cos_cache", cos_cache), ("sin_cache", sin_cache),
+                       ("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight),
+                       ("slot_mapping", slot_mapping), ("q_out", q_out)))
     sections = [int(n) for n in axis_sections]
     if not 1 <= len(sections) <= capi.PA_MAX_AXES:
         raise ValueError(f"PagedAttention: axis_sections must name 1..{capi.PA_MAX_AXES} axes")
@@ -346,71 +353,72 @@ def multi_axis_rotary_append(query, key, value, key_cache, value_cache, cum, pas
                             _ptr(cos_cache), _ptr(sin_cache), pa_dtype(cos_cache.dtype),
                             cos_cache.shape[0], cos_cache.shape[1], rotary_offset,
                             rotary_interleaved)
-    with torch.cuda.device(ref.device):
-        capi.check(lib.pa_multi_axis_rotary_append(
-            C.byref(cache), C.byref(batch), num_heads, pa_dtype(key.dtype), _ptr(query), ql,
-            _ptr(key), kl, _ptr(value), vl, C.byref(rot), _ptr(q_norm_weight),
-            _ptr(k_norm_weight), qk_norm_epsilon, _ptr(q_out), _stream(ref.device)))
+    capi.check(_on_device(
+        dev, capi.load().pa_multi_axis_rotary_append, C.byref(cache), C.byref(batch), num_heads,
+        pa_dtype(key.dtype), _ptr(query), ql, _ptr(key), kl, _ptr(value), vl, C.byref(rot),
+        _ptr(q_norm_weight), _ptr(k_norm_weight), qk_norm_epsilon, _ptr(q_out)))
     return q_out
 
 
-def _mask_desc(q, cum, num_heads, distance_slopes, prefix_lens, document_starts):
-    batch, T = cum.numel() - 1, q.shape[0]
+def _mask_desc(index, batch, T, num_heads, distance_slopes, prefix_lens, document_starts):
+    if distance_slopes is None and prefix_lens is None and document_starts is None:
+        return None
     for name, t, dt, n in (("distance_slopes", distance_slopes, torch.float32, num_heads),
                            ("prefix_lens", prefix_lens, torch.int32, batch),
                            ("document_starts", document_starts, torch.int32, T)):
         if t is not None and (t.dtype != dt or t.numel() != n):
             raise ValueError(f"PagedAttention: {name} must be {dt} with {n} elements")
-    _same_device(q, {"distance_slopes": distance_slopes, "prefix_lens": prefix_lens,
-                     "document_starts": document_starts})
-    return capi.PaMask(_ptr(distance_slopes), _ptr(prefix_lens), _ptr(document_starts))
+    _same_device(index, (("distance_slopes", distance_slopes), ("prefix_lens", prefix_lens),
+                         ("document_starts", document_starts)))
+    return C.byref(capi.PaMask(_ptr(distance_slopes), _ptr(prefix_lens), _ptr(document_starts)))
 
 
-def _masked_call(q, key_cache, value_cache, cum, past, block_table, share, *, num_heads, scale,
+def _masked_call(q, key_cache, value_cache, cum, past, block_table, share, num_heads, scale,
                  softcap, local_window_size, is_causal, head_sink, distance_slopes, prefix_lens,
                  document_starts, k_scale, v_scale, k_quant_type, v_quant_type, max_query_len,
                  max_context_len, out, workspace):
     lib = capi.load()
     _need_cuda("query", q)
-    _contig("query", q)
+    dev = q.get_device()
     if q.dim() != 2 or num_heads <= 0 or q.shape[1] % num_heads:
         raise ValueError("PagedAttention: query must be [num_tokens, num_heads * head_size]")
     if value_cache is None:
         raise ValueError("PagedAttention: masked attention takes the SEPARATE cache layout")
-    _same_device(q, {"key_cache": key_cache, "value_cache": value_cache, "cum": cum, "past": past,
-                     "block_table": block_table, "head_sink": head_sink, "out": out,
-                     "k_scale": k_scale, "v_scale": v_scale, "workspace": workspace})
-    if past.numel() != cum.numel() - 1 or block_table.dim() != 2 or block_table.shape[0] != past.numel():
+    _same_device(dev, (("query", q), ("key_cache", key_cache), ("value_cache", value_cache), ("cum", cum),
+                       ("past", past), ("block_table", block_table), ("head_sink", head_sink),
+                       ("out", out), ("k_scale", k_scale), ("v_scale", v_scale),
+                       ("workspace", workspace)))
+    T, n = q.shape[0], past.numel()
+    if n != cum.numel() - 1 or block_table.dim() != 2 or block_table.shape[0] != n:
         raise ValueError("PagedAttention: inconsistent cumulative lengths, past lengths or block table")
     if head_sink is not None and (head_sink.dtype != q.dtype or head_sink.numel() != num_heads):
         raise ValueError("PagedAttention: head_sink must be [num_heads] in the activation dtype")
-    mask = _mask_desc(q, cum, num_heads, distance_slopes, prefix_lens, document_starts)
-    cache = cache_desc(key_cache, value_cache, k_scale, v_scale, head_dim=q.shape[1] // num_heads,
-                       k_quant_type=k_quant_type, v_quant_type=v_quant_type)
-    batch = batch_desc(cum, past, block_table, q.shape[0], None, max_query_len,
-                       capi.PA_BATCH_NEW_ROWS_IN_CACHE, max_context_len)
-    attn = attn_desc(num_heads, scale, softcap, local_window_size, is_causal, head_sink)
-    act = pa_dtype(q.dtype)
     if out is None:
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("PagedAttention: out must match query's shape and dtype")
-    head = (C.byref(cache), C.byref(batch), C.byref(attn))
-    tail = (C.byref(mask), act)
-    if share is not None:
-        head += (C.byref(share),)
-        size, call = (lib.pa_shared_prefix_attention_workspace_bytes, lib.pa_shared_prefix_attention)
-    else:
+    mask = _mask_desc(dev, n, T, num_heads, distance_slopes, prefix_lens, document_starts)
+    cache = cache_desc(key_cache, value_cache, k_scale, v_scale, head_dim=q.shape[1] // num_heads,
+                       k_quant_type=k_quant_type, v_quant_type=v_quant_type)
+    batch = batch_desc(cum, past, block_table, T, None, max_query_len,
+                       capi.PA_BATCH_NEW_ROWS_IN_CACHE, max_context_len)
+    attn = attn_desc(num_heads, scale, softcap, local_window_size, is_causal, head_sink)
+    act = pa_dtype(q.dtype)
+    args = (C.byref(cache), C.byref(batch), C.byref(attn))
+    if share is None:
         size, call = lib.pa_masked_attention_workspace_bytes, lib.pa_masked_attention
-    with torch.cuda.device(q.device):
-        nbytes = size(*head, *tail)
+        args += (mask, act)
+    else:
+        size, call = (lib.pa_shared_prefix_attention_workspace_bytes, lib.pa_shared_prefix_attention)
+        args += (C.byref(share), mask, act)
+    if workspace is None:
         # A workspace of the call's own: torch's allocator keeps it apart from work on other streams
         # and in other captured graphs.
-        if workspace is None:
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        have = 0 if workspace is None else workspace.numel() * workspace.element_size()
-        capi.check(call(*head, *tail, _ptr(q), _ptr(out), _ptr(workspace), have,
-                        _stream(q.device)))
+        have = size(*args)
+        workspace = torch.empty(have, dtype=torch.uint8, device=q.device) if have else None
+    else:
+        have = workspace.numel() * workspace.element_size()
+    capi.check(_on_device(dev, call, *args, q.data_ptr(), out.data_ptr(), _ptr(workspace), have))
     return out
 
 
@@ -429,14 +437,10 @@ def masked_attention(q, key_cache, value_cache, cum, past, block_table, *, num_h
     that see no key are zero.  ``max_query_len`` / ``max_context_len`` bound every sequence's new
     tokens / past + new tokens (0 = unknown).  ``workspace``: a uint8 tensor of at least the queried
     size, for callers that keep their own."""
-    return _masked_call(q, key_cache, value_cache, cum, past, block_table, None,
-                        num_heads=num_heads, scale=scale, softcap=softcap,
-                        local_window_size=local_window_size, is_causal=is_causal,
-                        head_sink=head_sink, distance_slopes=distance_slopes,
-                        prefix_lens=prefix_lens, document_starts=document_starts,
-                        k_scale=k_scale, v_scale=v_scale, k_quant_type=k_quant_type,
-                        v_quant_type=v_quant_type, max_query_len=max_query_len,
-                        max_context_len=max_context_len, out=out, workspace=workspace)
+    return _masked_call(q, key_cache, value_cache, cum, past, block_table, None, num_heads, scale,
+                        softcap, local_window_size, is_causal, head_sink, distance_slopes,
+                        prefix_lens, document_starts, k_scale, v_scale, k_quant_type, v_quant_type,
+                        max_query_len, max_context_len, out, workspace)
 
 
 def shared_prefix_attention(q, key_cache, value_cache, cum, past, block_table, group_cum,
@@ -458,17 +462,13 @@ def shared_prefix_attention(q, key_cache, value_cache, cum, past, block_table, g
     if group_cum.numel() != shared_lens.numel() + 1:
         raise ValueError("PagedAttention: group_cum must have one element more than shared_lens")
     _need_cuda("query", q)
-    _same_device(q, {"group_cum": group_cum, "shared_lens": shared_lens})
+    _same_device(q.get_device(), (("group_cum", group_cum), ("shared_lens", shared_lens)))
     share = capi.PaSharedPrefix(_ptr(group_cum), _ptr(shared_lens), shared_lens.numel(),
                                 max_prefix_len)
-    return _masked_call(q, key_cache, value_cache, cum, past, block_table, share,
-                        num_heads=num_heads, scale=scale, softcap=softcap,
-                        local_window_size=local_window_size, is_causal=is_causal,
-                        head_sink=head_sink, distance_slopes=distance_slopes,
-                        prefix_lens=prefix_lens, document_starts=document_starts,
-                        k_scale=k_scale, v_scale=v_scale, k_quant_type=k_quant_type,
-                        v_quant_type=v_quant_type, max_query_len=max_query_len,
-                        max_context_len=max_context_len, out=out, workspace=workspace)
+    return _masked_call(q, key_cache, value_cache, cum, past, block_table, share, num_heads, scale,
+                        softcap, local_window_size, is_causal, head_sink, distance_slopes,
+                        prefix_lens, document_starts, k_scale, v_scale, k_quant_type, v_quant_type,
+                        max_query_len, max_context_len, out, workspace)
 
 
 def paged_attention(query, key, value, key_cache, value_cache, cumulative_sequence_length,
