@@ -9,7 +9,8 @@
 //
 // Work.  Sources: every group (all its rows against the shared keys, read through its first
 // sequence's table) and every sequence (its rows against the keys behind the shared ones).  An item is a
-// block of rows of one source and kv-head, its cost the 64-key tiles that the block may see.  Sources of
+// block of rows of one source and kv-head, its cost the 64-key tiles that the block may see and a few more for
+// its start and end.  Sources of
 // more than 32 rows (prompts, shared prefixes) are wide: blocks of 128 rows, a workgroup each.  The others
 // (decode) are narrow: one block, a wavefront each.  Both kinds' tiles form a flat list which is cut into
 // equal stretches, whatever item borders lie inside, over workgroups and wavefronts in proportion to the
@@ -49,6 +50,7 @@ constexpr int kRTile = 64;     // keys per unit of cost
 constexpr int kRWide = 128;    // rows of a block of four wavefronts
 constexpr int kRNarrow = 32;   // rows of a block whose wavefronts split the keys
 constexpr int kRChunk = 256;   // sources scanned at a time, one per thread
+constexpr int kRStart = 4;     // what an item's start and end cost, in tiles
 constexpr int64_t kRMergeRows = 4096;  // rows up to which the merge gives each a workgroup
 
 template <typename TT>
@@ -104,6 +106,13 @@ __device__ __forceinline__ void dma_ptr(const char* ptr, uint32_t lds) {
 template <int N>
 __device__ __forceinline__ void wait_loads() {  // until at most N vector loads are outstanding
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// A barrier that waits for nothing itself: the tile loops' loads are waited for by hand, and what was read from
+// LDS has been used.
+__device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 __device__ __forceinline__ void wait_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
@@ -170,7 +179,7 @@ __device__ __forceinline__ bool r_wide(const RSource& s) { return s.rows > kRNar
 __device__ __forceinline__ int r_blocks(const RSource& s) {
   return r_wide(s) ? (s.rows + kRWide - 1) / kRWide : s.rows > 0;
 }
-// Tiles of one kv-head before block i: all of the source's (constant), or growing with the rows' positions
+// Places of one kv-head before block i, kRStart and the tiles of each: all of the source's (constant), or growing with the rows' positions
 // under a causal mask -- base + 2 i / g each, close to what block i can see, in closed form.
 __device__ __forceinline__ int r_before(const RSource& s, int i, int g, bool grows) {
   return i * s.base + (grows ? (int)((int64_t)i * (i - 1) / g) : 0);
@@ -210,7 +219,7 @@ __device__ __forceinline__ RSource r_source(const RangedParams& p, int i) {
     if (r_grows(p, s)) end = min(end, e.past + (kRWide + g - 1) / g);  // the last position of block 0
   }
   // (an item without keys keeps a tile, whose worker writes its empty rows)
-  s.base = max((end + kRTile - 1) / kRTile - s.ka / kRTile, 1);
+  s.base = kRStart + max((end + kRTile - 1) / kRTile - s.ka / kRTile, 1);
   return s;
 }
 
@@ -288,9 +297,10 @@ __device__ __forceinline__ RShare r_share(const RangedParams& p, const RTotals& 
   r.per[1] = p.whole ? 0 : max((t.tiles[1] + waves - 1) / waves, p.least[1]);
   return r;
 }
-// One item: block blk of source s and kv-head kh, its place and tiles in the flat list.
+// One item: block blk of source s and kv-head kh, its number and places in the flat list: kRStart for its start
+// and end, then its tiles.
 struct RItem {
-  int blk, kh, item, at, tiles;
+  int blk, kh, item, at, size;
 };
 __device__ __forceinline__ RItem r_item(const RangedParams& p, const RSource& s, int blk, int kh) {
   const int g = p.num_heads / p.kv_heads;
@@ -300,13 +310,13 @@ __device__ __forceinline__ RItem r_item(const RangedParams& p, const RSource& s,
   r.kh = kh;
   r.item = s.item + blk * p.kv_heads + kh;
   const int f = r_before(s, blk, g, grows);
-  r.tiles = r_before(s, blk + 1, g, grows) - f;
-  r.at = s.first + f * p.kv_heads + kh * r.tiles;
+  r.size = r_before(s, blk + 1, g, grows) - f;
+  r.at = s.first + f * p.kv_heads + kh * r.size;
   return r;
 }
 // Worker of tile x of an item; what lies behind its counted tiles belongs to its last worker.
 __device__ __forceinline__ int r_worker(int per, const RItem& q, int x) {
-  return per > 0 ? (q.at + min(x, q.tiles - 1)) / per : q.item;
+  return per > 0 ? (q.at + min(kRStart + x, q.size - 1)) / per : q.item;
 }
 
 // The range [lo, hi) of token t at position pos of sequence b (total keys).
@@ -351,12 +361,17 @@ struct RInfo {
   int t, h, pos, lo, hi, how;
 };
 constexpr int kRAny = 1, kRSingle = 2, kRZero = 4;
-__device__ __forceinline__ RInfo r_info(const RangedParams& p, const RUnit& u, int rl) {
+__device__ __forceinline__ RInfo r_place(const RangedParams& p, const RUnit& u, int rl) {
   const int g = p.num_heads / p.kv_heads, r = u.row0 + rl;
   const bool valid = r < u.s.rows;
   RInfo q;
   q.t = u.s.tok0 + (valid ? r / g : 0);
   q.h = u.kh * g + (valid ? r % g : 0);
+  return q;
+}
+__device__ __forceinline__ void r_keys(const RangedParams& p, const RUnit& u, int rl, RInfo& q) {
+  const int g = p.num_heads / p.kv_heads;
+  const bool valid = u.row0 + rl < u.s.rows;
   int b = u.s.b0, total = u.s.kb, shared = u.s.shared;
   if (u.group) {
     b = r_token_seq(p, u.s.b0, u.s.b1, q.t);
@@ -377,7 +392,6 @@ __device__ __forceinline__ RInfo r_info(const RangedParams& p, const RUnit& u, i
     q.how = kRAny | (a >= u.k0 && z <= u.k1 && !other ? kRSingle : 0);
   }
   if (valid && !u.group && x.lo >= x.hi && u.head) q.how |= kRZero;
-  return q;
 }
 
 template <typename TT>
@@ -629,32 +643,37 @@ __device__ __forceinline__ void r_values(RState<TT, D>& st, const char* vt, int 
 }
 
 template <typename TT, int D>
-__device__ __forceinline__ void r_init(const RangedParams& p, const RInfo& q, int lane, RState<TT, D>& st) {
-  const bool any = q.how & kRAny;
+__device__ __forceinline__ void r_queries(const RangedParams& p, const RInfo& q, int lane, RState<TT, D>& st) {
   const char* src = reinterpret_cast<const char*>(p.q) + ((int64_t)q.t * p.num_heads + q.h) * D * 2 +
                     16 * (lane >> 5);
-  // a negative scale goes into the queries' signs (p.scale_log2 has its magnitude)
+  // Rows beyond the block repeat its first and are not written.  A negative scale goes into the queries'
+  // signs (p.scale_log2 has its magnitude).
 #pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks)
-    st.q[ks] = any ? (ld16(src + 32 * ks) ^ p.qxor) : u32x4{0, 0, 0, 0};
+  for (int ks = 0; ks < D / 16; ++ks) st.q[ks] = ld16(src + 32 * ks) ^ p.qxor;
+  st.slope = p.slopes ? p.slopes[q.h] * kLog2e : 0.0f;
+}
+template <typename TT, int D>
+__device__ __forceinline__ void r_init(const RInfo& q, RState<TT, D>& st) {
 #pragma unroll
   for (int n = 0; n < D / 32; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) st.o[n][i] = 0.0f;
   st.m = kNegInf;
   st.l = 0.0f;
-  st.lo = any ? q.lo : 0;
-  st.hi = any ? q.hi : 0;
+  st.lo = (q.how & kRAny) ? q.lo : 0;
+  st.hi = (q.how & kRAny) ? q.hi : 0;
   st.pos = q.pos;
-  st.slope = p.slopes ? p.slopes[q.h] * kLog2e : 0.0f;
 }
 
-__device__ __forceinline__ int half_min(int v) {  // over the 32 rows of a wavefront (both halves alike)
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-  return uniform(v);
+__device__ __forceinline__ int half_max(int v) {  // over the 32 rows of a wavefront (both halves alike)
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));   // quad_perm 1,0,3,2
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));   // quad_perm 2,3,0,1
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));  // row_half_mirror
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));  // row_mirror
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xA, 0xF, false));  // row_bcast:15
+  return __builtin_amdgcn_readlane(v, 31);
 }
-__device__ __forceinline__ int half_max(int v) { return -half_min(-v); }
+__device__ __forceinline__ int half_min(int v) { return -half_max(-v); }
 
 // The lane, hidden from the compiler once per unit: what follows from it would otherwise be computed at the
 // kernel's start for both kinds of unit, and spilled.
@@ -729,11 +748,13 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
   constexpr int KB = G::KT / 32, SIDE = G::KT * G::PITCH;
   const int wave = uniform(threadIdx.x >> 6), lane = unit_lane();
   const int rl = 32 * wave + (lane & 31);
-  q = r_info(p, u, rl);
-  const bool any = q.how & kRAny;
   RState<TT, D> st;
-  r_init<TT, D>(p, q, lane, st);
+  q = r_place(p, u, rl);
+  r_queries<TT, D>(p, q, lane, st);
   const float sink = r_sink<TT>(p, q.h);
+  r_keys(p, u, rl, q);
+  const bool any = q.how & kRAny;
+  r_init<TT, D>(q, st);
   // keys that some / every row of the wavefront sees, and some row of the workgroup
   const int wlo = half_min(any ? q.lo : INT32_MAX), whi = half_max(any ? q.hi : 0);
   const int flo = half_max(any ? q.lo : 0), fhi = half_min(any ? q.hi : INT32_MAX);
@@ -751,8 +772,8 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
     const uint32_t base = lds_address(lds);
     // iteration t loads tile t + 1 and multiplies tile t (none in the first)
     for (int t = tb - 1; t < te; ++t) {
-      wait_loads<0>();
-      __syncthreads();
+      if (t >= tb) wait_loads<0>();
+      barrier();
       if (t + 1 < te) {
         const uint32_t buf = base + ((t + 1 - tb) & 1) * 2 * SIDE;
         feed_rows<D, G::KT / 4, 0, false>(p, f, (t + 1) * G::KT, wave * (G::KT / 4), buf, lane);
@@ -777,15 +798,17 @@ __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUn
   using G = RGeom<D>;
   constexpr int SIDE = 32 * G::PITCH, NI = 32 / G::RPI;
   const int lane = unit_lane(), rl = lane & 31;
-  q = r_info(p, u, rl);
+  RState<TT, D> st;
+  q = r_place(p, u, rl);
+  r_queries<TT, D>(p, q, lane, st);
+  const float sink = r_sink<TT>(p, q.h);
+  r_keys(p, u, rl, q);
   const bool any = q.how & kRAny;
+  r_init<TT, D>(q, st);
   RFeed f = r_feed(p, u, D);
   f.kmin = half_min(any ? q.lo : INT32_MAX);
   f.kmax = half_max(any ? q.hi : 0);
   const int flo = half_max(any ? q.lo : 0), fhi = half_min(any ? q.hi : INT32_MAX);
-  const float sink = r_sink<TT>(p, q.h);
-  RState<TT, D> st;
-  r_init<TT, D>(p, q, lane, st);
   if (f.kmin < f.kmax) {
     const int tb = f.kmin / 32, te = (f.kmax + 31) / 32;
     const uint32_t base = lds_address(mine);
@@ -920,10 +943,12 @@ ranged_kernel(const RangedParams p) {
       u.kh = kh;
       u.row0 = blk * kRWide;
       const int x0 = per > 0 ? at - it.at : 0, kt = u.s.ka / kRTile;
-      const int x1 = per > 0 ? min(it.tiles, end - it.at) : it.tiles;
-      u.head = x0 == 0;
-      u.k0 = u.head ? 0 : (kt + x0) * kRTile;
-      u.k1 = x1 == it.tiles ? INT32_MAX : (kt + x1) * kRTile;
+      const int x1 = per > 0 ? min(it.size, end - it.at) : it.size;
+      if (per > 0) at = it.at + x1;
+      if (x1 <= kRStart) continue;  // (the places of its start alone)
+      u.head = x0 <= kRStart;
+      u.k0 = u.head ? 0 : (kt + x0 - kRStart) * kRTile;
+      u.k1 = x1 == it.size ? INT32_MAX : (kt + x1 - kRStart) * kRTile;
       u.slot = r_slot(p, kind, per > 0 ? me : it.item, it.item, u.head);
       RInfo q;
       uint32_t odd;
@@ -940,7 +965,6 @@ ranged_kernel(const RangedParams p) {
                       uniform(__shfl(q.lo, k, 64)), uniform(__shfl(q.hi, k, 64)), uniform(__shfl(q.how, k, 64))};
         slow_row<TT, D>(p, u, w, (wide ? 32 * wave : 0) + k);
       }
-      if (per > 0) at = it.at + x1;
     }
   }
 }
