@@ -444,6 +444,7 @@ struct RangedParams {
   int32_t batch, max_blocks, num_tokens;
   int32_t window, causal;
   float scale, scale_log2, softcap;  // scale_log2: |scale| log2(e)
+  float slope_unit;                  // slopes times this: in raw products, with a softcap in log2 units
   uint32_t qxor;                     // 0x80008000 where scale is negative
   int32_t slots;     // workgroups
   int32_t least[2];  // tiles per worker, at least (wide, narrow)

@@ -79,21 +79,39 @@ __device__ __forceinline__ u32x4 pack8(const float* x) {
   return __builtin_bit_cast(u32x4, __builtin_convertvector(v, typename TT::vec8));
 }
 
-// Direct LDS loads of 16 bytes per lane to lds + 16 * lane, as inline assembly so that the compiler's
-// memory counters do not see them and nothing waits for them but the tile loops (wait_loads).
+// Direct LDS loads of 16 bytes per lane to M0 + 16 * lane, as inline assembly so that the compiler's
+// memory counters do not see them and nothing waits for them but the tile loops (wait_loads).  The
+// immediate offset counts for both addresses.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-template <bool NT>
-__device__ __forceinline__ void dma_base(const char* base, uint32_t off, uint32_t lds) {
-  if constexpr (NT)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt"
+template <int N, bool NT>
+__device__ __forceinline__ void dma_rows(const char* base, const uint32_t* off, uint32_t lds) {
+  static_assert(N == 2 || N == 4, "two or four KiB");
+  if constexpr (N == 4 && NT)
+    asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4 nt\n\t"
+                 "global_load_lds_dwordx4 %1, %4 offset:1024 nt\n\t"
+                 "global_load_lds_dwordx4 %2, %4 offset:2048 nt\n\tglobal_load_lds_dwordx4 %3, %4 offset:3072 nt"
                  :
-                 : "v"(off), "s"(base), "s"(lds)
+                 : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(lds)
+                 : "memory", "m0");
+  else if constexpr (N == 4)
+    asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
+                 "global_load_lds_dwordx4 %1, %4 offset:1024\n\t"
+                 "global_load_lds_dwordx4 %2, %4 offset:2048\n\tglobal_load_lds_dwordx4 %3, %4 offset:3072"
+                 :
+                 : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(lds)
+                 : "memory", "m0");
+  else if constexpr (NT)
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2 nt\n\t"
+                 "global_load_lds_dwordx4 %1, %2 offset:1024 nt"
+                 :
+                 : "v"(off[0]), "v"(off[1]), "s"(base), "s"(lds)
                  : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2\n\t"
+                 "global_load_lds_dwordx4 %1, %2 offset:1024"
                  :
-                 : "v"(off), "s"(base), "s"(lds)
+                 : "v"(off[0]), "v"(off[1]), "s"(base), "s"(lds)
                  : "memory", "m0");
 }
 __device__ __forceinline__ void dma_ptr(const char* ptr, uint32_t lds) {
@@ -477,57 +495,91 @@ struct RGeom {
   __device__ static int vx(int row) { return D == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3); }
 };
 
-// Loads of rows [R0, R0 + 16 or 8 * ..) of a tile by one wavefront: where its pieces come from.
+// A wavefront's loads of tile rows: groups of GR rows (16; 8 where a wavefront has no more of a tile), each in
+// one page where pages hold a power of two of at least 16 rows.
+template <int D, int GR>
 struct RFeed {
+  using G = RGeom<D>;
+  static constexpr int NI = GR / G::RPI;          // load instructions per group and side
+  static constexpr int NB = NI < 4 ? NI : 4;      // ... per base
+  static constexpr int kBias = 1024 * (NB - 1);   // (offsets stay positive: the immediate goes up, they go down)
   const char *kc, *vc;
   const int32_t* bt;
-  int64_t rowb, hoff;  // bytes of a cache row, of the kv-head's place in it
+  uint32_t rowb;       // bytes of a cache row
+  int pages, last;     // pages of the pool, last entry of the table
   int kmin, kmax;      // keys that may be read
   int bs, sh;          // block size, its logarithm if it is a power of two of at least 16, else -1
-};
+  uint32_t ko[NI], vo[NI];
 
-// Tile rows [row0, row0 + ROWS) (row0 a multiple of ROWS, at most 32), keys t0 + row, into lds + PITCH row.  SIDE: 0 keys, 1 values.
-// NT: streamed once (nt), else kept for the other workgroups that read the same keys.
-template <int D, int ROWS, int SIDE, bool NT>
-__device__ __forceinline__ void feed_rows(const RangedParams& p, const RFeed& f, int t0, int row0,
-                                          uint32_t lds, int lane) {
-  using G = RGeom<D>;
-  constexpr int NI = ROWS / G::RPI;
-  const char* cache = SIDE ? f.vc : f.kc;
-  auto piece = [&](int row) {
-    int c = (lane % G::CPR) ^ (SIDE ? G::vx(row) : G::kx(row));
+  __device__ __forceinline__ uint32_t piece(int row, int lane, bool value) const {
+    int c = (lane % G::CPR) ^ (value ? G::vx(row) : G::kx(row));
     if (D == 96 && c >= 12) c -= 8;
-    return c;
-  };
-  const int lr = lane / G::CPR;
-  if (f.sh >= 0 && t0 + row0 >= f.kmin && t0 + row0 + ROWS <= f.kmax) {
-    // every 16 rows lie in one page
-    constexpr int GR = ROWS < 16 ? ROWS : 16;
+    return 16 * c;
+  }
+  // Group rows r0 .. (its place in the tile modulo 16) of this lane.
+  __device__ __forceinline__ void begin(const RangedParams& p, int b, int kh, int r0, int lane) {
+    bt = p.block_table + (int64_t)b * p.max_blocks;
+    rowb = (uint32_t)p.kv_heads * D * 2;
+    const int64_t hoff = (int64_t)kh * D * 2 - kBias;
+    kc = reinterpret_cast<const char*>(p.key_cache) + hoff;
+    vc = reinterpret_cast<const char*>(p.value_cache) + hoff;
+    pages = (int)p.num_blocks;
+    last = p.max_blocks - 1;
+    bs = p.block_size;
+    sh = p.bs_shift;
 #pragma unroll
-    for (int gp = 0; gp < ROWS / GR; ++gp) {
-      const int pos = uniform(t0 + row0 + gp * GR);
-      int64_t page = scalar_load(f.bt + min(pos >> f.sh, p.max_blocks - 1));
-      page = min(max(page, (int64_t)0), p.num_blocks - 1);
-      const char* base = cache + ((page << f.sh) + (pos & (f.bs - 1))) * f.rowb + f.hoff;
-#pragma unroll
-      for (int i = 0; i < GR / G::RPI; ++i) {
-        const int rl = gp * GR + i * G::RPI;
-        dma_base<NT>(base + i * G::RPI * f.rowb, (uint32_t)(lr * (int)f.rowb + 16 * piece(row0 + rl + lr)),
-                 lds + (row0 + rl) * G::PITCH);
-      }
-    }
-  } else {
-#pragma unroll 1
     for (int i = 0; i < NI; ++i) {
-      const int row = row0 + i * G::RPI + lr;
-      const int pos = min(max(t0 + row, f.kmin), f.kmax - 1);
-      int64_t page = f.bt[min(pos / f.bs, p.max_blocks - 1)];
-      page = min(max(page, (int64_t)0), p.num_blocks - 1);
-      dma_ptr(cache + (page * f.bs + pos % f.bs) * f.rowb + f.hoff + 16 * piece(row),
-              lds + (row0 + i * G::RPI) * G::PITCH);
+      const int row = i * G::RPI + lane / G::CPR;
+      ko[i] = row * rowb + piece(r0 + row, lane, false) + kBias - 1024 * (i % NB);
+      vo[i] = row * rowb + piece(r0 + row, lane, true) + kBias - 1024 * (i % NB);
     }
   }
-}
+  // Page of the group at key pos, or of the nearest group that may be read.
+  __device__ __forceinline__ int page(int pos) const {
+    const int x = min(max(pos, kmin), kmax - 1);
+    return sh >= 0 ? min(max(scalar_load(bt + min(x >> sh, last)), 0), pages - 1) : 0;
+  }
+  // Loads of one group at key pos, page pg: keys and / or values of its rows.
+  template <bool KEYS, bool VALUES, bool NT>
+  __device__ __forceinline__ void load(int pos, int pg, uint32_t kl, uint32_t vl, int r0, int lane) const {
+    if (sh >= 0 && pos >= kmin && pos + GR <= kmax) {
+      const uint64_t off = (uint64_t)(((uint32_t)pg << sh) + (uint32_t)(pos & (bs - 1))) * rowb;
+#pragma unroll
+      for (int i = 0; i < NI; i += NB) {
+        if constexpr (KEYS) dma_rows<NB, NT>(kc + off, ko + i, kl + 1024 * i);
+        if constexpr (VALUES) dma_rows<NB, NT>(vc + off, vo + i, vl + 1024 * i);
+      }
+    } else if (sh >= 0) {
+      // an edge: rows that must not be read repeat the nearest that may
+      const int x = min(max(pos, kmin), kmax - 1) & ~(GR - 1);
+      const uint64_t off = (uint64_t)(((uint32_t)pg << sh) + (uint32_t)(x & (bs - 1))) * rowb;
+#pragma unroll
+      for (int i = 0; i < NI; i += NB) {
+        uint32_t k[NB], v[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const int row = (i + j) * G::RPI + lane / G::CPR;
+          const uint32_t at = (uint32_t)(min(max(pos + row, kmin), kmax - 1) - x) * rowb + kBias - 1024 * j;
+          k[j] = at + piece(r0 + row, lane, false);
+          v[j] = at + piece(r0 + row, lane, true);
+        }
+        if constexpr (KEYS) dma_rows<NB, NT>(kc + off, k, kl + 1024 * i);
+        if constexpr (VALUES) dma_rows<NB, NT>(vc + off, v, vl + 1024 * i);
+      }
+    } else {
+      // pages of any size: lane r finds the page of row r
+      const int mine = min(max(pos + (lane & (GR - 1)), kmin), kmax - 1), bi = mine / bs;
+      const int slot = min(max(bt[min(bi, last)], 0), pages - 1) * bs + (mine - bi * bs);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int row = i * G::RPI + lane / G::CPR;
+        const uint64_t off = (uint64_t)(uint32_t)__shfl(slot, row, 64) * rowb + kBias;
+        if constexpr (KEYS) dma_ptr(kc + off + piece(r0 + row, lane, false), kl + 1024 * i);
+        if constexpr (VALUES) dma_ptr(vc + off + piece(r0 + row, lane, true), vl + 1024 * i);
+      }
+    }
+  }
+};
 
 // A wavefront's 32 rows: lane l holds row l % 32, half h = l / 32 of the keys of a tile and of the dims.
 template <typename TT, int D>
@@ -537,10 +589,17 @@ struct RState {
   float m, l;
   int lo, hi;  // keys that the row sees in this unit
   int pos;
-  float slope;  // log2 units
+  float slope;  // in units of the scores it is taken from (r_softmax)
 };
 
-// Scores of 32 KB keys at t0: raw products.
+// Order of the instructions around it: groups of LDS reads, matrix products and others, as they should issue.
+constexpr int kSchedMfma = 0x8, kSchedRead = 0x100;
+template <int MASK, int N>
+__device__ __forceinline__ void sched() {
+  __builtin_amdgcn_sched_group_barrier(MASK, N, 0);
+}
+
+// Scores of 32 KB keys: raw products.
 template <typename TT, int D, int KB>
 __device__ __forceinline__ void r_scores(const RState<TT, D>& st, const char* kt, int lane,
                                          f32x16 (&s)[KB]) {
@@ -559,25 +618,55 @@ __device__ __forceinline__ void r_scores(const RState<TT, D>& st, const char* kt
     for (int kb = 0; kb < KB; ++kb)
       s[kb] = mfma_r<TT>(*reinterpret_cast<const u32x4*>(a + kb * 32 * G::PITCH), st.q[ks], s[kb]);
   }
+  // four reads ahead of the products (the compiler alone waits for each)
+  constexpr int N = D / 16 * KB, A = 4;
+  sched<kSchedRead, A>();
+#pragma unroll
+  for (int i = 0; i < N - A; ++i) {
+    sched<kSchedMfma, 1>();
+    sched<kSchedRead, 1>();
+  }
+  sched<kSchedMfma, A>();
 }
 
-// Bias, mask, the lazy maximum and the probabilities of 32 KB keys at t0, packed per 16 keys.
-template <typename TT, int D, int KB, bool EXTRA>
+// Forms of a score: as it is, less a slope times the distance, softcapped (and less that).
+enum RForm { kRPlain = 0, kRSlope = 1, kRCap = 2 };
+
+template <typename TT>
+__device__ __forceinline__ float add_pairs(u32x4 p, float l) {  // l + the eight values of p
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = p[i];  // (a bit_cast of the element itself reads element 0)
+    if constexpr (TT::code == PA_DTYPE_FLOAT16) {
+      typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+      l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)1.0f, (_Float16)1.0f}, l, false);
+    } else {
+      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+      l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w),
+                                          __builtin_bit_cast(bf16x2, 0x3f803f80u), l, false);
+    }
+  }
+  return l;
+}
+
+// Bias, mask, the lazy maximum and the probabilities of 32 KB keys at t0, packed per 16 keys.  The row's sum takes
+// the rounded probabilities, so that both sides of the quotient err alike.
+template <typename TT, int D, int KB, int FORM>
 __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& st, f32x16 (&s)[KB],
                                           int t0, bool masked, int lane, u32x4 (&pr)[2 * KB]) {
   const int h = lane >> 5;
-  // EXTRA: scores become log2 units here; otherwise the scale enters each exponent's FMA
-  const float sl = EXTRA ? 1.0f : p.scale_log2;
-  if constexpr (EXTRA) {
-    const float ck = p.softcap > 0.0f ? fabsf(p.scale) / p.softcap : 0.0f, cl = p.softcap * kLog2e;
+  // kRCap: scores become log2 units here; otherwise the scale enters each exponent's FMA, and the slope is in
+  // units of the raw products
+  const float sl = FORM == kRCap ? 1.0f : p.scale_log2;
+  const float ck = FORM == kRCap ? fabsf(p.scale) / p.softcap : 0.0f, cl = p.softcap * kLog2e;
+  if constexpr (FORM != kRPlain) {
     const float far = (float)(st.pos - t0 - 4 * h);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float x = p.softcap > 0.0f ? softcap_log2(s[kb][i], ck, cl) : s[kb][i] * p.scale_log2;
-        x -= st.slope * fabsf(far - (float)(32 * kb + 8 * (i >> 2) + (i & 3)));
-        s[kb][i] = x;
+        const float x = FORM == kRCap ? softcap_log2(s[kb][i], ck, cl) : s[kb][i];
+        s[kb][i] = __builtin_fmaf(fabsf(far - (float)(32 * kb + 8 * (i >> 2) + (i & 3))), -st.slope, x);
       }
   }
   if (masked) {
@@ -589,11 +678,11 @@ __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& 
       for (int i = 0; i < 16; ++i)
         s[kb][i] = rel + (unsigned)(32 * kb + 8 * (i >> 2) + (i & 3)) < span ? s[kb][i] : kNegInf;
   }
-  float mx = kNegInf;
+  float mx = s[0][0];
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+    for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(s[kb][i], s[kb][i + 1]), mx);
   mx *= sl;
   mx = fmaxf(mx, half_swap(mx));
   if (__any(mx > st.m + 8.0f)) {
@@ -606,15 +695,13 @@ __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& 
   }
   const float ms = st.m == kNegInf ? 0.0f : st.m;
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb) {
-    float e[16];
+  for (int t = 0; t < 2 * KB; ++t) {
+    float e[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], sl, -ms));
-      st.l += e[i];
-    }
-    pr[2 * kb] = pack8<TT>(e);
-    pr[2 * kb + 1] = pack8<TT>(e + 8);
+    for (int i = 0; i < 8; ++i)
+      e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][8 * (t & 1) + i], sl, -ms));
+    pr[t] = pack8<TT>(e);
+    st.l = add_pairs<TT>(pr[t], st.l);
   }
 }
 
@@ -628,10 +715,10 @@ __device__ __forceinline__ void r_values(RState<TT, D>& st, const char* vt, int 
   const char* row = vt + (4 * h + (i >> 2)) * G::PITCH + 8 * (i & 1);
   const int vx = G::vx(4 * h + (i >> 2)), sub = 2 * dh + ((i & 3) >> 1);
 #pragma unroll
-  for (int n = 0; n < D / 32; ++n) {
-    const char* a = row + ((((4 * n) ^ vx) + sub) << 4);
+  for (int t = 0; t < 2 * KB; ++t) {
 #pragma unroll
-    for (int t = 0; t < 2 * KB; ++t) {
+    for (int n = 0; n < D / 32; ++n) {
+      const char* a = row + ((((4 * n) ^ vx) + sub) << 4);
       const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) s16x4*)(a + t * 16 * G::PITCH));
       const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -640,6 +727,14 @@ __device__ __forceinline__ void r_values(RState<TT, D>& st, const char* vt, int 
       st.o[n] = mfma_r<TT>(u32x4{w0[0], w0[1], w1[0], w1[1]}, pr[t], st.o[n]);
     }
   }
+  constexpr int N = 2 * KB * (D / 32), A = 4;
+  sched<kSchedRead, 2 * A>();
+#pragma unroll
+  for (int k = 0; k < N - A; ++k) {
+    sched<kSchedMfma, 1>();
+    sched<kSchedRead, 2>();
+  }
+  sched<kSchedMfma, A>();
 }
 
 template <typename TT, int D>
@@ -650,7 +745,7 @@ __device__ __forceinline__ void r_queries(const RangedParams& p, const RInfo& q,
   // signs (p.scale_log2 has its magnitude).
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) st.q[ks] = ld16(src + 32 * ks) ^ p.qxor;
-  st.slope = p.slopes ? p.slopes[q.h] * kLog2e : 0.0f;
+  st.slope = p.slopes ? p.slopes[q.h] * p.slope_unit : 0.0f;
 }
 template <typename TT, int D>
 __device__ __forceinline__ void r_init(const RInfo& q, RState<TT, D>& st) {
@@ -681,19 +776,6 @@ __device__ __forceinline__ int unit_lane() {
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));
   return lane;
-}
-
-__device__ __forceinline__ RFeed r_feed(const RangedParams& p, const RUnit& u, int D) {
-  RFeed f;
-  f.kc = reinterpret_cast<const char*>(p.key_cache);
-  f.vc = reinterpret_cast<const char*>(p.value_cache);
-  f.bt = p.block_table + (int64_t)u.s.b0 * p.max_blocks;
-  f.rowb = (int64_t)p.kv_heads * D * 2;
-  f.hoff = (int64_t)u.kh * D * 2;
-  f.kmin = f.kmax = 0;
-  f.bs = p.block_size;
-  f.sh = p.bs_shift;
-  return f;
 }
 
 // ------------------------------------------------------------------------------------ a unit
@@ -741,7 +823,7 @@ __device__ __forceinline__ uint32_t r_store(const RangedParams& p, const RUnit& 
 }
 
 // A block of 128 rows, by the whole workgroup: wavefront w takes rows 32 w .. 32 w + 31 of every tile.
-template <typename TT, int D, bool EXTRA>
+template <typename TT, int D, int FORM>
 __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit& u, char* lds, RScan& sh,
                                               RInfo& q) {
   using G = RGeom<D>;
@@ -764,20 +846,24 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
     sh.red[2 * wave + 1] = whi;
   }
   __syncthreads();
-  RFeed f = r_feed(p, u, D);
+  constexpr int GR = G::KT / 4;  // a wavefront's rows of a tile
+  RFeed<D, GR> f;
+  f.begin(p, u.s.b0, u.kh, wave * GR & 15, lane);
   f.kmin = uniform(min(min(sh.red[0], sh.red[2]), min(sh.red[4], sh.red[6])));
   f.kmax = uniform(max(max(sh.red[1], sh.red[3]), max(sh.red[5], sh.red[7])));
   if (f.kmin < f.kmax) {
     const int tb = f.kmin / G::KT, te = (f.kmax + G::KT - 1) / G::KT;
-    const uint32_t base = lds_address(lds);
+    const uint32_t base = lds_address(lds) + wave * GR * G::PITCH;
+    int pg = f.page(tb * G::KT + wave * GR);  // of the tile to be loaded next
     // iteration t loads tile t + 1 and multiplies tile t (none in the first)
     for (int t = tb - 1; t < te; ++t) {
       if (t >= tb) wait_loads<0>();
       barrier();
       if (t + 1 < te) {
         const uint32_t buf = base + ((t + 1 - tb) & 1) * 2 * SIDE;
-        feed_rows<D, G::KT / 4, 0, false>(p, f, (t + 1) * G::KT, wave * (G::KT / 4), buf, lane);
-        feed_rows<D, G::KT / 4, 1, false>(p, f, (t + 1) * G::KT, wave * (G::KT / 4), buf + SIDE, lane);
+        const int pos = (t + 1) * G::KT + wave * GR;
+        f.template load<true, true, false>(pos, pg, buf, buf + SIDE, wave * GR & 15, lane);
+        pg = f.page(pos + G::KT);
       }
       const int t0 = t * G::KT;
       if (t < tb || t0 >= whi || t0 + G::KT <= wlo) continue;
@@ -785,7 +871,7 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
       f32x16 s[KB];
       u32x4 pr[2 * KB];
       r_scores<TT, D, KB>(st, buf, lane, s);
-      r_softmax<TT, D, KB, EXTRA>(p, st, s, t0, t0 < flo || t0 + G::KT > fhi, lane, pr);
+      r_softmax<TT, D, KB, FORM>(p, st, s, t0, t0 < flo || t0 + G::KT > fhi, lane, pr);
       r_values<TT, D, KB>(st, buf + SIDE, lane, pr);
     }
   }
@@ -793,7 +879,7 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
 }
 
 // At most 32 rows, by one wavefront on 32-key tiles in `mine`.
-template <typename TT, int D, bool EXTRA>
+template <typename TT, int D, int FORM>
 __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUnit& u, char* mine, RInfo& q) {
   using G = RGeom<D>;
   constexpr int SIDE = 32 * G::PITCH, NI = 32 / G::RPI;
@@ -805,7 +891,8 @@ __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUn
   r_keys(p, u, rl, q);
   const bool any = q.how & kRAny;
   r_init<TT, D>(q, st);
-  RFeed f = r_feed(p, u, D);
+  RFeed<D, 16> f;
+  f.begin(p, u.s.b0, u.kh, 0, lane);
   f.kmin = half_min(any ? q.lo : INT32_MAX);
   f.kmax = half_max(any ? q.hi : 0);
   const int flo = half_max(any ? q.lo : 0), fhi = half_min(any ? q.hi : INT32_MAX);
@@ -813,6 +900,8 @@ __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUn
     const int tb = f.kmin / 32, te = (f.kmax + 31) / 32;
     const uint32_t base = lds_address(mine);
     wait_lds_reads();
+    int p0 = f.page(tb * 32), p1 = f.page(tb * 32 + 16);  // pages of the tile to be loaded next
+    constexpr int HALF = 16 * G::PITCH;
     // iteration t loads tile t + 1 and multiplies tile t (none in the first)
     for (int t = tb - 1; t < te; ++t) {
       const bool more = t + 1 < te, have = t >= tb;
@@ -824,9 +913,12 @@ __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUn
         r_scores<TT, D, 1>(st, mine, lane, s);
         wait_lds_reads();
       }
-      if (more) feed_rows<D, 32, 0, true>(p, f, t0 + 32, 0, base, lane);
+      if (more) {
+        f.template load<true, false, true>(t0 + 32, p0, base, 0, 0, lane);
+        f.template load<true, false, true>(t0 + 48, p1, base + HALF, 0, 0, lane);
+      }
       if (have) {
-        r_softmax<TT, D, 1, EXTRA>(p, st, s, t0, t0 < flo || t0 + 32 > fhi, lane, pr);
+        r_softmax<TT, D, 1, FORM>(p, st, s, t0, t0 < flo || t0 + 32 > fhi, lane, pr);
         if (more)
           wait_loads<NI>();
         else
@@ -834,7 +926,12 @@ __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUn
         r_values<TT, D, 1>(st, mine + SIDE, lane, pr);
         wait_lds_reads();
       }
-      if (more) feed_rows<D, 32, 1, true>(p, f, t0 + 32, 0, base + SIDE, lane);
+      if (more) {
+        f.template load<false, true, true>(t0 + 32, p0, 0, base + SIDE, 0, lane);
+        f.template load<false, true, true>(t0 + 48, p1, 0, base + SIDE + HALF, 0, lane);
+        p0 = f.page(t0 + 64);
+        p1 = f.page(t0 + 80);
+      }
     }
   }
   return r_store<TT, D>(p, u, q, rl, st, sink, lane);
@@ -842,7 +939,7 @@ __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUn
 
 // WIDE: the batch may have wide items.
 // Workgroups per CU: two by LDS and registers, three at head 64, one at head 256.
-template <typename TT, int D, bool EXTRA, bool WIDE>
+template <typename TT, int D, int FORM, bool WIDE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : D == 64 ? 3 : 2))) void
 ranged_kernel(const RangedParams p) {
   constexpr int kMine = 2 * 32 * RGeom<D>::PITCH;  // a wavefront's tile
@@ -955,9 +1052,9 @@ ranged_kernel(const RangedParams p) {
       bool wide = false;
       if constexpr (WIDE) wide = kind == 0;
       if (wide)
-        odd = wide_unit<TT, D, EXTRA>(p, u, lds, sh, q);
+        odd = wide_unit<TT, D, FORM>(p, u, lds, sh, q);
       else
-        odd = narrow_unit<TT, D, EXTRA>(p, u, lds + wave * kMine, q);
+        odd = narrow_unit<TT, D, FORM>(p, u, lds + wave * kMine, q);
       // rows that came out not finite, again
       for (; odd; odd &= odd - 1) {
         const int k = __builtin_ctz(odd);
@@ -1095,13 +1192,15 @@ __global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p)
 template <typename TT, int D>
 hipError_t launch_d(const RangedParams& p, hipStream_t s) {
   const dim3 grid(p.slots), block(256);
-  const bool extra = p.softcap > 0.0f || p.slopes;
+  const int form = p.softcap > 0.0f ? kRCap : p.slopes ? kRSlope : kRPlain;
   if (p.wide) {
-    if (extra) hipLaunchKernelGGL((ranged_kernel<TT, D, true, true>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((ranged_kernel<TT, D, false, true>), grid, block, 0, s, p);
+    if (form == kRCap) hipLaunchKernelGGL((ranged_kernel<TT, D, kRCap, true>), grid, block, 0, s, p);
+    else if (form == kRSlope) hipLaunchKernelGGL((ranged_kernel<TT, D, kRSlope, true>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((ranged_kernel<TT, D, kRPlain, true>), grid, block, 0, s, p);
   } else {
-    if (extra) hipLaunchKernelGGL((ranged_kernel<TT, D, true, false>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((ranged_kernel<TT, D, false, false>), grid, block, 0, s, p);
+    if (form == kRCap) hipLaunchKernelGGL((ranged_kernel<TT, D, kRCap, false>), grid, block, 0, s, p);
+    else if (form == kRSlope) hipLaunchKernelGGL((ranged_kernel<TT, D, kRSlope, false>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((ranged_kernel<TT, D, kRPlain, false>), grid, block, 0, s, p);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.merge) return e;
