@@ -1276,7 +1276,7 @@ RunOpts masked_opts(const pa_mask* mask) {
 // Launch shape and workspace of the matrix-core kernel over key ranges (pa_ranged.hip).
 struct RangedPlan {
   bool on = false, whole = false, merge = false, wide = false;
-  int slots = 0, narrow_rows = 0;
+  int slots = 0, per_cu = 0, narrow_rows = 0;
   int64_t part_rows = 0, part_narrow = 0;
   size_t o_bytes = 0, ml_bytes = 0, table_bytes = 0;
   size_t bytes() const { return o_bytes + ml_bytes + table_bytes; }
@@ -1306,15 +1306,15 @@ RangedPlan ranged_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a,
     return r;
   r.on = true;
   r.wide = wide > 0;
-  const int per_cu = c->head_dim > 128 ? 1 : c->head_dim == 64 ? 3 : 2;
+  r.per_cu = c->head_dim > 128 ? 1 : c->head_dim == 64 ? 3 : 2;
   r.whole = ctx <= kRangedWhole && groups == 0;
   r.merge = !r.whole;
   // no more workgroups than there are tiles for
   const int64_t most = wide * ((ctx + 63) / 64 + 1) + (narrow * ((ctx + 63) / 64 + 1) + 3) / 4;
-  r.slots = (int)std::max<int64_t>(std::min<int64_t>((int64_t)per_cu * device_cus(), most), 2);
+  r.slots = (int)std::max<int64_t>(std::min<int64_t>((int64_t)r.per_cu * device_cus(), most), 2);
   r.narrow_rows = (int)std::min<int64_t>(groups ? 32 : mq * g, 32);
   if (r.merge) {
-    r.part_narrow = 128 * (wide == 0 ? 0 : groups ? std::max(r.slots + std::min(wide, 4 * (int64_t)r.slots), 2 * wide)
+    r.part_narrow = 128 * (wide == 0 ? 0 : groups ? wide + std::max<int64_t>(r.slots, wide)
                                                   : 2 * (int64_t)r.slots);
     r.part_rows = r.part_narrow +
                   (int64_t)r.narrow_rows * (groups ? 4 * r.slots + narrow : 8 * (int64_t)r.slots);
@@ -1397,6 +1397,7 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
   p.slope_unit = a->softcap > 0.0f ? pa::kLog2e : 1.0f / std::fabs(p.scale);
   p.qxor = p.scale < 0.0f ? 0x80008000u : 0u;
   p.slots = r.slots;
+  p.per_cu = r.per_cu;
   p.least[0] = 4;
   p.least[1] = 3;
   p.whole = r.whole ? 1 : 0;

@@ -447,6 +447,7 @@ struct RangedParams {
   float slope_unit;                  // slopes times this: in raw products, with a softcap in log2 units
   uint32_t qxor;                     // 0x80008000 where scale is negative
   int32_t slots;     // workgroups
+  int32_t per_cu;    // ... that a CU holds at once
   int32_t least[2];  // tiles per worker, at least (wide, narrow)
   int32_t whole;     // every item whole (short contexts)
   int32_t merge;     // some row may have several pieces

@@ -14,7 +14,7 @@
 // more than 32 rows (prompts, shared prefixes) are wide: blocks of 128 rows, a workgroup each.  The others
 // (decode) are narrow: one block, a wavefront each.  Both kinds' tiles form a flat list which is cut into
 // equal stretches, whatever item borders lie inside, over workgroups and wavefronts in proportion to the
-// tiles: an item that meets several workers leaves (m, l, O) of each in fp32 and ranged_merge_kernel joins
+// tiles: an item that meets several workers leaves (m, l, O) of each in fp32 and the merge joins
 // them, as it joins a row's shared and own keys.  Where wide items are many, workgroups take whole ones in
 // turns, longest first, every other turn backwards.  The plan is a scan over the lengths that every
 // workgroup makes for itself, from the device's metadata.
@@ -50,8 +50,16 @@ constexpr int kRTile = 64;     // keys per unit of cost
 constexpr int kRWide = 128;    // rows of a block of four wavefronts
 constexpr int kRNarrow = 32;   // rows of a block whose wavefronts split the keys
 constexpr int kRChunk = 256;   // sources scanned at a time, one per thread
-constexpr int kRStart = 4;     // what an item's start and end cost, in tiles
-constexpr int64_t kRMergeRows = 4096;  // rows up to which the merge gives each a workgroup
+// What an item's start and end cost, in tiles (8 instead: 64 samples of a prompt 53 us for 49).
+constexpr int kRStart = 4;
+// What partial rows and their merge cost, in tiles of every worker: 3, 8 and 20 gave 640, 641 and 556 us over a
+// prompt of 8192, 244, 210 and 210 over prompts of 1001 - 2500 at head 64; at 20, 36 us for systems' prompts as at 3.
+constexpr float kRCut = 20.0f;
+// Time of a tile where a workgroup has its CU to itself (1.0 instead: a prompt of 1024 44.6 us for 41.7).
+constexpr float kRAlone = 0.65f;
+// Rows up to which the merge gives each a workgroup, a wavefront; workgroups of the merge of more.
+constexpr int64_t kRJoinWide = 1024, kRJoinRows = 16384;
+constexpr int kRMergeGrid = 2048;
 
 template <typename TT>
 __device__ __forceinline__ f32x16 mfma_r(u32x4 a, u32x4 b, f32x16 c) {
@@ -77,6 +85,20 @@ __device__ __forceinline__ u32x4 pack8(const float* x) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = x[i];
   return __builtin_bit_cast(u32x4, __builtin_convertvector(v, typename TT::vec8));
+}
+template <typename TT>
+__device__ __forceinline__ u32x2 pack4(float a, float b, float c, float d) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef decltype(__builtin_shufflevector(typename TT::vec8{}, typename TT::vec8{}, 0, 1)) vec2;
+  return u32x2{__builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, vec2)),
+               __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{c, d}, vec2))};
+}
+
+// x, hidden from the compiler: what follows from it would otherwise be computed at the kernel's start for every path
+// there is, and keep registers there that the tile loops need.
+__device__ __forceinline__ int hidden(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 // Direct LDS loads of 16 bytes per lane to M0 + 16 * lane, as inline assembly so that the compiler's
@@ -137,6 +159,18 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(lds_char*)p;
 }
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// Maximum of v over lanes 0 .. 31 in lane 31, over lanes 32 .. 63 in lane 63.
+__device__ __forceinline__ int half_top(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));   // quad_perm 1,0,3,2
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));   // quad_perm 2,3,0,1
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));  // row_half_mirror
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));  // row_mirror
+  return max(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xA, 0xF, false));  // row_bcast:15
+}
+// Over the 32 rows of a wavefront (both halves alike).
+__device__ __forceinline__ int half_max(int v) { return __builtin_amdgcn_readlane(half_top(v), 31); }
+__device__ __forceinline__ int half_min(int v) { return -half_max(-v); }
+
 // A table entry at a wave-uniform place, through the scalar cache (no kernel writes the tables).
 __device__ __forceinline__ int scalar_load(const int32_t* p) {
   typedef const __attribute__((address_space(4))) int32_t* cptr;
@@ -247,9 +281,11 @@ struct RScan {
   RSource src[kRChunk];
   int64_t wt[4][2];
   int red[8];
+  int most[4];
 };
 struct RTotals {
   int tiles[2], items[2];  // wide, narrow
+  int most;                // places of the largest wide item
 };
 __device__ __forceinline__ int pick(const int (&x)[2], int kind) { return kind ? x[1] : x[0]; }
 __device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
@@ -263,11 +299,14 @@ __device__ __forceinline__ int64_t scan64(int64_t v, int lane) {
 // Sources base .. base + 255 with their places in the flat lists into sh.src; t: tiles and items before
 // them, moved past them.  Called by all 256 threads.
 __device__ __forceinline__ void scan_chunk(const RangedParams& p, int base, RScan& sh, RTotals& t) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = hidden(threadIdx.x), lane = tid & 63, wave = tid >> 6;
   RSource s = r_source(p, base + tid);
-  const int blocks = r_blocks(s), kind = r_wide(s) ? 0 : 1;
+  const int blocks = r_blocks(s), kind = r_wide(s) ? 0 : 1, g = p.num_heads / p.kv_heads;
+  const bool grows = r_grows(p, s);
+  const int largest = kind ? 0 : r_before(s, blocks, g, grows) - r_before(s, blocks - 1, g, grows);
   const int64_t mine = ((int64_t)(blocks * p.kv_heads) << kRItemShift) +
-                       (int64_t)p.kv_heads * r_before(s, blocks, p.num_heads / p.kv_heads, r_grows(p, s));
+                       (int64_t)p.kv_heads * r_before(s, blocks, g, grows);
+  const int top = max(half_max(largest), __builtin_amdgcn_readlane(half_top(largest), 63));
   int64_t before[2], all[2] = {0, 0};
 #pragma unroll
   for (int k = 0; k < 2; ++k) before[k] = scan64(kind == k ? mine : 0, lane);
@@ -275,6 +314,7 @@ __device__ __forceinline__ void scan_chunk(const RangedParams& p, int base, RSca
   if (lane == 63) {
     sh.wt[wave][0] = before[0];
     sh.wt[wave][1] = before[1];
+    sh.most[wave] = top;
   }
   __syncthreads();
 #pragma unroll
@@ -296,6 +336,7 @@ __device__ __forceinline__ void scan_chunk(const RangedParams& p, int base, RSca
     t.tiles[k] += uniform((int)(all[k] & low));
     t.items[k] += uniform((int)(all[k] >> kRItemShift));
   }
+  t.most = uniform(max(t.most, max(max(sh.most[0], sh.most[1]), max(sh.most[2], sh.most[3]))));
   __syncthreads();
 }
 // Who takes what: workgroups [0, wide) the wide items, the wavefronts of the others the narrow ones; tiles
@@ -311,8 +352,21 @@ __device__ __forceinline__ RShare r_share(const RangedParams& p, const RTotals& 
                ? p.slots
                : min(max((int)((float)p.slots * ((float)t.tiles[0] / (float)all)), 1), p.slots - 1);
   const int waves = max((p.slots - r.wide) * 4, 1);
-  r.per[0] = p.whole || t.items[0] >= 4 * r.wide ? 0 : max((t.tiles[0] + r.wide - 1) / max(r.wide, 1), p.least[0]);
-  r.per[1] = p.whole ? 0 : max((t.tiles[1] + waves - 1) / waves, p.least[1]);
+  // Whole wide items, or equal stretches of their tiles.  Whole, a worker takes the largest item, or its share
+  // of all in turns: items of equal cost as many as there are turns, of evenly spread costs little over an even
+  // share; an item that has its CU to itself runs faster.  Stretches take an even share and what the partial rows
+  // and their merge cost (kRCut tiles; little where shared prefixes leave them anyway).  Documents hide what items
+  // cost, and go whole.
+  const float even = (float)t.tiles[0] / (float)max(r.wide, 1), avg = (float)t.tiles[0] / (float)max(t.items[0], 1);
+  const int turns = (t.items[0] + r.wide - 1) / max(r.wide, 1);
+  const float spread = fminf(fmaxf((float)t.most / fmaxf(avg, 1.0f) - 1.0f, 0.0f), 1.0f);
+  const float whole =
+      turns <= 1 ? t.most * (2 * t.items[0] <= r.wide && p.per_cu > 1 ? kRAlone : 1.0f)
+                 : fmaxf((float)t.most, avg * turns * (1.0f - spread) + 1.05f * even * spread);
+  const bool take = p.whole || (p.doc_starts && 2 * t.items[0] >= r.wide) ||
+                    whole <= even + (p.groups ? 0.25f : 1.0f) * kRCut;
+  r.per[0] = take || t.items[0] == 0 ? 0 : max((t.tiles[0] + r.wide - 1) / max(r.wide, 1), p.least[0]);
+  r.per[1] = p.whole || t.items[1] == 0 ? 0 : max((t.tiles[1] + waves - 1) / waves, p.least[1]);
   return r;
 }
 // One item: block blk of source s and kv-head kh, its number and places in the flat list: kRStart for its start
@@ -430,7 +484,7 @@ __device__ __forceinline__ int64_t r_offset(const RangedParams& p, int b, int kh
 template <typename TT, int D>
 __device__ __forceinline__ void slow_row(const RangedParams& p, const RUnit& u, const RInfo& q, int rl) {
   constexpr int NE = (D + 63) / 64;
-  const int lane = threadIdx.x & 63;
+  const int lane = hidden(threadIdx.x & 63);
   using raw = typename TT::raw;
   float qv[NE], o[NE], m = kNegInf, l = 0.0f;
   const float slope = p.slopes ? p.slopes[q.h] : 0.0f;
@@ -487,8 +541,10 @@ struct RGeom {
   static constexpr int PITCH = D == 96 ? 256 : 2 * D;
   static constexpr int CPR = PITCH / 16;     // pieces per row
   static constexpr int RPI = 64 / CPR;       // rows per load instruction
-  static constexpr int KT = D > 128 ? 32 : 64;  // keys of a wide tile
-  static constexpr int WIDE = 2 * 2 * KT * PITCH;     // two buffers of keys and values
+  // Keys of a wide tile, two of which are buffered.  (Tiles of 32 keys, four deep: 626 us for 554 over a prompt of
+  // 8192 at head 128; four deep at head 256 664 for 647: what is loaded a tile ahead is there in time.)
+  static constexpr int KT = D > 128 ? 32 : 64;
+  static constexpr int WIDE = 2 * 2 * KT * PITCH;
   static constexpr int NARROW = 4 * 2 * 32 * PITCH;   // four wavefronts' tiles of 32 keys
   static constexpr int LDS = WIDE > NARROW ? WIDE : NARROW;
   __device__ static int kx(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
@@ -541,7 +597,7 @@ struct RFeed {
   }
   // Loads of one group at key pos, page pg: keys and / or values of its rows.
   template <bool KEYS, bool VALUES, bool NT>
-  __device__ __forceinline__ void load(int pos, int pg, uint32_t kl, uint32_t vl, int r0, int lane) const {
+  __device__ __forceinline__ void load(int pos, int pg, uint32_t kl, uint32_t vl, int r0, int lane0) const {
     if (sh >= 0 && pos >= kmin && pos + GR <= kmax) {
       const uint64_t off = (uint64_t)(((uint32_t)pg << sh) + (uint32_t)(pos & (bs - 1))) * rowb;
 #pragma unroll
@@ -551,6 +607,7 @@ struct RFeed {
       }
     } else if (sh >= 0) {
       // an edge: rows that must not be read repeat the nearest that may
+      const int lane = hidden(lane0);
       const int x = min(max(pos, kmin), kmax - 1) & ~(GR - 1);
       const uint64_t off = (uint64_t)(((uint32_t)pg << sh) + (uint32_t)(x & (bs - 1))) * rowb;
 #pragma unroll
@@ -568,6 +625,7 @@ struct RFeed {
       }
     } else {
       // pages of any size: lane r finds the page of row r
+      const int lane = hidden(lane0);
       const int mine = min(max(pos + (lane & (GR - 1)), kmin), kmax - 1), bi = mine / bs;
       const int slot = min(max(bt[min(bi, last)], 0), pages - 1) * bs + (mine - bi * bs);
 #pragma unroll
@@ -592,18 +650,18 @@ struct RState {
   float slope;  // in units of the scores it is taken from (r_softmax)
 };
 
-// Order of the instructions around it: groups of LDS reads, matrix products and others, as they should issue.
-constexpr int kSchedMfma = 0x8, kSchedRead = 0x100;
-template <int MASK, int N>
-__device__ __forceinline__ void sched() {
-  __builtin_amdgcn_sched_group_barrier(MASK, N, 0);
-}
+// Matrix products run in groups, whose operands are read from LDS while the group before multiplies: reads and
+// products keep their order (the compiler alone reuses one operand's registers and waits for every read), vector
+// and scalar instructions may move.
+__device__ __forceinline__ void r_order() { __builtin_amdgcn_sched_barrier(0x0406); }
 
 // Scores of 32 KB keys: raw products.
 template <typename TT, int D, int KB>
 __device__ __forceinline__ void r_scores(const RState<TT, D>& st, const char* kt, int lane,
                                          f32x16 (&s)[KB]) {
   using G = RGeom<D>;
+  constexpr int N = D / 16 * KB, A = N % 4 ? 3 : 4;  // products, of a group
+  static_assert(N % A == 0, "whole groups");
   const int c = lane & 31, h = lane >> 5;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
@@ -611,22 +669,23 @@ __device__ __forceinline__ void r_scores(const RState<TT, D>& st, const char* kt
     for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
   const char* row = kt + c * G::PITCH;
   const int x = G::kx(c) ^ h;
+  u32x4 k[2][A];
+  auto read = [&](int g) {
 #pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) {
-    const char* a = row + (((2 * ks) ^ x) << 4);
+    for (int i = 0; i < A; ++i) {
+      const int ks = (g * A + i) / KB, kb = (g * A + i) % KB;
+      k[g & 1][i] = *reinterpret_cast<const u32x4*>(row + (((2 * ks) ^ x) << 4) + kb * 32 * G::PITCH);
+    }
+  };
+  read(0);
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-      s[kb] = mfma_r<TT>(*reinterpret_cast<const u32x4*>(a + kb * 32 * G::PITCH), st.q[ks], s[kb]);
+  for (int g = 0; g < N / A; ++g) {
+    if (g + 1 < N / A) read(g + 1);
+    r_order();
+#pragma unroll
+    for (int i = 0; i < A; ++i) s[(g * A + i) % KB] = mfma_r<TT>(k[g & 1][i], st.q[(g * A + i) / KB], s[(g * A + i) % KB]);
+    r_order();
   }
-  // four reads ahead of the products (the compiler alone waits for each)
-  constexpr int N = D / 16 * KB, A = 4;
-  sched<kSchedRead, A>();
-#pragma unroll
-  for (int i = 0; i < N - A; ++i) {
-    sched<kSchedMfma, 1>();
-    sched<kSchedRead, 1>();
-  }
-  sched<kSchedMfma, A>();
 }
 
 // Forms of a score: as it is, less a slope times the distance, softcapped (and less that).
@@ -707,35 +766,48 @@ __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& 
 
 // O^T += V^T P^T over 32 KB keys.
 template <typename TT, int D, int KB>
-__device__ __forceinline__ void r_values(RState<TT, D>& st, const char* vt, int lane,
-                                         const u32x4 (&pr)[2 * KB]) {
+struct RValues {
   using G = RGeom<D>;
-  const int h = lane >> 5, dh = (lane >> 4) & 1, i = lane & 15;
-  // rows 4 h + i / 4 (+ 8) of each 16 keys, dims 32 n + 16 dh + 4 (i % 4) .. + 3
-  const char* row = vt + (4 * h + (i >> 2)) * G::PITCH + 8 * (i & 1);
-  const int vx = G::vx(4 * h + (i >> 2)), sub = 2 * dh + ((i & 3) >> 1);
+  static constexpr int NB = D / 32, N = 2 * KB * NB, A = NB == 3 ? 3 : 4;  // products, of a group
+  static_assert(N % A == 0, "whole groups");
+  const char* row;
+  int vx, sub;
+  u32x4 v[2][A];
+  __device__ __forceinline__ void read(int g) {
 #pragma unroll
-  for (int t = 0; t < 2 * KB; ++t) {
-#pragma unroll
-    for (int n = 0; n < D / 32; ++n) {
+    for (int k = 0; k < A; ++k) {
+      const int t = (g * A + k) / NB, n = (g * A + k) % NB;
       const char* a = row + ((((4 * n) ^ vx) + sub) << 4);
       const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) s16x4*)(a + t * 16 * G::PITCH));
       const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) s16x4*)(a + (t * 16 + 8) * G::PITCH));
       const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
-      st.o[n] = mfma_r<TT>(u32x4{w0[0], w0[1], w1[0], w1[1]}, pr[t], st.o[n]);
+      v[g & 1][k] = u32x4{w0[0], w0[1], w1[0], w1[1]};
     }
   }
-  constexpr int N = 2 * KB * (D / 32), A = 4;
-  sched<kSchedRead, 2 * A>();
-#pragma unroll
-  for (int k = 0; k < N - A; ++k) {
-    sched<kSchedMfma, 1>();
-    sched<kSchedRead, 2>();
+  // Reads the first group.
+  __device__ __forceinline__ RValues(const char* vt, int lane) {
+    const int h = lane >> 5, dh = (lane >> 4) & 1, i = lane & 15;
+    // rows 4 h + i / 4 (+ 8) of each 16 keys, dims 32 n + 16 dh + 4 (i % 4) .. + 3
+    row = vt + (4 * h + (i >> 2)) * G::PITCH + 8 * (i & 1);
+    vx = G::vx(4 * h + (i >> 2));
+    sub = 2 * dh + ((i & 3) >> 1);
+    read(0);
+    r_order();
   }
-  sched<kSchedMfma, A>();
-}
+  __device__ __forceinline__ void multiply(RState<TT, D>& st, const u32x4 (&pr)[2 * KB]) {
+#pragma unroll
+    for (int g = 0; g < N / A; ++g) {
+      if (g + 1 < N / A) read(g + 1);
+      r_order();
+#pragma unroll
+      for (int k = 0; k < A; ++k)
+        st.o[(g * A + k) % NB] = mfma_r<TT>(v[g & 1][k], pr[(g * A + k) / NB], st.o[(g * A + k) % NB]);
+      r_order();
+    }
+  }
+};
 
 template <typename TT, int D>
 __device__ __forceinline__ void r_queries(const RangedParams& p, const RInfo& q, int lane, RState<TT, D>& st) {
@@ -760,24 +832,6 @@ __device__ __forceinline__ void r_init(const RInfo& q, RState<TT, D>& st) {
   st.pos = q.pos;
 }
 
-__device__ __forceinline__ int half_max(int v) {  // over the 32 rows of a wavefront (both halves alike)
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));   // quad_perm 1,0,3,2
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));   // quad_perm 2,3,0,1
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));  // row_half_mirror
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));  // row_mirror
-  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xA, 0xF, false));  // row_bcast:15
-  return __builtin_amdgcn_readlane(v, 31);
-}
-__device__ __forceinline__ int half_min(int v) { return -half_max(-v); }
-
-// The lane, hidden from the compiler once per unit: what follows from it would otherwise be computed at the
-// kernel's start for both kinds of unit, and spilled.
-__device__ __forceinline__ int unit_lane() {
-  int lane = threadIdx.x & 63;
-  asm volatile("" : "+v"(lane));
-  return lane;
-}
-
 // ------------------------------------------------------------------------------------ a unit
 // The wavefront's rows, final where the unit has all their keys, else as partial rows; returns those that came
 // out not finite, which want slow_row.
@@ -798,14 +852,10 @@ __device__ __forceinline__ uint32_t r_store(const RangedParams& p, const RUnit& 
 #pragma unroll
     for (int n = 0; n < D / 32; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u32x2 w;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          w[k] = (uint32_t)TT::from_f32(st.o[n][4 * i + 2 * k] * fct) |
-                 ((uint32_t)TT::from_f32(st.o[n][4 * i + 2 * k + 1] * fct) << 16);
-        *reinterpret_cast<u32x2*>(dst + 32 * n + 8 * i) = w;
-      }
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<u32x2*>(dst + 32 * n + 8 * i) =
+            pack4<TT>(st.o[n][4 * i] * fct, st.o[n][4 * i + 1] * fct, st.o[n][4 * i + 2] * fct,
+                      st.o[n][4 * i + 3] * fct);
   } else if (any) {
     const int64_t row = u.slot + rl;
     if (row < p.part_rows) {
@@ -828,7 +878,7 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
                                               RInfo& q) {
   using G = RGeom<D>;
   constexpr int KB = G::KT / 32, SIDE = G::KT * G::PITCH;
-  const int wave = uniform(threadIdx.x >> 6), lane = unit_lane();
+  const int wave = uniform(threadIdx.x >> 6), lane = hidden(threadIdx.x & 63);
   const int rl = 32 * wave + (lane & 31);
   RState<TT, D> st;
   q = r_place(p, u, rl);
@@ -871,8 +921,9 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
       f32x16 s[KB];
       u32x4 pr[2 * KB];
       r_scores<TT, D, KB>(st, buf, lane, s);
+      RValues<TT, D, KB> v(buf + SIDE, lane);
       r_softmax<TT, D, KB, FORM>(p, st, s, t0, t0 < flo || t0 + G::KT > fhi, lane, pr);
-      r_values<TT, D, KB>(st, buf + SIDE, lane, pr);
+      v.multiply(st, pr);
     }
   }
   return r_store<TT, D>(p, u, q, rl, st, sink, lane);
@@ -883,7 +934,7 @@ template <typename TT, int D, int FORM>
 __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUnit& u, char* mine, RInfo& q) {
   using G = RGeom<D>;
   constexpr int SIDE = 32 * G::PITCH, NI = 32 / G::RPI;
-  const int lane = unit_lane(), rl = lane & 31;
+  const int lane = hidden(threadIdx.x & 63), rl = lane & 31;
   RState<TT, D> st;
   q = r_place(p, u, rl);
   r_queries<TT, D>(p, q, lane, st);
@@ -923,7 +974,7 @@ __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUn
           wait_loads<NI>();
         else
           wait_loads<0>();
-        r_values<TT, D, 1>(st, mine + SIDE, lane, pr);
+        RValues<TT, D, 1>(mine + SIDE, lane).multiply(st, pr);
         wait_lds_reads();
       }
       if (more) {
@@ -1067,125 +1118,166 @@ ranged_kernel(const RangedParams p) {
 }
 
 // ------------------------------------------------------------------------------------ the merge
-// Rows whose keys several workgroups took: their (m, l, O) joined.  A workgroup takes RM consecutive rows
-// (token, head of the group) of a kv-head; thread k < RM finds the pieces of row k -- the workgroups from
-// the one that holds the row's first key to the one that holds its last, for the shared keys and for its
-// own -- and groups of lanes, each lane 16 bytes of the row, sum them, several pieces in flight.
+// Rows whose keys several workers took: their (m, l, O) joined.  A row's pieces are those of the workers from the
+// one that holds its first key to the one that holds its last, for the shared keys and for its own.
 struct RPieces {
   int n;             // pieces
   int64_t first;     // the first one's partial row
   int64_t next, step;  // piece k > 0: next + k * step
 };
 struct RJoin {
-  int t, h;
   RPieces a, b;      // of the shared and of its own keys
+  __device__ __forceinline__ int64_t row(int k) const {
+    const RPieces& q = k < a.n ? a : b;
+    const int y = k < a.n ? k : k - a.n;
+    return y == 0 ? q.first : q.next + y * q.step;
+  }
+};
+__device__ __forceinline__ RJoin r_join(const RangedParams& p, int t, int h, int b, const int (&per)[2]) {
+  const int g = p.num_heads / p.kv_heads, kh = h / g;
+  auto source = [&](int i) {
+    const RTable e = p.table[1 + i];
+    return RSource{e.v[0], e.v[1], e.v[2], e.v[3], e.v[4], e.v[5], e.v[6], e.v[7], e.v[8], e.v[9], e.v[10]};
+  };
+  const RSource own = source(p.groups + b);
+  const RRange r = r_range(p, t, own.kb - own.rows / g + (t - own.tok0), b, own.kb);
+  auto pieces = [&](const RSource& e, int a, int z) {
+    const int kind = r_wide(e) ? 0 : 1, pr = pick(per, kind);
+    const int rr = (t - e.tok0) * g + h - kh * g, blk = kind ? 0 : rr / kRWide, kt = e.ka / kRTile;
+    const RItem it = r_item(p, e, blk, kh);
+    const int w0 = r_worker(pr, it, a / kRTile - kt), w1 = r_worker(pr, it, (z - 1) / kRTile - kt);
+    const int rl = rr - blk * kRWide;
+    RPieces q;
+    q.n = w1 - w0 + 1;
+    q.first = r_slot(p, kind, w0, it.item, w0 == r_worker(pr, it, 0)) + rl;
+    q.next = r_slot(p, kind, w0, it.item, false) + rl;
+    q.step = r_slot(p, kind, w0 + 1, it.item, false) + rl - q.next;
+    if (q.first >= p.part_rows || q.next + (q.n - 1) * q.step >= p.part_rows) q.n = 0;  // (metadata beyond its bounds)
+    return q;
+  };
+  RJoin j{};
+  const int sh_hi = min(r.hi, own.shared), own_lo = max(r.lo, own.shared);
+  if (r.lo < sh_hi) j.a = pieces(source(own.group), r.lo, sh_hi);
+  if (own_lo < r.hi) j.b = pieces(own, own_lo, r.hi);
+  return j;
+}
+// (m, l) and four elements of a row from the pieces, and the join of two of them.
+struct RSum {
+  float m, l;
+  f32x4 o;
+  __device__ __forceinline__ void meet(float m2, float l2, f32x4 o2) {
+    const float mn = fmaxf(m, m2);
+    const float wa = m == kNegInf ? 0.0f : exp2f(m - mn), wb = m2 == kNegInf ? 0.0f : exp2f(m2 - mn);
+    // (pieces whose scores are all NaN have no maximum, but a sum)
+    l = (l == l ? l * wa : l) + (l2 == l2 ? l2 * wb : l2);
+    o = o * wa + o2 * wb;
+    m = mn;
+  }
 };
 constexpr int kRDepth = 4;
-template <typename TT, int D, int RM>
-__global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p) {
-  constexpr int LP = D == 96 ? 32 : D / 4, NG = 256 / LP;
-  constexpr int GPR = NG / (RM < NG ? RM : NG);  // groups of lanes per row
-  __shared__ RJoin join[RM];
-  __shared__ f32x4 sh_o[GPR > 1 ? NG : 1][LP];
-  __shared__ float2 sh_ml[GPR > 1 ? NG : 1];
-  const int per0 = p.table[0].v[0], per1 = p.table[0].v[1];
-  if (per0 == 0 && per1 == 0 && p.groups == 0) return;
-  const int tid = threadIdx.x, g = p.num_heads / p.kv_heads;
-  const int kh = blockIdx.x % p.kv_heads;
-  int b1 = 0;  // one row: its sequence, searched by the whole wavefront
-  if constexpr (RM == 1)
-    if (tid < 64) b1 = seq_of_token(p.cum, p.batch, (int)min((int64_t)(blockIdx.x / p.kv_heads) / g, (int64_t)p.num_tokens));
-  if (tid < RM) {
-    const int64_t gr = (int64_t)(blockIdx.x / p.kv_heads) * RM + tid;
-    const int t = (int)min(gr / g, (int64_t)p.num_tokens);
-    RJoin j{t, kh * g + (int)(gr % g), RPieces{}, RPieces{}};
-    if (t < p.num_tokens && t >= p.cum[0] && t < p.cum[p.batch]) {
-      const int b = RM == 1 ? b1 : r_token_seq(p, 0, p.batch, t);
-      auto source = [&](int i) {
-        const RTable e = p.table[1 + i];
-        return RSource{e.v[0], e.v[1], e.v[2], e.v[3], e.v[4], e.v[5], e.v[6], e.v[7], e.v[8], e.v[9], e.v[10]};
-      };
-      const RSource own = source(p.groups + b);
-      const RRange r = r_range(p, t, own.kb - own.rows / g + (t - own.tok0), b, own.kb);
-      auto pieces = [&](const RSource& e, int a, int z) {
-        const int kind = r_wide(e) ? 0 : 1, per = kind ? per1 : per0;
-        const int rr = (t - e.tok0) * g + j.h - kh * g, blk = kind ? 0 : rr / kRWide, kt = e.ka / kRTile;
-        const RItem it = r_item(p, e, blk, kh);
-        const int w0 = r_worker(per, it, a / kRTile - kt), w1 = r_worker(per, it, (z - 1) / kRTile - kt);
-        const int rl = rr - blk * kRWide;
-        RPieces q;
-        q.n = w1 - w0 + 1;
-        q.first = r_slot(p, kind, w0, it.item, w0 == r_worker(per, it, 0)) + rl;
-        q.next = r_slot(p, kind, w0, it.item, false) + rl;
-        q.step = r_slot(p, kind, w0 + 1, it.item, false) + rl - q.next;
-        if (q.first >= p.part_rows || q.next + (q.n - 1) * q.step >= p.part_rows) q.n = 0;
-        return q;
-      };
-      const int sh_hi = min(r.hi, own.shared), own_lo = max(r.lo, own.shared);
-      if (r.lo < sh_hi) j.a = pieces(source(own.group), r.lo, sh_hi);
-      if (own_lo < r.hi) j.b = pieces(own, own_lo, r.hi);
+// Pieces k0, k0 + stride, ... of a row, several in flight.
+__device__ __forceinline__ RSum r_pieces(const RangedParams& p, const RJoin& j, int k0, int stride, int D, int d0) {
+  RSum s{kNegInf, 0.0f, f32x4{0.f, 0.f, 0.f, 0.f}};
+  const int n = j.a.n + j.b.n;
+  for (int i0 = k0; i0 < n; i0 += stride * kRDepth) {
+    float2 ml[kRDepth];
+    f32x4 o[kRDepth];
+#pragma unroll
+    for (int i = 0; i < kRDepth; ++i) {
+      const int64_t row = j.row(min(i0 + i * stride, n - 1));
+      ml[i] = p.part_ml[row];
+      o[i] = *reinterpret_cast<const f32x4*>(p.part_o + row * D + d0);
     }
-    join[tid] = j;
+    float mn = s.m;
+#pragma unroll
+    for (int i = 0; i < kRDepth; ++i)
+      if (i0 + i * stride < n) mn = fmaxf(mn, ml[i].x);
+    const float a = s.m == kNegInf ? 0.0f : exp2f(s.m - mn);
+    s.l = s.l == s.l ? s.l * a : s.l;
+    s.o *= a;
+#pragma unroll
+    for (int i = 0; i < kRDepth; ++i)
+      if (i0 + i * stride < n) {
+        const float w = ml[i].x == kNegInf ? 0.0f : exp2f(ml[i].x - mn);
+        s.l += ml[i].y == ml[i].y ? ml[i].y * w : ml[i].y;
+        s.o += o[i] * w;
+      }
+    s.m = mn;
   }
-  __syncthreads();
-  const int grp = tid / LP, d0 = 4 * min(tid % LP, D / 4 - 1);
-  for (int k = grp / GPR; k < RM; k += NG / GPR) {
-    const RJoin j = join[k];
-    const int n = j.a.n + j.b.n;
-    if (n < 2) continue;  // (with several groups per row: RM == 1, and every thread goes)
-    float M = kNegInf, L = 0.0f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int i0 = grp % GPR; i0 < n; i0 += GPR * kRDepth) {
-      float2 ml[kRDepth];
-      f32x4 o[kRDepth];
+  return s;
+}
+template <typename TT>
+__device__ __forceinline__ void r_finish(const RangedParams& p, const RSum& s, int64_t t, int h, int D, int d0) {
+  const float f = s.l == s.l ? finalize_factor(s.m, s.l, r_sink<TT>(p, h)) : s.l;
+  *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + (t * p.num_heads + h) * D + d0) =
+      pack4<TT>(s.o[0] * f, s.o[1] * f, s.o[2] * f, s.o[3] * f);
+}
+
+// Few rows: NW wavefronts per row, whose groups of lanes (16 bytes of the row per lane) take pieces in turn and meet
+// through lane exchanges and, with four wavefronts, LDS.  Bound by its chain of loads.
+template <typename TT, int D, int NW>
+__global__ __launch_bounds__(256) void ranged_join_kernel(const RangedParams p) {
+  constexpr int LP = D == 96 ? 32 : D / 4, NG = 64 / LP * NW;
+  __shared__ f32x4 sh_o[NW > 1 ? 4 : 1][LP];
+  __shared__ float2 sh_ml[NW > 1 ? 4 : 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int64_t row = (int64_t)blockIdx.x * (4 / NW) + (NW > 1 ? 0 : wave);
+  const int t = uniform((int)(row / p.num_heads)), h = uniform((int)(row % p.num_heads));
+  if (t >= p.num_tokens) return;
+  const int per[2] = {p.table[0].v[0], p.table[0].v[1]};
+  const int c0 = p.cum[0], c1 = p.cum[p.batch];
+  const int b = uniform(seq_of_token(p.cum, p.batch, t));
+  if (t < c0 || t >= c1 || (per[0] == 0 && per[1] == 0 && p.groups == 0)) return;
+  const RJoin j = r_join(p, t, h, b, per);
+  if (j.a.n + j.b.n < 2) return;
+  const int d0 = 4 * min(lane % LP, D / 4 - 1);
+  RSum s = r_pieces(p, j, (NW > 1 ? wave * (64 / LP) : 0) + lane / LP, NG, D, d0);
 #pragma unroll
-      for (int i = 0; i < kRDepth; ++i) {
-        const int x = min(i0 + i * GPR, n - 1);
-        const RPieces& q = x < j.a.n ? j.a : j.b;
-        const int y = x < j.a.n ? x : x - j.a.n;
-        const int64_t row = y == 0 ? q.first : q.next + y * q.step;
-        ml[i] = p.part_ml[row];
-        o[i] = *reinterpret_cast<const f32x4*>(p.part_o + row * D + d0);
-      }
-      float mn = M;
+  for (int o = LP; o < 64; o <<= 1)
+    s.meet(__shfl_xor(s.m, o, 64), __shfl_xor(s.l, o, 64),
+           f32x4{__shfl_xor(s.o[0], o, 64), __shfl_xor(s.o[1], o, 64), __shfl_xor(s.o[2], o, 64),
+                 __shfl_xor(s.o[3], o, 64)});
+  if constexpr (NW > 1) {
+    if (lane < LP) sh_o[wave][lane] = s.o;
+    if (lane == 0) sh_ml[wave] = float2{s.m, s.l};
+    __syncthreads();
+    if (wave > 0 || lane >= LP) return;
 #pragma unroll
-      for (int i = 0; i < kRDepth; ++i)
-        if (i0 + i * GPR < n) mn = fmaxf(mn, ml[i].x);
-      const float a = M == kNegInf ? 0.0f : exp2f(M - mn);
-      L = L == L ? L * a : L;
-      acc *= a;
-#pragma unroll
-      for (int i = 0; i < kRDepth; ++i)
-        if (i0 + i * GPR < n) {
-          const float w = ml[i].x == kNegInf ? 0.0f : exp2f(ml[i].x - mn);
-          L += ml[i].y == ml[i].y ? ml[i].y * w : ml[i].y;
-          acc += o[i] * w;
-        }
-      M = mn;
+    for (int w = 1; w < 4; ++w) s.meet(sh_ml[w].x, sh_ml[w].y, sh_o[w][lane]);
+  }
+  if (lane < D / 4) r_finish<TT>(p, s, t, h, D, d0);
+}
+
+// Many rows: workgroups take 32 rows (token, head of the group) of a kv-head at a time; thread k finds the pieces of
+// row k, then groups of lanes sum a row each.
+template <typename TT, int D>
+__global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p, int blocks) {
+  constexpr int LP = D == 96 ? 32 : D / 4, NG = 256 / LP, RM = 32;
+  __shared__ RJoin join[RM];
+  __shared__ int2 place[RM];
+  const int per[2] = {p.table[0].v[0], p.table[0].v[1]};
+  if (per[0] == 0 && per[1] == 0 && p.groups == 0) return;
+  const int tid = threadIdx.x, g = p.num_heads / p.kv_heads;
+  for (int blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
+    const int kh = blk % p.kv_heads;
+    if (tid < RM) {
+      const int64_t gr = (int64_t)(blk / p.kv_heads) * RM + tid;
+      const int t = (int)min(gr / g, (int64_t)p.num_tokens), h = kh * g + (int)(gr % g);
+      RJoin j{};
+      if (t < p.num_tokens && t >= p.cum[0] && t < p.cum[p.batch])
+        j = r_join(p, t, h, r_token_seq(p, 0, p.batch, t), per);
+      join[tid] = j;
+      place[tid] = int2{t, h};
     }
-    if constexpr (GPR > 1) {
-      static_assert(RM == 1, "one row per workgroup");
-      sh_o[grp][tid % LP] = acc;
-      if (tid % LP == 0) sh_ml[grp] = float2{M, L};
-      __syncthreads();
-      if (grp > 0) return;
-#pragma unroll
-      for (int w = 1; w < NG; ++w) {
-        const float2 ml = sh_ml[w];
-        const float mn = fmaxf(M, ml.x);
-        const float wa = M == kNegInf ? 0.0f : exp2f(M - mn), wb = ml.x == kNegInf ? 0.0f : exp2f(ml.x - mn);
-        L = (L == L ? L * wa : L) + (ml.y == ml.y ? ml.y * wb : ml.y);
-        acc = acc * wa + sh_o[w][tid % LP] * wb;
-        M = mn;
-      }
+    __syncthreads();
+    const int d0 = 4 * min(tid % LP, D / 4 - 1);
+    for (int k = tid / LP; k < RM; k += NG) {
+      const RJoin j = join[k];
+      if (j.a.n + j.b.n < 2) continue;
+      const RSum s = r_pieces(p, j, 0, 1, D, d0);
+      if (tid % LP < D / 4) r_finish<TT>(p, s, place[k].x, place[k].y, D, d0);
     }
-    if (tid % LP >= D / 4) continue;
-    const float f = L == L ? finalize_factor(M, L, r_sink<TT>(p, j.h)) : L;
-    u32x2 w;
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-      w[m] = (uint32_t)TT::from_f32(acc[2 * m] * f) | ((uint32_t)TT::from_f32(acc[2 * m + 1] * f) << 16);
-    *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + ((int64_t)j.t * p.num_heads + j.h) * D + d0) = w;
+    __syncthreads();
   }
 }
 
@@ -1204,11 +1296,16 @@ hipError_t launch_d(const RangedParams& p, hipStream_t s) {
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.merge) return e;
-  const int64_t rows = (int64_t)p.num_tokens * (p.num_heads / p.kv_heads);
-  if (rows * p.kv_heads <= kRMergeRows)
-    hipLaunchKernelGGL((ranged_merge_kernel<TT, D, 1>), dim3((unsigned)(rows * p.kv_heads)), block, 0, s, p);
-  else
-    hipLaunchKernelGGL((ranged_merge_kernel<TT, D, 32>), dim3((unsigned)((rows + 31) / 32 * p.kv_heads)), block, 0, s, p);
+  const int64_t rows = (int64_t)p.num_tokens * p.num_heads;
+  if (rows <= kRJoinWide) {
+    hipLaunchKernelGGL((ranged_join_kernel<TT, D, 4>), dim3((unsigned)rows), block, 0, s, p);
+  } else if (rows <= kRJoinRows) {
+    hipLaunchKernelGGL((ranged_join_kernel<TT, D, 1>), dim3((unsigned)((rows + 3) / 4)), block, 0, s, p);
+  } else {
+    const int blocks = (int)((rows / p.kv_heads + 31) / 32 * p.kv_heads);
+    hipLaunchKernelGGL((ranged_merge_kernel<TT, D>), dim3((unsigned)std::min(blocks, kRMergeGrid)), block, 0, s, p,
+                       blocks);
+  }
   return hipGetLastError();
 }
 
