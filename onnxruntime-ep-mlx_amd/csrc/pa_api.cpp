@@ -1321,7 +1321,7 @@ RangedPlan ranged_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a,
   }
   r.o_bytes = align256((size_t)r.part_rows * c->head_dim * sizeof(float));
   r.ml_bytes = align256((size_t)r.part_rows * 2 * sizeof(float));
-  r.table_bytes = align256((size_t)(1 + groups + b->batch) * sizeof(pa::RTable));
+  r.table_bytes = align256((size_t)(1 + groups + b->batch) * sizeof(pa::RTable)) + pa::kRQueueBytes;
   return r;
 }
 
@@ -1376,6 +1376,9 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
   p.part_o = reinterpret_cast<float*>(base);
   p.part_ml = reinterpret_cast<float2*>(base + r.o_bytes);
   p.table = reinterpret_cast<pa::RTable*>(base + r.o_bytes + r.ml_bytes);
+  // Documents hide what items cost: where every workgroup has several, they take them from a queue.
+  if (p.doc_starts && (int64_t)b->num_tokens * (a->num_heads / c->kv_heads) / 128 * c->kv_heads >= 2 * r.slots)
+    p.queue = reinterpret_cast<int32_t*>(base + r.bytes() - pa::kRQueueBytes);
   p.num_blocks = c->num_blocks;
   p.part_rows = r.part_rows;
   p.part_narrow = r.part_narrow;

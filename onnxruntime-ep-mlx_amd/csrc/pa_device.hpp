@@ -416,6 +416,8 @@ struct AttnParams {
 struct RTable {
   int32_t v[12];
 };
+// Counters of the queues of wide items, 64 bytes apart.
+constexpr int kRQueues = 8, kRQueueStep = 16, kRQueueBytes = 4 * kRQueues * kRQueueStep;
 struct RangedParams {
   const void* q;
   const void* key_cache;
@@ -431,6 +433,7 @@ struct RangedParams {
   const int32_t* doc_starts;
   const int32_t* group_cum;
   const int32_t* shared_lens;
+  int32_t* queue;  // or null
   // Workspace: part_rows partial rows [head_dim] (those of wide blocks, then from part_narrow on those of
   // narrow ones, narrow_rows each), their (m, l), and the table
   float* part_o;

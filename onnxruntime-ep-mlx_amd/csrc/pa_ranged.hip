@@ -57,6 +57,9 @@ constexpr int kRStart = 4;
 constexpr float kRCut = 20.0f;
 // Time of a tile where a workgroup has its CU to itself (1.0 instead: a prompt of 1024 44.6 us for 41.7).
 constexpr float kRAlone = 0.65f;
+// Time of a wide tile on a workgroup over a narrow one's on a wavefront, in the sharing out of workgroups (1, 2 and 3:
+// 64 samples of a prompt of 8190 45, 46 and 47 us for 40; elsewhere within 2 %).
+constexpr float kRWideCost = 1.5f;
 // Rows up to which the merge gives each a workgroup, a wavefront; workgroups of the merge of more.
 constexpr int64_t kRJoinWide = 1024, kRJoinRows = 16384;
 constexpr int kRMergeGrid = 2048;
@@ -282,6 +285,7 @@ struct RScan {
   int64_t wt[4][2];
   int red[8];
   int most[4];
+  int next;  // from the queue
 };
 struct RTotals {
   int tiles[2], items[2];  // wide, narrow
@@ -346,11 +350,11 @@ struct RShare {
 };
 __device__ __forceinline__ RShare r_share(const RangedParams& p, const RTotals& t) {
   RShare r;
-  const int64_t all = (int64_t)t.tiles[0] + t.tiles[1];
+  const float cost = kRWideCost * (float)t.tiles[0];
   r.wide = t.tiles[0] == 0 ? 0
            : t.tiles[1] == 0
                ? p.slots
-               : min(max((int)((float)p.slots * ((float)t.tiles[0] / (float)all)), 1), p.slots - 1);
+               : min(max((int)((float)p.slots * (cost / (cost + (float)t.tiles[1]))), 1), p.slots - 1);
   const int waves = max((p.slots - r.wide) * 4, 1);
   // Whole wide items, or equal stretches of their tiles.  Whole, a worker takes the largest item, or its share
   // of all in turns: items of equal cost as many as there are turns, of evenly spread costs little over an even
@@ -712,37 +716,54 @@ __device__ __forceinline__ float add_pairs(u32x4 p, float l) {  // l + the eight
 // the rounded probabilities, so that both sides of the quotient err alike.
 template <typename TT, int D, int KB, int FORM>
 __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& st, f32x16 (&s)[KB],
-                                          int t0, bool masked, int lane, u32x4 (&pr)[2 * KB]) {
+                                          int t0, bool low, bool high, bool before, int lane, u32x4 (&pr)[2 * KB]) {
   const int h = lane >> 5;
   // kRCap: scores become log2 units here; otherwise the scale enters each exponent's FMA, and the slope is in
   // units of the raw products
   const float sl = FORM == kRCap ? 1.0f : p.scale_log2;
   const float ck = FORM == kRCap ? fabsf(p.scale) / p.softcap : 0.0f, cl = p.softcap * kLog2e;
+  float off = 0.0f;  // what the tile's scores share, in log2 units
   if constexpr (FORM != kRPlain) {
     const float far = (float)(st.pos - t0 - 4 * h);
+    if (FORM == kRSlope && before) {
+      // no key behind the row (that it sees): the distance is far less the key's place
+      off = -st.slope * far * sl;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float x = FORM == kRCap ? softcap_log2(s[kb][i], ck, cl) : s[kb][i];
-        s[kb][i] = __builtin_fmaf(fabsf(far - (float)(32 * kb + 8 * (i >> 2) + (i & 3))), -st.slope, x);
-      }
+        for (int i = 0; i < 16; ++i)
+          s[kb][i] = __builtin_fmaf(st.slope, (float)(32 * kb + 8 * (i >> 2) + (i & 3)), s[kb][i]);
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = FORM == kRCap ? softcap_log2(s[kb][i], ck, cl) : s[kb][i];
+          s[kb][i] = __builtin_fmaf(fabsf(far - (float)(32 * kb + 8 * (i >> 2) + (i & 3))), -st.slope, x);
+        }
+    }
   }
-  if (masked) {
-    const unsigned span = st.hi > st.lo ? (unsigned)(st.hi - st.lo) : 0u;
-    const unsigned rel = (unsigned)(t0 + 4 * h) - (unsigned)st.lo;
+  if (low) {  // some row's keys begin inside the tile
+    const int lo = st.lo - t0 - 4 * h;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        s[kb][i] = rel + (unsigned)(32 * kb + 8 * (i >> 2) + (i & 3)) < span ? s[kb][i] : kNegInf;
+      for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i >> 2) + (i & 3) >= lo ? s[kb][i] : kNegInf;
+  }
+  if (high) {  // ... end inside it
+    const int hi = st.hi - t0 - 4 * h;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i >> 2) + (i & 3) < hi ? s[kb][i] : kNegInf;
   }
   float mx = s[0][0];
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(s[kb][i], s[kb][i + 1]), mx);
-  mx *= sl;
+  // (the halves' keys are four apart, and off with them)
+  mx = FORM == kRSlope ? __builtin_fmaf(mx, sl, off) : mx * sl;
   mx = fmaxf(mx, half_swap(mx));
   if (__any(mx > st.m + 8.0f)) {
     const float mn = fmaxf(st.m, mx);
@@ -752,7 +773,7 @@ __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& 
 #pragma unroll
     for (int n = 0; n < D / 32; ++n) st.o[n] *= a;
   }
-  const float ms = st.m == kNegInf ? 0.0f : st.m;
+  const float ms = st.m == kNegInf ? 0.0f : st.m - off;
 #pragma unroll
   for (int t = 0; t < 2 * KB; ++t) {
     float e[8];
@@ -832,6 +853,13 @@ __device__ __forceinline__ void r_init(const RInfo& q, RState<TT, D>& st) {
   st.pos = q.pos;
 }
 
+// Keys below it lie before every row of the wavefront that sees them (see r_softmax).
+template <int FORM>
+__device__ __forceinline__ int r_near(const RangedParams& p, const RInfo& q) {
+  if (FORM != kRSlope) return 0;
+  return p.causal && !p.prefix_lens ? INT32_MAX : half_min((q.how & kRAny) ? q.pos : INT32_MAX);
+}
+
 // ------------------------------------------------------------------------------------ a unit
 // The wavefront's rows, final where the unit has all their keys, else as partial rows; returns those that came
 // out not finite, which want slow_row.
@@ -848,14 +876,20 @@ __device__ __forceinline__ uint32_t r_store(const RangedParams& p, const RUnit& 
     for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(st.o[n][i], 0.0f, sum);
   if ((q.how & kRZero) || (any && (q.how & kRSingle))) {
     const float fct = (q.how & kRZero) ? 0.0f : finalize_factor(st.m, l, sink);
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((int64_t)q.t * p.num_heads + q.h) * D + 4 * h;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((int64_t)q.t * p.num_heads + q.h) * D + 8 * h;
+    // (the halves exchange every other four dims, so that each stores eight at a time)
 #pragma unroll
     for (int n = 0; n < D / 32; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<u32x2*>(dst + 32 * n + 8 * i) =
-            pack4<TT>(st.o[n][4 * i] * fct, st.o[n][4 * i + 1] * fct, st.o[n][4 * i + 2] * fct,
-                      st.o[n][4 * i + 3] * fct);
+      for (int i = 0; i < 4; i += 2) {
+        const u32x2 a = pack4<TT>(st.o[n][4 * i] * fct, st.o[n][4 * i + 1] * fct, st.o[n][4 * i + 2] * fct,
+                                  st.o[n][4 * i + 3] * fct);
+        const u32x2 b = pack4<TT>(st.o[n][4 * i + 4] * fct, st.o[n][4 * i + 5] * fct, st.o[n][4 * i + 6] * fct,
+                                  st.o[n][4 * i + 7] * fct);
+        const auto x = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
+        const auto y = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+        *reinterpret_cast<u32x4*>(dst + 32 * n + 8 * i) = u32x4{x[0], y[0], x[1], y[1]};
+      }
   } else if (any) {
     const int64_t row = u.slot + rl;
     if (row < p.part_rows) {
@@ -890,6 +924,7 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
   // keys that some / every row of the wavefront sees, and some row of the workgroup
   const int wlo = half_min(any ? q.lo : INT32_MAX), whi = half_max(any ? q.hi : 0);
   const int flo = half_max(any ? q.lo : 0), fhi = half_min(any ? q.hi : INT32_MAX);
+  const int near = r_near<FORM>(p, q);
   __syncthreads();  // the last unit's readers are done
   if (lane == 0) {
     sh.red[2 * wave] = wlo;
@@ -909,10 +944,11 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
     for (int t = tb - 1; t < te; ++t) {
       if (t >= tb) wait_loads<0>();
       barrier();
+      // (at once: between the products they cost more, 735 us for 627 over a prompt of 8192 at head 256)
       if (t + 1 < te) {
-        const uint32_t buf = base + ((t + 1 - tb) & 1) * 2 * SIDE;
+        const uint32_t put = base + ((t + 1 - tb) & 1) * 2 * SIDE;
         const int pos = (t + 1) * G::KT + wave * GR;
-        f.template load<true, true, false>(pos, pg, buf, buf + SIDE, wave * GR & 15, lane);
+        f.template load<true, true, false>(pos, pg, put, put + SIDE, wave * GR & 15, lane);
         pg = f.page(pos + G::KT);
       }
       const int t0 = t * G::KT;
@@ -922,7 +958,7 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
       u32x4 pr[2 * KB];
       r_scores<TT, D, KB>(st, buf, lane, s);
       RValues<TT, D, KB> v(buf + SIDE, lane);
-      r_softmax<TT, D, KB, FORM>(p, st, s, t0, t0 < flo || t0 + G::KT > fhi, lane, pr);
+      r_softmax<TT, D, KB, FORM>(p, st, s, t0, t0 < flo, t0 + G::KT > fhi, t0 + G::KT <= near, lane, pr);
       v.multiply(st, pr);
     }
   }
@@ -947,6 +983,7 @@ __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUn
   f.kmin = half_min(any ? q.lo : INT32_MAX);
   f.kmax = half_max(any ? q.hi : 0);
   const int flo = half_max(any ? q.lo : 0), fhi = half_min(any ? q.hi : INT32_MAX);
+  const int near = r_near<FORM>(p, q);
   if (f.kmin < f.kmax) {
     const int tb = f.kmin / 32, te = (f.kmax + 31) / 32;
     const uint32_t base = lds_address(mine);
@@ -969,7 +1006,7 @@ __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUn
         f.template load<true, false, true>(t0 + 48, p1, base + HALF, 0, 0, lane);
       }
       if (have) {
-        r_softmax<TT, D, 1, FORM>(p, st, s, t0, t0 < flo || t0 + 32 > fhi, lane, pr);
+        r_softmax<TT, D, 1, FORM>(p, st, s, t0, t0 < flo, t0 + 32 > fhi, t0 + 32 <= near, lane, pr);
         if (more)
           wait_loads<NI>();
         else
@@ -1003,6 +1040,7 @@ ranged_kernel(const RangedParams p) {
   RTotals t{}, tb{};
   RShare r{};
   int me = 0, per = 0, kind = 0, at = 0, end = 0, stride = 0, turn = 0;
+  bool queued = false;
   for (int c = chunks > 1 ? -chunks : 0; c < chunks; ++c) {
     const int base = (c < 0 ? c + chunks : c) * kRChunk;
     tb = t;
@@ -1011,6 +1049,7 @@ ranged_kernel(const RangedParams p) {
     if (c == -1 || chunks == 1) {
       r = r_share(p, t);
       kind = (int)blockIdx.x < r.wide ? 0 : 1;
+      queued = p.queue && kind == 0 && r.per[0] == 0;
       me = kind ? ((int)blockIdx.x - r.wide) * 4 + wave : (int)blockIdx.x;
       per = kind ? r.per[1] : r.per[0];
       // my stretch of tiles, or my first item
@@ -1033,6 +1072,8 @@ ranged_kernel(const RangedParams p) {
     for (;;) {
       if (per > 0) {
         if (at >= min(end, pick(t.tiles, kind))) break;
+      } else if (queued) {
+        if (at >= t.items[0]) break;
       } else {
         // whole items in turns; wide ones alternately up and down the list, in runs of eight (neighbours share
         // keys, and runs keep them on their XCD)
@@ -1102,6 +1143,11 @@ ranged_kernel(const RangedParams p) {
       uint32_t odd;
       bool wide = false;
       if constexpr (WIDE) wide = kind == 0;
+      // The next one from the queue: eight queues, of every eighth item each, so that neighbours, which share keys,
+      // keep their XCDs.
+      const int queues = (r.wide & (kRQueues - 1)) == 0 ? kRQueues : 1, mine = me & (queues - 1);
+      int ticket = 0;
+      if (queued && threadIdx.x == 0) ticket = atomicAdd(p.queue + mine * kRQueueStep, 1);
       if (wide)
         odd = wide_unit<TT, D, FORM>(p, u, lds, sh, q);
       else
@@ -1112,6 +1158,11 @@ ranged_kernel(const RangedParams p) {
         const RInfo w{uniform(__shfl(q.t, k, 64)),  uniform(__shfl(q.h, k, 64)),  uniform(__shfl(q.pos, k, 64)),
                       uniform(__shfl(q.lo, k, 64)), uniform(__shfl(q.hi, k, 64)), uniform(__shfl(q.how, k, 64))};
         slow_row<TT, D>(p, u, w, (wide ? 32 * wave : 0) + k);
+      }
+      if (queued) {
+        if (threadIdx.x == 0) sh.next = r.wide + queues * ticket + mine;
+        __syncthreads();
+        at = uniform(sh.next);
       }
     }
   }
@@ -1281,9 +1332,14 @@ __global__ __launch_bounds__(256) void ranged_merge_kernel(const RangedParams p,
   }
 }
 
+__global__ __launch_bounds__(64) void ranged_queue_kernel(const RangedParams p) {
+  if (threadIdx.x < kRQueues) p.queue[threadIdx.x * kRQueueStep] = 0;
+}
+
 template <typename TT, int D>
 hipError_t launch_d(const RangedParams& p, hipStream_t s) {
   const dim3 grid(p.slots), block(256);
+  if (p.queue) hipLaunchKernelGGL(ranged_queue_kernel, dim3(1), dim3(64), 0, s, p);
   const int form = p.softcap > 0.0f ? kRCap : p.slopes ? kRSlope : kRPlain;
   if (p.wide) {
     if (form == kRCap) hipLaunchKernelGGL((ranged_kernel<TT, D, kRCap, true>), grid, block, 0, s, p);
