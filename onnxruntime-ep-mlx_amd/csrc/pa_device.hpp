@@ -447,7 +447,7 @@ struct RangedParams {
   int32_t batch, max_blocks, num_tokens;
   int32_t window, causal;
   float scale, scale_log2, softcap;  // scale_log2: |scale| log2(e)
-  float slope_unit;                  // slopes times this: in raw products, with a softcap in log2 units
+  float slope_unit;                  // slopes times this: in raw products, with a softcap in twice the softcap
   uint32_t qxor;                     // 0x80008000 where scale is negative
   int32_t slots;     // workgroups
   int32_t per_cu;    // ... that a CU holds at once

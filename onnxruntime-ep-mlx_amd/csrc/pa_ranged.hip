@@ -718,16 +718,23 @@ template <typename TT, int D, int KB, int FORM>
 __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& st, f32x16 (&s)[KB],
                                           int t0, bool low, bool high, bool before, int lane, u32x4 (&pr)[2 * KB]) {
   const int h = lane >> 5;
-  // kRCap: scores become log2 units here; otherwise the scale enters each exponent's FMA, and the slope is in
-  // units of the raw products
-  const float sl = FORM == kRCap ? 1.0f : p.scale_log2;
-  const float ck = FORM == kRCap ? fabsf(p.scale) / p.softcap : 0.0f, cl = p.softcap * kLog2e;
-  float off = 0.0f;  // what the tile's scores share, in log2 units
-  if constexpr (FORM != kRPlain) {
+  // A score in log2 units is s * sl + off.  kRCap: softcap tanh(y) = softcap (1 - 2 / (1 + exp(2 y))), of which s keeps
+  // the quotient, so that the exponent's FMA ends it (about 2^-23 of the softcap, far below the types' resolution).
+  const float sl = FORM == kRCap ? 2.0f * kLog2e * p.softcap : p.scale_log2;
+  float off = FORM == kRCap ? kLog2e * p.softcap : 0.0f;
+  if constexpr (FORM == kRCap) {
+    const float ck = 2.0f * p.scale_log2 / p.softcap;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        s[kb][i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[kb][i] * ck));
+  }
+  if (FORM == kRSlope || (FORM == kRCap && p.slopes)) {
     const float far = (float)(st.pos - t0 - 4 * h);
-    if (FORM == kRSlope && before) {
+    if (before) {
       // no key behind the row (that it sees): the distance is far less the key's place
-      off = -st.slope * far * sl;
+      off = __builtin_fmaf(-st.slope * far, sl, off);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -737,10 +744,8 @@ __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& 
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = FORM == kRCap ? softcap_log2(s[kb][i], ck, cl) : s[kb][i];
-          s[kb][i] = __builtin_fmaf(fabsf(far - (float)(32 * kb + 8 * (i >> 2) + (i & 3))), -st.slope, x);
-        }
+        for (int i = 0; i < 16; ++i)
+          s[kb][i] = __builtin_fmaf(fabsf(far - (float)(32 * kb + 8 * (i >> 2) + (i & 3))), -st.slope, s[kb][i]);
     }
   }
   if (low) {  // some row's keys begin inside the tile
@@ -763,7 +768,7 @@ __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& 
 #pragma unroll
     for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(s[kb][i], s[kb][i + 1]), mx);
   // (the halves' keys are four apart, and off with them)
-  mx = FORM == kRSlope ? __builtin_fmaf(mx, sl, off) : mx * sl;
+  mx = FORM == kRPlain ? mx * sl : __builtin_fmaf(mx, sl, off);
   mx = fmaxf(mx, half_swap(mx));
   if (__any(mx > st.m + 8.0f)) {
     const float mn = fmaxf(st.m, mx);
@@ -856,7 +861,7 @@ __device__ __forceinline__ void r_init(const RInfo& q, RState<TT, D>& st) {
 // Keys below it lie before every row of the wavefront that sees them (see r_softmax).
 template <int FORM>
 __device__ __forceinline__ int r_near(const RangedParams& p, const RInfo& q) {
-  if (FORM != kRSlope) return 0;
+  if (FORM == kRPlain || !p.slopes) return 0;
   return p.causal && !p.prefix_lens ? INT32_MAX : half_min((q.how & kRAny) ? q.pos : INT32_MAX);
 }
 
