@@ -104,6 +104,12 @@ def test_masked_attention_refuses(kw, code, text):
     assert text in error()
 
 
+@pytest.mark.parametrize("kw", [dict(q=FAKE + 8), dict(out=FAKE + 2), dict(ws=FAKE + 8)])
+def test_rows_and_workspaces_at_odd_addresses_are_refused(kw):
+    assert masked(**kw) == capi.PA_ERR_INVALID_ARGUMENT
+    assert "16-byte aligned" in error()
+
+
 def test_null_descriptors_are_refused():
     lib, c, b, a = capi.load(), cache(), batch(), attn()
     for i in range(3):
