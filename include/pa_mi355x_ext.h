@@ -73,7 +73,9 @@ typedef struct pa_mask {
 
 /* Attention over the pages under such a mask (mask NULL: plain paged attention).  Layouts of q and
  * out and the attributes as pa_attention; the SEPARATE cache layout.  Workspace: at least the
- * queried size. */
+ * queried size.  fp16 / bf16 activations and pages at heads 64, 96, 128 and 256, from caches that
+ * begin at 16 bytes, run on matrix cores and want q, out and the workspace at 16 bytes too (refused
+ * otherwise); everything else runs without them. */
 size_t pa_masked_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
                                            const pa_attn* attn, const pa_mask* mask,
                                            pa_dtype act_dtype);
