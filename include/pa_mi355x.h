@@ -496,6 +496,31 @@ typedef struct pa_gqa_node_info {
 
 int pa_group_query_attention_claim(const pa_gqa_node_info* node, char* reason, size_t reason_len);
 
+/* Entries whose descriptors and contracts are in pa_mi355x_ext.h. */
+struct pa_axis_rotary;
+struct pa_mask;
+struct pa_shared_prefix;
+int pa_multi_axis_rotary_append(const pa_cache* cache, const pa_batch* batch, int32_t num_heads,
+                                pa_dtype act_dtype, const void* query, int64_t q_stride,
+                                const void* key, int64_t k_stride, const void* value,
+                                int64_t v_stride, const struct pa_axis_rotary* rotary,
+                                const void* q_norm, const void* k_norm, float norm_eps,
+                                void* q_out, pa_stream_t stream);
+size_t pa_masked_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
+                                           const pa_attn* attn, const struct pa_mask* mask,
+                                           pa_dtype act_dtype);
+int pa_masked_attention(const pa_cache* cache, const pa_batch* batch, const pa_attn* attn,
+                        const struct pa_mask* mask, pa_dtype act_dtype, const void* q, void* out,
+                        void* workspace, size_t workspace_bytes, pa_stream_t stream);
+size_t pa_shared_prefix_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
+                                                  const pa_attn* attn,
+                                                  const struct pa_shared_prefix* share,
+                                                  const struct pa_mask* mask, pa_dtype act_dtype);
+int pa_shared_prefix_attention(const pa_cache* cache, const pa_batch* batch, const pa_attn* attn,
+                               const struct pa_shared_prefix* share, const struct pa_mask* mask,
+                               pa_dtype act_dtype, const void* q, void* out, void* workspace,
+                               size_t workspace_bytes, pa_stream_t stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif
