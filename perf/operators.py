@@ -466,17 +466,12 @@ def _plain_shared(st):
 
 # ------------------------------------------------------------------------------------------ runs
 
-_ep = None
-
-
 def _library():
-    """The package, found and imported once."""
-    global _ep
-    if _ep is None:
-        sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "onnxruntime-ep-mlx_amd"))
-        import onnxruntime_ep_mlx_amd
-        _ep = onnxruntime_ep_mlx_amd
-    return _ep
+    place = str(Path(__file__).resolve().parent.parent / "onnxruntime-ep-mlx_amd")
+    if place not in sys.path:
+        sys.path.insert(0, place)
+    import onnxruntime_ep_mlx_amd as ep
+    return ep
 
 
 def _own(st):
