@@ -24,8 +24,10 @@
 //   O^T[dim][row] = V^T P^T (A: 32 dims x 16 keys by transposing LDS reads, B: the probabilities as the
 //                            score product leaves them)
 // A row's maximum and sum need one exchange between the lane halves, and its range, slope and position
-// are scalars of the lane.  Probabilities enter the second product rounded to the activation type (half
-// a step of it, the output's own rounding); scores, statistics and sums are fp32.
+// are scalars of the lane.  Probabilities enter the second product in two parts of the activation type
+// (off by at most 2^-17 of themselves in bf16, 2^-20 in fp16, as in the other attention kernels: one part
+// alone erred as much as the output's own rounding), two products against one read of the values; scores,
+// statistics and sums are fp32.
 //
 // Wide items: four wavefronts of 32 rows each on the same 64-key tile (32 keys at head 256), staged by
 // direct loads from the pages into two LDS buffers, one barrier per tile.  Narrow items: a wavefront with a
@@ -86,14 +88,15 @@ __device__ __forceinline__ float half_swap(float x) {  // lane l ^ 32's x
   return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-// Eight probabilities in T, rounded to nearest even.
+// Eight probabilities as the sum of two parts in T.
+struct RPair {
+  u32x4 hi, lo;
+};
 template <typename TT>
-__device__ __forceinline__ u32x4 pack8(const float* x) {
-  typedef float f32x8 __attribute__((ext_vector_type(8)));
-  f32x8 v;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = x[i];
-  return __builtin_bit_cast(u32x4, __builtin_convertvector(v, typename TT::vec8));
+__device__ __forceinline__ RPair split_pair(const float (&x)[8]) {
+  typename TT::vec8 h, l;
+  TT::split8(x, h, l);
+  return RPair{__builtin_bit_cast(u32x4, h), __builtin_bit_cast(u32x4, l)};
 }
 template <typename TT>
 __device__ __forceinline__ u32x2 pack4(float a, float b, float c, float d) {
@@ -701,28 +704,10 @@ __device__ __forceinline__ void r_scores(const RState<TT, D>& st, const char* kt
 // Forms of a score: as it is, less a slope times the distance, softcapped (and less that).
 enum RForm { kRPlain = 0, kRSlope = 1, kRCap = 2 };
 
-template <typename TT>
-__device__ __forceinline__ float add_pairs(u32x4 p, float l) {  // l + the eight values of p
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t w = p[i];  // (a bit_cast of the element itself reads element 0)
-    if constexpr (TT::code == PA_DTYPE_FLOAT16) {
-      typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-      l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{(_Float16)1.0f, (_Float16)1.0f}, l, false);
-    } else {
-      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-      l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w),
-                                          __builtin_bit_cast(bf16x2, 0x3f803f80u), l, false);
-    }
-  }
-  return l;
-}
-
-// Bias, mask, the lazy maximum and the probabilities of 32 KB keys at t0, packed per 16 keys.  The row's sum takes
-// the rounded probabilities, so that both sides of the quotient err alike.
+// Bias, mask, the lazy maximum and the probabilities of 32 KB keys at t0, in two parts per 16 keys.
 template <typename TT, int D, int KB, int FORM>
 __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& st, f32x16 (&s)[KB],
-                                          int t0, bool low, bool high, bool before, int lane, u32x4 (&pr)[2 * KB]) {
+                                          int t0, bool low, bool high, bool before, int lane, RPair (&pr)[2 * KB]) {
   const int h = lane >> 5;
   // A score in log2 units is s * sl + off.  kRCap: softcap tanh(y) = softcap (1 - 2 / (1 + exp(2 y))), of which s keeps
   // the quotient, so that the exponent's FMA ends it (about 2^-23 of the softcap, far below the types' resolution).
@@ -791,8 +776,8 @@ __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& 
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][8 * (t & 1) + i], sl, -ms));
-    pr[t] = pack8<TT>(e);
-    st.l = add_pairs<TT>(pr[t], st.l);
+    pr[t] = split_pair<TT>(e);
+    st.l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
   }
 }
 
@@ -828,14 +813,17 @@ struct RValues {
     read(0);
     r_order();
   }
-  __device__ __forceinline__ void multiply(RState<TT, D>& st, const u32x4 (&pr)[2 * KB]) {
+  __device__ __forceinline__ void multiply(RState<TT, D>& st, const RPair (&pr)[2 * KB]) {
 #pragma unroll
     for (int g = 0; g < N / A; ++g) {
       if (g + 1 < N / A) read(g + 1);
       r_order();
 #pragma unroll
       for (int k = 0; k < A; ++k)
-        st.o[(g * A + k) % NB] = mfma_r<TT>(v[g & 1][k], pr[(g * A + k) / NB], st.o[(g * A + k) % NB]);
+        st.o[(g * A + k) % NB] = mfma_r<TT>(v[g & 1][k], pr[(g * A + k) / NB].hi, st.o[(g * A + k) % NB]);
+#pragma unroll
+      for (int k = 0; k < A; ++k)
+        st.o[(g * A + k) % NB] = mfma_r<TT>(v[g & 1][k], pr[(g * A + k) / NB].lo, st.o[(g * A + k) % NB]);
       r_order();
     }
   }
@@ -966,7 +954,7 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
       if (t < tb || t0 >= whi || t0 + G::KT <= wlo) continue;
       const char* buf = lds + ((t - tb) & 1) * 2 * SIDE;
       f32x16 s[KB];
-      u32x4 pr[2 * KB];
+      RPair pr[2 * KB];
       r_scores<TT, D, KB>(st, buf, lane, s);
       RValues<TT, D, KB> v(buf + SIDE, lane);
       r_softmax<TT, D, KB, FORM>(p, st, s, t0, t0 < flo, t0 + G::KT > fhi, t0 + G::KT <= near, lane, pr);
@@ -1006,7 +994,7 @@ __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUn
       const bool more = t + 1 < te, have = t >= tb;
       const int t0 = t * 32;
       f32x16 s[1];
-      u32x4 pr[2];
+      RPair pr[2];
       if (have) {
         wait_loads<NI>();  // the keys; the values are younger
         r_scores<TT, D, 1>(st, mine, lane, s);
