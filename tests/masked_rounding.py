@@ -72,24 +72,3 @@ def slopes_of(H):
 
 BATCHES = {"decode": ([1] * 6, [0, 1, 40, 63, 200, 900]), "few": ([2, 0, 5, 1], [9, 100, 31, 700]),
            "prompts": ([33, 1, 200, 65], [0, 0, 30, 333])}
-
-
-@pytest.mark.parametrize("batch", list(BATCHES))
-@pytest.mark.parametrize("D", [64, 96, 128, 256])
-@pytest.mark.parametrize("dt", [BF16, F16])
-def test_probabilities_keep_two_parts(dt, D, batch):
-    new, past = BATCHES[batch]
-    st = make_batch(new, past, H=8, KV=2, D=D, block=16, dtype=dt, seed=40)
-    forms = [{}, dict(slopes=slopes_of(8)), dict(window=37, prefix=[3, 0, 150, 70, 5, 9][:len(new)])]
-    for form in forms:
-        check(run(st, **form), *narrow64(st, **form))
-    check(run(st, softcap=20.0), *narrow64(st, softcap=20.0))
-
-
-@pytest.mark.parametrize("dt", [BF16, F16])
-def test_shared_prefixes_keep_two_parts(dt):
-    group_cum, shared = [0, 3, 5], [640, 320]
-    for new in ([1, 1, 2, 1, 1, 1], [30, 1, 20, 1, 70, 40]):
-        st = make_batch(new, [640, 700, 655, 320, 900, 17], H=8, KV=2, D=128, block=16, dtype=dt, seed=41,
-                        group_cum=group_cum, shared=shared)
-        check(run(st, group_cum=group_cum, shared=shared), *narrow64(st))
