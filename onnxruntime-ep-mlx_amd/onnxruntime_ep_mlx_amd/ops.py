@@ -302,8 +302,8 @@ def multi_axis_rotary_append(query, key, value, key_cache, value_cache, cum, pas
                              k_quant_type="NONE", v_quant_type="NONE", q_out=None):
     """Fused RMSNorm + rotary positions of several axes + append (pa_multi_axis_rotary_append).
 
-    ``positions`` int64 [axes, num_tokens] (time, height, width); frequency i turns at the position
-    of its axis: ``axis_sections`` frequencies per axis one section after the other, or in turns
+    ``positions`` int64 [axes, num_tokens] (time, height, width), rows dense or one row expanded over
+    the axes; frequency i turns at the position of its axis: ``axis_sections`` frequencies per axis one section after the other, or in turns
     with ``axes_interleaved``.  cos / sin tables [positions, sum(axis_sections)] in the activation
     dtype or float32.  ``query``, ``key`` and ``value`` are [num_tokens, width] with dense rows
     (slices of packed QKV rows, too).  Keys and values go to their pages; returns the query rows
@@ -347,6 +347,10 @@ def multi_axis_rotary_append(query, key, value, key_cache, value_cache, cum, pas
                        k_quant_type=k_quant_type, v_quant_type=v_quant_type)
     batch = batch_desc(cum, past, block_table, T, slot_mapping, 0,
                        capi.PA_BATCH_SLOTS_DISTINCT if slots_distinct else 0)
+    if len(sections) > 1 and positions.stride(0) == 0:
+        # one row for every axis (text tokens): a single axis turns alike, and the library's stride 0
+        # would stand for dense rows
+        sections = [sum(sections)]
     rot = capi.PaAxisRotary(_ptr(positions), positions.stride(0) if len(sections) > 1 else 0,
                             len(sections),
                             (C.c_int32 * capi.PA_MAX_AXES)(*sections), int(bool(axes_interleaved)),
