@@ -291,7 +291,11 @@ def _rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> int:
         raise ValueError(f"PagedAttention: {name} must be [num_tokens, width] with dense rows")
     if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0]):
         raise ValueError(f"PagedAttention: {name} must match the other rows' dtype and tokens")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if t.shape[0] <= 1:
+        return t.shape[1]
+    if t.stride(0) < t.shape[1]:  # (the library takes a stride of 0 for dense rows)
+        raise ValueError(f"PagedAttention: {name} rows must not overlap (broadcast rows are not taken)")
+    return t.stride(0)
 
 
 def multi_axis_rotary_append(query, key, value, key_cache, value_cache, cum, past, block_table,

@@ -64,3 +64,28 @@ def test_positions_stay_in_their_tensor(calls, T, form):
     flat = pos.as_strided((behind(pos),), (1,))
     for i in range(HALF):
         assert torch.equal(flat[axis[i] * stride:axis[i] * stride + T], pos[want[i]])
+
+
+@pytest.mark.parametrize("T", [1, 2, 7])
+@pytest.mark.parametrize("name,n", [("query", H), ("key", KV), ("value", KV)])
+def test_broadcast_rows_are_refused(calls, name, n, T):
+    row = torch.zeros(1, n * D, dtype=BF16).expand(T, n * D)
+    if T > 1:
+        with pytest.raises(ValueError, match=f"{name} .*overlap"):
+            ep.multi_axis_rotary_append(**inputs(T, **{name: row}))
+        # ... and rows that begin inside the one before
+        with pytest.raises(ValueError, match=f"{name} .*overlap"):
+            ep.multi_axis_rotary_append(**inputs(T, **{name: torch.zeros(T * n * D, dtype=BF16).as_strided((T, n * D), (8, 1))}))
+        assert not calls
+    else:  # a single row is dense whatever its stride
+        ep.multi_axis_rotary_append(**inputs(T, **{name: row}))
+
+
+@pytest.mark.parametrize("T", [1, 7])
+def test_rows_stay_in_their_tensors(calls, T):
+    wide = torch.zeros(T, (H + 2 * KV) * D + 24, dtype=BF16)
+    q, k, v, _ = wide.split([H * D, KV * D, KV * D, 24], 1)
+    ep.multi_axis_rotary_append(**inputs(T, query=q, key=k, value=v))
+    args = calls[0]
+    for t, ptr, ld in ((q, *args[4:6]), (k, *args[6:8]), (v, *args[8:10])):
+        assert ptr == t.data_ptr() and ld >= t.shape[1] and (T - 1) * ld + t.shape[1] <= behind(t)
