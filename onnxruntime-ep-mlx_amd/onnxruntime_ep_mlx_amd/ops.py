@@ -298,6 +298,20 @@ def _rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> int:
     return t.stride(0)
 
 
+def _scales_hold(cache: capi.PaCache, k_scale, v_scale) -> None:
+    """Scales hold what the library reads: fp8 one per block and head, integers one or one per channel."""
+    for name, t, mode in (("k_scale", k_scale, cache.k_quant_type), ("v_scale", v_scale, cache.v_quant_type)):
+        if t is None:
+            continue
+        n = 0
+        if cache.dtype == capi.PA_DTYPE_FP8_E4M3:
+            n = cache.num_blocks * cache.kv_heads
+        elif cache.dtype in (capi.PA_DTYPE_INT8, capi.PA_DTYPE_INT4):
+            n = cache.kv_heads * cache.head_dim if mode == capi.QUANT_TYPES["PER_CHANNEL"] else 1
+        if t.numel() < n:
+            raise ValueError(f"PagedAttention: {name} must hold {n} scales, got {t.numel()}")
+
+
 def multi_axis_rotary_append(query, key, value, key_cache, value_cache, cum, past, block_table,
                              positions, cos_cache, sin_cache, *, num_heads, axis_sections,
                              axes_interleaved=False, rotary_interleaved=0, rotary_offset=0,
@@ -321,7 +335,15 @@ def multi_axis_rotary_append(query, key, value, key_cache, value_cache, cum, pas
     _same_device(dev, (("key_cache", key_cache), ("value_cache", value_cache), ("cum", cum), ("past", past),
                        ("block_table", block_table), ("cos_cache", cos_cache), ("sin_cache", sin_cache),
                        ("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight),
-                       ("slot_mapping", slot_mapping), ("q_out", q_out)))
+                       ("slot_mapping", slot_mapping), ("q_out", q_out), ("k_scale", k_scale),
+                       ("v_scale", v_scale)))
+    if key_cache.dim() != 4 or value_cache is None:
+        raise ValueError("PagedAttention: key_cache and value_cache must be [num_blocks,block_size,kv_num_heads,head_size]")
+    n = cum.numel() - 1
+    if past.numel() < n or block_table.dim() != 2 or block_table.shape[0] < n:
+        raise ValueError("PagedAttention: inconsistent cumulative lengths, past lengths or block table")
+    if slot_mapping is not None and slot_mapping.numel() < key.shape[0]:
+        raise ValueError("PagedAttention: slot_mapping must hold num_tokens slots")
     sections = [int(n) for n in axis_sections]
     if not 1 <= len(sections) <= capi.PA_MAX_AXES:
         raise ValueError(f"PagedAttention: axis_sections must name 1..{capi.PA_MAX_AXES} axes")
@@ -349,6 +371,7 @@ def multi_axis_rotary_append(query, key, value, key_cache, value_cache, cum, pas
         raise ValueError("PagedAttention: q_out without query")
     cache = cache_desc(key_cache, value_cache, k_scale, v_scale, head_dim=head,
                        k_quant_type=k_quant_type, v_quant_type=v_quant_type)
+    _scales_hold(cache, k_scale, v_scale)
     batch = batch_desc(cum, past, block_table, T, slot_mapping, 0,
                        capi.PA_BATCH_SLOTS_DISTINCT if slots_distinct else 0)
     if len(sections) > 1 and positions.stride(0) == 0:
@@ -408,6 +431,7 @@ def _masked_call(q, key_cache, value_cache, cum, past, block_table, share, num_h
     mask = _mask_desc(dev, n, T, num_heads, distance_slopes, prefix_lens, document_starts)
     cache = cache_desc(key_cache, value_cache, k_scale, v_scale, head_dim=q.shape[1] // num_heads,
                        k_quant_type=k_quant_type, v_quant_type=v_quant_type)
+    _scales_hold(cache, k_scale, v_scale)
     batch = batch_desc(cum, past, block_table, T, None, max_query_len,
                        capi.PA_BATCH_NEW_ROWS_IN_CACHE, max_context_len)
     attn = attn_desc(num_heads, scale, softcap, local_window_size, is_causal, head_sink)

@@ -89,3 +89,46 @@ def test_rows_stay_in_their_tensors(calls, T):
     args = calls[0]
     for t, ptr, ld in ((q, *args[4:6]), (k, *args[6:8]), (v, *args[8:10])):
         assert ptr == t.data_ptr() and ld >= t.shape[1] and (T - 1) * ld + t.shape[1] <= behind(t)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(past=torch.zeros(0, dtype=torch.int32)), "inconsistent"),
+    (dict(cum=torch.zeros(3, dtype=torch.int32)), "inconsistent"),
+    (dict(block_table=torch.zeros(4, dtype=torch.int32)), "inconsistent"),
+    (dict(block_table=torch.zeros(1, 2, 2, dtype=torch.int32)), "inconsistent"),
+    (dict(past=torch.zeros(2, dtype=torch.int32), cum=torch.tensor([0, 3, 5], dtype=torch.int32)), "inconsistent"),
+    (dict(slot_mapping=torch.zeros(4, dtype=torch.int32)), "slot_mapping"),
+    (dict(key_cache=torch.zeros(5, 16, KV * D, dtype=BF16)), "key_cache"),
+    (dict(value_cache=None), "value_cache"),
+    (dict(key_cache=torch.zeros(5, 16, KV, D).to(torch.float8_e4m3fn), value_cache=torch.zeros(5, 16, KV, D).to(torch.float8_e4m3fn),
+          k_scale=torch.ones(5, KV), v_scale=torch.ones(4, KV)), "v_scale"),
+    (dict(key_cache=torch.zeros(5, 16, KV, D, dtype=torch.int8), value_cache=torch.zeros(5, 16, KV, D, dtype=torch.int8),
+          k_quant_type="PER_CHANNEL", v_quant_type="PER_TENSOR", k_scale=torch.ones(1), v_scale=torch.ones(1)), "k_scale"),
+    (dict(key_cache=torch.zeros(5, 16, KV, D, dtype=torch.int8), value_cache=torch.zeros(5, 16, KV, D, dtype=torch.int8),
+          k_quant_type="PER_TENSOR", v_quant_type="PER_TENSOR", k_scale=torch.ones(1), v_scale=torch.ones(0)), "v_scale"),
+], ids=lambda x: x if isinstance(x, str) else None)
+def test_short_tensors_are_refused(calls, kw, text):
+    """Every tensor that the library reads by the batch's and the cache's sizes holds as much."""
+    with pytest.raises(ValueError, match=text):
+        ep.multi_axis_rotary_append(**inputs(5, **kw))
+    assert not calls
+
+
+@pytest.mark.parametrize("kw", [
+    dict(k_scale=torch.ones(5, KV), v_scale=torch.ones(4, KV)),
+    dict(k_scale=torch.ones(KV), v_scale=torch.ones(5, KV))])
+def test_masked_attention_refuses_short_scales(calls, kw):
+    x = inputs(5)
+    cache = torch.zeros(5, 16, KV, D).to(torch.float8_e4m3fn)
+    with pytest.raises(ValueError, match="_scale"):
+        ep.masked_attention(x["query"], cache, cache, x["cum"], x["past"], x["block_table"], num_heads=H, **kw)
+    assert not calls
+
+
+def test_every_tensor_is_looked_for_on_the_device(calls, monkeypatch):
+    seen = set()
+    monkeypatch.setattr(ops, "_same_device", lambda index, tensors, contiguous=True: seen.update(n for n, _ in tensors))
+    cache = torch.zeros(5, 16, KV, D).to(torch.float8_e4m3fn)
+    ep.multi_axis_rotary_append(**inputs(5, key_cache=cache, value_cache=cache, v_scale=torch.ones(5, KV), k_scale=torch.ones(5, KV)))
+    assert seen == {"query", "value", "positions", "key_cache", "value_cache", "cum", "past", "block_table", "cos_cache",
+                    "sin_cache", "q_norm_weight", "k_norm_weight", "slot_mapping", "q_out", "k_scale", "v_scale"}
