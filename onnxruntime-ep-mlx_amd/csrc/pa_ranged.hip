@@ -874,17 +874,20 @@ __device__ __forceinline__ uint32_t r_store(const RangedParams& p, const RUnit& 
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(st.o[n][i], 0.0f, sum);
   if ((q.how & kRZero) || (any && (q.how & kRSingle))) {
-    const float fct = (q.how & kRZero) ? 0.0f : finalize_factor(st.m, l, sink);
+    // (zeros outright: an empty row went through the tiles that the others see, and what it summed may be anything)
+    const bool none = q.how & kRZero;
+    const float fct = finalize_factor(st.m, l, sink);
+    auto four = [&](int n, int i) {
+      auto x = [&](int k) { return none ? 0.0f : st.o[n][4 * i + k] * fct; };
+      return pack4<TT>(x(0), x(1), x(2), x(3));
+    };
     uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((int64_t)q.t * p.num_heads + q.h) * D + 8 * h;
     // (the halves exchange every other four dims, so that each stores eight at a time)
 #pragma unroll
     for (int n = 0; n < D / 32; ++n)
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
-        const u32x2 a = pack4<TT>(st.o[n][4 * i] * fct, st.o[n][4 * i + 1] * fct, st.o[n][4 * i + 2] * fct,
-                                  st.o[n][4 * i + 3] * fct);
-        const u32x2 b = pack4<TT>(st.o[n][4 * i + 4] * fct, st.o[n][4 * i + 5] * fct, st.o[n][4 * i + 6] * fct,
-                                  st.o[n][4 * i + 7] * fct);
+        const u32x2 a = four(n, i), b = four(n, i + 1);
         const auto x = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
         const auto y = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
         *reinterpret_cast<u32x4*>(dst + 32 * n + 8 * i) = u32x4{x[0], y[0], x[1], y[1]};
