@@ -72,7 +72,7 @@ typedef struct pa_mask {
 } pa_mask;
 
 /* Attention over the pages under such a mask (mask NULL: plain paged attention).  Layouts of q and
- * out and the attributes as pa_attention; the SEPARATE cache layout.  Workspace: at least the
+ * out and the attributes as pa_attention; the SEPARATE cache layout; out apart from q.  Workspace: at least the
  * queried size.  fp16 / bf16 activations and pages at heads 64, 96, 128 and 256, from caches that
  * begin at 16 bytes, run on matrix cores and want q, out and the workspace at 16 bytes too (refused
  * otherwise); everything else runs without them. */

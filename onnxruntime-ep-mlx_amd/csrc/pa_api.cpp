@@ -895,6 +895,18 @@ pa::AttnParams attn_params(const pa_cache* c, const pa_batch* b, const pa_attn* 
   return p;
 }
 
+// Whether out meets q: pa_masked_attention reads a row's queries in several places, some of them after
+// another has stored that row's output.
+bool out_meets_q(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dtype act, const void* q,
+                 const void* out) {
+  const uintptr_t n = (uintptr_t)b->num_tokens * a->num_heads * c->head_dim * elem_size(act);
+  const uintptr_t x = reinterpret_cast<uintptr_t>(q), y = reinterpret_cast<uintptr_t>(out);
+  return x < y + n && y < x + n;
+}
+int fail_out_meets_q() {
+  return fail(PA_ERR_INVALID_ARGUMENT, "masked attention: out must not overlap q");
+}
+
 int run_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dtype act,
                   const void* q, const void* kn, const void* vn, void* out, void* ws,
                   size_t ws_bytes, int kind, int chunk, hipStream_t s, RunOpts opts = RunOpts()) {
@@ -947,6 +959,7 @@ int run_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dty
   if (need > 0 && (!ws || ws_bytes < need))
     return fail(PA_ERR_INVALID_ARGUMENT, "workspace too small: need %zu bytes, got %zu", need,
                 ws_bytes);
+  if (opts.masked && out_meets_q(c, b, a, act, q, out)) return fail_out_meets_q();
   if (!plain_only(c, b, a, act, pl, opts.host)) {
     const Plan pr = make_plan(c, b, a, act, kind, chunk, opts.linear_cap > 0, opts.linear_cap,
                               plan_images(opts), opts.bias != nullptr, opts.host, true);
@@ -1353,6 +1366,7 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) ||
       (reinterpret_cast<uintptr_t>(ws) & 15))
     return fail(PA_ERR_INVALID_ARGUMENT, "q, out and workspace must be 16-byte aligned");
+  if (out_meets_q(c, b, a, act, q, out)) return fail_out_meets_q();
   pa::RangedParams p{};
   p.q = q;
   p.key_cache = c->key_cache;
