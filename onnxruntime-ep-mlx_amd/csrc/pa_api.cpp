@@ -1410,8 +1410,9 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
   p.causal = a->is_causal ? 1 : 0;
   p.scale = a->scale != 0.0f ? a->scale : 1.0f / std::sqrt((float)c->head_dim);
   p.scale_log2 = std::fabs(p.scale) * pa::kLog2e;
-  p.softcap = a->softcap;
-  p.slope_unit = a->softcap > 0.0f ? 0.5f / a->softcap : 1.0f / std::fabs(p.scale);
+  // (no score comes near a cap of 2^100, and twice a larger one passes fp32)
+  p.softcap = a->softcap < 0x1p100f ? a->softcap : 0.0f;
+  p.slope_unit = p.softcap > 0.0f ? 0.5f / p.softcap : 1.0f / std::fabs(p.scale);
   p.qxor = p.scale < 0.0f ? 0x80008000u : 0u;
   p.slots = r.slots;
   p.per_cu = r.per_cu;

@@ -68,6 +68,8 @@ constexpr float kRAlone = 0.65f;
 // Time of a wide tile on a workgroup over a narrow one's on a wavefront, in the sharing out of workgroups (1, 2 and 3:
 // 64 samples of a prompt of 8190 45, 46 and 47 us for 40; elsewhere within 2 %).
 constexpr float kRWideCost = 1.5f;
+// Softcaps up to which a score may err by steps of the softcap (r_softmax).
+constexpr float kRCapNear = 64.0f;
 // Rows up to which the merge gives each a workgroup, a wavefront; workgroups of the merge of more.
 constexpr int64_t kRJoinWide = 1024, kRJoinRows = 16384;
 constexpr int kRMergeGrid = 2048;
@@ -704,22 +706,43 @@ __device__ __forceinline__ void r_scores(const RState<TT, D>& st, const char* kt
 // Forms of a score: as it is, less a slope times the distance, softcapped (and less that).
 enum RForm { kRPlain = 0, kRSlope = 1, kRCap = 2 };
 
+// tanh(y) / 2 of z = 2 y log2(e).  Near zero by its series (the next term is below 2^-26 of it at 1/4), elsewhere
+// from 1 - 2 / (1 + exp(2 y)), which holds its own bits there.
+__device__ __forceinline__ float half_tanh(float z) {
+  const float y = z * (0.5f / kLog2e), y2 = y * y;
+  float t = __builtin_fmaf(y2, 31.0f / 2835.0f, -17.0f / 630.0f);
+  t = __builtin_fmaf(y2, t, 1.0f / 15.0f);
+  t = __builtin_fmaf(y2, t, -1.0f / 6.0f);
+  t = __builtin_fmaf(y2, t, 0.5f);
+  const float far = 0.5f + __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(z));
+  return fabsf(y) < 0.25f ? y * t : far;
+}
+
 // Bias, mask, the lazy maximum and the probabilities of 32 KB keys at t0, in two parts per 16 keys.
 template <typename TT, int D, int KB, int FORM>
 __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& st, f32x16 (&s)[KB],
                                           int t0, bool low, bool high, bool before, int lane, RPair (&pr)[2 * KB]) {
   const int h = lane >> 5;
-  // A score in log2 units is s * sl + off.  kRCap: softcap tanh(y) = softcap (1 - 2 / (1 + exp(2 y))), of which s keeps
-  // the quotient, so that the exponent's FMA ends it (about 2^-23 of the softcap, far below the types' resolution).
+  // A score in log2 units is s * sl + off.  kRCap: softcap tanh(y), whose last product the exponent's FMA makes.
+  // Up to kRCapNear s keeps the quotient of softcap (1 - 2 / (1 + exp(2 y))): its error, a few steps of 2^-24 of the
+  // softcap, stays below 2^-16, the probabilities' own.  Beyond it s is tanh(y) / 2 to its own bits.
   const float sl = FORM == kRCap ? 2.0f * kLog2e * p.softcap : p.scale_log2;
-  float off = FORM == kRCap ? kLog2e * p.softcap : 0.0f;
+  float off = 0.0f;
   if constexpr (FORM == kRCap) {
     const float ck = 2.0f * p.scale_log2 / p.softcap;
+    if (p.softcap <= kRCapNear) {
+      off = kLog2e * p.softcap;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        s[kb][i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[kb][i] * ck));
+        for (int i = 0; i < 16; ++i)
+          s[kb][i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[kb][i] * ck));
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = half_tanh(s[kb][i] * ck);
+    }
   }
   if (FORM == kRSlope || (FORM == kRCap && p.slopes)) {
     const float far = (float)(st.pos - t0 - 4 * h);
