@@ -796,6 +796,10 @@ struct RunOpts {
 bool plan_images(const RunOpts& o) { return o.images && o.bias == nullptr; }
 
 // Kernel parameters of one launch (plan pl of batch b) of an attention call over workspace ws.
+// The softcap that kernels run with: none for caps from 2^100 on, which no score comes near and
+// which they would take out of fp32's range.
+float capped(float softcap) { return softcap < 0x1p100f ? softcap : 0.0f; }
+
 pa::AttnParams attn_params(const pa_cache* c, const pa_batch* b, const pa_attn* a, const void* q,
                            const void* kn, const void* vn, void* out, void* ws, const Plan& pl,
                            const RunOpts& opts) {
@@ -865,7 +869,7 @@ pa::AttnParams attn_params(const pa_cache* c, const pa_batch* b, const pa_attn* 
   p.max_query_len = b->max_query_len > 0 ? b->max_query_len : b->num_tokens;
   p.scale = a->scale != 0.0f ? a->scale : 1.0f / std::sqrt((float)c->head_dim);
   p.scale_log2 = p.scale * pa::kLog2e;
-  p.softcap = a->softcap;
+  p.softcap = capped(a->softcap);
   p.window = a->local_window_size;
   p.causal = a->is_causal ? 1 : 0;
   p.read_all_from_cache = quant || opts.masked ? 1 : 0;
@@ -1410,8 +1414,7 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
   p.causal = a->is_causal ? 1 : 0;
   p.scale = a->scale != 0.0f ? a->scale : 1.0f / std::sqrt((float)c->head_dim);
   p.scale_log2 = std::fabs(p.scale) * pa::kLog2e;
-  // (no score comes near a cap of 2^100, and twice a larger one passes fp32)
-  p.softcap = a->softcap < 0x1p100f ? a->softcap : 0.0f;
+  p.softcap = capped(a->softcap);
   p.slope_unit = p.softcap > 0.0f ? 0.5f / p.softcap : 1.0f / std::fabs(p.scale);
   p.qxor = p.scale < 0.0f ? 0x80008000u : 0u;
   p.slots = r.slots;

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "pa_mi355x.h"
 #include "pa_mi355x_ext.h"
 
@@ -540,14 +542,37 @@ __host__ __device__ constexpr bool img_head(int d) {
 
 // Softcapped score in log2 units for the matrix-core kernels: cap * tanh(y) * log2(e), y = v * k
 // with k = scale / cap, from the identity tanh(y) = sign(y) (1 - e) / (1 + e), e = exp(-2 |y|):
-// one exponential and one reciprocal (about one ulp each, ~2^-22 absolute in tanh: far below
-// the resolution of bf16 / fp16 scores) instead of a division and the library tanh per score.
-// |y| large: e = 0, tanh = +-1; NaN stays NaN.
+// one exponential and one reciprocal (about one ulp each, ~2^-22 absolute in tanh: below 2^-16
+// of a score's exponent for caps up to kCapNear) instead of a division and the library tanh per
+// score.  |y| large: e = 0, tanh = +-1; NaN stays NaN.
+// FAR (caps beyond kCapNear, which a step of tanh would show in the scores): small arguments by
+// the series of tanh, to their own bits.
+constexpr float kCapNear = 64.0f;
+// tanh(y) / (2 y) for |y| < 1/4 and y2 = y * y (the next term is below 2^-26 of it).
+__device__ __forceinline__ float half_tanh_series(float y2) {
+  float t = __builtin_fmaf(y2, 31.0f / 2835.0f, -17.0f / 630.0f);
+  t = __builtin_fmaf(y2, t, 1.0f / 15.0f);
+  t = __builtin_fmaf(y2, t, -1.0f / 6.0f);
+  return __builtin_fmaf(y2, t, 0.5f);
+}
+template <bool FAR = false>
 __device__ __forceinline__ float softcap_log2(float v, float k, float cap_log2) {
   const float y = v * k;
   const float e = __builtin_amdgcn_exp2f(-2.0f * kLog2e * fabsf(y));
   const float t = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
-  return __builtin_copysignf(t, y) * cap_log2;
+  float x = __builtin_copysignf(t, y);
+  if constexpr (FAR) {
+    x = fabsf(y) < 0.25f ? 2.0f * y * half_tanh_series(y * y) : x;
+    __builtin_amdgcn_sched_barrier(0);  // one score after the other, so that the branch keeps few registers
+  }
+  return x * cap_log2;
+}
+// f(std::true_type) where the cap is beyond kCapNear, else f(std::false_type): one uniform branch
+// around the scores of a step.
+template <typename F>
+__device__ __forceinline__ void softcap_either(float cap_log2, F f) {
+  if (cap_log2 > kCapNear * kLog2e) f(std::true_type{});
+  else f(std::false_type{});
 }
 
 // Final normalisation shared by every attention kernel: the factor that turns an output

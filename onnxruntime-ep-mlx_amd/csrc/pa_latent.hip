@@ -260,10 +260,15 @@ latent_kernel(const AttnParams p) {
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       float x[8];
+      if constexpr (CAP) {
+        softcap_either(cap_l2, [&](auto far) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float sv = e < 4 ? fa[j][e & 3] : fb[j][e & 3];
-        x[e] = CAP ? softcap_log2(sv, cap_k, cap_l2) : sv * scale_log2;
+          for (int e = 0; e < 8; ++e)
+            x[e] = softcap_log2<decltype(far)::value>(e < 4 ? fa[j][e & 3] : fb[j][e & 3], cap_k, cap_l2);
+        });
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (e < 4 ? fa[j][e & 3] : fb[j][e & 3]) * scale_log2;
       }
       if (masked) {
         // positions [vis_lo, min(end, vis_hi)) of the row, one unsigned range test per score

@@ -320,9 +320,16 @@ latent_wide_kernel(const AttnParams p, int rbs) {
             if (more) load_tail(k + 1);
             product(std::false_type{}, sb, sc);
           }
+          if constexpr (CAP) {
+            softcap_either(cap_l2, [&](auto far) __attribute__((always_inline)) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            x[i] = CAP ? softcap_log2(sc[i], cap_k, cap_l2) : sc[i] * scale_log2;
+              for (int i = 0; i < 16; ++i)
+                x[i] = softcap_log2<decltype(far)::value>(sc[i], cap_k, cap_l2);
+            });
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = sc[i] * scale_log2;
+          }
           const int t0 = t_first + kWideKeys * k + 32 * kh;
           if (!(t0 >= all_lo && t0 + 32 <= all_hi)) {
             // positions [vis_lo, vis_hi) of the row, one unsigned range test per score

@@ -630,11 +630,13 @@ __device__ __forceinline__ void img_issue(MxBufT<KB, D>& buf, int wave, int lane
 // same calls do: fp16 hi + lo, or bf16 hi + lo against the bf16 values as they are (kRaw).  (Both parts
 // of an fp16 pair end at 2^-25, so below 2^-8 it holds fewer bits than a bf16 pair and below 2^-25
 // none, which values 2^26 times their neighbours would show.)
+// FAR: softcaps beyond kCapNear (an instance of their own: the branch cost the others 17 registers at
+// head 64, and with them a workgroup per CU).
 // Workgroups per CU: two, bound by registers and from head 128 on by LDS; three to four at head 64
 // and up to three at 96 (33 and 49 KB of LDS).
 constexpr int mx_max_waves(bool img, int d) { return !img ? 2 : d == 64 ? 4 : d == 96 ? 3 : 2; }
 template <typename TT, bool CAP, bool IMG, int D = 128, bool INTC = false, bool F8S = false,
-          bool PREC = false>
+          bool PREC = false, bool FAR = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, mx_max_waves(IMG, D)))) void
 prefill_mx_kernel(const AttnParams p) {
   static_assert(!PREC || (IMG && !INTC && !F8S), "two-part probabilities over images of rows in T");
@@ -825,7 +827,7 @@ prefill_mx_kernel(const AttnParams p) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float v = sc[kb][i];
-        if constexpr (CAP) v = softcap_log2(v, ck, cap_l2);
+        if constexpr (CAP) v = softcap_log2<FAR>(v, ck, cap_l2);
         x[kb][i] = v;
       }
     // per-score position tests only on steps some row does not see whole (one scalar branch):
@@ -1867,6 +1869,17 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(const AttnParams p) 
 // Page kinds of the prefill launch: pages in the activation dtype, integer codes, fp8 codes.
 constexpr int kPkT = 0, kPkInt = 1, kPkF8 = 2;
 
+// prefill_mx_kernel by the call's softcap: none, a usual one, a far one.
+template <typename TT, bool IMG, int D, bool INTC, bool F8S, bool PREC>
+void launch_mx(const AttnParams& p, dim3 grid, hipStream_t s) {
+  if (p.softcap > kCapNear)
+    hipLaunchKernelGGL((prefill_mx_kernel<TT, true, IMG, D, INTC, F8S, PREC, true>), grid, dim3(256), 0, s, p);
+  else if (p.softcap > 0.0f)
+    hipLaunchKernelGGL((prefill_mx_kernel<TT, true, IMG, D, INTC, F8S, PREC>), grid, dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((prefill_mx_kernel<TT, false, IMG, D, INTC, F8S, PREC>), grid, dim3(256), 0, s, p);
+}
+
 template <typename TT, int D>
 hipError_t launch_d(const AttnParams& p, dim3 grid, hipStream_t s, int pk = kPkT) {
   constexpr int NG = kPrefillGroups;
@@ -1882,26 +1895,10 @@ hipError_t launch_d(const AttnParams& p, dim3 grid, hipStream_t s, int pk = kPkT
   }
   if constexpr (img_head(D)) {
     if (p.vimg != nullptr) {
-      if (pk == kPkInt) {
-        if (p.softcap > 0.0f)
-          hipLaunchKernelGGL((prefill_mx_kernel<TT, true, true, D, true>), grid, dim3(256), 0, s, p);
-        else
-          hipLaunchKernelGGL((prefill_mx_kernel<TT, false, true, D, true>), grid, dim3(256), 0, s, p);
-      } else if (pk == kPkF8) {
-        if (p.softcap > 0.0f)
-          hipLaunchKernelGGL((prefill_mx_kernel<TT, true, true, D, false, true>), grid, dim3(256), 0, s, p);
-        else
-          hipLaunchKernelGGL((prefill_mx_kernel<TT, false, true, D, false, true>), grid, dim3(256), 0, s, p);
-      } else if (p.plan_prec) {
-        if (p.softcap > 0.0f)
-          hipLaunchKernelGGL((prefill_mx_kernel<TT, true, true, D, false, false, true>), grid, dim3(256), 0, s, p);
-        else
-          hipLaunchKernelGGL((prefill_mx_kernel<TT, false, true, D, false, false, true>), grid, dim3(256), 0, s, p);
-      } else if (p.softcap > 0.0f) {
-        hipLaunchKernelGGL((prefill_mx_kernel<TT, true, true, D>), grid, dim3(256), 0, s, p);
-      } else {
-        hipLaunchKernelGGL((prefill_mx_kernel<TT, false, true, D>), grid, dim3(256), 0, s, p);
-      }
+      if (pk == kPkInt) launch_mx<TT, true, D, true, false, false>(p, grid, s);
+      else if (pk == kPkF8) launch_mx<TT, true, D, false, true, false>(p, grid, s);
+      else if (p.plan_prec) launch_mx<TT, true, D, false, false, true>(p, grid, s);
+      else launch_mx<TT, true, D, false, false, false>(p, grid, s);
       return hipGetLastError();
     }
   }
@@ -1911,12 +1908,7 @@ hipError_t launch_d(const AttnParams& p, dim3 grid, hipStream_t s, int pk = kPkT
   // probabilities) -- the in-loop fp16 conversion of bf16 values keeps a running power of two per
   // quarter, under which values 2^-29 below the largest seen so far lose bits.
   if constexpr (D == 128 && !std::is_same<TT, TBF16>::value) {
-    const bool cap = p.softcap > 0.0f;
-    if (cap) {
-      hipLaunchKernelGGL((prefill_mx_kernel<TT, true, false>), grid, dim3(256), 0, s, p);
-    } else {
-      hipLaunchKernelGGL((prefill_mx_kernel<TT, false, false>), grid, dim3(256), 0, s, p);
-    }
+    launch_mx<TT, false, D, false, false, false>(p, grid, s);
     return hipGetLastError();
   }
   if (p.softcap > 0.0f)

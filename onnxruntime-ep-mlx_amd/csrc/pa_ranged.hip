@@ -68,8 +68,6 @@ constexpr float kRAlone = 0.65f;
 // Time of a wide tile on a workgroup over a narrow one's on a wavefront, in the sharing out of workgroups (1, 2 and 3:
 // 64 samples of a prompt of 8190 45, 46 and 47 us for 40; elsewhere within 2 %).
 constexpr float kRWideCost = 1.5f;
-// Softcaps up to which a score may err by steps of the softcap (r_softmax).
-constexpr float kRCapNear = 64.0f;
 // Rows up to which the merge gives each a workgroup, a wavefront; workgroups of the merge of more.
 constexpr int64_t kRJoinWide = 1024, kRJoinRows = 16384;
 constexpr int kRMergeGrid = 2048;
@@ -706,16 +704,11 @@ __device__ __forceinline__ void r_scores(const RState<TT, D>& st, const char* kt
 // Forms of a score: as it is, less a slope times the distance, softcapped (and less that).
 enum RForm { kRPlain = 0, kRSlope = 1, kRCap = 2 };
 
-// tanh(y) / 2 of z = 2 y log2(e).  Near zero by its series (the next term is below 2^-26 of it at 1/4), elsewhere
-// from 1 - 2 / (1 + exp(2 y)), which holds its own bits there.
+// tanh(y) / 2 of z = 2 y log2(e).  Near zero by its series, elsewhere from 1 - 2 / (1 + exp(2 y)), which holds its own bits there.
 __device__ __forceinline__ float half_tanh(float z) {
-  const float y = z * (0.5f / kLog2e), y2 = y * y;
-  float t = __builtin_fmaf(y2, 31.0f / 2835.0f, -17.0f / 630.0f);
-  t = __builtin_fmaf(y2, t, 1.0f / 15.0f);
-  t = __builtin_fmaf(y2, t, -1.0f / 6.0f);
-  t = __builtin_fmaf(y2, t, 0.5f);
+  const float y = z * (0.5f / kLog2e);
   const float far = 0.5f + __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(z));
-  return fabsf(y) < 0.25f ? y * t : far;
+  return fabsf(y) < 0.25f ? y * half_tanh_series(y * y) : far;
 }
 
 // Bias, mask, the lazy maximum and the probabilities of 32 KB keys at t0, in two parts per 16 keys.
@@ -724,13 +717,13 @@ __device__ __forceinline__ void r_softmax(const RangedParams& p, RState<TT, D>& 
                                           int t0, bool low, bool high, bool before, int lane, RPair (&pr)[2 * KB]) {
   const int h = lane >> 5;
   // A score in log2 units is s * sl + off.  kRCap: softcap tanh(y), whose last product the exponent's FMA makes.
-  // Up to kRCapNear s keeps the quotient of softcap (1 - 2 / (1 + exp(2 y))): its error, a few steps of 2^-24 of the
+  // Up to kCapNear s keeps the quotient of softcap (1 - 2 / (1 + exp(2 y))): its error, a few steps of 2^-24 of the
   // softcap, stays below 2^-16, the probabilities' own.  Beyond it s is tanh(y) / 2 to its own bits.
   const float sl = FORM == kRCap ? 2.0f * kLog2e * p.softcap : p.scale_log2;
   float off = 0.0f;
   if constexpr (FORM == kRCap) {
     const float ck = 2.0f * p.scale_log2 / p.softcap;
-    if (p.softcap <= kRCapNear) {
+    if (p.softcap <= kCapNear) {
       off = kLog2e * p.softcap;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)

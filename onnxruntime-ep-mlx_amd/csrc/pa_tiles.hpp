@@ -250,11 +250,17 @@ __device__ __forceinline__ float step_scores(const RowState<TT, D>& rs, KeyOp ko
   const float xa = SC ? ksA * scale_log2 : scale_log2, xb = SC ? ksB * scale_log2 : scale_log2;
   const float kxa = KOFF ? koff * xa : 0.0f, kxb = KOFF ? koff * xb : 0.0f;
   const float cap_k = CAP ? scale / cap : 0.0f, cap_l2 = cap * kLog2e;
+  if constexpr (CAP)
+    softcap_either(cap_l2, [&](auto far) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[e] = softcap_log2<decltype(far)::value>((e < 4) ? sa[e & 3] : sb[e & 3], cap_k, cap_l2);
+    });
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float sv = (e < 4) ? sa[e & 3] : sb[e & 3];
     if constexpr (CAP)
-      x[e] = softcap_log2(sv, cap_k, cap_l2);
+      ;  // above
     else if constexpr (FOLD)
       x[e] = sv;
     else if constexpr (KOFF)
