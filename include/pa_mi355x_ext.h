@@ -62,7 +62,7 @@ int pa_multi_axis_rotary_append(const pa_cache* cache, const pa_batch* batch, in
 /* Masks and a bias by distance, each optional (NULL).  Token t = row r of sequence b stands at
  * position i = past[b] + r and sees key j of its sequence iff
  *   max(document_starts[t], i - local_window_size + 1) <= j < max(i + 1, prefix_lens[b])
- * (is_causal 0: up to the sequence's last key), and its score there is
+ * (is_causal 0: up to the sequence's last key; local_window_size -1: no window, else at least 1), and its score there is
  *   softcap(scale * q.k) - distance_slopes[h] * |i - j|.
  * A row that sees no key is zero. */
 typedef struct pa_mask {

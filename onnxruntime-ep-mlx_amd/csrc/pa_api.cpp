@@ -1273,6 +1273,8 @@ int check_masked(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dtyp
                 "masked attention reads the block-table pages: slot_mapping must be NULL");
   if (!std::isfinite(a->scale))
     return fail(PA_ERR_INVALID_ARGUMENT, "scale must be finite");
+  if (a->local_window_size != -1 && a->local_window_size <= 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "local_window_size must be -1 or positive");
   return PA_OK;
 }
 

@@ -465,8 +465,8 @@ def masked_attention(q, key_cache, value_cache, cum, past, block_table, *, num_h
     A token at position i of its sequence sees key j iff max(its document's start,
     i - local_window_size + 1) <= j < max(i + 1, the sequence's prefix length), and its score is
     softcap(scale * q.k) - distance_slopes[h] * |i - j|.  ``document_starts`` int32 [num_tokens],
-    ``prefix_lens`` int32 [batch], ``distance_slopes`` float32 [num_heads]; each may be None.  Rows
-    that see no key are zero.  ``max_query_len`` / ``max_context_len`` bound every sequence's new
+    ``prefix_lens`` int32 [batch], ``distance_slopes`` float32 [num_heads]; each may be None.
+    ``local_window_size`` -1 is no window.  Rows that see no key are zero.  ``max_query_len`` / ``max_context_len`` bound every sequence's new
     tokens / past + new tokens (0 = unknown).  ``out`` may not overlap the queries.  ``workspace``: a uint8 tensor of at least the queried
     size, for callers that keep their own."""
     return _masked_call(q, key_cache, value_cache, cum, past, block_table, None, num_heads, scale,

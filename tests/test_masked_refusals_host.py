@@ -1,5 +1,5 @@
-"""Outputs of pa_masked_attention and pa_shared_prefix_attention that meet the queries are refused on the host,
-before any device work (the pointers are not memory)."""
+"""Calls of pa_masked_attention and pa_shared_prefix_attention that are refused on the host, before any device work
+(the pointers are not memory): outputs that meet the queries, windows of no key."""
 from __future__ import annotations
 
 import ctypes as C
@@ -35,3 +35,12 @@ def test_out_over_the_queries_is_refused_by_the_other_kernel_too(share, off):
     f32 = capi.PA_DTYPE_FLOAT32
     assert call(share, FAKE + off, cache(dt=f32), f32) == capi.PA_ERR_INVALID_ARGUMENT
     assert "overlap" in error()
+
+
+@pytest.mark.parametrize("share", [False, True], ids=["masked", "shared"])
+@pytest.mark.parametrize("act", [BF16, capi.PA_DTYPE_FLOAT32])
+@pytest.mark.parametrize("window", [0, -2, -(1 << 31)])
+def test_windows_of_no_key_are_refused(monkeypatch, share, act, window):
+    monkeypatch.setitem(globals(), "attn", lambda: capi.PaAttn(8, 0.0, 0.0, window, 1, None, 0))
+    assert call(share, 8 * FAKE, cache(dt=act), act) == capi.PA_ERR_INVALID_ARGUMENT
+    assert "local_window_size" in error()
