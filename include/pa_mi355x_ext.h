@@ -92,7 +92,8 @@ typedef struct pa_shared_prefix {
   const int32_t* group_cum;   /* [groups + 1], non-decreasing, within [0, batch] */
   const int32_t* prefix_lens; /* [groups] */
   int32_t groups;             /* >= 1 */
-  int32_t max_prefix_len;     /* host-known bound on prefix_lens; 0 = the block-table capacity */
+  int32_t max_prefix_len;     /* host-known bound on prefix_lens, for the plan and its workspace;
+                               * 0 = the context's own bound */
 } pa_shared_prefix;
 
 /* pa_masked_attention for such groups: the same results up to rounding, the keys and values of a

@@ -1317,9 +1317,9 @@ RangedPlan ranged_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a,
   const int64_t cap = (int64_t)b->max_blocks * c->block_size;
   const int64_t ctx = b->max_context_len > 0 ? std::min<int64_t>(b->max_context_len, cap) : cap;
   // wide items (blocks of up to 128 rows of the sequences and groups with more than 32), narrow ones
-  const int64_t wide = kv * ((mq * g > 32 ? T * g / 128 + std::min<int64_t>(b->batch, T * g / 33) : 0) +
-                             (groups ? T * g / 128 + std::min<int64_t>(groups, T * g / 33) : 0));
-  const int64_t narrow = kv * (b->batch + groups);
+  const int64_t wide_own = kv * (mq * g > 32 ? T * g / 128 + std::min<int64_t>(b->batch, T * g / 33) : 0);
+  const int64_t wide_group = kv * (groups ? T * g / 128 + std::min<int64_t>(groups, T * g / 33) : 0);
+  const int64_t wide = wide_own + wide_group, narrow = kv * (b->batch + groups);
   const int64_t tiles = std::min<int64_t>(cap, INT32_MAX / 2) / 64 + 2;
   if (wide + narrow >= ((int64_t)1 << 23) || (wide + narrow) * tiles > INT32_MAX / 2 || T * g > INT32_MAX)
     return r;
@@ -1329,12 +1329,14 @@ RangedPlan ranged_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a,
   r.whole = ctx <= kRangedWhole && groups == 0;
   r.merge = !r.whole;
   // no more workgroups than there are tiles for
-  const int64_t most = wide * ((ctx + 63) / 64 + 1) + (narrow * ((ctx + 63) / 64 + 1) + 3) / 4;
+  const int64_t prefix = share && share->max_prefix_len > 0 ? std::min<int64_t>(share->max_prefix_len, ctx) : ctx;
+  const int64_t own_tiles = (ctx + 63) / 64 + 1, group_tiles = (prefix + 63) / 64 + 1;
+  const int64_t most = wide_own * own_tiles + wide_group * group_tiles +
+                       (kv * (b->batch * own_tiles + groups * group_tiles) + 3) / 4;
   r.slots = (int)std::max<int64_t>(std::min<int64_t>((int64_t)r.per_cu * device_cus(), most), 2);
   r.narrow_rows = (int)std::min<int64_t>(groups ? 32 : mq * g, 32);
   if (r.merge) {
-    r.part_narrow = 128 * (wide == 0 ? 0 : groups ? wide + std::max<int64_t>(r.slots, wide)
-                                                  : 2 * (int64_t)r.slots);
+    r.part_narrow = 128 * (wide == 0 ? 0 : groups ? wide + r.slots : 2 * (int64_t)r.slots);
     r.part_rows = r.part_narrow +
                   (int64_t)r.narrow_rows * (groups ? 4 * r.slots + narrow : 8 * (int64_t)r.slots);
   }

@@ -399,9 +399,10 @@ __device__ __forceinline__ RItem r_item(const RangedParams& p, const RSource& s,
   r.at = s.first + f * p.kv_heads + kh * r.size;
   return r;
 }
-// Worker of tile x of an item; what lies behind its counted tiles belongs to its last worker.
+// Worker of tile x of an item; what lies behind its counted tiles belongs to its last worker.  (Whole items: 0, for
+// their places in the workspace go by the item alone.)
 __device__ __forceinline__ int r_worker(int per, const RItem& q, int x) {
-  return per > 0 ? (q.at + min(kRStart + x, q.size - 1)) / per : q.item;
+  return per > 0 ? (q.at + min(kRStart + x, q.size - 1)) / per : 0;
 }
 
 // The range [lo, hi) of token t at position pos of sequence b (total keys).
@@ -1156,7 +1157,7 @@ ranged_kernel(const RangedParams p) {
       u.head = x0 <= kRStart;
       u.k0 = u.head ? 0 : (kt + x0 - kRStart) * kRTile;
       u.k1 = x1 == it.size ? INT32_MAX : (kt + x1 - kRStart) * kRTile;
-      u.slot = r_slot(p, kind, per > 0 ? me : it.item, it.item, u.head);
+      u.slot = r_slot(p, kind, per > 0 ? me : 0, it.item, u.head);
       RInfo q;
       uint32_t odd;
       bool wide = false;
