@@ -33,8 +33,9 @@
 // direct loads from the pages into two LDS buffers, one barrier per tile.  Narrow items: a wavefront with a
 // 32-key tile of its own in LDS, the next keys in flight while the values are multiplied, no barrier.
 //
-// Masked keys weigh exactly zero, but zero times an infinite value is NaN in the product: rows that come
-// out not finite are computed again one key at a time, which skips what they do not see.  Tiles read no
+// Masked keys weigh exactly zero, but zero times an infinite value is NaN in the product: rows whose sums of
+// values come out not finite are computed again, a wavefront's together and one key at a time, which skips what
+// they do not see.  Tiles read no
 // key outside [first visible, last visible] of their rows (such places repeat a visible one), so pages
 // behind a sequence's end or before its window may hold anything.
 //
@@ -68,6 +69,8 @@ constexpr float kRAlone = 0.65f;
 // Time of a wide tile on a workgroup over a narrow one's on a wavefront, in the sharing out of workgroups (1, 2 and 3:
 // 64 samples of a prompt of 8190 45, 46 and 47 us for 40; elsewhere within 2 %).
 constexpr float kRWideCost = 1.5f;
+// Least weight of a key that a row sees, beside fp32's smallest: infinite values show however little they weigh.
+constexpr float kRTiny = 0x1p-126f;
 // Rows up to which the merge gives each a workgroup, a wavefront; workgroups of the merge of more.
 constexpr int64_t kRJoinWide = 1024, kRJoinRows = 16384;
 constexpr int kRMergeGrid = 2048;
@@ -494,57 +497,6 @@ __device__ __forceinline__ int64_t r_offset(const RangedParams& p, int b, int kh
   return ((page * p.block_size + pos % p.block_size) * p.kv_heads + kh) * D;
 }
 
-// One row of a unit one key at a time, by one wavefront, written like the others'.
-template <typename TT, int D>
-__device__ __forceinline__ void slow_row(const RangedParams& p, const RUnit& u, const RInfo& q, int rl) {
-  constexpr int NE = (D + 63) / 64;
-  const int lane = hidden(threadIdx.x & 63);
-  using raw = typename TT::raw;
-  float qv[NE], o[NE], m = kNegInf, l = 0.0f;
-  const float slope = p.slopes ? p.slopes[q.h] : 0.0f;
-#pragma unroll
-  for (int k = 0; k < NE; ++k) {
-    const int e = lane + 64 * k;
-    qv[k] = e < D ? TT::to_f32(reinterpret_cast<const raw*>(p.q)[((int64_t)q.t * p.num_heads + q.h) * D + e])
-                  : 0.0f;
-    o[k] = 0.0f;
-  }
-#pragma unroll 1
-  for (int j = q.lo; j < q.hi; ++j) {
-    const int64_t at = r_offset(p, u.s.b0, u.kh, j, D);
-    float part = 0.0f, v[NE];
-#pragma unroll
-    for (int k = 0; k < NE; ++k) {
-      const int e = lane + 64 * k;
-      v[k] = e < D ? TT::to_f32(reinterpret_cast<const raw*>(p.value_cache)[at + e]) : 0.0f;
-      if (e < D) part += qv[k] * TT::to_f32(reinterpret_cast<const raw*>(p.key_cache)[at + e]);
-    }
-    float x = wave_sum(part) * p.scale;
-    if (p.softcap > 0.0f) x = p.softcap * tanhf(x / p.softcap);
-    x = (x - slope * fabsf((float)(q.pos - j))) * kLog2e;
-    const float mn = fmaxf(m, x), ms = mn == kNegInf ? 0.0f : mn;
-    const float a = m == kNegInf ? 0.0f : exp2f(m - mn), w = exp2f(x - ms);
-    l = l * a + w;
-#pragma unroll
-    for (int k = 0; k < NE; ++k) o[k] = o[k] * a + w * v[k];
-    m = mn;
-  }
-  const bool single = q.how & kRSingle;
-  const int64_t row = u.slot + rl;
-  if (!single && row >= p.part_rows) return;
-  const float f = l == l ? finalize_factor(m, l, r_sink<TT>(p, q.h)) : l;
-#pragma unroll
-  for (int k = 0; k < NE; ++k) {
-    const int e = lane + 64 * k;
-    if (e >= D) continue;
-    if (single)
-      reinterpret_cast<raw*>(p.out)[((int64_t)q.t * p.num_heads + q.h) * D + e] = TT::from_f32(o[k] * f);
-    else
-      p.part_o[row * D + e] = o[k];
-  }
-  if (!single && lane == 0) p.part_ml[row] = float2{m, l};
-}
-
 // ------------------------------------------------------------------------------------ the tiles
 // LDS rows of one tile: PITCH bytes each, 16-byte pieces exchanged by an XOR with the row so that the
 // operand reads of 16 lanes meet 16 different bank groups.  Keys are read a row per lane: piece ^ row.
@@ -878,7 +830,7 @@ __device__ __forceinline__ int r_near(const RangedParams& p, const RInfo& q) {
 
 // ------------------------------------------------------------------------------------ a unit
 // The wavefront's rows, final where the unit has all their keys, else as partial rows; returns those that came
-// out not finite, which want slow_row.
+// out not finite, which want slow_rows.
 template <typename TT, int D>
 __device__ __forceinline__ uint32_t r_store(const RangedParams& p, const RUnit& u, const RInfo& q, int rl,
                                             const RState<TT, D>& st, float sink, int lane) {
@@ -893,7 +845,7 @@ __device__ __forceinline__ uint32_t r_store(const RangedParams& p, const RUnit& 
   if ((q.how & kRZero) || (any && (q.how & kRSingle))) {
     // (zeros outright: an empty row went through the tiles that the others see, and what it summed may be anything)
     const bool none = q.how & kRZero;
-    const float fct = finalize_factor(st.m, l, sink);
+    const float fct = fmaxf(finalize_factor(st.m, l, sink), kRTiny);
     auto four = [&](int n, int i) {
       auto x = [&](int k) { return none ? 0.0f : st.o[n][4 * i + k] * fct; };
       return pack4<TT>(x(0), x(1), x(2), x(3));
@@ -921,8 +873,61 @@ __device__ __forceinline__ uint32_t r_store(const RangedParams& p, const RUnit& 
       if (h == 0) p.part_ml[row] = float2{st.m, l};
     }
   }
-  const uint64_t odd = __ballot(any && !(sum == 0.0f && l < __builtin_huge_valf()));
+  // (A sum that is NaN has seen a score that is NaN or infinite: its row is NaN, as it came out.)
+  const uint64_t odd = __ballot(any && sum != 0.0f && l == l);
   return (uint32_t)(odd | (odd >> 32));
+}
+
+// The rows of `odd` again, a key at a time for all of them, so that a key that a row does not see takes no part
+// in it whatever its value; written like the others.  About 1 us per key: a prompt of 8192 with one
+// infinite value 37 ms for 0.9 (row by row 800).
+template <typename TT, int D>
+__device__ __forceinline__ void slow_rows(const RangedParams& p, const RUnit& u, RInfo q, int rl, uint32_t odd) {
+  const int lane = hidden(threadIdx.x & 63), h = lane >> 5;
+  if (!((odd >> (lane & 31)) & 1)) q.how = 0;
+  RState<TT, D> st;
+  r_queries<TT, D>(p, q, lane, st);
+  r_init<TT, D>(q, st);
+  const float sink = r_sink<TT>(p, q.h), slope = p.slopes ? p.slopes[q.h] : 0.0f, scale = fabsf(p.scale);
+  const bool any = q.how & kRAny;
+  const int k0 = half_min(any ? q.lo : INT32_MAX), k1 = half_max(any ? q.hi : 0);
+#pragma unroll 1
+  for (int j = k0; j < k1; ++j) {
+    const int64_t at = r_offset(p, u.s.b0, u.kh, j, D);
+    const uint16_t* kr = reinterpret_cast<const uint16_t*>(p.key_cache) + at + 8 * h;
+    const uint16_t* vr = reinterpret_cast<const uint16_t*>(p.value_cache) + at + 4 * h;
+    float x = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const u32x4 k = *reinterpret_cast<const u32x4*>(kr + 16 * ks);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x = __builtin_fmaf(TT::to_f32((uint16_t)k[i]), TT::to_f32((uint16_t)st.q[ks][i]), x);
+        x = __builtin_fmaf(TT::to_f32((uint16_t)(k[i] >> 16)), TT::to_f32((uint16_t)(st.q[ks][i] >> 16)), x);
+      }
+    }
+    x = (x + half_swap(x)) * scale;
+    if (p.softcap > 0.0f) x = p.softcap * tanhf(x / p.softcap);
+    x = (x - slope * fabsf((float)(q.pos - j))) * kLog2e;
+    const bool seen = j >= st.lo && j < st.hi && x != kNegInf;
+    const float mn = seen ? fmaxf(st.m, x) : st.m, ms = mn == kNegInf ? 0.0f : mn;
+    const float a = st.m == kNegInf ? 0.0f : fmaxf(exp2f(st.m - ms), kRTiny);
+    const float w = seen ? fmaxf(exp2f(x - ms), kRTiny) : 0.0f;
+    st.l = st.l * a + (h == 0 ? w : 0.0f);  // (the halves' sums are added)
+    st.m = mn;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(vr + 32 * n + 2 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = TT::to_f32((uint16_t)(v[e >> 1] >> (16 * (e & 1))));
+          st.o[n][i + e] = st.o[n][i + e] * a + (seen ? w * y : 0.0f);
+        }
+      }
+  }
+  r_store<TT, D>(p, u, q, rl, st, sink, lane);
 }
 
 // A block of 128 rows, by the whole workgroup: wavefront w takes rows 32 w .. 32 w + 31 of every tile.
@@ -1054,7 +1059,7 @@ ranged_kernel(const RangedParams p) {
       lds[WIDE && RGeom<D>::WIDE > 4 * kMine ? RGeom<D>::WIDE : 4 * kMine];
   __shared__ RScan sh;
   const int n = p.groups + p.batch, chunks = (n + kRChunk - 1) / kRChunk;
-  const int wave = uniform(threadIdx.x >> 6);
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   // Pass 0 adds up tiles and items of all sources, pass 1 walks them; both at once if one chunk has them all.
   RTotals t{}, tb{};
   RShare r{};
@@ -1172,12 +1177,7 @@ ranged_kernel(const RangedParams p) {
       else
         odd = narrow_unit<TT, D, FORM>(p, u, lds + wave * kMine, q);
       // rows that came out not finite, again
-      for (; odd; odd &= odd - 1) {
-        const int k = __builtin_ctz(odd);
-        const RInfo w{uniform(__shfl(q.t, k, 64)),  uniform(__shfl(q.h, k, 64)),  uniform(__shfl(q.pos, k, 64)),
-                      uniform(__shfl(q.lo, k, 64)), uniform(__shfl(q.hi, k, 64)), uniform(__shfl(q.how, k, 64))};
-        slow_row<TT, D>(p, u, w, (wide ? 32 * wave : 0) + k);
-      }
+      if (odd) slow_rows<TT, D>(p, u, q, (wide ? 32 * wave : 0) + (lane & 31), odd);
       if (queued) {
         if (threadIdx.x == 0) sh.next = r.wide + queues * ticket + mine;
         __syncthreads();
@@ -1237,7 +1237,8 @@ struct RSum {
   f32x4 o;
   __device__ __forceinline__ void meet(float m2, float l2, f32x4 o2) {
     const float mn = fmaxf(m, m2);
-    const float wa = m == kNegInf ? 0.0f : exp2f(m - mn), wb = m2 == kNegInf ? 0.0f : exp2f(m2 - mn);
+    const float wa = m == kNegInf ? 0.0f : fmaxf(exp2f(m - mn), kRTiny);
+    const float wb = m2 == kNegInf ? 0.0f : fmaxf(exp2f(m2 - mn), kRTiny);
     // (pieces whose scores are all NaN have no maximum, but a sum)
     l = (l == l ? l * wa : l) + (l2 == l2 ? l2 * wb : l2);
     o = o * wa + o2 * wb;
@@ -1262,13 +1263,13 @@ __device__ __forceinline__ RSum r_pieces(const RangedParams& p, const RJoin& j, 
 #pragma unroll
     for (int i = 0; i < kRDepth; ++i)
       if (i0 + i * stride < n) mn = fmaxf(mn, ml[i].x);
-    const float a = s.m == kNegInf ? 0.0f : exp2f(s.m - mn);
+    const float a = s.m == kNegInf ? 0.0f : fmaxf(exp2f(s.m - mn), kRTiny);
     s.l = s.l == s.l ? s.l * a : s.l;
     s.o *= a;
 #pragma unroll
     for (int i = 0; i < kRDepth; ++i)
       if (i0 + i * stride < n) {
-        const float w = ml[i].x == kNegInf ? 0.0f : exp2f(ml[i].x - mn);
+        const float w = ml[i].x == kNegInf ? 0.0f : fmaxf(exp2f(ml[i].x - mn), kRTiny);
         s.l += ml[i].y == ml[i].y ? ml[i].y * w : ml[i].y;
         s.o += o[i] * w;
       }
@@ -1278,7 +1279,7 @@ __device__ __forceinline__ RSum r_pieces(const RangedParams& p, const RJoin& j, 
 }
 template <typename TT>
 __device__ __forceinline__ void r_finish(const RangedParams& p, const RSum& s, int64_t t, int h, int D, int d0) {
-  const float f = s.l == s.l ? finalize_factor(s.m, s.l, r_sink<TT>(p, h)) : s.l;
+  const float f = s.l == s.l ? fmaxf(finalize_factor(s.m, s.l, r_sink<TT>(p, h)), kRTiny) : s.l;
   *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + (t * p.num_heads + h) * D + d0) =
       pack4<TT>(s.o[0] * f, s.o[1] * f, s.o[2] * f, s.o[3] * f);
 }
