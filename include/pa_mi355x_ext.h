@@ -2,7 +2,8 @@
  * pa_mi355x_ext.h — entries of the same library for models beyond the reference operator's
  * attributes: rotary positions of several axes, masks by document and prefix with a bias by
  * distance, and prefixes that several sequences hold in the same pages.  They have no counterpart
- * in the reference; conventions, layouts and descriptors are pa_mi355x.h's.
+ * in the reference; conventions and layouts are pa_mi355x.h's, which declares the entries beside the
+ * others.  Here are their descriptors and contracts.
  *
  * The attention entries read every key and value, the new tokens' rows included, from the
  * block-table pages (pa_multi_axis_rotary_append, pa_rotary_append or pa_reshape_and_cache wrote
@@ -14,10 +15,6 @@
 #define PA_MI355X_EXT_H
 
 #include "pa_mi355x.h"
-
-#ifdef __cplusplus
-extern "C" {
-#endif
 
 /* Rotary positions of several axes (time, height and width of images and video).  Frequency i of
  * [0, rotary_half) turns by the cos / sin row of positions[axis(i)][t].  axes_interleaved 0: the
@@ -41,7 +38,7 @@ typedef struct pa_axis_rotary {
   int32_t rotary_interleaved; /* 0: pairs (i, rotary_half + i); 1: pairs (2 i, 2 i + 1) */
 } pa_axis_rotary;
 
-/* RMSNorm (optional) and multi-axis rotary positions on the query and key rows, queries into
+/* pa_multi_axis_rotary_append: RMSNorm (optional) and multi-axis rotary positions on the query and key rows, queries into
  * q_out, keys and values into their pages.
  *   query/key/value  [num_tokens, heads * head_dim] in act_dtype, consecutive tokens q_stride /
  *                    k_stride / v_stride elements apart (0 = dense; views of packed QKV rows)
@@ -52,17 +49,12 @@ typedef struct pa_axis_rotary {
  * A row is normalised, scaled by the weights and turned in fp32 and rounded to act_dtype once;
  * fp8 and integer caches encode that rounded row.  Slots, -1 entries of batch->slot_mapping and
  * tokens that share a slot are treated as by pa_rotary_append. */
-int pa_multi_axis_rotary_append(const pa_cache* cache, const pa_batch* batch, int32_t num_heads,
-                                pa_dtype act_dtype, const void* query, int64_t q_stride,
-                                const void* key, int64_t k_stride, const void* value,
-                                int64_t v_stride, const pa_axis_rotary* rotary,
-                                const void* q_norm, const void* k_norm, float norm_eps,
-                                void* q_out, pa_stream_t stream);
 
 /* Masks and a bias by distance, each optional (NULL).  Token t = row r of sequence b stands at
  * position i = past[b] + r and sees key j of its sequence iff
  *   max(document_starts[t], i - local_window_size + 1) <= j < max(i + 1, prefix_lens[b])
- * (is_causal 0: up to the sequence's last key; local_window_size -1: no window, else at least 1), and its score there is
+ * (is_causal 0: up to the sequence's last key; local_window_size -1: no window, else at least 1),
+ * and its score there is
  *   softcap(scale * q.k) - distance_slopes[h] * |i - j|.
  * A row that sees no key is zero. */
 typedef struct pa_mask {
@@ -71,17 +63,14 @@ typedef struct pa_mask {
   const int32_t* document_starts; /* [num_tokens]: first key of the token's document */
 } pa_mask;
 
-/* Attention over the pages under such a mask (mask NULL: plain paged attention).  Layouts of q and
- * out and the attributes as pa_attention; the SEPARATE cache layout; out apart from q.  Workspace: at least the
- * queried size.  fp16 / bf16 activations and pages at heads 64, 96, 128 and 256, from caches that
- * begin at 16 bytes, run on matrix cores and want q, out and the workspace at 16 bytes too (refused
- * otherwise); everything else runs without them. */
-size_t pa_masked_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
-                                           const pa_attn* attn, const pa_mask* mask,
-                                           pa_dtype act_dtype);
-int pa_masked_attention(const pa_cache* cache, const pa_batch* batch, const pa_attn* attn,
-                        const pa_mask* mask, pa_dtype act_dtype, const void* q, void* out,
-                        void* workspace, size_t workspace_bytes, pa_stream_t stream);
+/* pa_masked_attention: attention over the pages under such a mask (mask NULL: plain paged
+ * attention).  Layouts of q and out and the attributes as pa_attention; the SEPARATE cache layout; out
+ * apart from q.  Workspace: at least the size that pa_masked_attention_workspace_bytes gives.
+ * fp16 / bf16 activations and pages at heads 64, 96, 128 and 256, from caches that begin at 16 bytes,
+ * run on matrix cores and want q, out and the workspace at 16 bytes too (refused otherwise).
+ * Everything else runs without them, many times as long on prompts: other types and heads, byte-coded
+ * pages, and calls whose blocks of 128 rows times their tables' tiles of 64 keys pass 2^30 (a prompt of
+ * 400,000 tokens at 64 heads). */
 
 /* Groups of consecutive sequences whose first keys are the same, in the same pages: group i holds
  * sequences [group_cum[i], group_cum[i + 1]) and their first prefix_lens[i] keys.  The caller
@@ -96,19 +85,8 @@ typedef struct pa_shared_prefix {
                                * 0 = the context's own bound */
 } pa_shared_prefix;
 
-/* pa_masked_attention for such groups: the same results up to rounding, the keys and values of a
- * prefix read once for all the rows of its group. */
-size_t pa_shared_prefix_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
-                                                  const pa_attn* attn,
-                                                  const pa_shared_prefix* share,
-                                                  const pa_mask* mask, pa_dtype act_dtype);
-int pa_shared_prefix_attention(const pa_cache* cache, const pa_batch* batch, const pa_attn* attn,
-                               const pa_shared_prefix* share, const pa_mask* mask,
-                               pa_dtype act_dtype, const void* q, void* out, void* workspace,
-                               size_t workspace_bytes, pa_stream_t stream);
-
-#ifdef __cplusplus
-} /* extern "C" */
-#endif
+/* pa_shared_prefix_attention: pa_masked_attention for such groups, with the same results up to
+ * rounding.  On matrix cores the keys and values of a prefix are read once for all the rows of its
+ * group (once per 128 of them), otherwise for every row. */
 
 #endif /* PA_MI355X_EXT_H */

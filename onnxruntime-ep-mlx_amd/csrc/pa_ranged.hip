@@ -15,7 +15,8 @@
 // between both kinds by their tiles.  A kind's tiles form a flat list, cut into equal stretches whatever
 // item borders lie inside: an item that meets several workers leaves (m, l, O) of each in fp32 and the
 // merge joins them, as it joins a row's shared and own keys.  Where it costs no more (r_share), workgroups
-// take whole wide items instead, in turns, longest first, every other turn backwards; or, where documents
+// take whole wide items instead, in turns, each sequence's longest first and the sequences in their order, every
+// other turn backwards; or, where documents
 // hide what items cost, from queues.  The plan is a scan over the lengths that every workgroup makes for
 // itself, from the device's metadata.
 //
@@ -1081,7 +1082,7 @@ ranged_kernel(const RangedParams p) {
       end = per > 0 ? min(at + per, pick(t.tiles, kind)) : pick(t.items, kind);
       stride = kind ? (p.slots - r.wide) * 4 : r.wide;
       // the sources' places, for the merge
-      if (blockIdx.x == 0 && threadIdx.x == 0) p.table[0] = RTable{{r.per[0], r.per[1], t.items[0], r.wide}};
+      if (blockIdx.x == 0 && threadIdx.x == 0) p.table[0] = RTable{{r.per[0], r.per[1]}};
       if (c == -1) {
         t = RTotals{};
         continue;

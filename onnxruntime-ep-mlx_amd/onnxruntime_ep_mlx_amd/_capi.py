@@ -41,11 +41,6 @@ PA_ERR_OUT_OF_MEMORY = 4
 
 # Every function the header declares, in declaration order (checked by the CPU test suite).
 EXPORTS = (
-    "pa_masked_attention",
-    "pa_masked_attention_workspace_bytes",
-    "pa_multi_axis_rotary_append",
-    "pa_shared_prefix_attention",
-    "pa_shared_prefix_attention_workspace_bytes",
     "pa_last_error", "pa_version",
     "pa_pool_create", "pa_pool_destroy", "pa_pool_k_ptr", "pa_pool_v_ptr",
     "pa_pool_k_scale_ptr", "pa_pool_v_scale_ptr", "pa_pool_bytes",
@@ -53,9 +48,11 @@ EXPORTS = (
     "pa_attention_workspace_bytes", "pa_attention_workspace_bytes_ex",
     "pa_attention", "pa_attention_ex",
     "pa_paged_attention_workspace_bytes", "pa_paged_attention", "pa_paged_attention_static",
-    "pa_paged_attention_claim",
     "pa_group_query_attention_workspace_bytes", "pa_group_query_attention",
-    "pa_group_query_attention_claim",
+    "pa_paged_attention_claim", "pa_group_query_attention_claim",
+    "pa_multi_axis_rotary_append",
+    "pa_masked_attention_workspace_bytes", "pa_masked_attention",
+    "pa_shared_prefix_attention_workspace_bytes", "pa_shared_prefix_attention",
 )
 
 

@@ -484,7 +484,8 @@ def shared_prefix_attention(q, key_cache, value_cache, cum, past, block_table, g
                             workspace=None):
     """masked_attention for groups of consecutive sequences whose first keys lie in the same pages
     (pa_shared_prefix_attention): sequences [group_cum[i], group_cum[i + 1]) share their first
-    ``shared_lens[i]`` keys, which are read once for all of them.  ``group_cum`` int32 [groups + 1],
+    ``shared_lens[i]`` keys, which are read once for all of them where matrix cores take the call (fp16 /
+    bf16 rows and pages at heads 64, 96, 128 and 256).  ``group_cum`` int32 [groups + 1],
     ``shared_lens`` int32 [groups]; the block tables of a group name the same pages for those keys.
     ``max_prefix_len`` bounds ``shared_lens`` (0 = unknown).  ``prefix_lens`` are masked_attention's:
     leading keys that every row of a sequence sees."""
