@@ -15,10 +15,9 @@
 // between both kinds by their tiles.  A kind's tiles form a flat list, cut into equal stretches whatever
 // item borders lie inside: an item that meets several workers leaves (m, l, O) of each in fp32 and the
 // merge joins them, as it joins a row's shared and own keys.  Where it costs no more (r_share), workgroups
-// take whole wide items instead, in turns, each sequence's longest first and the sequences in their order, every
-// other turn backwards; or, where documents
-// hide what items cost, from queues.  The plan is a scan over the lengths that every workgroup makes for
-// itself, from the device's metadata.
+// take whole wide items instead, in turns, each sequence's longest first and the sequences in their order,
+// every other turn backwards; or, where documents hide what items cost, from queues.  The plan is a scan over
+// the lengths that every workgroup makes for itself, from the device's metadata.
 //
 // Both products run transposed on 32x32x16 tiles, so that a lane holds one query row:
 //   S^T[key][row] = K Q^T   (A: 32 keys x 16 dims from LDS, B: the queries in registers)
@@ -26,7 +25,7 @@
 //                            score product leaves them)
 // A row's maximum and sum need one exchange between the lane halves, and its range, slope and position
 // are scalars of the lane.  Probabilities enter the second product in two parts of the activation type
-// (off by at most 2^-17 of themselves in bf16, 2^-20 in fp16, as in the other attention kernels: one part
+// (off by at most 2^-17 of themselves in bf16, 2^-20 in fp16, as in the streaming decode: one part
 // alone erred as much as the output's own rounding), two products against one read of the values; scores,
 // statistics and sums are fp32.
 //
@@ -36,15 +35,14 @@
 //
 // Masked keys weigh exactly zero, but zero times an infinite value is NaN in the product: rows whose sums of
 // values come out not finite are computed again, a wavefront's together and one key at a time, which skips what
-// they do not see.  Tiles read no
-// key outside [first visible, last visible] of their rows (such places repeat a visible one), so pages
-// behind a sequence's end or before its window may hold anything.
+// they do not see.  Tiles read no key outside [first visible, last visible] of their rows (such places repeat a
+// visible one), so pages behind a sequence's end or before its window may hold anything.
 //
-// What bounds it (GPU times of a call, merge included).  A prompt of 8192, 32 heads of 128: 547 us, 1004
-// TFLOP/s, products and the softmax's vector instructions about equal; head 64, with twice the scores per
-// product, 745 us, head 256 630 us.  64 sequences of up to 8192 keys, one token each: 213 us, 5.5 TB/s
-// from HBM.  Small calls: 5 us of dependent loads and the scan before the first item, 2 us to its first
-// tile, 3 us per launch.
+// What bounds it (GPU times of a call, merge included).  Prompts of 8192: 32 heads of 128 in 746 us, 737
+// TFLOP/s of the two products, 1105 with the second part of the probabilities, the softmax's vector instructions
+// behind them in turn; 64 heads of 64 in 945 us (twice the scores per product), 16 heads of 256 in 767.  64
+// sequences of up to 8192 keys, one token each: 212 us, 5.8 TB/s from HBM.  Small calls: 5 us of dependent
+// loads and the scan before the first item, 2 us to its first tile, 3 us per launch.
 #include <algorithm>
 
 #include "pa_tiles.hpp"
@@ -60,15 +58,16 @@ constexpr int kRTile = 64;     // keys per unit of cost
 constexpr int kRWide = 128;    // rows of a block of four wavefronts
 constexpr int kRNarrow = 32;   // rows of a block whose wavefronts split the keys
 constexpr int kRChunk = 256;   // sources scanned at a time, one per thread
-// What an item's start and end cost, in tiles (8 instead: 64 samples of a prompt 53 us for 49).
+// What an item's start and end cost, in tiles (8 instead: 64 samples of a prompt of 8176 41 us for 39).
 constexpr int kRStart = 4;
-// What partial rows and their merge cost, in tiles of every worker: 3, 8 and 20 gave 640, 641 and 556 us over a
-// prompt of 8192, 244, 210 and 210 over prompts of 1001 - 2500 at head 64; at 20, 36 us for systems' prompts as at 3.
+// What partial rows and their merge cost, in tiles of every worker: 3, 8 and 20 gave 826, 836 and 748 us over a
+// prompt of 8192, 236, 214 and 213 over six prompts of 1001 - 2500 at head 64; 25 each for 40 samples of 1500.
 constexpr float kRCut = 20.0f;
-// Time of a tile where a workgroup has its CU to itself (1.0 instead: a prompt of 1024 44.6 us for 41.7).
+// Time of a tile where a workgroup has its CU to itself (1.0 instead: 1024 tokens over 1000 keys 70 us for
+// 62, over 3000 115 for 109).
 constexpr float kRAlone = 0.65f;
 // Time of a wide tile on a workgroup over a narrow one's on a wavefront, in the sharing out of workgroups (1, 2 and 3:
-// 64 samples of a prompt of 8190 45, 46 and 47 us for 40; elsewhere within 2 %).
+// 64 samples of a prompt of 8176 40, 45 and 44 us for 39; 40 samples of 1500 26, 25 and 25 for 25).
 constexpr float kRWideCost = 1.5f;
 // Least weight of a key that a row sees, beside fp32's smallest: infinite values show however little they weigh.
 constexpr float kRTiny = 0x1p-126f;
@@ -508,8 +507,9 @@ struct RGeom {
   static constexpr int PITCH = D == 96 ? 256 : 2 * D;
   static constexpr int CPR = PITCH / 16;     // pieces per row
   static constexpr int RPI = 64 / CPR;       // rows per load instruction
-  // Keys of a wide tile, two of which are buffered.  (Tiles of 32 keys, four deep: 626 us for 554 over a prompt of
-  // 8192 at head 128; four deep at head 256 664 for 647: what is loaded a tile ahead is there in time.)
+  // Keys of a wide tile, two of which are buffered.  (Tiles of 32 keys, four deep: 626 us for 554 over a
+  // prompt of 8192 at head 128, four deep at head 256 664 for 647, with one part of the probabilities: what is
+  // loaded a tile ahead is there in time.)
   static constexpr int KT = D > 128 ? 32 : 64;
   static constexpr int WIDE = 2 * 2 * KT * PITCH;
   static constexpr int NARROW = 4 * 2 * 32 * PITCH;   // four wavefronts' tiles of 32 keys
@@ -969,7 +969,8 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
     for (int t = tb - 1; t < te; ++t) {
       if (t >= tb) wait_loads<0>();
       barrier();
-      // (at once: between the products they cost more, 735 us for 627 over a prompt of 8192 at head 256)
+      // (at once: between the products they cost more, 735 us for 627 over a prompt of 8192 at head 256,
+      // with one part of the probabilities)
       if (t + 1 < te) {
         const uint32_t put = base + ((t + 1 - tb) & 1) * 2 * SIDE;
         const int pos = (t + 1) * G::KT + wave * GR;
