@@ -21,7 +21,7 @@
  * axes' sections follow each other (the first sections[0] frequencies on axis 0, the next
  * sections[1] on axis 1, ...); 1: they take turns, axis(i) = i % axes while i < axes *
  * sections[i % axes], axis 0 beyond.  A pair whose position lies outside [0, rotary_positions) is
- * left unturned. */
+ * left unturned.  (One row of positions for every axis: axes 1 and one section.) */
 #define PA_MAX_AXES 4
 typedef struct pa_axis_rotary {
   const int64_t* positions; /* [axes, num_tokens] */
