@@ -521,6 +521,26 @@ int pa_shared_prefix_attention(const pa_cache* cache, const pa_batch* batch, con
                                pa_dtype act_dtype, const void* q, void* out, void* workspace,
                                size_t workspace_bytes, pa_stream_t stream);
 
+/* Entries whose descriptors and contracts are in pa_mi355x_upkeep.h. */
+struct pa_drafts;
+struct pa_eviction;
+size_t pa_tree_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
+                                         const pa_attn* attn, pa_dtype act_dtype);
+int pa_tree_attention(const pa_cache* cache, const pa_batch* batch, const pa_attn* attn,
+                      const int32_t* parents, pa_dtype act_dtype, const void* q, void* out,
+                      void* workspace, size_t workspace_bytes, pa_stream_t stream);
+int pa_accept_drafts(const pa_cache* cache, const pa_batch* batch, const struct pa_drafts* drafts,
+                     pa_stream_t stream);
+size_t pa_accumulating_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
+                                                 const pa_attn* attn, int32_t observed_rows,
+                                                 pa_dtype act_dtype);
+int pa_accumulating_attention(const pa_cache* cache, const pa_batch* batch, const pa_attn* attn,
+                              float* key_weights, int32_t observed_rows, pa_dtype act_dtype,
+                              const void* q, void* out, void* workspace, size_t workspace_bytes,
+                              pa_stream_t stream);
+int pa_evict_keys(const pa_cache* cache, const pa_batch* batch, const struct pa_eviction* eviction,
+                  pa_stream_t stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -19,6 +19,7 @@
 #include "pa_device.hpp"
 #include "pa_mi355x.h"
 #include "pa_mi355x_ext.h"
+#include "pa_mi355x_upkeep.h"
 
 namespace {
 
@@ -786,6 +787,11 @@ struct RunOpts {
   // pa_masked_attention: its mask, and every key and value, the new rows included, from the pages
   bool masked = false;
   const pa_mask* mask = nullptr;
+  // drafted trees and accounts (see RangedParams)
+  const uint32_t* tree_bits = nullptr;
+  const int32_t* tree_lag = nullptr;
+  int tree_words = 0;
+  float* row_stats = nullptr;
   bool images = true;  // operand images allowed (see make_plan)
   HostLens host;       // host metadata lengths (LATENT chunk sizing)
 };
@@ -879,6 +885,10 @@ pa::AttnParams attn_params(const pa_cache* c, const pa_batch* b, const pa_attn* 
     p.prefix_lens = opts.mask->prefix_lens;
     p.doc_starts = opts.mask->document_starts;
   }
+  p.tree_bits = opts.tree_bits;
+  p.tree_lag = opts.tree_lag;
+  p.tree_words = opts.tree_words;
+  p.row_stats = opts.row_stats;
   p.k_quant = c->k_quant_type;
   p.v_quant = c->v_quant_type;
   p.v_head_dim = a->v_head_size > 0 ? a->v_head_size : c->head_dim;
@@ -1353,28 +1363,28 @@ size_t masked_workspace(const pa_cache* c, const pa_batch* b, const pa_attn* a,
   return r.on ? r.bytes() : ws_need(c, b, a, act, 3, 0).best;
 }
 
-int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, const pa_mask* mask,
-                     const pa_shared_prefix* share, pa_dtype act, const void* q, void* out,
-                     void* ws, size_t ws_bytes, hipStream_t s) {
-  const int rc = check_masked(c, b, a, act);
-  if (rc) return rc;
-  const RangedPlan r = ranged_plan(c, b, a, share, act);
-  // Other types and head sizes: the VALU kernel, which reads a shared prefix for every row
-  if (!r.on)
-    return run_attention(c, b, a, act, q, nullptr, nullptr, out, ws, ws_bytes, 3, 0, s,
-                         masked_opts(mask));
+// Checks beyond check_masked's of a call on the matrix-core kernel, or (matrix false) on another one.
+int check_ranged(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dtype act, const void* q,
+                 const void* out, const void* ws, size_t ws_bytes, size_t need, bool matrix) {
   if (!q || !out) return fail(PA_ERR_INVALID_ARGUMENT, "q/out pointers are NULL");
   if (a->v_head_size > 0 && a->v_head_size != c->head_dim)
     return fail(PA_ERR_INVALID_ARGUMENT, "SEPARATE layout requires equal key and value head sizes");
   if (!(a->softcap >= 0.0f) || !std::isfinite(a->softcap))
     return fail(PA_ERR_INVALID_ARGUMENT, "softcap must be finite and non-negative");
-  if (!ws || ws_bytes < r.bytes())
-    return fail(PA_ERR_INVALID_ARGUMENT, "workspace too small: need %zu bytes, got %zu", r.bytes(),
+  if (!ws || ws_bytes < need)
+    return fail(PA_ERR_INVALID_ARGUMENT, "workspace too small: need %zu bytes, got %zu", need,
                 ws_bytes);
-  if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) ||
-      (reinterpret_cast<uintptr_t>(ws) & 15))
+  if (matrix && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15))
+    return fail(PA_ERR_INVALID_ARGUMENT, "q, out and workspace must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(ws) & 15)
     return fail(PA_ERR_INVALID_ARGUMENT, "q, out and workspace must be 16-byte aligned");
   if (out_meets_q(c, b, a, act, q, out)) return fail_out_meets_q();
+  return PA_OK;
+}
+
+// Its parameters over workspace ws (NULL: another kernel runs, and these hold the call alone).
+pa::RangedParams ranged_params(const pa_cache* c, const pa_batch* b, const pa_attn* a, const void* q,
+                               void* out, void* ws, const RangedPlan& r) {
   pa::RangedParams p{};
   p.q = q;
   p.key_cache = c->key_cache;
@@ -1384,23 +1394,12 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
   p.block_table = b->block_table;
   p.head_sink = a->head_sink;
   p.out = out;
-  if (mask) {
-    p.slopes = mask->distance_slopes;
-    p.prefix_lens = mask->prefix_lens;
-    p.doc_starts = mask->document_starts;
-  }
-  if (share) {
-    p.group_cum = share->group_cum;
-    p.shared_lens = share->prefix_lens;
-    p.groups = share->groups;
-  }
   char* base = reinterpret_cast<char*>(ws);
-  p.part_o = reinterpret_cast<float*>(base);
-  p.part_ml = reinterpret_cast<float2*>(base + r.o_bytes);
-  p.table = reinterpret_cast<pa::RTable*>(base + r.o_bytes + r.ml_bytes);
-  // Documents hide what items cost: where every workgroup has several, they take them from a queue.
-  if (p.doc_starts && (int64_t)b->num_tokens * (a->num_heads / c->kv_heads) / 128 * c->kv_heads >= 2 * r.slots)
-    p.queue = reinterpret_cast<int32_t*>(base + r.bytes() - pa::kRQueueBytes);
+  if (base) {
+    p.part_o = reinterpret_cast<float*>(base);
+    p.part_ml = reinterpret_cast<float2*>(base + r.o_bytes);
+    p.table = reinterpret_cast<pa::RTable*>(base + r.o_bytes + r.ml_bytes);
+  }
   p.num_blocks = c->num_blocks;
   p.part_rows = r.part_rows;
   p.part_narrow = r.part_narrow;
@@ -1428,9 +1427,123 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
   p.whole = r.whole ? 1 : 0;
   p.merge = r.merge ? 1 : 0;
   p.wide = r.wide ? 1 : 0;
+  return p;
+}
+
+int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, const pa_mask* mask,
+                     const pa_shared_prefix* share, pa_dtype act, const void* q, void* out,
+                     void* ws, size_t ws_bytes, hipStream_t s) {
+  int rc = check_masked(c, b, a, act);
+  if (rc) return rc;
+  const RangedPlan r = ranged_plan(c, b, a, share, act);
+  // Other types and head sizes: the VALU kernel, which reads a shared prefix for every row
+  if (!r.on)
+    return run_attention(c, b, a, act, q, nullptr, nullptr, out, ws, ws_bytes, 3, 0, s,
+                         masked_opts(mask));
+  if ((rc = check_ranged(c, b, a, act, q, out, ws, ws_bytes, r.bytes(), true))) return rc;
+  pa::RangedParams p = ranged_params(c, b, a, q, out, ws, r);
+  if (mask) {
+    p.slopes = mask->distance_slopes;
+    p.prefix_lens = mask->prefix_lens;
+    p.doc_starts = mask->document_starts;
+  }
+  if (share) {
+    p.group_cum = share->group_cum;
+    p.shared_lens = share->prefix_lens;
+    p.groups = share->groups;
+  }
+  // Documents hide what items cost: where every workgroup has several, they take them from a queue.
+  if (p.doc_starts && (int64_t)b->num_tokens * (a->num_heads / c->kv_heads) / 128 * c->kv_heads >= 2 * r.slots)
+    p.queue = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(ws) + r.bytes() - pa::kRQueueBytes);
   const hipError_t e = pa::launch_ranged(p, act, s);
   if (e != hipSuccess) return hip_fail(e, "masked attention launch");
   return PA_OK;
+}
+
+// ------------------------------------------------------------------------------ drafted trees
+// Words of a node's bits, and the workspace: the bits and lags, then the attention's own.
+struct TreePlan {
+  int words = 0;
+  size_t bits_bytes = 0, lag_bytes = 0, attn_bytes = 0;
+  RangedPlan r;
+  size_t bytes() const { return bits_bytes + lag_bytes + attn_bytes; }
+};
+TreePlan tree_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dtype act) {
+  TreePlan t;
+  const int nodes = std::min(b->max_query_len > 0 ? std::min(b->max_query_len, b->num_tokens) : b->num_tokens,
+                             PA_MAX_TREE_NODES);
+  t.words = std::max((nodes + 31) / 32, 1);
+  t.bits_bytes = align256((size_t)b->num_tokens * t.words * sizeof(uint32_t));
+  t.lag_bytes = align256((size_t)b->num_tokens * sizeof(int32_t));
+  t.r = ranged_plan(c, b, a, nullptr, act);
+  t.attn_bytes = t.r.on ? t.r.bytes() : ws_need(c, b, a, act, 3, 0).best;
+  return t;
+}
+
+// ------------------------------------------------------------------------------ accounts
+// Rows of a chunk whose sums over the rows a workgroup keeps, and the workspace: the rows' constants, then their scores
+// or the chunks' sums, then the attention's own.
+struct AccountPlan {
+  bool scores = false;
+  int chunks = 0, chunk_rows = 0, keys = 0;
+  int64_t ld = 0;
+  size_t stat_bytes = 0, sum_bytes = 0, attn_bytes = 0;
+  RangedPlan r;
+  size_t bytes() const { return stat_bytes + sum_bytes + attn_bytes; }
+};
+AccountPlan account_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a, int observed, pa_dtype act) {
+  AccountPlan t;
+  const int64_t g = a->num_heads / c->kv_heads, T = b->num_tokens, z = (int64_t)b->batch * c->kv_heads;
+  const int64_t mq = std::min<int64_t>(b->max_query_len > 0 ? b->max_query_len : T, T);
+  t.keys = max_ctx_bound(c, b);
+  if (b->max_context_len > 0) t.keys = std::min(t.keys, b->max_context_len);
+  t.ld = ((int64_t)t.keys + 63) / 64 * 64;
+  t.r = ranged_plan(c, b, a, nullptr, act);
+  t.attn_bytes = t.r.on ? t.r.bytes() : ws_need(c, b, a, act, 3, 0).best;
+  t.stat_bytes = align256((size_t)T * a->num_heads * sizeof(float));
+  // every sequence's rows of a kv-head on a wavefront of their own
+  t.scores = t.r.on && !t.r.wide;
+  if (t.scores) {
+    t.sum_bytes = align256((size_t)T * a->num_heads * t.ld * sizeof(float));
+    return t;
+  }
+  // as many chunks as fill the GPU several times, of 512 rows at least
+  const int64_t rows = std::max<int64_t>((observed > 0 ? std::min<int64_t>(observed, mq) : mq) * g, 1);
+  const int64_t blocks = (t.ld + 255) / 256 * z;
+  const int64_t want = std::min<int64_t>((8 * (int64_t)device_cus() + blocks - 1) / std::max<int64_t>(blocks, 1), (rows + 511) / 512);
+  t.chunk_rows = (int)(((rows + want - 1) / want + 31) / 32 * 32);
+  t.chunks = (int)((rows + t.chunk_rows - 1) / t.chunk_rows);
+  t.sum_bytes = align256((size_t)t.chunks * z * t.ld * sizeof(float));
+  return t;
+}
+
+// Checks of the entries that move rows, and what the kernels need of the caches.
+int check_rows(const pa_cache* c, int batch, int max_blocks, const int32_t* table, const int32_t* lens) {
+  if (!c) return fail(PA_ERR_INVALID_ARGUMENT, "cache descriptor is NULL");
+  const bool coded = c->dtype == PA_DTYPE_FP8_E4M3 || is_int_cache(c->dtype);
+  const int rc = check_cache(c, coded ? PA_DTYPE_BFLOAT16 : c->dtype);
+  if (rc) return rc;
+  if (!c->value_cache) return fail(PA_ERR_UNSUPPORTED, "the SEPARATE cache layout is required");
+  if (batch < 1 || batch > 65535 || max_blocks < 1)
+    return fail(PA_ERR_INVALID_ARGUMENT, "batch must be 1..65535 sequences with at least one block each");
+  if (!table || !lens) return fail(PA_ERR_INVALID_ARGUMENT, "metadata pointers are NULL");
+  return PA_OK;
+}
+pa::RowsParams rows_params(const pa_cache* c, const pa_batch* b) {
+  pa::RowsParams p{};
+  p.key_cache = reinterpret_cast<char*>(c->key_cache);
+  p.value_cache = reinterpret_cast<char*>(c->value_cache);
+  p.k_scale = c->k_scale;
+  p.v_scale = c->v_scale;
+  p.block_table = b->block_table;
+  p.num_blocks = c->num_blocks;
+  p.block_size = c->block_size;
+  p.kv_heads = c->kv_heads;
+  p.head_bytes = (int32_t)cache_head_bytes(c->dtype, c->head_dim);
+  p.batch = b->batch;
+  p.max_blocks = b->max_blocks;
+  p.fp8 = c->dtype == PA_DTYPE_FP8_E4M3 ? 1 : 0;
+  return p;
 }
 
 }  // namespace
@@ -1464,6 +1577,186 @@ int pa_shared_prefix_attention(const pa_cache* cache, const pa_batch* batch, con
   if (rc) return rc;
   return masked_attention(cache, batch, attn, mask, share, act_dtype, q, out, workspace,
                           workspace_bytes, reinterpret_cast<hipStream_t>(stream));
+}
+
+// ------------------------------------------------------------------------------ drafted trees
+size_t pa_tree_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
+                                         const pa_attn* attn, pa_dtype act_dtype) {
+  if (!cache || !batch || !attn || cache->kv_heads <= 0 || batch->batch <= 0 || batch->num_tokens <= 0) return 0;
+  return tree_plan(cache, batch, attn, act_dtype).bytes();
+}
+
+int pa_tree_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, const int32_t* parents,
+                      pa_dtype act, const void* q, void* out, void* ws, size_t ws_bytes,
+                      pa_stream_t stream) {
+  int rc = check_masked(c, b, a, act);
+  if (rc) return rc;
+  if (!a->is_causal) return fail(PA_ERR_INVALID_ARGUMENT, "tree attention: is_causal must be 1");
+  if (a->num_heads <= 0 || a->num_heads % c->kv_heads != 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "PagedAttention: bad num_heads/kv_num_heads");
+  if (b->max_query_len > PA_MAX_TREE_NODES)
+    return fail(PA_ERR_UNSUPPORTED, "tree attention: at most %d nodes to a sequence, got max_query_len %d",
+                PA_MAX_TREE_NODES, b->max_query_len);
+  if (b->num_tokens == 0) return PA_OK;
+  if (!parents) return fail(PA_ERR_INVALID_ARGUMENT, "tree attention: parents is NULL");
+  const TreePlan t = tree_plan(c, b, a, act);
+  if ((rc = check_ranged(c, b, a, act, q, out, ws, ws_bytes, t.bytes(), t.r.on))) return rc;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  char* base = reinterpret_cast<char*>(ws);
+  pa::TreeParams tp{};
+  tp.parents = parents;
+  tp.cum = b->cumulative_sequence_length;
+  tp.bits = reinterpret_cast<uint32_t*>(base);
+  tp.lag = reinterpret_cast<int32_t*>(base + t.bits_bytes);
+  tp.batch = b->batch;
+  tp.num_tokens = b->num_tokens;
+  tp.words = t.words;
+  tp.window = a->local_window_size;
+  hipError_t e = pa::launch_tree_bits(tp, s);
+  if (e != hipSuccess) return hip_fail(e, "tree attention launch");
+  char* rest = base + t.bits_bytes + t.lag_bytes;
+  if (!t.r.on) {
+    RunOpts o = masked_opts(nullptr);
+    o.tree_bits = tp.bits;
+    o.tree_lag = tp.lag;
+    o.tree_words = t.words;
+    return run_attention(c, b, a, act, q, nullptr, nullptr, out, rest, t.attn_bytes, 3, 0, s, o);
+  }
+  pa::RangedParams p = ranged_params(c, b, a, q, out, rest, t.r);
+  p.tree_bits = tp.bits;
+  p.tree_lag = tp.lag;
+  p.tree_words = t.words;
+  e = pa::launch_ranged_tree(p, act, s);
+  if (e != hipSuccess) return hip_fail(e, "tree attention launch");
+  return PA_OK;
+}
+
+int pa_accept_drafts(const pa_cache* c, const pa_batch* b, const pa_drafts* d, pa_stream_t stream) {
+  if (!b) return fail(PA_ERR_INVALID_ARGUMENT, "batch descriptor is NULL");
+  const int rc = check_rows(c, b->batch, b->max_blocks, b->block_table, b->past_seqlens);
+  if (rc) return rc;
+  if (!b->cumulative_sequence_length) return fail(PA_ERR_INVALID_ARGUMENT, "metadata pointers are NULL");
+  if (b->num_tokens < 0 || b->slot_mapping)
+    return fail(PA_ERR_INVALID_ARGUMENT, "accepting drafts: num_tokens must not be negative, slot_mapping must be NULL");
+  if (b->max_query_len > PA_MAX_TREE_NODES)
+    return fail(PA_ERR_UNSUPPORTED, "accepting drafts: at most %d nodes to a sequence, got max_query_len %d",
+                PA_MAX_TREE_NODES, b->max_query_len);
+  if (!d || d->max_path < 1 || !d->path || !d->path_lens)
+    return fail(PA_ERR_INVALID_ARGUMENT, "accepting drafts: path, path_lens and a positive max_path are required");
+  if ((d->parents == nullptr) != (d->tokens == nullptr) || (d->parents == nullptr) != (d->targets == nullptr))
+    return fail(PA_ERR_INVALID_ARGUMENT, "accepting drafts: parents, tokens and targets must be provided together");
+  if (!d->parents && d->next_tokens)
+    return fail(PA_ERR_INVALID_ARGUMENT, "accepting drafts: next_tokens without targets");
+  pa::AcceptParams p{};
+  p.c = rows_params(c, b);
+  p.cum = b->cumulative_sequence_length;
+  p.past = b->past_seqlens;
+  p.parents = d->parents;
+  p.tokens = d->tokens;
+  p.targets = d->targets;
+  p.path = d->path;
+  p.path_lens = d->path_lens;
+  p.next_tokens = d->next_tokens;
+  p.num_tokens = b->num_tokens;
+  p.max_path = d->max_path;
+  const hipError_t e = pa::launch_accept(p, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "accepting drafts launch");
+  return PA_OK;
+}
+
+// ------------------------------------------------------------------------------ accounts, eviction
+size_t pa_accumulating_attention_workspace_bytes(const pa_cache* cache, const pa_batch* batch,
+                                                 const pa_attn* attn, int32_t observed_rows,
+                                                 pa_dtype act_dtype) {
+  if (!cache || !batch || !attn || cache->kv_heads <= 0 || batch->batch <= 0 || batch->num_tokens <= 0 ||
+      attn->num_heads < cache->kv_heads)
+    return 0;
+  return account_plan(cache, batch, attn, observed_rows, act_dtype).bytes();
+}
+
+int pa_accumulating_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, float* key_weights,
+                              int32_t observed_rows, pa_dtype act, const void* q, void* out, void* ws,
+                              size_t ws_bytes, pa_stream_t stream) {
+  int rc = check_masked(c, b, a, act);
+  if (rc) return rc;
+  if (a->num_heads <= 0 || a->num_heads % c->kv_heads != 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "PagedAttention: bad num_heads/kv_num_heads");
+  if (observed_rows < 0) return fail(PA_ERR_INVALID_ARGUMENT, "observed_rows must not be negative");
+  if ((int64_t)b->num_tokens * a->num_heads > INT32_MAX)
+    return fail(PA_ERR_UNSUPPORTED, "accumulating attention: more than 2^31 rows");
+  if (b->num_tokens == 0) return PA_OK;
+  if (!key_weights || (reinterpret_cast<uintptr_t>(key_weights) & 3))
+    return fail(PA_ERR_INVALID_ARGUMENT, "key_weights must be given, 4-byte aligned");
+  const AccountPlan t = account_plan(c, b, a, observed_rows, act);
+  if ((rc = check_ranged(c, b, a, act, q, out, ws, ws_bytes, t.bytes(), t.r.on))) return rc;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  char* base = reinterpret_cast<char*>(ws);
+  char* rest = base + t.stat_bytes + t.sum_bytes;
+  pa::WeighParams w{};
+  w.r = ranged_params(c, b, a, q, out, t.r.on ? rest : nullptr, t.r);
+  w.r.row_stats = reinterpret_cast<float*>(base);
+  w.r.observed = observed_rows;
+  if (t.scores) {
+    w.r.scores = reinterpret_cast<float*>(base + t.stat_bytes);
+    w.r.score_ld = t.ld;
+  } else {
+    w.part = reinterpret_cast<float*>(base + t.stat_bytes);
+    w.part_ld = t.ld;
+    w.chunks = t.chunks;
+    w.chunk_rows = t.chunk_rows;
+  }
+  w.k_scale = c->k_scale;
+  w.k_quant = c->k_quant_type;
+  w.weights = key_weights;
+  w.max_keys = t.keys;
+  hipError_t e;
+  if (t.r.on) {
+    e = pa::launch_ranged_weigh(w.r, act, s);
+    if (e != hipSuccess) return hip_fail(e, "accumulating attention launch");
+  } else {
+    RunOpts o = masked_opts(nullptr);
+    o.row_stats = w.r.row_stats;
+    if ((rc = run_attention(c, b, a, act, q, nullptr, nullptr, out, rest, t.attn_bytes, 3, 0, s, o))) return rc;
+  }
+  e = pa::launch_weigh(w, act, c->dtype, s);
+  if (e != hipSuccess) return hip_fail(e, "accumulating attention launch");
+  return PA_OK;
+}
+
+int pa_evict_keys(const pa_cache* c, const pa_batch* b, const pa_eviction* v, pa_stream_t stream) {
+  if (!b) return fail(PA_ERR_INVALID_ARGUMENT, "batch descriptor is NULL");
+  const int rc = check_rows(c, b->batch, b->max_blocks, b->block_table, b->past_seqlens);
+  if (rc) return rc;
+  if (!v || !v->key_weights || !v->kept || !v->lens_out)
+    return fail(PA_ERR_INVALID_ARGUMENT, "eviction: key_weights, kept and lens_out are required");
+  if (v->budget < 1 || v->sinks < 0 || v->recent < 0 || (int64_t)v->sinks + v->recent > v->budget)
+    return fail(PA_ERR_INVALID_ARGUMENT, "eviction: sinks + recent must lie within a positive budget");
+  const int cap = max_ctx_bound(c, b), keys = b->max_context_len > 0 ? std::min(b->max_context_len, cap) : cap;
+  if (v->block_table_out) {
+    if (v->block_table_out == b->block_table)
+      return fail(PA_ERR_INVALID_ARGUMENT, "eviction: block_table_out must name other pages (NULL: in place)");
+    if (v->max_blocks_out < 1 || (int64_t)v->max_blocks_out * c->block_size < std::min(v->budget, keys))
+      return fail(PA_ERR_INVALID_ARGUMENT, "eviction: block_table_out must hold min(budget, context) rows");
+  }
+  if (v->lens_out == b->past_seqlens)
+    return fail(PA_ERR_INVALID_ARGUMENT, "eviction: lens_out must not be past_seqlens");
+  if ((int64_t)b->batch * c->kv_heads * v->budget > INT32_MAX)
+    return fail(PA_ERR_UNSUPPORTED, "eviction: more than 2^31 kept positions");
+  pa::EvictParams p{};
+  p.c = rows_params(c, b);
+  p.lens = b->past_seqlens;
+  p.weights = v->key_weights;
+  p.table_out = v->block_table_out;
+  p.kept = v->kept;
+  p.lens_out = v->lens_out;
+  p.max_blocks_out = v->max_blocks_out;
+  p.budget = v->budget;
+  p.sinks = v->sinks;
+  p.recent = v->recent;
+  p.max_keys = keys;
+  const hipError_t e = pa::launch_evict(p, reinterpret_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "eviction launch");
+  return PA_OK;
 }
 
 // ------------------------------------------------------------------------------ multi-axis append

@@ -14,58 +14,11 @@
 // x = s*log2(e), which is the same function.
 #include <type_traits>
 
-#include "pa_device.hpp"
+#include "pa_cache_read.hpp"
 
 namespace pa {
 
 namespace {
-
-// Element e of a cache row starting at storage index `base`, widened to fp32.  `scale` is the
-// fp8 per-(block, kv-head) scale or the integer per-tensor / per-channel scale of element e.
-template <typename CT>
-struct CacheRead;
-
-template <>
-struct CacheRead<TF16> {
-  __device__ static float at(const void* c, int64_t base, int e, float) {
-    return f16_to_f32(reinterpret_cast<const uint16_t*>(c)[base + e]);
-  }
-};
-template <>
-struct CacheRead<TBF16> {
-  __device__ static float at(const void* c, int64_t base, int e, float) {
-    return bf16_to_f32(reinterpret_cast<const uint16_t*>(c)[base + e]);
-  }
-};
-template <>
-struct CacheRead<TF32> {
-  __device__ static float at(const void* c, int64_t base, int e, float) {
-    return reinterpret_cast<const float*>(c)[base + e];
-  }
-};
-struct Fp8Cache {};
-template <>
-struct CacheRead<Fp8Cache> {
-  __device__ static float at(const void* c, int64_t base, int e, float scale) {
-    return e4m3_to_f32(reinterpret_cast<const uint8_t*>(c)[base + e]) * scale;
-  }
-};
-// Integer caches: QuantizedCache::decode (kv_cache.rs:222-256), code * scale in fp32.
-struct I8Cache {};
-template <>
-struct CacheRead<I8Cache> {
-  __device__ static float at(const void* c, int64_t base, int e, float scale) {
-    return (float)reinterpret_cast<const int8_t*>(c)[base + e] * scale;
-  }
-};
-struct I4Cache {};
-template <>
-struct CacheRead<I4Cache> {
-  __device__ static float at(const void* c, int64_t base, int e, float scale) {
-    const uint32_t byte = reinterpret_cast<const uint8_t*>(c)[base + (e >> 1)];
-    return (float)((int)((byte >> ((e & 1) * 4)) & 15u) - 8) * scale;
-  }
-};
 
 // Keys of sequence b: past + query rows, bounded by key_limit[b] when given (GroupQueryAttention
 // sequences shorter than the query rows of a ragged first prompt) and by the capacity of a
@@ -76,12 +29,11 @@ __device__ __forceinline__ int64_t seq_keys(const AttnParams& p, int b, int64_t 
   return p.linear_cap > 0 ? min(t, (int64_t)p.linear_cap) : t;
 }
 
-template <typename CT>
-constexpr bool kIntCache = false;
-template <>
-constexpr bool kIntCache<I8Cache> = true;
-template <>
-constexpr bool kIntCache<I4Cache> = true;
+// Whether token t sees new row n of its sequence: of a drafted tree, what its bits name (n < 0: a key before it).
+__device__ __forceinline__ bool tree_sees(const AttnParams& p, int t, int64_t n) {
+  if (!p.tree_bits || n < 0) return true;
+  return (n >> 5) < p.tree_words && ((p.tree_bits[(int64_t)t * p.tree_words + (n >> 5)] >> (n & 31)) & 1u);
+}
 
 // Elements per lane: NE = 1, 2, 4 cover head_dim <= 64, 128, 256, NE = 10 head_dim <= 640 (latent
 // heads).  (Bound by instruction issue: with the four of head 256 at every size one fp32 token of head
@@ -120,7 +72,8 @@ __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams 
   if (p.doc_starts) lo = max(lo, (int64_t)p.doc_starts[t]);
   // window end point: the row's position, or the last key for rows past it (a right-padded
   // first prompt, causal_window_mask attention.rs:328-353)
-  if (p.window > 0) lo = max(lo, min(rp, total - 1) - p.window + 1);
+  // (a drafted node's place goes by its depth)
+  if (p.window > 0) lo = max(lo, min(rp, total - 1) - (p.tree_lag ? p.tree_lag[t] : 0) - p.window + 1);
   const typename TT::raw* bias_row =
       p.bias ? reinterpret_cast<const typename TT::raw*>(p.bias) +
                    ((((int64_t)(p.bias_b == 1 ? 0 : b) * p.bias_h + (p.bias_h == 1 ? 0 : h)) *
@@ -158,7 +111,7 @@ __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams 
       for (int u = 0; u < U; ++u) {
         // a surplus key repeats the last one: weight 0 below, and no values (theirs may be infinite)
         const int64_t pos = min(p0 + NW * u, hi - 1);
-        const int vd = NW * u < left ? VD : 0;
+        const int vd = NW * u < left && tree_sees(p, t, pos - pastb) ? VD : 0;
         const void *kb, *vb;
         int64_t off;
         float ks = 1.0f, vs = 1.0f;
@@ -216,7 +169,7 @@ __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams 
         if (bias_row)
           s += TT::to_f32(
               bias_row[min(max(min(pos, hi - 1) + bias_off, (int64_t)0), (int64_t)p.bias_cols - 1)]);
-        x[u] = pos < hi ? s * kLog2e : kNegInf;
+        x[u] = pos < hi && tree_sees(p, t, pos - pastb) ? s * kLog2e : kNegInf;
       }
     }
     float mn = m;
@@ -268,6 +221,7 @@ __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams 
   if (!single && p.part_o == nullptr) return;  // beyond planned capacity: nothing to write into
   if (single) {
     float f = finalize_factor(m, l, sink_logit<TT>(p, h));
+    if (p.row_stats && lane == 0) p.row_stats[stat_row(p, t, h)] = softmax_stat(m, l, sink_logit<TT>(p, h));
     typename TT::raw* out = reinterpret_cast<typename TT::raw*>(p.out);
 #pragma unroll
     for (int k = 0; k < NE; ++k) {
@@ -326,6 +280,7 @@ __global__ __launch_bounds__(NT) void split_reduce_kernel(const AttnParams p) {
   }
   L = wave_sum(L);
   const float f = finalize_factor(M, L, sink_logit<TT>(p, h));
+  if (p.row_stats && tid == 0) p.row_stats[stat_row(p, t, h)] = softmax_stat(M, L, sink_logit<TT>(p, h));
   typename TT::raw* out = reinterpret_cast<typename TT::raw*>(p.out);
   const float* po = p.part_o + base * D;
   float acc[NE];

@@ -9,6 +9,7 @@
 
 #include "pa_mi355x.h"
 #include "pa_mi355x_ext.h"
+#include "pa_mi355x_upkeep.h"
 
 namespace pa {
 
@@ -388,6 +389,11 @@ struct AttnParams {
   const float* slopes;
   const int32_t* prefix_lens;
   const int32_t* doc_starts;
+  // Drafted trees and accounts, as RangedParams has them (VALU kernel).
+  const uint32_t* tree_bits;
+  const int32_t* tree_lag;
+  int32_t tree_words;
+  float* row_stats;
   int32_t* plan;
   int32_t* plan_info;
   int32_t* plan_split;
@@ -412,7 +418,7 @@ struct AttnParams {
   int32_t* plan_seq;
 };
 
-// Attention over key ranges per row, with shared prefixes (pa_ranged.hip).
+// Attention over key ranges per row, with shared prefixes (pa_ranged.hpp).
 // The plan as the merge reads it: entry 0 tiles per worker (wide, narrow), then the groups' and sequences'
 // places in the flat lists of 64-key tiles.
 struct RTable {
@@ -457,8 +463,82 @@ struct RangedParams {
   int32_t whole;     // every item whole (short contexts)
   int32_t merge;     // some row may have several pieces
   int32_t wide;      // some block may hold more than 32 rows
+  // Drafted trees (launch_ranged_tree): tree_words words per token, bit n: it sees its sequence's new row n (itself
+  // and its ancestors in the window); and how far behind its row a node's place in the text is
+  const uint32_t* tree_bits;
+  const int32_t* tree_lag;
+  int32_t tree_words;
+  // Accounts (launch_ranged_weigh): the constants of the rows' softmax (2^(x - it) is a probability), rows by kv-head,
+  // token and head of the group; on narrow items the scores x of the last `observed` tokens (0: all) of each sequence,
+  // score_ld of them per row, or null
+  float* row_stats;
+  float* scores;
+  int64_t score_ld;
+  int32_t observed;
 };
 hipError_t launch_ranged(const RangedParams& p, pa_dtype act, hipStream_t s);
+hipError_t launch_ranged_tree(const RangedParams& p, pa_dtype act, hipStream_t s);
+hipError_t launch_ranged_weigh(const RangedParams& p, pa_dtype act, hipStream_t s);
+
+// Ancestors' bits and lags of drafted trees (pa_tree.hip) from parents [num_tokens], rows of their sequence.
+struct TreeParams {
+  const int32_t* parents;
+  const int32_t* cum;
+  uint32_t* bits;
+  int32_t* lag;
+  int32_t batch, num_tokens, words, window;
+};
+hipError_t launch_tree_bits(const TreeParams& p, hipStream_t s);
+
+// Keys' accounts (pa_weigh.hip): what the rows' probabilities (r: its row_stats, scores, observed and the call) add to
+// weights [num_blocks, kv_heads, block_size].
+struct WeighParams {
+  RangedParams r;
+  const float* k_scale;
+  int32_t k_quant;
+  float* weights;
+  float* part;  // [chunks][batch * kv_heads][part_ld] sums over chunk_rows rows each, where no scores are held
+  int64_t part_ld;
+  int32_t chunks, chunk_rows;
+  int32_t max_keys;  // of any sequence
+};
+hipError_t launch_weigh(const WeighParams& p, pa_dtype act, pa_dtype cache_dtype, hipStream_t s);
+
+// Rows that move within the pages (pa_upkeep.hip).
+struct RowsParams {  // the caches
+  char* key_cache;
+  char* value_cache;
+  const float* k_scale;  // fp8 pages: codes are written for their new page's scale
+  const float* v_scale;
+  const int32_t* block_table;
+  int64_t num_blocks;
+  int32_t block_size, kv_heads, head_bytes;  // head_bytes: of a kv-head's row
+  int32_t batch, max_blocks, fp8;
+};
+struct AcceptParams {
+  RowsParams c;
+  const int32_t* cum;
+  const int32_t* past;
+  const int32_t* parents;   // null: path and path_lens are given
+  const int64_t* tokens;
+  const int64_t* targets;
+  int32_t* path;            // [batch, max_path]
+  int32_t* path_lens;
+  int64_t* next_tokens;     // or null
+  int32_t num_tokens, max_path;
+};
+hipError_t launch_accept(const AcceptParams& p, hipStream_t s);
+struct EvictParams {
+  RowsParams c;
+  const int32_t* lens;
+  float* weights;               // [num_blocks, kv_heads, block_size]
+  const int32_t* table_out;     // null: in place
+  int32_t* kept;                // [batch, kv_heads, budget]
+  int32_t* lens_out;
+  int32_t max_blocks_out, budget, sinks, recent;
+  int32_t max_keys;
+};
+hipError_t launch_evict(const EvictParams& p, hipStream_t s);
 bool ranged_supported(int head_dim, pa_dtype act, pa_dtype cache_dtype);
 
 // Parts of an item of a short planned prefill, at most, their keys in percent of an even share of
@@ -584,6 +664,20 @@ __device__ __forceinline__ float finalize_factor(float m, float l, float sink_x)
   float f = (m == kNegInf) ? 0.0f : exp2f(m - mm);
   float lt = l * f + ((sink_x == kNegInf) ? 0.0f : exp2f(sink_x - mm));
   return lt > 0.0f ? f / lt : 0.0f;
+}
+
+// Constant of a row's softmax from its maximum m and sum l: probabilities are 2^(x - it), 0 where nothing weighs.
+__device__ __forceinline__ float softmax_stat(float m, float l, float sink_x) {
+  const float mm = fmaxf(m, sink_x);
+  if (l != l) return l;
+  if (mm == kNegInf) return -kNegInf;
+  return mm + __log2f(l * (m == kNegInf ? 0.0f : exp2f(m - mm)) + (sink_x == kNegInf ? 0.0f : exp2f(sink_x - mm)));
+}
+// Its place: rows by kv-head, token and head of the group.
+template <typename P>
+__device__ __forceinline__ int64_t stat_row(const P& p, int64_t t, int h) {
+  const int g = p.num_heads / p.kv_heads, kh = h / g;
+  return ((int64_t)kh * p.num_tokens + t) * g + (h - kh * g);
 }
 
 template <typename TT>

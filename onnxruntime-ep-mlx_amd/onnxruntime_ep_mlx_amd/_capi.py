@@ -53,6 +53,8 @@ EXPORTS = (
     "pa_multi_axis_rotary_append",
     "pa_masked_attention_workspace_bytes", "pa_masked_attention",
     "pa_shared_prefix_attention_workspace_bytes", "pa_shared_prefix_attention",
+    "pa_tree_attention_workspace_bytes", "pa_tree_attention", "pa_accept_drafts",
+    "pa_accumulating_attention_workspace_bytes", "pa_accumulating_attention", "pa_evict_keys",
 )
 
 
@@ -203,6 +205,21 @@ class PaSharedPrefix(C.Structure):
                 ("max_prefix_len", C.c_int32)]
 
 
+PA_MAX_TREE_NODES = 4096  # include/pa_mi355x_upkeep.h
+
+
+class PaDrafts(C.Structure):
+    _fields_ = [("parents", C.c_void_p), ("tokens", C.c_void_p), ("targets", C.c_void_p),
+                ("path", C.c_void_p), ("path_lens", C.c_void_p), ("next_tokens", C.c_void_p),
+                ("max_path", C.c_int32)]
+
+
+class PaEviction(C.Structure):
+    _fields_ = [("key_weights", C.c_void_p), ("budget", C.c_int32), ("sinks", C.c_int32),
+                ("recent", C.c_int32), ("block_table_out", C.c_void_p),
+                ("max_blocks_out", C.c_int32), ("kept", C.c_void_p), ("lens_out", C.c_void_p)]
+
+
 class PagedAttentionError(RuntimeError):
     """Raised when a C-ABI call returns a non-zero status; the message is pa_last_error()."""
 
@@ -262,6 +279,19 @@ def load() -> C.CDLL:
         "pa_shared_prefix_attention": (C.c_int, [C.POINTER(PaCache), C.POINTER(PaBatch),
                                                  C.POINTER(PaAttn), C.POINTER(PaSharedPrefix),
                                                  C.POINTER(PaMask), C.c_int, P, P, P, SZ, P]),
+        "pa_tree_attention_workspace_bytes": (SZ, [C.POINTER(PaCache), C.POINTER(PaBatch),
+                                                   C.POINTER(PaAttn), C.c_int]),
+        "pa_tree_attention": (C.c_int, [C.POINTER(PaCache), C.POINTER(PaBatch),
+                                        C.POINTER(PaAttn), P, C.c_int, P, P, P, SZ, P]),
+        "pa_accept_drafts": (C.c_int, [C.POINTER(PaCache), C.POINTER(PaBatch),
+                                       C.POINTER(PaDrafts), P]),
+        "pa_accumulating_attention_workspace_bytes": (SZ, [C.POINTER(PaCache), C.POINTER(PaBatch),
+                                                           C.POINTER(PaAttn), I32, C.c_int]),
+        "pa_accumulating_attention": (C.c_int, [C.POINTER(PaCache), C.POINTER(PaBatch),
+                                                C.POINTER(PaAttn), P, I32, C.c_int, P, P, P, SZ,
+                                                P]),
+        "pa_evict_keys": (C.c_int, [C.POINTER(PaCache), C.POINTER(PaBatch),
+                                    C.POINTER(PaEviction), P]),
         "pa_paged_attention_workspace_bytes": (SZ, [C.POINTER(PaNode), C.POINTER(PaIO)]),
         "pa_paged_attention": (C.c_int, [C.POINTER(PaNode), C.POINTER(PaIO), P, SZ, P]),
         "pa_paged_attention_static": (C.c_int, [C.POINTER(PaNode), C.POINTER(PaIO), P]),

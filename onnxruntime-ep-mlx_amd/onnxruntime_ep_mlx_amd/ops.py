@@ -404,11 +404,10 @@ def _mask_desc(index, batch, T, num_heads, distance_slopes, prefix_lens, documen
     return C.byref(capi.PaMask(_ptr(distance_slopes), _ptr(prefix_lens), _ptr(document_starts)))
 
 
-def _masked_call(q, key_cache, value_cache, cum, past, block_table, share, num_heads, scale,
-                 softcap, local_window_size, is_causal, head_sink, distance_slopes, prefix_lens,
-                 document_starts, k_scale, v_scale, k_quant_type, v_quant_type, max_query_len,
-                 max_context_len, out, workspace):
-    lib = capi.load()
+def _paged_call(q, key_cache, value_cache, cum, past, block_table, num_heads, scale, softcap,
+                local_window_size, is_causal, head_sink, k_scale, v_scale, k_quant_type, v_quant_type,
+                max_query_len, max_context_len, out, workspace):
+    """The checked descriptors of attention over the pages, and its output."""
     _need_cuda("query", q)
     dev = q.get_device()
     if q.dim() != 2 or num_heads <= 0 or q.shape[1] % num_heads:
@@ -428,30 +427,45 @@ def _masked_call(q, key_cache, value_cache, cum, past, block_table, share, num_h
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("PagedAttention: out must match query's shape and dtype")
-    mask = _mask_desc(dev, n, T, num_heads, distance_slopes, prefix_lens, document_starts)
     cache = cache_desc(key_cache, value_cache, k_scale, v_scale, head_dim=q.shape[1] // num_heads,
                        k_quant_type=k_quant_type, v_quant_type=v_quant_type)
     _scales_hold(cache, k_scale, v_scale)
     batch = batch_desc(cum, past, block_table, T, None, max_query_len,
                        capi.PA_BATCH_NEW_ROWS_IN_CACHE, max_context_len)
     attn = attn_desc(num_heads, scale, softcap, local_window_size, is_causal, head_sink)
-    act = pa_dtype(q.dtype)
-    args = (C.byref(cache), C.byref(batch), C.byref(attn))
-    if share is None:
-        size, call = lib.pa_masked_attention_workspace_bytes, lib.pa_masked_attention
-        args += (mask, act)
-    else:
-        size, call = (lib.pa_shared_prefix_attention_workspace_bytes, lib.pa_shared_prefix_attention)
-        args += (C.byref(share), mask, act)
+    return (C.byref(cache), C.byref(batch), C.byref(attn)), out
+
+
+def _with_workspace(q, out, workspace, size, size_args, call, args):
     if workspace is None:
         # A workspace of the call's own: torch's allocator keeps it apart from work on other streams
         # and in other captured graphs.
-        have = size(*args)
+        have = size(*size_args)
         workspace = torch.empty(have, dtype=torch.uint8, device=q.device) if have else None
     else:
         have = workspace.numel() * workspace.element_size()
-    capi.check(_on_device(dev, call, *args, q.data_ptr(), out.data_ptr(), _ptr(workspace), have))
+    capi.check(_on_device(q.get_device(), call, *args, q.data_ptr(), out.data_ptr(), _ptr(workspace), have))
     return out
+
+
+def _masked_call(q, key_cache, value_cache, cum, past, block_table, share, num_heads, scale,
+                 softcap, local_window_size, is_causal, head_sink, distance_slopes, prefix_lens,
+                 document_starts, k_scale, v_scale, k_quant_type, v_quant_type, max_query_len,
+                 max_context_len, out, workspace):
+    lib = capi.load()
+    descs, out = _paged_call(q, key_cache, value_cache, cum, past, block_table, num_heads, scale, softcap,
+                             local_window_size, is_causal, head_sink, k_scale, v_scale, k_quant_type,
+                             v_quant_type, max_query_len, max_context_len, out, workspace)
+    mask = _mask_desc(q.get_device(), past.numel(), q.shape[0], num_heads, distance_slopes, prefix_lens,
+                      document_starts)
+    act = pa_dtype(q.dtype)
+    if share is None:
+        size, call = lib.pa_masked_attention_workspace_bytes, lib.pa_masked_attention
+        args = (*descs, mask, act)
+    else:
+        size, call = (lib.pa_shared_prefix_attention_workspace_bytes, lib.pa_shared_prefix_attention)
+        args = (*descs, C.byref(share), mask, act)
+    return _with_workspace(q, out, workspace, size, args, call, args)
 
 
 def masked_attention(q, key_cache, value_cache, cum, past, block_table, *, num_heads, scale=0.0,
@@ -502,6 +516,159 @@ def shared_prefix_attention(q, key_cache, value_cache, cum, past, block_table, g
                         softcap, local_window_size, is_causal, head_sink, distance_slopes,
                         prefix_lens, document_starts, k_scale, v_scale, k_quant_type, v_quant_type,
                         max_query_len, max_context_len, out, workspace)
+
+
+def tree_attention(q, key_cache, value_cache, cum, past, block_table, parents, *, num_heads, scale=0.0,
+                   softcap=0.0, local_window_size=-1, head_sink=None, k_scale=None, v_scale=None,
+                   k_quant_type="NONE", v_quant_type="NONE", max_query_len=0, max_context_len=0, out=None,
+                   workspace=None):
+    """Attention of drafted trees over the pages, the new tokens' keys and values among them
+    (pa_tree_attention).
+
+    The new tokens of a sequence are the nodes of its tree: ``parents`` int32 [num_tokens] names the row
+    (within the sequence's new tokens) of each one's parent, an earlier one; -1 is a root.  A node sees
+    the cached keys, its ancestors and itself, those less than ``local_window_size`` positions before it;
+    its position is past + its depth (what its rotary positions should be: multi_axis_rotary_append takes
+    them), its slot past + its row.  Everything else as in masked_attention.  At most 4096 nodes to a
+    sequence; ``max_query_len`` bounds them (0 = unknown)."""
+    lib = capi.load()
+    descs, out = _paged_call(q, key_cache, value_cache, cum, past, block_table, num_heads, scale, softcap,
+                             local_window_size, 1, head_sink, k_scale, v_scale, k_quant_type, v_quant_type,
+                             max_query_len, max_context_len, out, workspace)
+    if parents.dtype != torch.int32 or parents.numel() != q.shape[0]:
+        raise ValueError("PagedAttention: parents must be int32 with num_tokens elements")
+    _same_device(q.get_device(), (("parents", parents),))
+    act = pa_dtype(q.dtype)
+    return _with_workspace(q, out, workspace, lib.pa_tree_attention_workspace_bytes, (*descs, act),
+                           lib.pa_tree_attention, (*descs, _ptr(parents), act))
+
+
+def _rows_call(key_cache, value_cache, block_table, lens, k_scale, v_scale, k_quant_type, v_quant_type, more):
+    """The checked cache descriptor of entries that move rows; `more`: (name, tensor) on the same device."""
+    _need_cuda("key_cache", key_cache)
+    if value_cache is None:
+        raise ValueError("PagedAttention: the SEPARATE cache layout is required")
+    _same_device(key_cache.get_device(), (("key_cache", key_cache), ("value_cache", value_cache),
+                                          ("block_table", block_table), ("past", lens), ("k_scale", k_scale),
+                                          ("v_scale", v_scale), *more))
+    if block_table.dim() != 2 or block_table.shape[0] != lens.numel() or block_table.dtype != torch.int32 \
+            or lens.dtype != torch.int32:
+        raise ValueError("PagedAttention: block_table and lengths must be int32 [batch, max_blocks] and [batch]")
+    cache = cache_desc(key_cache, value_cache, k_scale, v_scale, k_quant_type=k_quant_type,
+                       v_quant_type=v_quant_type)
+    # (codes move as they are: only fp8 pages have scales of their own)
+    if cache.dtype in (capi.PA_DTYPE_INT8, capi.PA_DTYPE_INT4) and k_scale is None:
+        one = _ptr(key_cache)
+        cache.k_scale = cache.v_scale = one
+        cache.k_quant_type = cache.v_quant_type = capi.PA_QUANT_PER_TENSOR
+    _scales_hold(cache, k_scale, v_scale)
+    return cache
+
+
+def accept_drafts(key_cache, value_cache, cum, past, block_table, parents=None, draft_tokens=None,
+                  target_tokens=None, *, path=None, path_lens=None, max_path=0, k_scale=None, v_scale=None,
+                  k_quant_type="NONE", v_quant_type="NONE", max_query_len=0):
+    """The accepted path of every drafted tree, its rows moved to where the sequence goes on
+    (pa_accept_drafts): row path[i] of a sequence's new tokens to slot past + i.
+
+    The path begins with row 0 and goes on, while there is one, to the first child of its last node whose
+    ``draft_tokens`` entry is that node's ``target_tokens`` entry (the model's choice after it; both int64
+    [num_tokens], ``parents`` as in tree_attention), up to ``max_path`` nodes (0: max_query_len, else
+    num_tokens).  Returns (path int32 [batch, max_path], -1 behind its end; path_lens int32 [batch]; the
+    target of the last node, int64 [batch]): the sequences go on with past + path_lens keys.  For a path chosen
+    otherwise give ``path`` (rising rows) and ``path_lens`` instead; the third result is then None.  The
+    pages of the new tokens must belong to their sequence alone."""
+    given = path is not None
+    if given == (parents is not None) or given != (path_lens is not None):
+        raise ValueError("PagedAttention: give parents, draft_tokens and target_tokens, or path and path_lens")
+    cache = _rows_call(key_cache, value_cache, block_table, past, k_scale, v_scale, k_quant_type, v_quant_type,
+                       (("cum", cum), ("parents", parents), ("draft_tokens", draft_tokens),
+                        ("target_tokens", target_tokens), ("path", path), ("path_lens", path_lens)))
+    B, dev = past.numel(), key_cache.device
+    if cum.numel() != B + 1:
+        raise ValueError("PagedAttention: inconsistent cumulative lengths, past lengths or block table")
+    after = None
+    if given:
+        if path.dtype != torch.int32 or path_lens.dtype != torch.int32 or path.dim() != 2 \
+                or path.shape[0] != B or path.shape[1] < 1 or path_lens.numel() != B:
+            raise ValueError("PagedAttention: path and path_lens must be int32 [batch, max_path] and [batch]")
+        # (no sequence has more new tokens than there are slots)
+        tokens = min(key_cache.shape[0] * key_cache.shape[1], 2**31 - 1)
+    else:
+        tokens = parents.numel()
+        if parents.dtype != torch.int32 or draft_tokens is None or target_tokens is None \
+                or draft_tokens.dtype != torch.int64 or target_tokens.dtype != torch.int64 \
+                or draft_tokens.numel() != tokens or target_tokens.numel() != tokens:
+            raise ValueError("PagedAttention: parents must be int32, draft_tokens and target_tokens int64 [num_tokens]")
+        path = torch.empty((B, max_path or max_query_len or max(tokens, 1)), dtype=torch.int32, device=dev)
+        path_lens = torch.empty(B, dtype=torch.int32, device=dev)
+        after = torch.empty(B, dtype=torch.int64, device=dev)
+    batch = batch_desc(cum, past, block_table, tokens, None, max_query_len)
+    drafts = capi.PaDrafts(_ptr(parents), _ptr(draft_tokens), _ptr(target_tokens), _ptr(path), _ptr(path_lens),
+                           _ptr(after), path.shape[1])
+    capi.check(_on_device(key_cache.get_device(), capi.load().pa_accept_drafts, C.byref(cache), C.byref(batch),
+                          C.byref(drafts)))
+    return path, path_lens, after
+
+
+def _account(key_weights, key_cache) -> None:
+    nb, bs, kv = key_cache.shape[:3]
+    if key_weights.dtype != torch.float32 or tuple(key_weights.shape) != (nb, kv, bs):
+        raise ValueError("PagedAttention: key_weights must be float32 [num_blocks, kv_num_heads, block_size]")
+    _same_device(key_cache.get_device(), (("key_weights", key_weights),))
+
+
+def accumulating_attention(q, key_cache, value_cache, cum, past, block_table, key_weights, *, num_heads,
+                           observed_rows=0, scale=0.0, softcap=0.0, local_window_size=-1, is_causal=1,
+                           head_sink=None, k_scale=None, v_scale=None, k_quant_type="NONE",
+                           v_quant_type="NONE", max_query_len=0, max_context_len=0, out=None, workspace=None):
+    """Attention over the pages, the new tokens' keys and values among them, that adds to every key's
+    account what it weighed (pa_accumulating_attention).
+
+    ``key_weights`` float32 [num_blocks, kv_num_heads, block_size] lies beside the pages: a key's entry
+    grows by its probabilities (sinks in their denominator) in the last ``observed_rows`` new tokens of its
+    sequence (0: in all of them), summed over the heads of its kv-head; entries of the new tokens begin at
+    zero.  The same call gives the same bits.  Returns the output; everything else as in masked_attention
+    without its masks."""
+    lib = capi.load()
+    descs, out = _paged_call(q, key_cache, value_cache, cum, past, block_table, num_heads, scale, softcap,
+                             local_window_size, is_causal, head_sink, k_scale, v_scale, k_quant_type,
+                             v_quant_type, max_query_len, max_context_len, out, workspace)
+    _account(key_weights, key_cache)
+    act = pa_dtype(q.dtype)
+    return _with_workspace(q, out, workspace, lib.pa_accumulating_attention_workspace_bytes,
+                           (*descs, observed_rows, act), lib.pa_accumulating_attention,
+                           (*descs, _ptr(key_weights), observed_rows, act))
+
+
+def evict_keys(key_cache, value_cache, key_weights, lens, block_table, *, budget, sinks=0, recent=0,
+               block_table_out=None, k_scale=None, v_scale=None, k_quant_type="NONE", v_quant_type="NONE",
+               max_context_len=0):
+    """The keys of every sequence and kv-head that stay by their account (pa_evict_keys).
+
+    Of ``lens[b]`` keys beyond ``budget`` stay the first ``sinks``, the last ``recent`` and the heaviest of
+    the others (the lower position of equals), in their order: row i of the pages becomes row kept[b, h, i],
+    key, value and ``key_weights`` (as in accumulating_attention), in place or in the pages of
+    ``block_table_out``, none of which a sequence of the batch holds.  Pages that are written belong to one
+    sequence alone.  Returns (kept int32 [batch, kv_num_heads, budget], -1 behind the end; the lengths that are
+    left, int32 [batch]).  ``max_context_len`` bounds ``lens`` (0 = the tables' capacity; keys beyond it
+    are not looked at)."""
+    cache = _rows_call(key_cache, value_cache, block_table, lens, k_scale, v_scale, k_quant_type, v_quant_type,
+                       (("block_table_out", block_table_out),))
+    _account(key_weights, key_cache)
+    B, kv, dev = lens.numel(), key_cache.shape[2], key_cache.device
+    if block_table_out is not None and (block_table_out.dtype != torch.int32 or block_table_out.dim() != 2
+                                        or block_table_out.shape[0] != B):
+        raise ValueError("PagedAttention: block_table_out must be int32 [batch, max_blocks]")
+    kept = torch.empty((B, kv, max(budget, 0)), dtype=torch.int32, device=dev)
+    lens_out = torch.empty(B, dtype=torch.int32, device=dev)
+    batch = capi.PaBatch(None, _ptr(lens), _ptr(block_table), None, B, block_table.shape[1], 0, 0, 0,
+                         max_context_len)
+    ev = capi.PaEviction(_ptr(key_weights), budget, sinks, recent, _ptr(block_table_out),
+                         0 if block_table_out is None else block_table_out.shape[1], _ptr(kept), _ptr(lens_out))
+    capi.check(_on_device(key_cache.get_device(), capi.load().pa_evict_keys, C.byref(cache), C.byref(batch),
+                          C.byref(ev)))
+    return kept, lens_out
 
 
 def paged_attention(query, key, value, key_cache, value_cache, cumulative_sequence_length,
