@@ -1539,6 +1539,7 @@ pa::RowsParams rows_params(const pa_cache* c, const pa_batch* b) {
   p.num_blocks = c->num_blocks;
   p.block_size = c->block_size;
   p.kv_heads = c->kv_heads;
+  p.bs_shift = (c->block_size & (c->block_size - 1)) == 0 ? __builtin_ctz((unsigned)c->block_size) : -1;
   p.head_bytes = (int32_t)cache_head_bytes(c->dtype, c->head_dim);
   p.batch = b->batch;
   p.max_blocks = b->max_blocks;
@@ -1727,8 +1728,8 @@ int pa_evict_keys(const pa_cache* c, const pa_batch* b, const pa_eviction* v, pa
   if (!b) return fail(PA_ERR_INVALID_ARGUMENT, "batch descriptor is NULL");
   const int rc = check_rows(c, b->batch, b->max_blocks, b->block_table, b->past_seqlens);
   if (rc) return rc;
-  if (!v || !v->key_weights || !v->kept || !v->lens_out)
-    return fail(PA_ERR_INVALID_ARGUMENT, "eviction: key_weights, kept and lens_out are required");
+  if (!v || !v->key_weights || !v->kept || !v->lens_out || (reinterpret_cast<uintptr_t>(v->key_weights) & 3))
+    return fail(PA_ERR_INVALID_ARGUMENT, "eviction: key_weights (4-byte aligned), kept and lens_out are required");
   if (v->budget < 1 || v->sinks < 0 || v->recent < 0 || (int64_t)v->sinks + v->recent > v->budget)
     return fail(PA_ERR_INVALID_ARGUMENT, "eviction: sinks + recent must lie within a positive budget");
   const int cap = max_ctx_bound(c, b), keys = b->max_context_len > 0 ? std::min(b->max_context_len, cap) : cap;
@@ -1754,6 +1755,7 @@ int pa_evict_keys(const pa_cache* c, const pa_batch* b, const pa_eviction* v, pa
   p.sinks = v->sinks;
   p.recent = v->recent;
   p.max_keys = keys;
+  p.four = c->block_size % 4 == 0 && (reinterpret_cast<uintptr_t>(v->key_weights) & 15) == 0 ? 1 : 0;
   const hipError_t e = pa::launch_evict(p, reinterpret_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "eviction launch");
   return PA_OK;

@@ -513,6 +513,7 @@ struct RowsParams {  // the caches
   const int32_t* block_table;
   int64_t num_blocks;
   int32_t block_size, kv_heads, head_bytes;  // head_bytes: of a kv-head's row
+  int32_t bs_shift;                          // log2 of a power of two, else -1
   int32_t batch, max_blocks, fp8;
 };
 struct AcceptParams {
@@ -537,6 +538,7 @@ struct EvictParams {
   int32_t* lens_out;
   int32_t max_blocks_out, budget, sinks, recent;
   int32_t max_keys;
+  int32_t four;                 // four weights of a page may be read at once
 };
 hipError_t launch_evict(const EvictParams& p, hipStream_t s);
 bool ranged_supported(int head_dim, pa_dtype act, pa_dtype cache_dtype);

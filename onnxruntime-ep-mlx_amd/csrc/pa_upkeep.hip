@@ -8,8 +8,10 @@
 // Accepting moves a few whole tokens of every sequence: a thread keeps to its 16 bytes of the token's row and takes
 // the rows in turn, eight loads in flight.  Evicting moves thousands of rows of single kv-heads, which stay by
 // different positions: the bytes of a head's row are independent of each other, so a workgroup takes 64 of them (of
-// keys or of values) for all rows, a thousand rows per round with a barrier between its loads and its stores;
-// between pages of different sequences no round waits.
+// keys or of values), or all of them where the heads are many, for all rows, hundreds per round with a barrier between
+// its loads and its stores; to other pages no round waits for another.
+#include <algorithm>
+
 #include "pa_device.hpp"
 
 namespace pa {
@@ -37,7 +39,7 @@ struct Slot {
   int64_t page;
 };
 __device__ __forceinline__ Slot slot_of(const RowsParams& c, const int32_t* table, int max_blocks, int b, int pos) {
-  const int bi = pos / c.block_size;
+  const int bi = c.bs_shift >= 0 ? pos >> c.bs_shift : pos / c.block_size;
   int64_t page = table[(int64_t)b * max_blocks + min(bi, max_blocks - 1)];
   page = min(max(page, (int64_t)0), c.num_blocks - 1);
   return Slot{page * c.block_size + (pos - bi * c.block_size), page};
@@ -168,7 +170,7 @@ constexpr int kEThreads = 1024, kEWaves = kEThreads / 64, kEBins = 2048;
 // stretches of their own.  HELD weights stay in LDS, more are read again in every round.
 template <int HELD>
 __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictParams p) {
-  __shared__ uint32_t held[HELD > 0 ? HELD : 1];
+  __shared__ __attribute__((aligned(16))) uint32_t held[HELD];
   __shared__ uint32_t bins[kEBins];
   __shared__ uint32_t part[kEWaves];
   __shared__ uint32_t found[2];
@@ -188,16 +190,34 @@ __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictPara
   for (int i = tid; i < p.recent; i += kEThreads) kept[p.budget - p.recent + i] = n - p.recent + i;
   uint32_t need = p.budget - p.sinks - p.recent;
   if (need == 0) return;
-  const int first = p.sinks, m = n - p.recent - first;  // the weights [first, first + m)
+  const int first = p.sinks, end = n - p.recent;  // the weights of positions [first, end), lowest order elsewhere
+  const bool hold = end <= HELD;
   auto load = [&](int i) {
-    const Slot s = slot_of(c, c.block_table, c.max_blocks, b, first + i);
+    const Slot s = slot_of(c, c.block_table, c.max_blocks, b, i);
     const int64_t off = s.slot - s.page * c.block_size;
-    return weight_order(p.weights[(s.page * c.kv_heads + kh) * c.block_size + off]);
+    return p.weights + (s.page * c.kv_heads + kh) * c.block_size + off;
   };
-  const bool hold = m <= HELD;
-  if (hold)
-    for (int i = tid; i < m; i += kEThreads) held[i] = load(i);
-  auto weight = [&](int i) { return hold ? held[HELD > 0 ? i : 0] : load(i); };
+  if (hold) {
+    // four at a time where pages hold a multiple of four, eight loads in flight
+    if (p.four) {
+      for (int i0 = 4 * tid; i0 < end; i0 += 8 * 4 * kEThreads) {
+        f32x4 w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          w[k] = *reinterpret_cast<const f32x4*>(load(min(i0 + 4 * kEThreads * k, (end - 1) & ~3)));
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int i = i0 + 4 * kEThreads * k;
+          if (i < end)
+            *reinterpret_cast<u32x4*>(held + i) = u32x4{weight_order(w[k][0]), weight_order(w[k][1]),
+                                                        weight_order(w[k][2]), weight_order(w[k][3])};
+        }
+      }
+    } else {
+      for (int i = tid; i < end; i += kEThreads) held[i] = weight_order(*load(i));
+    }
+  }
+  auto weight = [&](int i) { return hold ? held[i] : weight_order(*load(i)); };
   uint32_t prefix = 0, mask = 0;
 #pragma unroll 1
   for (int round = 0; round < 3; ++round) {
@@ -205,7 +225,7 @@ __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictPara
     const uint32_t digit = round == 2 ? 1023u : 2047u;
     for (int i = tid; i < kEBins; i += kEThreads) bins[i] = 0;
     __syncthreads();
-    for (int i = tid; i < m; i += kEThreads) {
+    for (int i = first + tid; i < end; i += kEThreads) {
       const uint32_t w = weight(i);
       if ((w & mask) == prefix) atomicAdd(&bins[(w >> shift) & digit], 1u);
     }
@@ -234,8 +254,8 @@ __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictPara
     __syncthreads();
   }
   // `need` of the weights that equal prefix stay, and all above it
-  const int stretch = ((m + kEWaves - 1) / kEWaves + 63) & ~63;
-  const int i0 = min(wave * stretch, m), i1 = min(i0 + stretch, m);
+  const int stretch = ((end - first + kEWaves - 1) / kEWaves + 63) & ~63;
+  const int i0 = min(first + wave * stretch, end), i1 = min(i0 + stretch, end);
   uint32_t na = 0, ns = 0;
   for (int i = i0 + lane; i - lane < i1; i += 64) {
     const uint32_t w = i < i1 ? weight(i) : 0u;
@@ -258,20 +278,22 @@ __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictPara
     const uint64_t a = __ballot(i < i1 && w > prefix), s = __ballot(i < i1 && w == prefix);
     const uint32_t ra = ba + __builtin_popcountll(a & below), rs = bs + __builtin_popcountll(s & below);
     const bool mine = i < i1 && (w > prefix || (w == prefix && rs < need));
-    if (mine) kept[first + ra + min(rs, need)] = first + i;
+    if (mine) kept[first + ra + min(rs, need)] = i;
     ba += __builtin_popcountll(a);
     bs += __builtin_popcountll(s);
   }
 }
 
-// Units [unit0, unit0 + per) of a head's row, of keys (side 0) or values (side 1), for all rows that stay.
-constexpr int kMThreads = 512, kMBytes = 64, kMDepth = 8;
-template <int U>
-__global__ __launch_bounds__(kMThreads) void evict_move_kernel(const EvictParams p, int slices) {
+// A head's rows that stay, of keys, of values (slices of W bytes of each) or the weights: in place all of them, a
+// round after the other; to other pages one round to a workgroup.  W is 256 where that gives every CU a workgroup,
+// else 64: 128-byte lines are then fetched by two workgroups, but four times as many share the rows.
+constexpr int kMThreads = 512, kMDepth = 8;
+template <int U, int W>
+__global__ __launch_bounds__(kMThreads) void evict_move_kernel(const EvictParams p) {
   typedef typename Unit<U>::type unit;
   const RowsParams& c = p.c;
-  const int tid = threadIdx.x;
-  const int z = blockIdx.x / (2 * slices + 1), part = blockIdx.x - z * (2 * slices + 1);
+  const int tid = threadIdx.x, slices = (c.head_bytes + W - 1) / W, parts = 2 * slices + 1;
+  const int z = blockIdx.x / parts, part = blockIdx.x - z * parts;
   const int b = z / c.kv_heads, kh = z - b * c.kv_heads;
   const int cap = (int)min((int64_t)c.max_blocks * c.block_size, (int64_t)(INT32_MAX / 2));
   const int n = min(max(p.lens[b], 0), min(cap, p.max_keys)), rows = min(n, p.budget);
@@ -280,20 +302,27 @@ __global__ __launch_bounds__(kMThreads) void evict_move_kernel(const EvictParams
   const int32_t* kept = p.kept + (int64_t)z * p.budget;
   const int32_t* to = inplace ? c.block_table : p.table_out;
   const int to_blocks = inplace ? c.max_blocks : p.max_blocks_out;
-  if (part == 2 * slices) {  // the weights
-    for (int i0 = 0; i0 < rows; i0 += kMThreads * kMDepth) {
+  constexpr int PER = W / U, ROWS = kMThreads / PER;  // units of a slice, rows at once
+  const bool weights = part == 2 * slices;
+  const int step = (weights ? kMThreads : ROWS) * kMDepth;
+  const int first = inplace ? 0 : (int)blockIdx.y * step;
+  const int last = inplace ? rows : (int)min((int64_t)first + step, (int64_t)rows);
+  if (weights) {
+    for (int i0 = first; i0 < last; i0 += step) {
       float w[kMDepth];
 #pragma unroll
       for (int k = 0; k < kMDepth; ++k) {
         const Slot s = slot_of(c, c.block_table, c.max_blocks, b, max(kept[min(i0 + k * kMThreads + tid, rows - 1)], 0));
         w[k] = p.weights[(s.page * c.kv_heads + kh) * c.block_size + (s.slot - s.page * c.block_size)];
       }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
+      if (inplace) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+      }
 #pragma unroll
       for (int k = 0; k < kMDepth; ++k) {
         const int i = i0 + k * kMThreads + tid;
-        if (i >= rows) continue;
+        if (i >= last) continue;
         const Slot d = slot_of(c, to, to_blocks, b, i);
         p.weights[(d.page * c.kv_heads + kh) * c.block_size + (d.slot - d.page * c.block_size)] = w[k];
       }
@@ -303,11 +332,10 @@ __global__ __launch_bounds__(kMThreads) void evict_move_kernel(const EvictParams
   const bool value = part >= slices;
   char* cache = value ? c.value_cache : c.key_cache;
   const float* scale = value ? c.v_scale : c.k_scale;
-  constexpr int PER = kMBytes / U, ROWS = kMThreads / PER;  // units of a slice, rows at once
   const int at = ((value ? part - slices : part) * PER + tid % PER) * U;
   const bool mine = at < c.head_bytes;
   const int64_t row = (int64_t)c.kv_heads * c.head_bytes, off = (int64_t)kh * c.head_bytes + (mine ? at : 0);
-  for (int i0 = 0; i0 < rows; i0 += ROWS * kMDepth) {
+  for (int i0 = first; i0 < last; i0 += step) {
     unit v[kMDepth];
     int from[kMDepth];
 #pragma unroll
@@ -328,10 +356,26 @@ __global__ __launch_bounds__(kMThreads) void evict_move_kernel(const EvictParams
 #pragma unroll
     for (int k = 0; k < kMDepth; ++k) {
       const int i = i0 + k * ROWS + tid / PER;
-      if (mine && i < rows && (!inplace || from[k] != i))
+      if (mine && i < last && (!inplace || from[k] != i))
         *reinterpret_cast<unit*>(cache + slot_of(c, to, to_blocks, b, i).slot * row + off) = v[k];
     }
   }
+}
+template <int U, int W>
+hipError_t launch_move(const EvictParams& p, hipStream_t s) {
+  const int64_t parts = 2 * ((p.c.head_bytes + W - 1) / W) + 1, wgs = parts * p.c.batch * p.c.kv_heads;
+  constexpr int step = kMThreads / (W / U) * kMDepth;
+  const int rows = std::min(p.budget, p.max_keys), rounds = p.table_out ? (rows + step - 1) / step : 1;
+  if (wgs > INT32_MAX || rounds > 65535) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((evict_move_kernel<U, W>), dim3((unsigned)wgs, (unsigned)rounds), dim3(kMThreads), 0, s, p);
+  return hipGetLastError();
+}
+template <int U>
+hipError_t launch_move_u(const EvictParams& p, hipStream_t s) {
+  // (units of one byte: rows of odd sizes, 64 of them to a row at once)
+  if constexpr (U == 16)
+    if (p.table_out || (int64_t)p.c.batch * p.c.kv_heads * ((p.c.head_bytes + 255) / 256) >= 128) return launch_move<U, 256>(p, s);
+  return launch_move<U, 64>(p, s);
 }
 
 // Bytes that rows of both caches allow at once.
@@ -358,19 +402,14 @@ hipError_t launch_accept(const AcceptParams& p, hipStream_t s) {
 hipError_t launch_evict(const EvictParams& p, hipStream_t s) {
   if (p.c.batch <= 0) return hipSuccess;
   const int64_t z = (int64_t)p.c.batch * p.c.kv_heads;
-  const int u = unit_of(p.c), slices = (p.c.head_bytes + kMBytes - 1) / kMBytes;
-  if (z * (2 * slices + 1) > INT32_MAX) return hipErrorInvalidValue;
+  const int u = unit_of(p.c);
   if (p.max_keys <= 8192)
     hipLaunchKernelGGL((evict_select_kernel<8192>), dim3((unsigned)z), dim3(kEThreads), 0, s, p);
   else
     hipLaunchKernelGGL((evict_select_kernel<32768>), dim3((unsigned)z), dim3(kEThreads), 0, s, p);
-  hipError_t e = hipGetLastError();
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const dim3 grid((unsigned)(z * (2 * slices + 1)));
-  if (u == 16) hipLaunchKernelGGL((evict_move_kernel<16>), grid, dim3(kMThreads), 0, s, p, slices);
-  else if (u == 4) hipLaunchKernelGGL((evict_move_kernel<4>), grid, dim3(kMThreads), 0, s, p, slices);
-  else hipLaunchKernelGGL((evict_move_kernel<1>), grid, dim3(kMThreads), 0, s, p, slices);
-  return hipGetLastError();
+  return u == 16 ? launch_move_u<16>(p, s) : u == 4 ? launch_move_u<4>(p, s) : launch_move_u<1>(p, s);
 }
 
 }  // namespace pa

@@ -30,26 +30,43 @@ __device__ __forceinline__ WRows key_rows(const RangedParams& p, const RSeq& e, 
   return WRows{lo * g, hi * g};
 }
 
-// Score in log2 units of a raw product.
-template <bool CAP>
-__device__ __forceinline__ float w_score(float s, float sl, float ck) {
-  return CAP ? half_tanh(s * ck) * sl : s * sl;
+// Forms of a score: as it is; under a softcap as a quotient, whose constant the exponent takes along, up to
+// kCapNear, and beyond it by tanh to its own bits -- the attention's own arithmetic (r_softmax), so that what the two
+// round alike cancels between a score and its row's constant.
+enum WForm { kWPlain = 0, kWNear = 1, kWFar = 2 };
+template <int FORM>
+__device__ __forceinline__ float w_raw(float s, float ck) {
+  if constexpr (FORM == kWNear) return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s * ck));
+  if constexpr (FORM == kWFar) return half_tanh(s * ck);
+  return s;
 }
 
-template <typename TT, int D, bool CAP>
-__global__ __launch_bounds__(256) void weigh_columns_kernel(const WeighParams wp) {
+// Query rows in tiles of 32, which the workgroup's wavefronts share in LDS, two of them: the next one arrives while
+// one is multiplied.  Blocks of keys over the same chunk of rows follow each other on one XCD, whose L2 then holds
+// the rows.
+template <typename TT, int D, int FORM>
+__global__ __launch_bounds__(256, 2) void weigh_columns_kernel(const WeighParams wp) {
+  using G = RGeom<D>;
+  constexpr int TILE = 32 * G::PITCH, NI = 8 / G::RPI;  // bytes of a tile; loads of a wavefront's eight rows
+  __shared__ __attribute__((aligned(1024))) char lds[2 * TILE];
+  __shared__ __attribute__((aligned(16))) float consts[2][32];
   const RangedParams& p = wp.r;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
-  const int blocks = (wp.max_keys + kWBlock - 1) / kWBlock, z = blockIdx.x / blocks;
-  const int kb0 = (blockIdx.x - z * blocks) * kWBlock, chunk = blockIdx.y;
+  const int blocks = (wp.max_keys + kWBlock - 1) / kWBlock, seqs = p.batch * p.kv_heads;
+  const int turn = blockIdx.x >> 3, group = (turn / blocks) * 8 + (blockIdx.x & 7);
+  if (group >= seqs * wp.chunks) return;
+  const int chunk = group / seqs, z = group - chunk * seqs, kb0 = (turn % blocks) * kWBlock;
   const int b = z / p.kv_heads, kh = z - b * p.kv_heads, g = p.num_heads / p.kv_heads;
   const RSeq e = r_seq(p, b);
+  if (kb0 >= e.total) return;
   const int k0 = kb0 + wave * kWKeys;
-  if (k0 >= e.total) return;
   const int first = p.observed > 0 ? max(e.nq - p.observed, 0) * g : 0;
   const int64_t from = (int64_t)first + (int64_t)chunk * wp.chunk_rows;
   const int rb = (int)min(from, (int64_t)e.nq * g), re = (int)min(from + wp.chunk_rows, (int64_t)e.nq * g);
-  float acc[2] = {0.0f, 0.0f};
+  // rows that some key of the workgroup counts, those that some and that all keys of the wavefront do
+  const int last = min(kb0 + kWBlock, e.total) - 1;
+  const int wg_lo = max(p.causal ? max(kb0 - e.past, 0) * g : 0, rb);
+  const int wg_hi = p.window > 0 ? (int)min((int64_t)re, max((int64_t)last - e.past + p.window, (int64_t)0) * g) : re;
   WRows rows[2];
   int some_lo = INT32_MAX, some_hi = 0, all_lo = 0, all_hi = INT32_MAX;
 #pragma unroll
@@ -59,54 +76,100 @@ __global__ __launch_bounds__(256) void weigh_columns_kernel(const WeighParams wp
     some_hi = max(some_hi, rows[kb].hi);
     all_lo = max(all_lo, rows[kb].lo);
     all_hi = min(all_hi, rows[kb].hi);
+    rows[kb].hi = min(rows[kb].hi, re);
   }
-  some_lo = max(half_min(some_lo), rb);
-  some_hi = min(half_max(some_hi), re);
+  some_lo = half_min(some_lo);
+  some_hi = half_max(some_hi);
   all_lo = half_max(all_lo);
   all_hi = min(half_min(all_hi), re);
-  if (some_lo < some_hi) {
+  float acc[2] = {0.0f, 0.0f};
+  if (wg_lo < wg_hi) {
     u32x4 k[2][D / 16];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       const char* src = reinterpret_cast<const char*>(p.key_cache) +
                         (r_offset(p, b, kh, min(k0 + 32 * kb + c, e.total - 1), D) + 8 * h) * 2;
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) k[kb][ks] = ld16(src + 32 * ks);
+      for (int ks = 0; ks < D / 16; ++ks) k[kb][ks] = ld16(src + 32 * ks) ^ p.qxor;
     }
     const float* stats = p.row_stats + ((int64_t)kh * p.num_tokens + e.s0) * g;
-    const float sl = CAP ? 2.0f * kLog2e * p.softcap : p.scale_log2, ck = CAP ? 2.0f * p.scale_log2 / p.softcap : 0.0f;
-    for (int r0 = some_lo; r0 < some_hi; r0 += 32) {
-      const int row = min(r0 + c, some_hi - 1), t = row / g;
-      const char* src = reinterpret_cast<const char*>(p.q) +
-                        (((int64_t)(e.s0 + t) * p.num_heads + kh * g + (row - t * g)) * D + 8 * h) * 2;
-      f32x4 st[4];
+    const char* q0 = reinterpret_cast<const char*>(p.q) + ((int64_t)e.s0 * p.num_heads + kh * g) * D * 2;
+    const uint32_t base = lds_address(lds) + wave * 8 * G::PITCH;
+    auto load = [&](int r0, int buf) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) st[i][j] = stats[min(r0 + 8 * i + 4 * h + j, some_hi - 1)];
-      f32x16 s[2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const u32x4 a = ld16(src + 32 * ks) ^ p.qxor;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) s[kb] = mfma_r<TT>(a, k[kb][ks], s[kb]);
+      for (int i = 0; i < NI; ++i) {
+        const int rr = wave * 8 + i * G::RPI + lane / G::CPR, r = min(r0 + rr, wg_hi - 1), t = r / g;
+        int piece = (lane % G::CPR) ^ G::kx(rr);
+        if (D == 96 && piece >= 12) piece -= 8;
+        dma_ptr(q0 + ((int64_t)t * p.num_heads + (r - t * g)) * D * 2 + 16 * piece, base + buf * TILE + 1024 * i);
       }
-      const bool whole = r0 >= all_lo && r0 + 32 <= all_hi;
+    };
+    const float sl = FORM == kWPlain ? p.scale_log2 : 2.0f * kLog2e * p.softcap;
+    const float off = FORM == kWNear ? kLog2e * p.softcap : 0.0f;
+    const float ck = FORM == kWPlain ? 0.0f : 2.0f * p.scale_log2 / p.softcap;
+    if (threadIdx.x < 32) consts[0][threadIdx.x] = off - stats[min(wg_lo + (int)threadIdx.x, wg_hi - 1)];
+    load(wg_lo, 0);
+    int buf = 0;
+    for (int r0 = wg_lo; r0 < wg_hi; r0 += 32, buf ^= 1) {
+      wait_loads<0>();
+      wait_lds_reads();
+      barrier();
+      const bool more = r0 + 32 < wg_hi;
+      float next = 0.0f;
+      if (more) {
+        if (threadIdx.x < 32) next = stats[min(r0 + 32 + (int)threadIdx.x, wg_hi - 1)];
+        load(r0 + 32, buf ^ 1);
+      }
+      if (r0 < some_hi && r0 + 32 > some_lo) {
+        const char* row = lds + buf * TILE + c * G::PITCH;
+        const int x = G::kx(c) ^ h;
+        f32x16 s[2];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = __builtin_amdgcn_exp2f(w_score<CAP>(s[kb][i], sl, ck) - st[i >> 2][i & 3]);
-          const int r = r0 + 8 * (i >> 2) + 4 * h + (i & 3);
-          acc[kb] += whole || (r >= rows[kb].lo && r < min(rows[kb].hi, re)) ? x : 0.0f;
+          for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+        constexpr int A = D / 16 % 4 ? 3 : 4;  // operands read a group of products ahead
+        u32x4 a[2][A];
+        auto read = [&](int gi) {
+#pragma unroll
+          for (int i = 0; i < A; ++i)
+            a[gi & 1][i] = *reinterpret_cast<const u32x4*>(row + (((2 * (gi * A + i)) ^ x) << 4));
+        };
+        read(0);
+#pragma unroll
+        for (int gi = 0; gi < D / 16 / A; ++gi) {
+          if (gi + 1 < D / 16 / A) read(gi + 1);
+          r_order();
+#pragma unroll
+          for (int i = 0; i < A; ++i)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) s[kb] = mfma_r<TT>(a[gi & 1][i], k[kb][gi * A + i], s[kb]);
+          r_order();
         }
+        f32x4 st[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st[i] = *reinterpret_cast<const f32x4*>(&consts[buf][8 * i + 4 * h]);
+        auto sum = [&](auto masked) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            f32x4 part = {0.0f, 0.0f, 0.0f, 0.0f};
+            const int lo = rows[kb].lo - r0 - 4 * h, hi = rows[kb].hi - r0 - 4 * h;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(w_raw<FORM>(s[kb][i], ck), sl, st[i >> 2][i & 3]));
+              const int r = 8 * (i >> 2) + (i & 3);
+              part[i & 3] += !decltype(masked)::value || (r >= lo && r < hi) ? w : 0.0f;
+            }
+            acc[kb] += (part[0] + part[1]) + (part[2] + part[3]);
+          }
+        };
+        if (r0 >= all_lo && r0 + 32 <= all_hi) sum(std::false_type{});
+        else sum(std::true_type{});
+      }
+      if (more && threadIdx.x < 32) consts[buf ^ 1][threadIdx.x] = off - next;
     }
   }
-  float* dst = wp.part + ((int64_t)chunk * p.batch * p.kv_heads + z) * wp.part_ld;
+  float* dst = wp.part + ((int64_t)chunk * seqs + z) * wp.part_ld;
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb) {
     const float sum = acc[kb] + half_swap(acc[kb]);
@@ -230,13 +293,19 @@ __global__ __launch_bounds__(256) void fold_kernel(const WeighParams wp) {
 
 template <typename TT, int D>
 void launch_columns(const WeighParams& p, dim3 grid, hipStream_t s) {
-  if (p.r.softcap > 0.0f)
-    hipLaunchKernelGGL((weigh_columns_kernel<TT, D, true>), grid, dim3(256), 0, s, p);
+  if (p.r.softcap > kCapNear)
+    hipLaunchKernelGGL((weigh_columns_kernel<TT, D, kWFar>), grid, dim3(256), 0, s, p);
+  else if (p.r.softcap > 0.0f)
+    hipLaunchKernelGGL((weigh_columns_kernel<TT, D, kWNear>), grid, dim3(256), 0, s, p);
   else
-    hipLaunchKernelGGL((weigh_columns_kernel<TT, D, false>), grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL((weigh_columns_kernel<TT, D, kWPlain>), grid, dim3(256), 0, s, p);
 }
 template <typename TT>
-hipError_t launch_matrix(const WeighParams& p, dim3 grid, hipStream_t s) {
+hipError_t launch_matrix(const WeighParams& p, hipStream_t s) {
+  const int64_t groups = (int64_t)p.r.batch * p.r.kv_heads * p.chunks, blocks = (p.max_keys + kWBlock - 1) / kWBlock;
+  const int64_t all = (groups + 7) / 8 * 8 * blocks;
+  if (all > INT32_MAX) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)all);
   switch (p.r.head_dim) {
     case 64: launch_columns<TT, 64>(p, grid, s); break;
     case 96: launch_columns<TT, 96>(p, grid, s); break;
@@ -271,11 +340,10 @@ hipError_t launch_weigh(const WeighParams& p, pa_dtype act, pa_dtype cache_dtype
     return hipErrorInvalidValue;
   if (!r.scores) {
     const bool matrix = ranged_supported(r.head_dim, act, cache_dtype) && r.slots > 0;
-    const int keys = matrix ? kWBlock : 16;
-    const dim3 grid((unsigned)((p.max_keys + keys - 1) / keys * z), p.chunks);
+    const dim3 grid((unsigned)((p.max_keys + 15) / 16 * z), p.chunks);
     hipError_t e;
     if (matrix)
-      e = act == PA_DTYPE_FLOAT16 ? launch_matrix<TF16>(p, grid, s) : launch_matrix<TBF16>(p, grid, s);
+      e = act == PA_DTYPE_FLOAT16 ? launch_matrix<TF16>(p, s) : launch_matrix<TBF16>(p, s);
     else
       e = act == PA_DTYPE_FLOAT16    ? launch_valu<TF16>(p, cache_dtype, grid, s)
           : act == PA_DTYPE_BFLOAT16 ? launch_valu<TBF16>(p, cache_dtype, grid, s)
