@@ -1510,7 +1510,7 @@ AccountPlan account_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a,
   // as many chunks as fill the GPU several times, of 512 rows at least
   const int64_t rows = std::max<int64_t>((observed > 0 ? std::min<int64_t>(observed, mq) : mq) * g, 1);
   const int64_t blocks = (t.ld + 255) / 256 * z;
-  const int64_t want = std::min<int64_t>((8 * (int64_t)device_cus() + blocks - 1) / std::max<int64_t>(blocks, 1), (rows + 511) / 512);
+  const int64_t want = std::min<int64_t>((24 * (int64_t)device_cus() + blocks - 1) / std::max<int64_t>(blocks, 1), (rows + 511) / 512);
   t.chunk_rows = (int)(((rows + want - 1) / want + 31) / 32 * 32);
   t.chunks = (int)((rows + t.chunk_rows - 1) / t.chunk_rows);
   t.sum_bytes = align256((size_t)t.chunks * z * t.ld * sizeof(float));

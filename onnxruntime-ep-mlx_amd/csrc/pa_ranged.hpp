@@ -70,6 +70,9 @@ constexpr int kRStart = 4;
 // What partial rows and their merge cost, in tiles of every worker: 3, 8 and 20 gave 826, 836 and 748 us over a
 // prompt of 8192, 236, 214 and 213 over six prompts of 1001 - 2500 at head 64; 25 each for 40 samples of 1500.
 constexpr float kRCut = 20.0f;
+// ... of drafted trees, whose few rows the merge joins in the 4 us that its launch takes anyway (a tree of 26 nodes after
+// 700 keys: 34 us with 10 or 20, 25 with 2 or 5; 24 trees of 9 - 33 nodes at head 64 45 with any).
+constexpr float kRCutTree = 5.0f;
 // Time of a tile where a workgroup has its CU to itself (1.0 instead: 1024 tokens over 1000 keys 70 us for
 // 62, over 3000 115 for 109).
 constexpr float kRAlone = 0.65f;
@@ -367,6 +370,7 @@ __device__ __forceinline__ void scan_chunk(const RangedParams& p, int base, RSca
 struct RShare {
   int wide, per[2];
 };
+template <int KIND>
 __device__ __forceinline__ RShare r_share(const RangedParams& p, const RTotals& t) {
   RShare r;
   const float cost = kRWideCost * (float)t.tiles[0];
@@ -387,7 +391,7 @@ __device__ __forceinline__ RShare r_share(const RangedParams& p, const RTotals& 
       turns <= 1 ? t.most * (2 * t.items[0] <= r.wide && p.per_cu > 1 ? kRAlone : 1.0f)
                  : fmaxf((float)t.most, avg * turns * (1.0f - spread) + 1.05f * even * spread);
   const bool take = p.whole || (p.doc_starts && 2 * t.items[0] >= r.wide) ||
-                    whole <= even + (p.groups ? 0.25f : 1.0f) * kRCut;
+                    whole <= even + (p.groups ? 0.25f : 1.0f) * (KIND == kRTree ? kRCutTree : kRCut);
   r.per[0] = take || t.items[0] == 0 ? 0 : max((t.tiles[0] + r.wide - 1) / max(r.wide, 1), p.least[0]);
   r.per[1] = p.whole || t.items[1] == 0 ? 0 : max((t.tiles[1] + waves - 1) / waves, p.least[1]);
   return r;
@@ -1149,7 +1153,7 @@ ranged_kernel(const RangedParams p) {
     scan_chunk(p, base, sh, t);
     if (c < -1) continue;
     if (c == -1 || chunks == 1) {
-      r = r_share(p, t);
+      r = r_share<KIND>(p, t);
       kind = (int)blockIdx.x < r.wide ? 0 : 1;
       queued = p.queue && kind == 0 && r.per[0] == 0;
       me = kind ? ((int)blockIdx.x - r.wide) * 4 + wave : (int)blockIdx.x;

@@ -287,26 +287,31 @@ __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictPara
 // A head's rows that stay, of keys, of values (slices of W bytes of each) or the weights: in place all of them, a
 // round after the other; to other pages one round to a workgroup.  W is 256 where that gives every CU a workgroup,
 // else 64: 128-byte lines are then fetched by two workgroups, but four times as many share the rows.
-constexpr int kMThreads = 512, kMDepth = 8;
-template <int U, int W>
-__global__ __launch_bounds__(kMThreads) void evict_move_kernel(const EvictParams p) {
+// Bound by HBM: 2048 of up to 9000 rows of 8 heads of 16 sequences, 268 MB read and written, to other pages in 58 us
+// (4.6 TB/s; a copy of 1 GiB 5.2; in rounds of 64 KB 75 us, with stores that stay in the cache 62).
+template <bool INPLACE>
+struct Round {  // threads, rows in flight of each
+  static constexpr int THREADS = INPLACE ? 512 : 256, DEPTH = INPLACE ? 8 : 4;
+};
+template <int U, int W, bool INPLACE>
+__global__ __launch_bounds__(Round<INPLACE>::THREADS) void evict_move_kernel(const EvictParams p) {
   typedef typename Unit<U>::type unit;
+  constexpr int kMThreads = Round<INPLACE>::THREADS, kMDepth = Round<INPLACE>::DEPTH;
   const RowsParams& c = p.c;
   const int tid = threadIdx.x, slices = (c.head_bytes + W - 1) / W, parts = 2 * slices + 1;
   const int z = blockIdx.x / parts, part = blockIdx.x - z * parts;
   const int b = z / c.kv_heads, kh = z - b * c.kv_heads;
   const int cap = (int)min((int64_t)c.max_blocks * c.block_size, (int64_t)(INT32_MAX / 2));
   const int n = min(max(p.lens[b], 0), min(cap, p.max_keys)), rows = min(n, p.budget);
-  const bool inplace = p.table_out == nullptr;
-  if (inplace && n <= p.budget) return;
+  if (INPLACE && n <= p.budget) return;
   const int32_t* kept = p.kept + (int64_t)z * p.budget;
-  const int32_t* to = inplace ? c.block_table : p.table_out;
-  const int to_blocks = inplace ? c.max_blocks : p.max_blocks_out;
+  const int32_t* to = INPLACE ? c.block_table : p.table_out;
+  const int to_blocks = INPLACE ? c.max_blocks : p.max_blocks_out;
   constexpr int PER = W / U, ROWS = kMThreads / PER;  // units of a slice, rows at once
   const bool weights = part == 2 * slices;
   const int step = (weights ? kMThreads : ROWS) * kMDepth;
-  const int first = inplace ? 0 : (int)blockIdx.y * step;
-  const int last = inplace ? rows : (int)min((int64_t)first + step, (int64_t)rows);
+  const int first = INPLACE ? 0 : (int)blockIdx.y * step;
+  const int last = INPLACE ? rows : (int)min((int64_t)first + step, (int64_t)rows);
   if (weights) {
     for (int i0 = first; i0 < last; i0 += step) {
       float w[kMDepth];
@@ -315,7 +320,7 @@ __global__ __launch_bounds__(kMThreads) void evict_move_kernel(const EvictParams
         const Slot s = slot_of(c, c.block_table, c.max_blocks, b, max(kept[min(i0 + k * kMThreads + tid, rows - 1)], 0));
         w[k] = p.weights[(s.page * c.kv_heads + kh) * c.block_size + (s.slot - s.page * c.block_size)];
       }
-      if (inplace) {
+      if (INPLACE) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
       }
@@ -349,33 +354,41 @@ __global__ __launch_bounds__(kMThreads) void evict_move_kernel(const EvictParams
         v[k] = recode_unit<U>(v[k], scale[s.page * c.kv_heads + kh], scale[d.page * c.kv_heads + kh]);
       }
     }
-    if (inplace) {  // every row of the round has been read
+    if (INPLACE) {  // every row of the round has been read
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
     }
 #pragma unroll
     for (int k = 0; k < kMDepth; ++k) {
       const int i = i0 + k * ROWS + tid / PER;
-      if (mine && i < last && (!inplace || from[k] != i))
-        *reinterpret_cast<unit*>(cache + slot_of(c, to, to_blocks, b, i).slot * row + off) = v[k];
+      if (!mine || i >= last || (INPLACE && from[k] == i)) continue;
+      unit* dst = reinterpret_cast<unit*>(cache + slot_of(c, to, to_blocks, b, i).slot * row + off);
+      if (INPLACE) *dst = v[k];
+      else __builtin_nontemporal_store(v[k], dst);
     }
   }
 }
+template <int U, int W, bool INPLACE>
+hipError_t launch_move_in(const EvictParams& p, hipStream_t s) {
+  const int64_t parts = 2 * ((p.c.head_bytes + W - 1) / W) + 1, wgs = parts * p.c.batch * p.c.kv_heads;
+  constexpr int step = Round<INPLACE>::THREADS / (W / U) * Round<INPLACE>::DEPTH;
+  const int rows = std::min(p.budget, p.max_keys);
+  const int64_t rounds = INPLACE ? 1 : (rows + step - 1) / step;
+  if (wgs > INT32_MAX || rounds > 65535) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((evict_move_kernel<U, W, INPLACE>), dim3((unsigned)wgs, (unsigned)rounds),
+                     dim3(Round<INPLACE>::THREADS), 0, s, p);
+  return hipGetLastError();
+}
 template <int U, int W>
 hipError_t launch_move(const EvictParams& p, hipStream_t s) {
-  const int64_t parts = 2 * ((p.c.head_bytes + W - 1) / W) + 1, wgs = parts * p.c.batch * p.c.kv_heads;
-  constexpr int step = kMThreads / (W / U) * kMDepth;
-  const int rows = std::min(p.budget, p.max_keys), rounds = p.table_out ? (rows + step - 1) / step : 1;
-  if (wgs > INT32_MAX || rounds > 65535) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((evict_move_kernel<U, W>), dim3((unsigned)wgs, (unsigned)rounds), dim3(kMThreads), 0, s, p);
-  return hipGetLastError();
+  return p.table_out ? launch_move_in<U, W, false>(p, s) : launch_move_in<U, W, true>(p, s);
 }
 template <int U>
 hipError_t launch_move_u(const EvictParams& p, hipStream_t s) {
-  // (units of one byte: rows of odd sizes, 64 of them to a row at once)
   if constexpr (U == 16)
-    if (p.table_out || (int64_t)p.c.batch * p.c.kv_heads * ((p.c.head_bytes + 255) / 256) >= 128) return launch_move<U, 256>(p, s);
-  return launch_move<U, 64>(p, s);
+    if (p.table_out || (int64_t)p.c.batch * p.c.kv_heads * ((p.c.head_bytes + 255) / 256) >= 128)
+      return launch_move<U, 256>(p, s);
+  return launch_move<U, 64>(p, s);  // (odd rows too: bytes, 64 of a row at once)
 }
 
 // Bytes that rows of both caches allow at once.

@@ -95,20 +95,38 @@ __global__ __launch_bounds__(256, 2) void weigh_columns_kernel(const WeighParams
     const float* stats = p.row_stats + ((int64_t)kh * p.num_tokens + e.s0) * g;
     const char* q0 = reinterpret_cast<const char*>(p.q) + ((int64_t)e.s0 * p.num_heads + kh * g) * D * 2;
     const uint32_t base = lds_address(lds) + wave * 8 * G::PITCH;
-    auto load = [&](int r0, int buf) {
+    // This lane's rows of the tile to be loaded next: token and head of the group, moved on by 32 rows a tile (a division
+    // for each instead was a quarter of the loop's vector instructions); rows behind the last one repeat it.
+    int tok[NI], head[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = wg_lo + wave * 8 + i * G::RPI + lane / G::CPR;
+      tok[i] = r / g;
+      head[i] = r - tok[i] * g;
+    }
+    const int dt = 32 / g, dh = 32 - dt * g, last_t = (wg_hi - 1) / g, last_h = wg_hi - 1 - last_t * g;
+    const uint32_t row_bytes = D * 2, tok_bytes = (uint32_t)p.num_heads * row_bytes;
+    auto load = [&](int buf) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int rr = wave * 8 + i * G::RPI + lane / G::CPR, r = min(r0 + rr, wg_hi - 1), t = r / g;
-        int piece = (lane % G::CPR) ^ G::kx(rr);
+        int piece = (lane % G::CPR) ^ G::kx(wave * 8 + i * G::RPI + lane / G::CPR);
         if (D == 96 && piece >= 12) piece -= 8;
-        dma_ptr(q0 + ((int64_t)t * p.num_heads + (r - t * g)) * D * 2 + 16 * piece, base + buf * TILE + 1024 * i);
+        const bool behind = tok[i] > last_t || (tok[i] == last_t && head[i] > last_h);
+        const uint32_t t = behind ? last_t : tok[i], hd = behind ? last_h : head[i];
+        dma_ptr(q0 + ((uint64_t)t * tok_bytes + hd * row_bytes + 16 * piece), base + buf * TILE + 1024 * i);
+        tok[i] += dt;
+        head[i] += dh;
+        if (head[i] >= g) {
+          head[i] -= g;
+          ++tok[i];
+        }
       }
     };
     const float sl = FORM == kWPlain ? p.scale_log2 : 2.0f * kLog2e * p.softcap;
     const float off = FORM == kWNear ? kLog2e * p.softcap : 0.0f;
     const float ck = FORM == kWPlain ? 0.0f : 2.0f * p.scale_log2 / p.softcap;
     if (threadIdx.x < 32) consts[0][threadIdx.x] = off - stats[min(wg_lo + (int)threadIdx.x, wg_hi - 1)];
-    load(wg_lo, 0);
+    load(0);
     int buf = 0;
     for (int r0 = wg_lo; r0 < wg_hi; r0 += 32, buf ^= 1) {
       wait_loads<0>();
@@ -118,7 +136,7 @@ __global__ __launch_bounds__(256, 2) void weigh_columns_kernel(const WeighParams
       float next = 0.0f;
       if (more) {
         if (threadIdx.x < 32) next = stats[min(r0 + 32 + (int)threadIdx.x, wg_hi - 1)];
-        load(r0 + 32, buf ^ 1);
+        load(buf ^ 1);
       }
       if (r0 < some_hi && r0 + 32 > some_lo) {
         const char* row = lds + buf * TILE + c * G::PITCH;
@@ -262,20 +280,31 @@ __global__ __launch_bounds__(256) void fold_kernel(const WeighParams wp) {
       hi = max(hi, rows[i].hi);
     }
     const int64_t first = ((int64_t)kh * p.num_tokens + e.s0) * g;
-    for (int r = lo; r < hi; ++r) {
-      float x[V];
-      load(p.scores + (first + r) * p.score_ld + key, x);
-      const float st = p.row_stats[first + r];
+    for (int r0 = lo; r0 < hi; r0 += 4) {  // (four rows in flight)
+      float x[4][V], st[4];
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        sum[i] += r >= rows[i].lo && r < rows[i].hi ? __builtin_amdgcn_exp2f(x[i] - st) : 0.0f;
+      for (int k = 0; k < 4; ++k) {
+        const int64_t row = first + min(r0 + k, hi - 1);
+        load(p.scores + row * p.score_ld + key, x[k]);
+        st[k] = p.row_stats[row];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          sum[i] += r0 + k >= rows[i].lo && r0 + k < rows[i].hi ? __builtin_amdgcn_exp2f(x[k][i] - st[k]) : 0.0f;
     }
   } else {
-    for (int ch = 0; ch < wp.chunks; ++ch) {
-      float x[V];
-      load(wp.part + ((int64_t)ch * p.batch * p.kv_heads + z) * wp.part_ld + key, x);
+    const float* part = wp.part + (int64_t)z * wp.part_ld + key;
+    const int64_t step = (int64_t)p.batch * p.kv_heads * wp.part_ld;
+    for (int c0 = 0; c0 < wp.chunks; c0 += 8) {  // (eight chunks in flight)
+      float x[8][V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum[i] += x[i];
+      for (int k = 0; k < 8; ++k) load(part + min(c0 + k, wp.chunks - 1) * step, x[k]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] += c0 + k < wp.chunks ? x[k][i] : 0.0f;
     }
   }
   int64_t page = p.block_table[(int64_t)b * p.max_blocks + min(key / p.block_size, p.max_blocks - 1)];

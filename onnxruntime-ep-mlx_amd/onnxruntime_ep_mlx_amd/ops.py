@@ -114,9 +114,11 @@ def batch_desc(cum: torch.Tensor, past: torch.Tensor, block_table: torch.Tensor,
                max_context_len: int = 0) -> capi.PaBatch:
     for name, t in (("cumulative_sequence_length", cum), ("past_seqlens", past),
                     ("block_table", block_table), ("slot_mapping", slot_mapping)):
-        if t is not None and t.dtype != torch.int32:
-            raise ValueError(f"input {name} must be int32")
-        _contig(name, t)
+        if t is not None:
+            if t.dtype != torch.int32:
+                raise ValueError(f"input {name} must be int32")
+            if not t.is_contiguous():
+                _contig(name, t)
     return capi.PaBatch(_ptr(cum), _ptr(past), _ptr(block_table), _ptr(slot_mapping),
                         cum.numel() - 1, block_table.shape[1], num_tokens, max_query_len, flags,
                         max_context_len)
