@@ -48,6 +48,8 @@ typedef struct pa_drafts {
   int32_t* path_lens;      /* [batch] */
   int64_t* next_tokens;    /* [batch]: the target of the path's last node (-1: no new tokens); or NULL */
   int32_t max_path;        /* >= 1; longer paths end there */
+  float* key_weights;      /* the cache's accounts (see below), which the path's rows begin anew at
+                            * zero; or NULL */
 } pa_drafts;
 
 /* ---- Accounts and eviction -------------------------------------------------------------------

@@ -1491,6 +1491,7 @@ struct AccountPlan {
   RangedPlan r;
   size_t bytes() const { return stat_bytes + sum_bytes + attn_bytes; }
 };
+constexpr size_t kAccountScores = (size_t)1 << 30;
 AccountPlan account_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a, int observed, pa_dtype act) {
   AccountPlan t;
   const int64_t g = a->num_heads / c->kv_heads, T = b->num_tokens, z = (int64_t)b->batch * c->kv_heads;
@@ -1501,13 +1502,16 @@ AccountPlan account_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a,
   t.r = ranged_plan(c, b, a, nullptr, act);
   t.attn_bytes = t.r.on ? t.r.bytes() : ws_need(c, b, a, act, 3, 0).best;
   t.stat_bytes = align256((size_t)T * a->num_heads * sizeof(float));
-  // every sequence's rows of a kv-head on a wavefront of their own
-  t.scores = t.r.on && !t.r.wide;
+  // Every sequence's rows of a kv-head on a wavefront of their own leave their scores, within a GiB: a step of 48 sequences
+  // of up to 8190 keys takes 30 us to write and 12 to read them where its keys take 77 to be read again.
+  const size_t scores = align256((size_t)T * a->num_heads * t.ld * sizeof(float));
+  t.scores = t.r.on && !t.r.wide && scores <= kAccountScores;
   if (t.scores) {
-    t.sum_bytes = align256((size_t)T * a->num_heads * t.ld * sizeof(float));
+    t.sum_bytes = scores;
     return t;
   }
-  // as many chunks as fill the GPU several times, of 512 rows at least
+  // as many chunks as fill the GPU several times, of 512 rows at least (4095 tokens after 600, 6 heads to a kv-head of 256:
+  // 8 workgroups to a CU 218 us and 10 to add the sums up, 24 208 and 7)
   const int64_t rows = std::max<int64_t>((observed > 0 ? std::min<int64_t>(observed, mq) : mq) * g, 1);
   const int64_t blocks = (t.ld + 255) / 256 * z;
   const int64_t want = std::min<int64_t>((24 * (int64_t)device_cus() + blocks - 1) / std::max<int64_t>(blocks, 1), (rows + 511) / 512);
@@ -1646,6 +1650,8 @@ int pa_accept_drafts(const pa_cache* c, const pa_batch* b, const pa_drafts* d, p
     return fail(PA_ERR_INVALID_ARGUMENT, "accepting drafts: path, path_lens and a positive max_path are required");
   if ((d->parents == nullptr) != (d->tokens == nullptr) || (d->parents == nullptr) != (d->targets == nullptr))
     return fail(PA_ERR_INVALID_ARGUMENT, "accepting drafts: parents, tokens and targets must be provided together");
+  if (reinterpret_cast<uintptr_t>(d->key_weights) & 3)
+    return fail(PA_ERR_INVALID_ARGUMENT, "accepting drafts: key_weights must be 4-byte aligned");
   if (!d->parents && d->next_tokens)
     return fail(PA_ERR_INVALID_ARGUMENT, "accepting drafts: next_tokens without targets");
   pa::AcceptParams p{};
@@ -1658,6 +1664,7 @@ int pa_accept_drafts(const pa_cache* c, const pa_batch* b, const pa_drafts* d, p
   p.path = d->path;
   p.path_lens = d->path_lens;
   p.next_tokens = d->next_tokens;
+  p.weights = d->key_weights;
   p.num_tokens = b->num_tokens;
   p.max_path = d->max_path;
   const hipError_t e = pa::launch_accept(p, reinterpret_cast<hipStream_t>(stream));
@@ -1689,6 +1696,8 @@ int pa_accumulating_attention(const pa_cache* c, const pa_batch* b, const pa_att
   if (!key_weights || (reinterpret_cast<uintptr_t>(key_weights) & 3))
     return fail(PA_ERR_INVALID_ARGUMENT, "key_weights must be given, 4-byte aligned");
   const AccountPlan t = account_plan(c, b, a, observed_rows, act);
+  if (t.ld / 16 * b->batch * c->kv_heads * std::max(t.chunks / 16, 1) > INT32_MAX)
+    return fail(PA_ERR_UNSUPPORTED, "accumulating attention: too many keys of all sequences; bound them by max_context_len");
   if ((rc = check_ranged(c, b, a, act, q, out, ws, ws_bytes, t.bytes(), t.r.on))) return rc;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   char* base = reinterpret_cast<char*>(ws);

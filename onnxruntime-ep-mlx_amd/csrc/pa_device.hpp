@@ -526,6 +526,7 @@ struct AcceptParams {
   int32_t* path;            // [batch, max_path]
   int32_t* path_lens;
   int64_t* next_tokens;     // or null
+  float* weights;           // accounts that the path's rows begin anew, or null
   int32_t num_tokens, max_path;
 };
 hipError_t launch_accept(const AcceptParams& p, hipStream_t s);

@@ -123,6 +123,12 @@ __global__ __launch_bounds__(256) void accept_kernel(const AcceptParams p) {
       if (p.next_tokens) p.next_tokens[b] = len > 0 ? p.targets[s0 + path[len - 1]] : -1;
     }
   }
+  if (p.weights && blockIdx.x == 0)
+    for (int i = tid; i < len * c.kv_heads; i += 256) {
+      const int r = i / c.kv_heads, kh = i - r * c.kv_heads;
+      const Slot d = slot_of(c, c.block_table, c.max_blocks, b, past + r);
+      p.weights[(d.page * c.kv_heads + kh) * c.block_size + (d.slot - d.page * c.block_size)] = 0.0f;
+    }
   // rows of whole tokens, keys then values
   const int64_t row = (int64_t)c.kv_heads * c.head_bytes;
   const int64_t x = ((int64_t)blockIdx.x * 256 + tid) * U;

@@ -211,7 +211,7 @@ PA_MAX_TREE_NODES = 4096  # include/pa_mi355x_upkeep.h
 class PaDrafts(C.Structure):
     _fields_ = [("parents", C.c_void_p), ("tokens", C.c_void_p), ("targets", C.c_void_p),
                 ("path", C.c_void_p), ("path_lens", C.c_void_p), ("next_tokens", C.c_void_p),
-                ("max_path", C.c_int32)]
+                ("max_path", C.c_int32), ("key_weights", C.c_void_p)]
 
 
 class PaEviction(C.Structure):

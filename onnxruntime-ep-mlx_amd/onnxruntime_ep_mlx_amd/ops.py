@@ -98,12 +98,13 @@ def cache_desc(key_cache: torch.Tensor, value_cache: torch.Tensor,
         head_dim = 2 * width if dt == capi.PA_DTYPE_INT4 else width
     elif (head_dim + 1) // 2 != width if dt == capi.PA_DTYPE_INT4 else head_dim != width:
         raise ValueError("key_cache must be [num_blocks,block_size,kv_num_heads,head_size]")
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t is not None:
-            if t.dtype != torch.float32:
-                raise ValueError(f"{name} must be float32")
-            _need_cuda(name, t)
-            _contig(name, t)
+    if k_scale is not None or v_scale is not None:
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t is not None:
+                if t.dtype != torch.float32:
+                    raise ValueError(f"{name} must be float32")
+                _need_cuda(name, t)
+                _contig(name, t)
     return capi.PaCache(_ptr(key_cache), _ptr(value_cache), _ptr(k_scale), _ptr(v_scale),
                         nb, bs, kv, head_dim, dt, _quant(k_quant_type), _quant(v_quant_type))
 
@@ -302,6 +303,8 @@ def _rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> int:
 
 def _scales_hold(cache: capi.PaCache, k_scale, v_scale) -> None:
     """Scales hold what the library reads: fp8 one per block and head, integers one or one per channel."""
+    if k_scale is None and v_scale is None:
+        return
     for name, t, mode in (("k_scale", k_scale, cache.k_quant_type), ("v_scale", v_scale, cache.v_quant_type)):
         if t is None:
             continue
@@ -568,8 +571,8 @@ def _rows_call(key_cache, value_cache, block_table, lens, k_scale, v_scale, k_qu
 
 
 def accept_drafts(key_cache, value_cache, cum, past, block_table, parents=None, draft_tokens=None,
-                  target_tokens=None, *, path=None, path_lens=None, max_path=0, k_scale=None, v_scale=None,
-                  k_quant_type="NONE", v_quant_type="NONE", max_query_len=0):
+                  target_tokens=None, *, path=None, path_lens=None, max_path=0, key_weights=None, k_scale=None,
+                  v_scale=None, k_quant_type="NONE", v_quant_type="NONE", max_query_len=0):
     """The accepted path of every drafted tree, its rows moved to where the sequence goes on
     (pa_accept_drafts): row path[i] of a sequence's new tokens to slot past + i.
 
@@ -578,7 +581,8 @@ def accept_drafts(key_cache, value_cache, cum, past, block_table, parents=None, 
     [num_tokens], ``parents`` as in tree_attention), up to ``max_path`` nodes (0: max_query_len, else
     num_tokens).  Returns (path int32 [batch, max_path], -1 behind its end; path_lens int32 [batch]; the
     target of the last node, int64 [batch]): the sequences go on with past + path_lens keys.  For a path chosen
-    otherwise give ``path`` (rising rows) and ``path_lens`` instead; the third result is then None.  The
+    otherwise give ``path`` (rising rows) and ``path_lens`` instead; the third result is then None.  The rows of
+    the path begin at zero in ``key_weights``, where that is given (the account of accumulating_attention).  The
     pages of the new tokens must belong to their sequence alone."""
     given = path is not None
     if given == (parents is not None) or given != (path_lens is not None):
@@ -586,6 +590,8 @@ def accept_drafts(key_cache, value_cache, cum, past, block_table, parents=None, 
     cache = _rows_call(key_cache, value_cache, block_table, past, k_scale, v_scale, k_quant_type, v_quant_type,
                        (("cum", cum), ("parents", parents), ("draft_tokens", draft_tokens),
                         ("target_tokens", target_tokens), ("path", path), ("path_lens", path_lens)))
+    if key_weights is not None:
+        _account(key_weights, key_cache)
     B, dev = past.numel(), key_cache.device
     if cum.numel() != B + 1:
         raise ValueError("PagedAttention: inconsistent cumulative lengths, past lengths or block table")
@@ -603,11 +609,11 @@ def accept_drafts(key_cache, value_cache, cum, past, block_table, parents=None, 
                 or draft_tokens.numel() != tokens or target_tokens.numel() != tokens:
             raise ValueError("PagedAttention: parents must be int32, draft_tokens and target_tokens int64 [num_tokens]")
         path = torch.empty((B, max_path or max_query_len or max(tokens, 1)), dtype=torch.int32, device=dev)
-        path_lens = torch.empty(B, dtype=torch.int32, device=dev)
+        path_lens = torch.empty_like(past)
         after = torch.empty(B, dtype=torch.int64, device=dev)
     batch = batch_desc(cum, past, block_table, tokens, None, max_query_len)
     drafts = capi.PaDrafts(_ptr(parents), _ptr(draft_tokens), _ptr(target_tokens), _ptr(path), _ptr(path_lens),
-                           _ptr(after), path.shape[1])
+                           _ptr(after), path.shape[1], _ptr(key_weights))
     capi.check(_on_device(key_cache.get_device(), capi.load().pa_accept_drafts, C.byref(cache), C.byref(batch),
                           C.byref(drafts)))
     return path, path_lens, after
@@ -663,7 +669,7 @@ def evict_keys(key_cache, value_cache, key_weights, lens, block_table, *, budget
                                         or block_table_out.shape[0] != B):
         raise ValueError("PagedAttention: block_table_out must be int32 [batch, max_blocks]")
     kept = torch.empty((B, kv, max(budget, 0)), dtype=torch.int32, device=dev)
-    lens_out = torch.empty(B, dtype=torch.int32, device=dev)
+    lens_out = torch.empty_like(lens)
     batch = capi.PaBatch(None, _ptr(lens), _ptr(block_table), None, B, block_table.shape[1], 0, 0, 0,
                          max_context_len)
     ev = capi.PaEviction(_ptr(key_weights), budget, sinks, recent, _ptr(block_table_out),

@@ -210,3 +210,10 @@ def test_two_streams_at_once_same_bits():
         for o, w in got[i]:
             assert torch.equal(o, want[i][0])
             assert torch.equal(w.view(torch.int32), want[i][1].view(torch.int32))
+
+
+def test_steps_behind_long_tables():
+    """More scores than are held: the keys are read again instead."""
+    st = make_batch([1] * 4, [100, 50, 900, 3], H=32, KV=2, D=64, block=16, dtype=F16, seed=16, spare=140000)
+    compare(st, call=dict(max_context_len=0))
+    compare(st, call=dict(max_context_len=0), observed=1)
