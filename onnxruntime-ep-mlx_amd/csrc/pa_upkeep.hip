@@ -223,7 +223,14 @@ __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictPara
       for (int i = tid; i < end; i += kEThreads) held[i] = weight_order(*load(i));
     }
   }
-  auto weight = [&](int i) { return hold ? held[i] : weight_order(*load(i)); };
+  // weights i .. i + 3 (i a multiple of four; what lies outside [first, end) may be anything)
+  auto quad = [&](int i) {
+    if (hold) return *reinterpret_cast<const u32x4*>(held + min(i, HELD - 4));
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = weight_order(*load(min(i + k, end - 1)));
+    return w;
+  };
   uint32_t prefix = 0, mask = 0;
 #pragma unroll 1
   for (int round = 0; round < 3; ++round) {
@@ -231,9 +238,11 @@ __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictPara
     const uint32_t digit = round == 2 ? 1023u : 2047u;
     for (int i = tid; i < kEBins; i += kEThreads) bins[i] = 0;
     __syncthreads();
-    for (int i = first + tid; i < end; i += kEThreads) {
-      const uint32_t w = weight(i);
-      if ((w & mask) == prefix) atomicAdd(&bins[(w >> shift) & digit], 1u);
+    for (int i = (first & ~3) + 4 * tid; i < end; i += 4 * kEThreads) {
+      const u32x4 w = quad(i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k >= first && i + k < end && (w[k] & mask) == prefix) atomicAdd(&bins[(w[k] >> shift) & digit], 1u);
     }
     __syncthreads();
     // bins from the top: thread t holds 2047 - 2 t and the one below
@@ -260,13 +269,22 @@ __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictPara
     __syncthreads();
   }
   // `need` of the weights that equal prefix stay, and all above it
-  const int stretch = ((end - first + kEWaves - 1) / kEWaves + 63) & ~63;
-  const int i0 = min(first + wave * stretch, end), i1 = min(i0 + stretch, end);
-  uint32_t na = 0, ns = 0;
-  for (int i = i0 + lane; i - lane < i1; i += 64) {
-    const uint32_t w = i < i1 ? weight(i) : 0u;
-    na += __builtin_popcountll(__ballot(i < i1 && w > prefix));
-    ns += __builtin_popcountll(__ballot(i < i1 && w == prefix));
+  const int stretch = ((end - (first & ~3) + kEWaves - 1) / kEWaves + 255) & ~255;  // four weights to a lane at a time
+  const int i0 = (first & ~3) + wave * stretch, i1 = min(i0 + stretch, end);
+  int na = 0, ns = 0;
+  for (int i = i0 + 4 * lane; i < i1; i += 256) {
+    const u32x4 w = quad(i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool in = i + k >= first && i + k < i1;
+      na += in && w[k] > prefix ? 1 : 0;
+      ns += in && w[k] == prefix ? 1 : 0;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    na += __shfl_xor(na, o, 64);
+    ns += __shfl_xor(ns, o, 64);
   }
   if (lane == 0) {
     above[wave] = na;
@@ -279,14 +297,27 @@ __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictPara
     bs += same[w];
   }
   const uint64_t below = ((uint64_t)1 << lane) - 1;
-  for (int i = i0 + lane; i - lane < i1; i += 64) {
-    const uint32_t w = i < i1 ? weight(i) : 0u;
-    const uint64_t a = __ballot(i < i1 && w > prefix), s = __ballot(i < i1 && w == prefix);
-    const uint32_t ra = ba + __builtin_popcountll(a & below), rs = bs + __builtin_popcountll(s & below);
-    const bool mine = i < i1 && (w > prefix || (w == prefix && rs < need));
-    if (mine) kept[first + ra + min(rs, need)] = i;
-    ba += __builtin_popcountll(a);
-    bs += __builtin_popcountll(s);
+  for (int i = i0 + 4 * lane; i - 4 * lane < i1; i += 256) {
+    const u32x4 w = quad(min(i, (end - 1) & ~3));
+    uint32_t ra = ba, rs = bs;  // of those that stay before this lane's four, and so on
+    bool a[4], e[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool in = i + k >= first && i + k < i1;
+      a[k] = in && w[k] > prefix;
+      e[k] = in && w[k] == prefix;
+      const uint64_t ma = __ballot(a[k]), me = __ballot(e[k]);
+      ra += __builtin_popcountll(ma & below);
+      rs += __builtin_popcountll(me & below);
+      ba += __builtin_popcountll(ma);
+      bs += __builtin_popcountll(me);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (a[k] || (e[k] && rs < need)) kept[first + ra + min(rs, need)] = i + k;
+      ra += a[k] ? 1 : 0;
+      rs += e[k] ? 1 : 0;
+    }
   }
 }
 
