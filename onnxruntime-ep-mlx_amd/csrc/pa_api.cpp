@@ -1461,7 +1461,8 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
 }
 
 // ------------------------------------------------------------------------------ drafted trees
-// Words of a node's bits, and the workspace: the bits and lags, then the attention's own.
+// Words of a node's bits (none: the matrix-core kernel makes those of small trees itself), and the workspace: the bits
+// and lags, then the attention's own.
 struct TreePlan {
   int words = 0;
   size_t bits_bytes = 0, lag_bytes = 0, attn_bytes = 0;
@@ -1472,10 +1473,10 @@ TreePlan tree_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dt
   TreePlan t;
   const int nodes = std::min(b->max_query_len > 0 ? std::min(b->max_query_len, b->num_tokens) : b->num_tokens,
                              PA_MAX_TREE_NODES);
-  t.words = std::max((nodes + 31) / 32, 1);
+  t.r = ranged_plan(c, b, a, nullptr, act);
+  t.words = t.r.on && nodes <= 64 ? 0 : std::max((nodes + 31) / 32, 1);
   t.bits_bytes = align256((size_t)b->num_tokens * t.words * sizeof(uint32_t));
   t.lag_bytes = align256((size_t)b->num_tokens * sizeof(int32_t));
-  t.r = ranged_plan(c, b, a, nullptr, act);
   t.attn_bytes = t.r.on ? t.r.bytes() : ws_need(c, b, a, act, 3, 0).best;
   return t;
 }
@@ -1525,7 +1526,13 @@ AccountPlan account_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a,
 int check_rows(const pa_cache* c, int batch, int max_blocks, const int32_t* table, const int32_t* lens) {
   if (!c) return fail(PA_ERR_INVALID_ARGUMENT, "cache descriptor is NULL");
   const bool coded = c->dtype == PA_DTYPE_FP8_E4M3 || is_int_cache(c->dtype);
-  const int rc = check_cache(c, coded ? PA_DTYPE_BFLOAT16 : c->dtype);
+  pa_cache rows = *c;
+  if (is_int_cache(c->dtype)) {  // integer codes move as they are: their scales are of no account
+    static const float none = 1.0f;
+    rows.k_scale = rows.v_scale = &none;
+    rows.k_quant_type = rows.v_quant_type = PA_QUANT_PER_TENSOR;
+  }
+  const int rc = check_cache(&rows, coded ? PA_DTYPE_BFLOAT16 : c->dtype);
   if (rc) return rc;
   if (!c->value_cache) return fail(PA_ERR_UNSUPPORTED, "the SEPARATE cache layout is required");
   if (batch < 1 || batch > 65535 || max_blocks < 1)
@@ -1617,7 +1624,7 @@ int pa_tree_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, co
   tp.num_tokens = b->num_tokens;
   tp.words = t.words;
   tp.window = a->local_window_size;
-  hipError_t e = pa::launch_tree_bits(tp, s);
+  hipError_t e = t.words ? pa::launch_tree_bits(tp, s) : hipSuccess;
   if (e != hipSuccess) return hip_fail(e, "tree attention launch");
   char* rest = base + t.bits_bytes + t.lag_bytes;
   if (!t.r.on) {
@@ -1629,6 +1636,7 @@ int pa_tree_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, co
   }
   pa::RangedParams p = ranged_params(c, b, a, q, out, rest, t.r);
   p.tree_bits = tp.bits;
+  p.tree_parents = t.words ? nullptr : parents;
   p.tree_lag = tp.lag;
   p.tree_words = t.words;
   e = pa::launch_ranged_tree(p, act, s);

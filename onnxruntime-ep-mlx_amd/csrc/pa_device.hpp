@@ -464,9 +464,11 @@ struct RangedParams {
   int32_t merge;     // some row may have several pieces
   int32_t wide;      // some block may hold more than 32 rows
   // Drafted trees (launch_ranged_tree): tree_words words per token, bit n: it sees its sequence's new row n (itself
-  // and its ancestors in the window); and how far behind its row a node's place in the text is
+  // and its ancestors in the window); and how far behind its row a node's place in the text is.  Of at most 64 nodes to
+  // a sequence the parents are enough, and the lags are written for the merge
   const uint32_t* tree_bits;
-  const int32_t* tree_lag;
+  const int32_t* tree_parents;
+  int32_t* tree_lag;
   int32_t tree_words;
   // Accounts (launch_ranged_weigh): the constants of the rows' softmax (2^(x - it) is a probability), rows by kv-head,
   // token and head of the group; on narrow items the scores x of the last `observed` tokens (0: all) of each sequence,

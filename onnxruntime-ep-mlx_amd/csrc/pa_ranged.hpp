@@ -424,13 +424,13 @@ struct RRange {
   int lo, hi;
 };
 template <int KIND>
-__device__ __forceinline__ RRange r_range(const RangedParams& p, int t, int pos, int b, int total) {
+__device__ __forceinline__ RRange r_range(const RangedParams& p, int t, int pos, int b, int total, int lag) {
   int hi = p.causal ? pos + 1 : total;
   if (p.causal && p.prefix_lens) hi = max(hi, p.prefix_lens[b]);
   int lo = p.window > 0 ? pos - p.window + 1 : 0;
   // (a node's place in its text goes by its depth; ancestors in the window lie above that place, for none has more
   // ancestors than rows before it)
-  if (KIND == kRTree && p.window > 0) lo -= p.tree_lag[t];
+  if (KIND == kRTree && p.window > 0) lo -= lag;
   if (p.doc_starts) lo = max(lo, p.doc_starts[t]);
   return RRange{max(lo, 0), min(hi, total)};
 }
@@ -463,8 +463,11 @@ __device__ __forceinline__ int r_token_seq(const RangedParams& p, int lo, int hi
 // kRSingle (all that it sees at all), kRZero (it sees nothing at all and this unit writes that).
 struct RInfo {
   int t, h, pos, lo, hi, how;
-  int past;              // kRTree: key of the sequence's first new row,
-  const uint32_t* bits;  // the row's bits
+  // kRTree: key of the sequence's first new row, and the new rows that the row sees, by bits: in memory, or of small
+  // trees here
+  int past;
+  const uint32_t* bits;
+  uint64_t mask;
 };
 constexpr int kRAny = 1, kRSingle = 2, kRZero = 4;
 __device__ __forceinline__ RInfo r_place(const RangedParams& p, const RUnit& u, int rl) {
@@ -475,11 +478,39 @@ __device__ __forceinline__ RInfo r_place(const RangedParams& p, const RUnit& u, 
   q.h = u.kh * g + (valid ? r % g : 0);
   return q;
 }
+// A tree of at most 64 nodes, one to a lane of the wavefront: the bits of node `node` and how far behind its row its
+// place in the text is.  Lines of ancestors double, six times at most.  (For a kernel of its own, before this one, a tree
+// of 26 nodes waited 5 us, 16 of 40 - 64 8.)
+struct RNode {
+  uint64_t mask;
+  int lag;
+};
+__device__ __forceinline__ RNode small_tree(const RangedParams& p, int tok0, int nodes, int node) {
+  const int lane = hidden(threadIdx.x & 63);
+  int up = lane < nodes ? p.tree_parents[tok0 + lane] : -1;
+  up = up >= 0 && up < lane ? up : -1;
+  uint64_t line = (uint64_t)1 << lane;
+  while (__any(up >= 0)) {  // line: 2^k nodes, up: the one behind them
+    const int from = max(up, 0), next = __shfl(up, from, 64);
+    const uint64_t more = __shfl((unsigned long long)line, from, 64);
+    if (up >= 0) {
+      line |= more;
+      up = next;
+    }
+  }
+  const int depth = __builtin_popcountll(line) - 1;
+  if (p.window > 0)
+    while (__builtin_popcountll(line) > p.window) line &= line - 1;  // the farthest ancestors are the lowest rows
+  const int at = min(node, 63);
+  const uint64_t mask = __shfl((unsigned long long)line, at, 64);
+  const int lag = node - __shfl(depth, at, 64);
+  return RNode{node < 64 ? mask : 0, lag};
+}
 template <int KIND>
 __device__ __forceinline__ void r_keys(const RangedParams& p, const RUnit& u, int rl, RInfo& q) {
   const int g = p.num_heads / p.kv_heads;
   const bool valid = u.row0 + rl < u.s.rows;
-  int b = u.s.b0, total = u.s.kb, shared = u.s.shared;
+  int b = u.s.b0, total = u.s.kb, shared = u.s.shared, lag = 0;
   if (u.group) {
     b = r_token_seq(p, u.s.b0, u.s.b1, q.t);
     const RSeq e = r_seq(p, b);
@@ -490,10 +521,18 @@ __device__ __forceinline__ void r_keys(const RangedParams& p, const RUnit& u, in
     q.pos = total - u.s.rows / g + (q.t - u.s.tok0);
     if constexpr (KIND == kRTree) {
       q.past = total - u.s.rows / g;
-      q.bits = p.tree_bits + (int64_t)q.t * p.tree_words;
+      if (p.tree_parents) {
+        const RNode node = small_tree(p, u.s.tok0, u.s.rows / g, q.t - u.s.tok0);
+        q.mask = node.mask;
+        lag = node.lag;
+        if (p.window > 0 && valid) p.tree_lag[q.t] = lag;  // for the merge
+      } else {
+        q.bits = p.tree_bits + (int64_t)q.t * p.tree_words;
+        if (p.window > 0) lag = p.tree_lag[q.t];
+      }
     }
   }
-  const RRange x = r_range<KIND>(p, q.t, q.pos, b, total);
+  const RRange x = r_range<KIND>(p, q.t, q.pos, b, total, lag);
   const int a = max(x.lo, u.group ? 0 : shared), z = min(x.hi, u.group ? shared : total);
   q.lo = max(a, u.k0);
   q.hi = min(z, u.k1);
@@ -642,9 +681,11 @@ struct RState {
 
 // Bits of keys t0 .. t0 + 31 of a row's mask over the new rows, the first of which is key `past`; the keys before
 // them are all seen.
-__device__ __forceinline__ uint32_t tree_mask(const uint32_t* bits, int words, int n) {  // n = t0 - past
+__device__ __forceinline__ uint32_t tree_mask(const RangedParams& p, const RInfo& q, int n) {  // n = t0 - past
   if (n <= -32) return ~0u;
-  const int w = n >> 5;
+  if (p.tree_parents) return (uint32_t)(n < 0 ? (q.mask << -n) | ((1u << -n) - 1u) : n < 64 ? q.mask >> n : 0);
+  const uint32_t* bits = q.bits;
+  const int words = p.tree_words, w = n >> 5;
   const uint32_t lo = w < 0 ? ~0u : w < words ? bits[w] : 0u, hi = w + 1 < words ? bits[w + 1] : 0u;
   return (uint32_t)((((uint64_t)hi << 32) | lo) >> (n & 31));
 }
@@ -968,7 +1009,7 @@ __device__ __forceinline__ void slow_rows(const RangedParams& p, const RUnit& u,
     if (p.softcap > 0.0f) x = p.softcap * tanhf(x / p.softcap);
     x = (x - slope * fabsf((float)(q.pos - j))) * kLog2e;
     bool seen = j >= st.lo && j < st.hi && x != kNegInf;
-    if constexpr (KIND == kRTree) seen = seen && (tree_mask(q.bits, p.tree_words, j - q.past) & 1u);
+    if constexpr (KIND == kRTree) seen = seen && (tree_mask(p, q, j - q.past) & 1u);
     const float mn = seen ? fmaxf(st.m, x) : st.m, ms = mn == kNegInf ? 0.0f : mn;
     const float a = st.m == kNegInf ? 0.0f : fmaxf(exp2f(st.m - ms), kRTiny);
     const float w = seen ? fmaxf(exp2f(x - ms), kRTiny) : 0.0f;
@@ -1046,7 +1087,7 @@ __device__ __forceinline__ uint32_t wide_unit(const RangedParams& p, const RUnit
       if constexpr (KIND == kRTree) {
         if (tree) {
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) tw[kb] = tree_mask(q.bits, p.tree_words, t0 + 32 * kb - past);
+          for (int kb = 0; kb < KB; ++kb) tw[kb] = tree_mask(p, q, t0 + 32 * kb - past);
         }
       }
       r_scores<TT, D, KB>(st, buf, lane, s);
@@ -1100,7 +1141,7 @@ __device__ __forceinline__ uint32_t narrow_unit(const RangedParams& p, const RUn
       RPair pr[2];
       uint32_t tw[1];
       const bool tree = KIND == kRTree && have && t0 + 32 > past;
-      if (tree) tw[0] = tree_mask(q.bits, p.tree_words, t0 - past);
+      if (tree) tw[0] = tree_mask(p, q, t0 - past);
       if (have) {
         wait_loads<NI>();  // the keys; the values are younger
         r_scores<TT, D, 1>(st, mine, lane, s);
@@ -1293,7 +1334,8 @@ __device__ __forceinline__ RJoin r_join(const RangedParams& p, int t, int h, int
     return RSource{e.v[0], e.v[1], e.v[2], e.v[3], e.v[4], e.v[5], e.v[6], e.v[7], e.v[8], e.v[9], e.v[10]};
   };
   const RSource own = source(p.groups + b);
-  const RRange r = r_range<KIND>(p, t, own.kb - own.rows / g + (t - own.tok0), b, own.kb);
+  const RRange r = r_range<KIND>(p, t, own.kb - own.rows / g + (t - own.tok0), b, own.kb,
+                                 KIND == kRTree && p.window > 0 ? p.tree_lag[t] : 0);
   auto pieces = [&](const RSource& e, int a, int z) {
     const int kind = r_wide(e) ? 0 : 1, pr = pick(per, kind);
     const int rr = (t - e.tok0) * g + h - kh * g, blk = kind ? 0 : rr / kRWide, kt = e.ka / kRTile;

@@ -270,6 +270,12 @@ __global__ __launch_bounds__(256) void fold_kernel(const WeighParams wp) {
       x[0] = src[0];
     }
   };
+  // (the entries come in while the sums are made)
+  int64_t page = p.block_table[(int64_t)b * p.max_blocks + min(key / p.block_size, p.max_blocks - 1)];
+  page = min(max(page, (int64_t)0), p.num_blocks - 1);
+  float* w = wp.weights + (page * p.kv_heads + kh) * p.block_size + key % p.block_size;
+  float old[V];
+  load(w, old);
   if (p.scores) {
     WRows rows[V];
     int lo = INT32_MAX, hi = 0;
@@ -307,11 +313,6 @@ __global__ __launch_bounds__(256) void fold_kernel(const WeighParams wp) {
         for (int i = 0; i < V; ++i) sum[i] += c0 + k < wp.chunks ? x[k][i] : 0.0f;
     }
   }
-  int64_t page = p.block_table[(int64_t)b * p.max_blocks + min(key / p.block_size, p.max_blocks - 1)];
-  page = min(max(page, (int64_t)0), p.num_blocks - 1);
-  float* w = wp.weights + (page * p.kv_heads + kh) * p.block_size + key % p.block_size;
-  float old[V];
-  load(w, old);
 #pragma unroll
   for (int i = 0; i < V; ++i) sum[i] = key + i < e.past ? old[i] + sum[i] : key + i < e.total ? sum[i] : old[i];
   if constexpr (V == 4)

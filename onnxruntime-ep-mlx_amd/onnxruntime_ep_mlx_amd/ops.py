@@ -115,11 +115,9 @@ def batch_desc(cum: torch.Tensor, past: torch.Tensor, block_table: torch.Tensor,
                max_context_len: int = 0) -> capi.PaBatch:
     for name, t in (("cumulative_sequence_length", cum), ("past_seqlens", past),
                     ("block_table", block_table), ("slot_mapping", slot_mapping)):
-        if t is not None:
-            if t.dtype != torch.int32:
-                raise ValueError(f"input {name} must be int32")
-            if not t.is_contiguous():
-                _contig(name, t)
+        if t is not None and t.dtype != torch.int32:
+            raise ValueError(f"input {name} must be int32")
+        _contig(name, t)
     return capi.PaBatch(_ptr(cum), _ptr(past), _ptr(block_table), _ptr(slot_mapping),
                         cum.numel() - 1, block_table.shape[1], num_tokens, max_query_len, flags,
                         max_context_len)
@@ -549,25 +547,27 @@ def tree_attention(q, key_cache, value_cache, cum, past, block_table, parents, *
 
 
 def _rows_call(key_cache, value_cache, block_table, lens, k_scale, v_scale, k_quant_type, v_quant_type, more):
-    """The checked cache descriptor of entries that move rows; `more`: (name, tensor) on the same device."""
+    """The checked cache descriptor of entries that move rows, its device and the sequences; `more`: (name,
+    tensor) on the same device."""
     _need_cuda("key_cache", key_cache)
     if value_cache is None:
         raise ValueError("PagedAttention: the SEPARATE cache layout is required")
-    _same_device(key_cache.get_device(), (("key_cache", key_cache), ("value_cache", value_cache),
-                                          ("block_table", block_table), ("past", lens), ("k_scale", k_scale),
-                                          ("v_scale", v_scale), *more))
-    if block_table.dim() != 2 or block_table.shape[0] != lens.numel() or block_table.dtype != torch.int32 \
+    index = key_cache.get_device()
+    _same_device(index, (("key_cache", key_cache), ("value_cache", value_cache), ("block_table", block_table),
+                         ("past", lens), ("k_scale", k_scale), ("v_scale", v_scale), *more))
+    n = lens.numel()
+    if block_table.dim() != 2 or block_table.shape[0] != n or block_table.dtype != torch.int32 \
             or lens.dtype != torch.int32:
         raise ValueError("PagedAttention: block_table and lengths must be int32 [batch, max_blocks] and [batch]")
     cache = cache_desc(key_cache, value_cache, k_scale, v_scale, k_quant_type=k_quant_type,
                        v_quant_type=v_quant_type)
-    # (codes move as they are: only fp8 pages have scales of their own)
-    if cache.dtype in (capi.PA_DTYPE_INT8, capi.PA_DTYPE_INT4) and k_scale is None:
-        one = _ptr(key_cache)
-        cache.k_scale = cache.v_scale = one
-        cache.k_quant_type = cache.v_quant_type = capi.PA_QUANT_PER_TENSOR
     _scales_hold(cache, k_scale, v_scale)
-    return cache
+    return cache, index, n
+
+
+def _account(key_weights, cache: capi.PaCache) -> None:
+    if key_weights.dtype != torch.float32 or key_weights.shape != (cache.num_blocks, cache.kv_heads, cache.block_size):
+        raise ValueError("PagedAttention: key_weights must be float32 [num_blocks, kv_num_heads, block_size]")
 
 
 def accept_drafts(key_cache, value_cache, cum, past, block_table, parents=None, draft_tokens=None,
@@ -587,13 +587,15 @@ def accept_drafts(key_cache, value_cache, cum, past, block_table, parents=None, 
     given = path is not None
     if given == (parents is not None) or given != (path_lens is not None):
         raise ValueError("PagedAttention: give parents, draft_tokens and target_tokens, or path and path_lens")
-    cache = _rows_call(key_cache, value_cache, block_table, past, k_scale, v_scale, k_quant_type, v_quant_type,
-                       (("cum", cum), ("parents", parents), ("draft_tokens", draft_tokens),
-                        ("target_tokens", target_tokens), ("path", path), ("path_lens", path_lens)))
+    cache, dev, B = _rows_call(key_cache, value_cache, block_table, past, k_scale, v_scale, k_quant_type,
+                               v_quant_type,
+                               (("cum", cum), ("parents", parents), ("draft_tokens", draft_tokens),
+                                ("target_tokens", target_tokens), ("key_weights", key_weights))
+                               if not given else
+                               (("cum", cum), ("path", path), ("path_lens", path_lens), ("key_weights", key_weights)))
     if key_weights is not None:
-        _account(key_weights, key_cache)
-    B, dev = past.numel(), key_cache.device
-    if cum.numel() != B + 1:
+        _account(key_weights, cache)
+    if cum.numel() != B + 1 or cum.dtype != torch.int32:
         raise ValueError("PagedAttention: inconsistent cumulative lengths, past lengths or block table")
     after = None
     if given:
@@ -608,22 +610,15 @@ def accept_drafts(key_cache, value_cache, cum, past, block_table, parents=None, 
                 or draft_tokens.dtype != torch.int64 or target_tokens.dtype != torch.int64 \
                 or draft_tokens.numel() != tokens or target_tokens.numel() != tokens:
             raise ValueError("PagedAttention: parents must be int32, draft_tokens and target_tokens int64 [num_tokens]")
-        path = torch.empty((B, max_path or max_query_len or max(tokens, 1)), dtype=torch.int32, device=dev)
+        path = past.new_empty((B, max_path or max_query_len or max(tokens, 1)))
         path_lens = torch.empty_like(past)
-        after = torch.empty(B, dtype=torch.int64, device=dev)
-    batch = batch_desc(cum, past, block_table, tokens, None, max_query_len)
+        after = draft_tokens.new_empty(B)
+    batch = capi.PaBatch(cum.data_ptr(), past.data_ptr(), block_table.data_ptr(), None, B, block_table.shape[1],
+                         tokens, max_query_len, 0, 0)
     drafts = capi.PaDrafts(_ptr(parents), _ptr(draft_tokens), _ptr(target_tokens), _ptr(path), _ptr(path_lens),
                            _ptr(after), path.shape[1], _ptr(key_weights))
-    capi.check(_on_device(key_cache.get_device(), capi.load().pa_accept_drafts, C.byref(cache), C.byref(batch),
-                          C.byref(drafts)))
+    capi.check(_on_device(dev, capi.load().pa_accept_drafts, C.byref(cache), C.byref(batch), C.byref(drafts)))
     return path, path_lens, after
-
-
-def _account(key_weights, key_cache) -> None:
-    nb, bs, kv = key_cache.shape[:3]
-    if key_weights.dtype != torch.float32 or tuple(key_weights.shape) != (nb, kv, bs):
-        raise ValueError("PagedAttention: key_weights must be float32 [num_blocks, kv_num_heads, block_size]")
-    _same_device(key_cache.get_device(), (("key_weights", key_weights),))
 
 
 def accumulating_attention(q, key_cache, value_cache, cum, past, block_table, key_weights, *, num_heads,
@@ -642,7 +637,8 @@ def accumulating_attention(q, key_cache, value_cache, cum, past, block_table, ke
     descs, out = _paged_call(q, key_cache, value_cache, cum, past, block_table, num_heads, scale, softcap,
                              local_window_size, is_causal, head_sink, k_scale, v_scale, k_quant_type,
                              v_quant_type, max_query_len, max_context_len, out, workspace)
-    _account(key_weights, key_cache)
+    _account(key_weights, descs[0]._obj)
+    _same_device(q.get_device(), (("key_weights", key_weights),))
     act = pa_dtype(q.dtype)
     return _with_workspace(q, out, workspace, lib.pa_accumulating_attention_workspace_bytes,
                            (*descs, observed_rows, act), lib.pa_accumulating_attention,
@@ -661,21 +657,19 @@ def evict_keys(key_cache, value_cache, key_weights, lens, block_table, *, budget
     sequence alone.  Returns (kept int32 [batch, kv_num_heads, budget], -1 behind the end; the lengths that are
     left, int32 [batch]).  ``max_context_len`` bounds ``lens`` (0 = the tables' capacity; keys beyond it
     are not looked at)."""
-    cache = _rows_call(key_cache, value_cache, block_table, lens, k_scale, v_scale, k_quant_type, v_quant_type,
-                       (("block_table_out", block_table_out),))
-    _account(key_weights, key_cache)
-    B, kv, dev = lens.numel(), key_cache.shape[2], key_cache.device
+    cache, dev, B = _rows_call(key_cache, value_cache, block_table, lens, k_scale, v_scale, k_quant_type,
+                               v_quant_type, (("block_table_out", block_table_out), ("key_weights", key_weights)))
+    _account(key_weights, cache)
     if block_table_out is not None and (block_table_out.dtype != torch.int32 or block_table_out.dim() != 2
                                         or block_table_out.shape[0] != B):
         raise ValueError("PagedAttention: block_table_out must be int32 [batch, max_blocks]")
-    kept = torch.empty((B, kv, max(budget, 0)), dtype=torch.int32, device=dev)
+    kept = lens.new_empty((B, cache.kv_heads, max(budget, 0)))
     lens_out = torch.empty_like(lens)
     batch = capi.PaBatch(None, _ptr(lens), _ptr(block_table), None, B, block_table.shape[1], 0, 0, 0,
                          max_context_len)
     ev = capi.PaEviction(_ptr(key_weights), budget, sinks, recent, _ptr(block_table_out),
                          0 if block_table_out is None else block_table_out.shape[1], _ptr(kept), _ptr(lens_out))
-    capi.check(_on_device(key_cache.get_device(), capi.load().pa_evict_keys, C.byref(cache), C.byref(batch),
-                          C.byref(ev)))
+    capi.check(_on_device(dev, capi.load().pa_evict_keys, C.byref(cache), C.byref(batch), C.byref(ev)))
     return kept, lens_out
 
 

@@ -40,6 +40,7 @@ LAYOUTS = [(BF16, 8, 2, 128, 16), (F16, 8, 2, 128, 32), (F16, 8, 1, 64, 16), (BF
 BATCHES = {"single": ([1, 1, 1, 1], [0, 63, 64, 700]),
            "small": ([7, 0, 1, 9, 4], [9, 100, 31, 511, 1200]),
            "trees": ([33, 1, 64, 65, 0, 129], [0, 1, 17, 40, 9, 333]),
+           "sixty_four": ([64, 33, 1, 63, 0], [70, 5, 0, 600, 8]),
            "wide": ([31, 32, 257], [65, 1000, 90])}
 
 
@@ -58,7 +59,7 @@ FORMS = {"window_one": dict(window=1), "window": dict(window=17), "window_past":
          "sink": dict(sink=True), "scale": dict(scale=0.3), "negative_scale": dict(scale=-0.1)}
 
 
-@pytest.mark.parametrize("batch", ["small", "trees"])
+@pytest.mark.parametrize("batch", ["small", "sixty_four", "trees"])
 @pytest.mark.parametrize("form", list(FORMS))
 @pytest.mark.parametrize("dt,D", [(BF16, 128), (F16, 64), (F32, 64)])
 def test_forms(dt, D, form, batch):

@@ -169,7 +169,11 @@ def test_workspaces():
     a = attn(heads=8)
     c, b = cache(nb=1000), batch(tokens=64, batch=64, mb=256, mq=1, ctx=4000)
     t, w, m = sizes(c, b, a, BF16)
-    assert t == m + 256 + 256  # one word and one lag to each of 64 nodes
+    assert t == m + 256  # one lag to each of 64 nodes
+    wide = sizes(c, batch(tokens=66, batch=2, mb=256, mq=65, ctx=4000), a, BF16)
+    assert wide[0] == wide[2] + 1024 + 512  # three words and one lag to each of 66
+    valu = sizes(cache(nb=1000, dt=F32), batch(tokens=64, batch=64, mb=256, mq=1, ctx=4000), a, F32)
+    assert valu[0] == valu[2] + 256 + 256
     assert w == m + 64 * 8 * 4 + 64 * 8 * 4032 * 4  # constants, scores of 4000 keys in tiles of 64
     # a longer bound than a GiB of scores: sums of chunks instead
     far = batch(tokens=64, batch=64, mb=1 << 18, mq=1, ctx=600000)
