@@ -322,13 +322,12 @@ __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictPara
 }
 
 // A head's rows that stay, of keys, of values (slices of W bytes of each) or the weights: in place all of them, a
-// round after the other; to other pages one round to a workgroup.  W is 256 where that gives every CU a workgroup,
-// else 64: 128-byte lines are then fetched by two workgroups, but four times as many share the rows.
+// round of 2048 after the other; to other pages one round to a workgroup, of whole rows.
 // Bound by HBM: 2048 of up to 9000 rows of 8 heads of 16 sequences, 268 MB read and written, to other pages in 58 us
 // (4.6 TB/s; a copy of 1 GiB 5.2; in rounds of 64 KB 75 us, with stores that stay in the cache 62).
 template <bool INPLACE>
 struct Round {  // threads, rows in flight of each
-  static constexpr int THREADS = INPLACE ? 512 : 256, DEPTH = INPLACE ? 8 : 4;
+  static constexpr int THREADS = INPLACE ? 1024 : 256, DEPTH = INPLACE ? 8 : 4;
 };
 template <int U, int W, bool INPLACE>
 __global__ __launch_bounds__(Round<INPLACE>::THREADS) void evict_move_kernel(const EvictParams p) {
@@ -336,7 +335,10 @@ __global__ __launch_bounds__(Round<INPLACE>::THREADS) void evict_move_kernel(con
   constexpr int kMThreads = Round<INPLACE>::THREADS, kMDepth = Round<INPLACE>::DEPTH;
   const RowsParams& c = p.c;
   const int tid = threadIdx.x, slices = (c.head_bytes + W - 1) / W, parts = 2 * slices + 1;
-  const int z = blockIdx.x / parts, part = blockIdx.x - z * parts;
+  // a head's slices, which share lines, all on one XCD (every eighth workgroup) and one after the other
+  const int group = blockIdx.x / (8 * parts), turn = blockIdx.x - group * 8 * parts;
+  const int part = turn >> 3, z = 8 * group + (turn & 7);
+  if (z >= c.batch * c.kv_heads) return;
   const int b = z / c.kv_heads, kh = z - b * c.kv_heads;
   const int cap = (int)min((int64_t)c.max_blocks * c.block_size, (int64_t)(INT32_MAX / 2));
   const int n = min(max(p.lens[b], 0), min(cap, p.max_keys)), rows = min(n, p.budget);
@@ -407,7 +409,8 @@ __global__ __launch_bounds__(Round<INPLACE>::THREADS) void evict_move_kernel(con
 }
 template <int U, int W, bool INPLACE>
 hipError_t launch_move_in(const EvictParams& p, hipStream_t s) {
-  const int64_t parts = 2 * ((p.c.head_bytes + W - 1) / W) + 1, wgs = parts * p.c.batch * p.c.kv_heads;
+  const int64_t parts = 2 * ((p.c.head_bytes + W - 1) / W) + 1;
+  const int64_t wgs = ((int64_t)p.c.batch * p.c.kv_heads + 7) / 8 * 8 * parts;
   constexpr int step = Round<INPLACE>::THREADS / (W / U) * Round<INPLACE>::DEPTH;
   const int rows = std::min(p.budget, p.max_keys);
   const int64_t rounds = INPLACE ? 1 : (rows + step - 1) / step;
@@ -423,8 +426,7 @@ hipError_t launch_move(const EvictParams& p, hipStream_t s) {
 template <int U>
 hipError_t launch_move_u(const EvictParams& p, hipStream_t s) {
   if constexpr (U == 16)
-    if (p.table_out || (int64_t)p.c.batch * p.c.kv_heads * ((p.c.head_bytes + 255) / 256) >= 128)
-      return launch_move<U, 256>(p, s);
+    if (p.table_out) return launch_move_in<U, 256, false>(p, s);
   return launch_move<U, 64>(p, s);  // (odd rows too: bytes, 64 of a row at once)
 }
 
