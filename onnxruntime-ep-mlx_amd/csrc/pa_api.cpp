@@ -792,6 +792,10 @@ struct RunOpts {
   const int32_t* tree_lag = nullptr;
   int tree_words = 0;
   float* row_stats = nullptr;
+  float* scores = nullptr;
+  int64_t score_ld = 0;
+  int observed = 0;
+  bool rows32 = false;
   bool images = true;  // operand images allowed (see make_plan)
   HostLens host;       // host metadata lengths (LATENT chunk sizing)
 };
@@ -889,6 +893,10 @@ pa::AttnParams attn_params(const pa_cache* c, const pa_batch* b, const pa_attn* 
   p.tree_lag = opts.tree_lag;
   p.tree_words = opts.tree_words;
   p.row_stats = opts.row_stats;
+  p.scores = opts.scores;
+  p.score_ld = opts.score_ld;
+  p.observed = opts.observed;
+  p.rows32 = opts.rows32 ? 1 : 0;
   p.k_quant = c->k_quant_type;
   p.v_quant = c->v_quant_type;
   p.v_head_dim = a->v_head_size > 0 ? a->v_head_size : c->head_dim;
@@ -1039,7 +1047,9 @@ int run_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dty
       }
       break;
     case 5: e = pa::launch_latent(p, act, c->dtype, s); break;
-    default: e = pa::launch_attn_generic(p, act, c->dtype, s); break;
+    default:
+      e = p.rows32 ? pa::launch_rows32(p, act, c->dtype, s) : pa::launch_attn_generic(p, act, c->dtype, s);
+      break;
   }
   if (e != hipSuccess) return hip_fail(e, "attention kernel launch");
   if (pl.max_splits > 1) {
@@ -1460,11 +1470,27 @@ int masked_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, con
   return PA_OK;
 }
 
+// Keys to a chunk of launch_rows32: chunks that all sequences together fill the GPU with once, of 128 keys at least; 0
+// where launch_attn_generic runs instead (heads beyond 256).
+int rows32_chunk(const pa_cache* c, const pa_batch* b, const pa_attn* a) {
+  if (c->head_dim > 256) return 0;
+  const int64_t g = a->num_heads / c->kv_heads, T = b->num_tokens;
+  const int64_t mq = std::min<int64_t>(b->max_query_len > 0 ? b->max_query_len : T, T);
+  const int64_t per = mq * g <= 32 ? 32 : 128, waves = per / 32;
+  const int64_t blocks = c->kv_heads * std::max<int64_t>(std::min<int64_t>(b->batch, T), T * g / per);
+  int64_t keys = max_ctx_bound(c, b);
+  if (b->max_context_len > 0) keys = std::min<int64_t>(keys, b->max_context_len);
+  // wavefronts that a CU holds, by LDS (workgroups of one) and registers
+  const int64_t held = c->head_dim <= 64 ? 8 : c->head_dim <= 128 ? (waves == 1 ? 4 : 8) : (waves == 1 ? 2 : 4);
+  const int64_t splits = std::max<int64_t>(held * device_cus() / std::max<int64_t>(blocks * waves, 1), 1);
+  return (int)std::max<int64_t>(((keys + splits - 1) / splits + 31) / 32 * 32, 128);
+}
+
 // ------------------------------------------------------------------------------ drafted trees
 // Words of a node's bits (none: the matrix-core kernel makes those of small trees itself), and the workspace: the bits
 // and lags, then the attention's own.
 struct TreePlan {
-  int words = 0;
+  int words = 0, chunk = 0;
   size_t bits_bytes = 0, lag_bytes = 0, attn_bytes = 0;
   RangedPlan r;
   size_t bytes() const { return bits_bytes + lag_bytes + attn_bytes; }
@@ -1477,7 +1503,8 @@ TreePlan tree_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dt
   t.words = t.r.on && nodes <= 64 ? 0 : std::max((nodes + 31) / 32, 1);
   t.bits_bytes = align256((size_t)b->num_tokens * t.words * sizeof(uint32_t));
   t.lag_bytes = align256((size_t)b->num_tokens * sizeof(int32_t));
-  t.attn_bytes = t.r.on ? t.r.bytes() : ws_need(c, b, a, act, 3, 0).best;
+  t.chunk = t.r.on ? 0 : rows32_chunk(c, b, a);
+  t.attn_bytes = t.r.on ? t.r.bytes() : ws_need(c, b, a, act, 3, t.chunk).best;
   return t;
 }
 
@@ -1486,7 +1513,7 @@ TreePlan tree_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dt
 // or the chunks' sums, then the attention's own.
 struct AccountPlan {
   bool scores = false;
-  int chunks = 0, chunk_rows = 0, keys = 0;
+  int chunks = 0, chunk_rows = 0, keys = 0, chunk = 0;
   int64_t ld = 0;
   size_t stat_bytes = 0, sum_bytes = 0, attn_bytes = 0;
   RangedPlan r;
@@ -1501,12 +1528,13 @@ AccountPlan account_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a,
   if (b->max_context_len > 0) t.keys = std::min(t.keys, b->max_context_len);
   t.ld = ((int64_t)t.keys + 63) / 64 * 64;
   t.r = ranged_plan(c, b, a, nullptr, act);
-  t.attn_bytes = t.r.on ? t.r.bytes() : ws_need(c, b, a, act, 3, 0).best;
+  t.chunk = t.r.on ? 0 : rows32_chunk(c, b, a);
+  t.attn_bytes = t.r.on ? t.r.bytes() : ws_need(c, b, a, act, 3, t.chunk).best;
   t.stat_bytes = align256((size_t)T * a->num_heads * sizeof(float));
   // Every sequence's rows of a kv-head on a wavefront of their own leave their scores, within a GiB: a step of 48 sequences
   // of up to 8190 keys takes 30 us to write and 12 to read them where its keys take 77 to be read again.
   const size_t scores = align256((size_t)T * a->num_heads * t.ld * sizeof(float));
-  t.scores = t.r.on && !t.r.wide && scores <= kAccountScores;
+  t.scores = (t.r.on ? !t.r.wide : t.chunk > 0 && mq * g <= 32) && scores <= kAccountScores;
   if (t.scores) {
     t.sum_bytes = scores;
     return t;
@@ -1632,7 +1660,8 @@ int pa_tree_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, co
     o.tree_bits = tp.bits;
     o.tree_lag = tp.lag;
     o.tree_words = t.words;
-    return run_attention(c, b, a, act, q, nullptr, nullptr, out, rest, t.attn_bytes, 3, 0, s, o);
+    o.rows32 = t.chunk > 0;
+    return run_attention(c, b, a, act, q, nullptr, nullptr, out, rest, t.attn_bytes, 3, t.chunk, s, o);
   }
   pa::RangedParams p = ranged_params(c, b, a, q, out, rest, t.r);
   p.tree_bits = tp.bits;
@@ -1734,7 +1763,11 @@ int pa_accumulating_attention(const pa_cache* c, const pa_batch* b, const pa_att
   } else {
     RunOpts o = masked_opts(nullptr);
     o.row_stats = w.r.row_stats;
-    if ((rc = run_attention(c, b, a, act, q, nullptr, nullptr, out, rest, t.attn_bytes, 3, 0, s, o))) return rc;
+    o.scores = w.r.scores;
+    o.score_ld = w.r.score_ld;
+    o.observed = observed_rows;
+    o.rows32 = t.chunk > 0;
+    if ((rc = run_attention(c, b, a, act, q, nullptr, nullptr, out, rest, t.attn_bytes, 3, t.chunk, s, o))) return rc;
   }
   e = pa::launch_weigh(w, act, c->dtype, s);
   if (e != hipSuccess) return hip_fail(e, "accumulating attention launch");

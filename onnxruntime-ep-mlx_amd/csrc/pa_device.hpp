@@ -394,6 +394,10 @@ struct AttnParams {
   const int32_t* tree_lag;
   int32_t tree_words;
   float* row_stats;
+  float* scores;
+  int64_t score_ld;
+  int32_t observed;
+  int32_t rows32;  // launch_rows32 instead of launch_attn_generic
   int32_t* plan;
   int32_t* plan_info;
   int32_t* plan_split;
@@ -671,6 +675,14 @@ __device__ __forceinline__ float finalize_factor(float m, float l, float sink_x)
   return lt > 0.0f ? f / lt : 0.0f;
 }
 
+// Bits n .. n + 31 of a mask over new rows (words of them); the keys before the new rows, n < 0, are all seen.
+__device__ __forceinline__ uint32_t tree_window(const uint32_t* bits, int words, int n) {
+  if (n <= -32) return ~0u;
+  const int w = n >> 5;
+  const uint32_t lo = w < 0 ? ~0u : w < words ? bits[w] : 0u, hi = w + 1 < words ? bits[w + 1] : 0u;
+  return (uint32_t)((((uint64_t)hi << 32) | lo) >> (n & 31));
+}
+
 // Constant of a row's softmax from its maximum m and sum l: probabilities are 2^(x - it), 0 where nothing weighs.
 __device__ __forceinline__ float softmax_stat(float m, float l, float sink_x) {
   const float mm = fmaxf(m, sink_x);
@@ -740,6 +752,8 @@ hipError_t launch_axes_append(const AppendParams& p, const AxisParams& ax, pa_dt
                               pa_dtype cache_dtype, hipStream_t s);
 hipError_t launch_attn_generic(const AttnParams& p, pa_dtype act, pa_dtype cache_dtype,
                                hipStream_t s);
+// Drafted trees and weighed rows of heads up to 256 (pa_rows32.hip); partials merged by launch_split_reduce.
+hipError_t launch_rows32(const AttnParams& p, pa_dtype act, pa_dtype cache_dtype, hipStream_t s);
 hipError_t launch_decode_mfma(const AttnParams& p, pa_dtype act, pa_dtype cache_dtype,
                               hipStream_t s);
 hipError_t launch_decode_balanced(const AttnParams& p, pa_dtype act, pa_dtype cache_dtype,

@@ -684,10 +684,7 @@ struct RState {
 __device__ __forceinline__ uint32_t tree_mask(const RangedParams& p, const RInfo& q, int n) {  // n = t0 - past
   if (n <= -32) return ~0u;
   if (p.tree_parents) return (uint32_t)(n < 0 ? (q.mask << -n) | ((1u << -n) - 1u) : n < 64 ? q.mask >> n : 0);
-  const uint32_t* bits = q.bits;
-  const int words = p.tree_words, w = n >> 5;
-  const uint32_t lo = w < 0 ? ~0u : w < words ? bits[w] : 0u, hi = w + 1 < words ? bits[w + 1] : 0u;
-  return (uint32_t)((((uint64_t)hi << 32) | lo) >> (n & 31));
+  return tree_window(q.bits, p.tree_words, n);
 }
 
 // Matrix products run in groups, whose operands are read from LDS while the group before multiplies: reads and

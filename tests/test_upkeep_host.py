@@ -172,8 +172,10 @@ def test_workspaces():
     assert t == m + 256  # one lag to each of 64 nodes
     wide = sizes(c, batch(tokens=66, batch=2, mb=256, mq=65, ctx=4000), a, BF16)
     assert wide[0] == wide[2] + 1024 + 512  # three words and one lag to each of 66
-    valu = sizes(cache(nb=1000, dt=F32), batch(tokens=64, batch=64, mb=256, mq=1, ctx=4000), a, F32)
-    assert valu[0] == valu[2] + 256 + 256
+    # other types: 64 x 2 blocks of rows in 8 chunks of 512 keys, their partial rows of 128 elements and (m, l)
+    f32, rows = sizes(cache(nb=1000, dt=F32), batch(tokens=64, batch=64, mb=256, mq=1, ctx=4000), a, F32), 64 * 8 * 8
+    assert f32[0] == 256 + 256 + rows * 128 * 4 + rows * 2 * 4
+    assert f32[1] == 64 * 8 * 4 + 64 * 8 * 4032 * 4 + rows * 128 * 4 + rows * 2 * 4
     assert w == m + 64 * 8 * 4 + 64 * 8 * 4032 * 4  # constants, scores of 4000 keys in tiles of 64
     # a longer bound than a GiB of scores: sums of chunks instead
     far = batch(tokens=64, batch=64, mb=1 << 18, mq=1, ctx=600000)
