@@ -26,8 +26,8 @@
 
 /* pa_tree_attention: attention in which a node sees the keys [0, past) and, of the new rows, its
  * ancestors and itself; under a window the keys and ancestors less than local_window_size positions
- * before it.  parents [num_tokens] int32.  Layouts, attributes (is_causal must be 1), types and the
- * kernels that run as pa_masked_attention's; out apart from q.  max_query_len bounds the nodes of a
+ * before it.  parents [num_tokens] int32.  Layouts, attributes (is_causal must be 1) and types as
+ * pa_masked_attention's; out apart from q.  max_query_len bounds the nodes of a
  * sequence (0: num_tokens, at most PA_MAX_TREE_NODES); nodes beyond the bound see the keys before
  * the tree at most, and what they yield is unspecified.  Workspace: at least the size that
  * pa_tree_attention_workspace_bytes gives; 16-byte aligned. */
@@ -60,8 +60,8 @@ typedef struct pa_drafts {
  * every key's account the probabilities, sinks in their denominator, that the rows which count gave
  * it, over the heads of its kv-head: the last `observed_rows` new tokens of each sequence (0: all of
  * them).  Keys of the new tokens begin at zero, whatever their slots held.  The same call on the
- * same inputs gives the same bits.  Windows, softcaps, sinks, types, layouts and the kernels that
- * run as pa_masked_attention's; out apart from q, key_weights 4-byte aligned and apart from
+ * same inputs gives the same bits.  Windows, softcaps, sinks, types and layouts as
+ * pa_masked_attention's; out apart from q, key_weights 4-byte aligned and apart from
  * everything else.  Workspace: at least the size that
  * pa_accumulating_attention_workspace_bytes gives (up to 32 rows of one kv-head per sequence: 4
  * bytes for every row and key of the context bound); 16-byte aligned.  A sequence whose context

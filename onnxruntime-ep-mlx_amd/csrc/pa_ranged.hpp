@@ -38,10 +38,15 @@
 // they do not see.  Tiles read no key outside [first visible, last visible] of their rows (such places repeat a
 // visible one), so pages behind a sequence's end or before its window may hold anything.
 //
+// Drafted trees (kRTree): a node's keys end with its own, and a word of its bits for every 32 new rows masks what lies
+// among them; only tiles with new rows look at it.  Weighed rows (kRWeigh): the constant m + log2(l) of a row goes beside
+// its output, and narrow items leave their scores (pa_weigh.hip).
+//
 // What bounds it (GPU times of a call, merge included).  Prompts of 8192: 32 heads of 128 in 746 us, 737
 // TFLOP/s of the two products, 1105 with the second part of the probabilities, the softmax's vector instructions
 // behind them in turn; 64 heads of 64 in 945 us (twice the scores per product), 16 heads of 256 in 767.  64
-// sequences of up to 8192 keys, one token each: 212 us, 5.8 TB/s from HBM.  Small calls: 5 us of dependent
+// sequences of up to 8192 keys, one token each: 212 us, 5.8 TB/s from HBM.  A tree of 257 nodes after 60001 keys, 32 heads
+// of 128: 427 us, 592 TFLOP/s (nine blocks of rows of which the last holds four); 16 trees of 40 - 64 nodes, 28 heads, 86.  Small calls: 5 us of dependent
 // loads and the scan before the first item, 2 us to its first tile, 3 us per launch.
 #pragma once
 
