@@ -5,6 +5,8 @@
  * conventions and layouts are pa_mi355x.h's, which declares the entries beside the others.  Here
  * are their descriptors and contracts.
  *
+ * A block-table entry that names no page is read as the nearest one and never written through.
+ *
  * The attention entries read every key and value, the new tokens' rows included, from the
  * block-table pages; batch->slot_mapping must be NULL.  A workspace carries nothing from one call to
  * the next; calls in flight on different streams, and captured graphs whose replays may overlap,
@@ -62,7 +64,8 @@ typedef struct pa_drafts {
  * them).  Keys of the new tokens begin at zero, whatever their slots held.  The same call on the
  * same inputs gives the same bits.  Windows, softcaps, sinks, types and layouts as
  * pa_masked_attention's; out apart from q, key_weights 4-byte aligned and apart from
- * everything else.  Workspace: at least the size that
+ * everything else.  Where several sequences of the call hold a page, each of them writes its entries,
+ * which are then unspecified (the outputs are not).  Workspace: at least the size that
  * pa_accumulating_attention_workspace_bytes gives (up to 32 rows of one kv-head per sequence: 4
  * bytes for every row and key of the context bound); 16-byte aligned.  A sequence whose context
  * exceeds max_context_len leaves its account unspecified. */

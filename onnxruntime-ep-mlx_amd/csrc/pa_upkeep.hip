@@ -33,16 +33,18 @@ struct Unit<1> {
   typedef uint8_t type;
 };
 
-// Slot (page * block_size + row) of position pos of sequence b, and its page.
+// Slot (page * block_size + row) of position pos of sequence b, and its page.  A table's entry that names no page reads
+// the nearest one and writes nothing.
 struct Slot {
   int64_t slot;
   int64_t page;
+  bool there;
 };
 __device__ __forceinline__ Slot slot_of(const RowsParams& c, const int32_t* table, int max_blocks, int b, int pos) {
   const int bi = c.bs_shift >= 0 ? pos >> c.bs_shift : pos / c.block_size;
-  int64_t page = table[(int64_t)b * max_blocks + min(bi, max_blocks - 1)];
-  page = min(max(page, (int64_t)0), c.num_blocks - 1);
-  return Slot{page * c.block_size + (pos - bi * c.block_size), page};
+  const int64_t named = table[(int64_t)b * max_blocks + min(bi, max_blocks - 1)];
+  const int64_t page = min(max(named, (int64_t)0), c.num_blocks - 1);
+  return Slot{page * c.block_size + (pos - bi * c.block_size), page, page == named};
 }
 
 // fp8 codes written for another page's scale: the value that they stand for, encoded as the append does.
@@ -130,7 +132,7 @@ __global__ __launch_bounds__(256) void accept_kernel(const AcceptParams p) {
     for (int i = tid; i < len * c.kv_heads; i += 256) {
       const int r = i / c.kv_heads, kh = i - r * c.kv_heads;
       const Slot d = slot_of(c, c.block_table, c.max_blocks, b, past + r);
-      p.weights[(d.page * c.kv_heads + kh) * c.block_size + (d.slot - d.page * c.block_size)] = 0.0f;
+      if (d.there) p.weights[(d.page * c.kv_heads + kh) * c.block_size + (d.slot - d.page * c.block_size)] = 0.0f;
     }
   // rows of whole tokens, keys then values
   const int64_t row = (int64_t)c.kv_heads * c.head_bytes;
@@ -157,8 +159,9 @@ __global__ __launch_bounds__(256) void accept_kernel(const AcceptParams p) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int i = i0 + k;
-      if (i < len && path[i] != i)
-        *reinterpret_cast<unit*>(cache + slot_of(c, c.block_table, c.max_blocks, b, past + i).slot * row + at) = v[k];
+      if (i >= len || path[i] == i) continue;
+      const Slot d = slot_of(c, c.block_table, c.max_blocks, b, past + i);
+      if (d.there) *reinterpret_cast<unit*>(cache + d.slot * row + at) = v[k];
     }
   }
 }
@@ -354,10 +357,9 @@ __global__ __launch_bounds__(Round<INPLACE>::THREADS) void evict_move_kernel(con
   constexpr int PER = W / U, ROWS = kMThreads / PER;  // units of a slice, rows at once
   const bool weights = part == 2 * slices;
   const int step = (weights ? kMThreads : ROWS) * kMDepth;
-  const int first = INPLACE ? 0 : (int)blockIdx.y * step;
-  const int last = INPLACE ? rows : (int)min((int64_t)first + step, (int64_t)rows);
+  const int first = INPLACE ? 0 : (int)blockIdx.y * step, next = INPLACE ? step : (int)gridDim.y * step;
   if (weights) {
-    for (int i0 = first; i0 < last; i0 += step) {
+    for (int i0 = first; i0 < rows; i0 += next) {
       float w[kMDepth];
 #pragma unroll
       for (int k = 0; k < kMDepth; ++k) {
@@ -371,9 +373,9 @@ __global__ __launch_bounds__(Round<INPLACE>::THREADS) void evict_move_kernel(con
 #pragma unroll
       for (int k = 0; k < kMDepth; ++k) {
         const int i = i0 + k * kMThreads + tid;
-        if (i >= last) continue;
+        if (i >= rows) continue;
         const Slot d = slot_of(c, to, to_blocks, b, i);
-        p.weights[(d.page * c.kv_heads + kh) * c.block_size + (d.slot - d.page * c.block_size)] = w[k];
+        if (d.there) p.weights[(d.page * c.kv_heads + kh) * c.block_size + (d.slot - d.page * c.block_size)] = w[k];
       }
     }
     return;
@@ -384,7 +386,7 @@ __global__ __launch_bounds__(Round<INPLACE>::THREADS) void evict_move_kernel(con
   const int at = ((value ? part - slices : part) * PER + tid % PER) * U;
   const bool mine = at < c.head_bytes;
   const int64_t row = (int64_t)c.kv_heads * c.head_bytes, off = (int64_t)kh * c.head_bytes + (mine ? at : 0);
-  for (int i0 = first; i0 < last; i0 += step) {
+  for (int i0 = first; i0 < rows; i0 += next) {
     unit v[kMDepth];
     int from[kMDepth];
 #pragma unroll
@@ -405,8 +407,10 @@ __global__ __launch_bounds__(Round<INPLACE>::THREADS) void evict_move_kernel(con
 #pragma unroll
     for (int k = 0; k < kMDepth; ++k) {
       const int i = i0 + k * ROWS + tid / PER;
-      if (!mine || i >= last || (INPLACE && from[k] == i)) continue;
-      unit* dst = reinterpret_cast<unit*>(cache + slot_of(c, to, to_blocks, b, i).slot * row + off);
+      if (!mine || i >= rows || (INPLACE && from[k] == i)) continue;
+      const Slot d = slot_of(c, to, to_blocks, b, i);
+      if (!d.there) continue;
+      unit* dst = reinterpret_cast<unit*>(cache + d.slot * row + off);
       if (INPLACE) *dst = v[k];
       else __builtin_nontemporal_store(v[k], dst);
     }
@@ -418,8 +422,8 @@ hipError_t launch_move_in(const EvictParams& p, hipStream_t s) {
   const int64_t wgs = ((int64_t)p.c.batch * p.c.kv_heads + 7) / 8 * 8 * parts;
   constexpr int step = Round<INPLACE>::THREADS / (W / U) * Round<INPLACE>::DEPTH;
   const int rows = std::min(p.budget, p.max_keys);
-  const int64_t rounds = INPLACE ? 1 : (rows + step - 1) / step;
-  if (wgs > INT32_MAX || rounds > 65535) return hipErrorInvalidValue;
+  const int rounds = INPLACE ? 1 : std::min((rows + step - 1) / step, 65535);
+  if (wgs > INT32_MAX) return hipErrorInvalidValue;
   hipLaunchKernelGGL((evict_move_kernel<U, W, INPLACE>), dim3((unsigned)wgs, (unsigned)rounds),
                      dim3(Round<INPLACE>::THREADS), 0, s, p);
   return hipGetLastError();

@@ -277,8 +277,8 @@ __global__ __launch_bounds__(256) void fold_kernel(const WeighParams wp) {
     }
   };
   // (the entries come in while the sums are made)
-  int64_t page = p.block_table[(int64_t)b * p.max_blocks + min(key / p.block_size, p.max_blocks - 1)];
-  page = min(max(page, (int64_t)0), p.num_blocks - 1);
+  const int64_t named = p.block_table[(int64_t)b * p.max_blocks + min(key / p.block_size, p.max_blocks - 1)];
+  const int64_t page = min(max(named, (int64_t)0), p.num_blocks - 1);
   float* w = wp.weights + (page * p.kv_heads + kh) * p.block_size + key % p.block_size;
   float old[V];
   load(w, old);
@@ -321,6 +321,7 @@ __global__ __launch_bounds__(256) void fold_kernel(const WeighParams wp) {
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) sum[i] = key + i < e.past ? old[i] + sum[i] : key + i < e.total ? sum[i] : old[i];
+  if (page != named) return;  // no page: nobody's entries
   if constexpr (V == 4)
     *reinterpret_cast<f32x4*>(w) = f32x4{sum[0], sum[1], sum[2], sum[3]};
   else

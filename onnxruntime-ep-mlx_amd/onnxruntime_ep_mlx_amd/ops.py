@@ -631,7 +631,7 @@ def accumulating_attention(q, key_cache, value_cache, cum, past, block_table, ke
     ``key_weights`` float32 [num_blocks, kv_num_heads, block_size] lies beside the pages: a key's entry
     grows by its probabilities (sinks in their denominator) in the last ``observed_rows`` new tokens of its
     sequence (0: in all of them), summed over the heads of its kv-head; entries of the new tokens begin at
-    zero.  The same call gives the same bits.  Returns the output; everything else as in masked_attention
+    zero, those of pages that several sequences of the call hold are unspecified.  The same call gives the same bits.  Returns the output; everything else as in masked_attention
     without its masks."""
     lib = capi.load()
     descs, out = _paged_call(q, key_cache, value_cache, cum, past, block_table, num_heads, scale, softcap,
