@@ -31,7 +31,7 @@ __device__ __forceinline__ int64_t seq_keys(const AttnParams& p, int b, int64_t 
 
 // Whether token t sees new row n of its sequence: of a drafted tree, what its bits name (n < 0: a key before it).
 __device__ __forceinline__ bool tree_sees(const AttnParams& p, int t, int64_t n) {
-  if (!p.tree_bits || n < 0) return true;
+  if (n < 0) return true;
   return (n >> 5) < p.tree_words && ((p.tree_bits[(int64_t)t * p.tree_words + (n >> 5)] >> (n & 31)) & 1u);
 }
 
@@ -44,9 +44,11 @@ __device__ __forceinline__ bool tree_sees(const AttnParams& p, int t, int64_t n)
 // latencies (block table, rows) and the sums, so a call of few (token, head) pairs takes as long as
 // its rounds: one fp32 token of 8 heads over 129 keys 79 us with one wavefront and one key at a
 // time, 8.7 with 16 (launch_generic_ne has the rule).
+// UPKEEP: drafted trees and rows that leave their softmax's constant, at heads beyond 256 (a build of its own: as branches
+// of every call they took one fp32 token each of 8 sequences from 285 to 347 us).
 template <int NE>
 constexpr int kGenKeys = NE <= 4 ? 8 : 2;
-template <typename TT, typename CT, int NE, int NW>
+template <typename TT, typename CT, int NE, int NW, bool UPKEEP>
 __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams p) {
   constexpr int U = kGenKeys<NE>;
   const int split = blockIdx.x, h = blockIdx.y, t = blockIdx.z;
@@ -73,7 +75,8 @@ __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams 
   // window end point: the row's position, or the last key for rows past it (a right-padded
   // first prompt, causal_window_mask attention.rs:328-353)
   // (a drafted node's place goes by its depth)
-  if (p.window > 0) lo = max(lo, min(rp, total - 1) - (p.tree_lag ? p.tree_lag[t] : 0) - p.window + 1);
+  const bool tree = UPKEEP && p.tree_bits;
+  if (p.window > 0) lo = max(lo, min(rp, total - 1) - (tree ? p.tree_lag[t] : 0) - p.window + 1);
   const typename TT::raw* bias_row =
       p.bias ? reinterpret_cast<const typename TT::raw*>(p.bias) +
                    ((((int64_t)(p.bias_b == 1 ? 0 : b) * p.bias_h + (p.bias_h == 1 ? 0 : h)) *
@@ -111,7 +114,7 @@ __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams 
       for (int u = 0; u < U; ++u) {
         // a surplus key repeats the last one: weight 0 below, and no values (theirs may be infinite)
         const int64_t pos = min(p0 + NW * u, hi - 1);
-        const int vd = NW * u < left && tree_sees(p, t, pos - pastb) ? VD : 0;
+        const int vd = NW * u < left && (!tree || tree_sees(p, t, pos - pastb)) ? VD : 0;
         const void *kb, *vb;
         int64_t off;
         float ks = 1.0f, vs = 1.0f;
@@ -169,7 +172,7 @@ __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams 
         if (bias_row)
           s += TT::to_f32(
               bias_row[min(max(min(pos, hi - 1) + bias_off, (int64_t)0), (int64_t)p.bias_cols - 1)]);
-        x[u] = pos < hi && tree_sees(p, t, pos - pastb) ? s * kLog2e : kNegInf;
+        x[u] = pos < hi && (!tree || tree_sees(p, t, pos - pastb)) ? s * kLog2e : kNegInf;
       }
     }
     float mn = m;
@@ -221,7 +224,8 @@ __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams 
   if (!single && p.part_o == nullptr) return;  // beyond planned capacity: nothing to write into
   if (single) {
     float f = finalize_factor(m, l, sink_logit<TT>(p, h));
-    if (p.row_stats && lane == 0) p.row_stats[stat_row(p, t, h)] = softmax_stat(m, l, sink_logit<TT>(p, h));
+    if (UPKEEP && p.row_stats && lane == 0)
+      p.row_stats[stat_row(p, t, h)] = softmax_stat(m, l, sink_logit<TT>(p, h));
     typename TT::raw* out = reinterpret_cast<typename TT::raw*>(p.out);
 #pragma unroll
     for (int k = 0; k < NE; ++k) {
@@ -337,22 +341,22 @@ constexpr int kMaxHeadDim = 640;
 template <int NE>
 constexpr bool ne_covers(int d) { return d <= 64 * NE; }
 
-template <typename TT, int NE, int NW>
+template <typename TT, int NE, int NW, bool UPKEEP>
 hipError_t launch_generic_nw(const AttnParams& p, pa_dtype cache_dtype, hipStream_t s) {
   dim3 grid(p.max_splits, p.num_heads, p.num_tokens), block(64 * NW);
   switch (cache_dtype) {
     case PA_DTYPE_FP8_E4M3:
-      hipLaunchKernelGGL((attn_generic_kernel<TT, Fp8Cache, NE, NW>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attn_generic_kernel<TT, Fp8Cache, NE, NW, UPKEEP>), grid, block, 0, s, p);
       break;
     case PA_DTYPE_INT8:
-      hipLaunchKernelGGL((attn_generic_kernel<TT, I8Cache, NE, NW>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attn_generic_kernel<TT, I8Cache, NE, NW, UPKEEP>), grid, block, 0, s, p);
       break;
     case PA_DTYPE_INT4:
-      hipLaunchKernelGGL((attn_generic_kernel<TT, I4Cache, NE, NW>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attn_generic_kernel<TT, I4Cache, NE, NW, UPKEEP>), grid, block, 0, s, p);
       break;
     default:
       if (cache_dtype != TT::code) return hipErrorInvalidValue;
-      hipLaunchKernelGGL((attn_generic_kernel<TT, TT, NE, NW>), grid, block, 0, s, p);
+      hipLaunchKernelGGL((attn_generic_kernel<TT, TT, NE, NW, UPKEEP>), grid, block, 0, s, p);
       break;
   }
   return hipGetLastError();
@@ -364,21 +368,22 @@ hipError_t launch_generic_nw(const AttnParams& p, pa_dtype cache_dtype, hipStrea
 // 2048 keys 25.1 / 42.0 / 132.6 us, 8 tokens over 600 25.9 / 42.6 / 133.2; 128 tokens over 128 keys 48.2 /
 // 39.6 / 94.2, 8 x 100 over 2048 2685 / 2000 / 2661; 16-token prompts 12.0 / 9.5 / 12.1 (one) and 89.9 /
 // 26.0 / 17.0 (32 of them).
-template <typename TT, int NE>
+template <typename TT, int NE, bool UPKEEP = false>
 hipError_t launch_generic_ne(const AttnParams& p, pa_dtype cache_dtype, hipStream_t s) {
   const int64_t groups = (int64_t)p.max_splits * p.num_heads * p.num_tokens;
   const int64_t keys =
       p.linear_cap > 0 ? (int64_t)p.linear_cap : (int64_t)p.max_blocks * p.block_size;
   const bool few = groups <= 512;
   if (keys <= 32)
-    return few ? launch_generic_nw<TT, NE, 4>(p, cache_dtype, s)
-               : launch_generic_nw<TT, NE, 1>(p, cache_dtype, s);
-  return few ? launch_generic_nw<TT, NE, 16>(p, cache_dtype, s)
-             : launch_generic_nw<TT, NE, 4>(p, cache_dtype, s);
+    return few ? launch_generic_nw<TT, NE, 4, UPKEEP>(p, cache_dtype, s)
+               : launch_generic_nw<TT, NE, 1, UPKEEP>(p, cache_dtype, s);
+  return few ? launch_generic_nw<TT, NE, 16, UPKEEP>(p, cache_dtype, s)
+             : launch_generic_nw<TT, NE, 4, UPKEEP>(p, cache_dtype, s);
 }
 
 template <typename TT>
 hipError_t launch_generic_t(const AttnParams& p, pa_dtype cache_dtype, hipStream_t s) {
+  if (p.tree_bits || p.row_stats) return launch_generic_ne<TT, 10, true>(p, cache_dtype, s);
   if (ne_covers<1>(p.head_dim)) return launch_generic_ne<TT, 1>(p, cache_dtype, s);
   if (ne_covers<2>(p.head_dim)) return launch_generic_ne<TT, 2>(p, cache_dtype, s);
   return ne_covers<4>(p.head_dim) ? launch_generic_ne<TT, 4>(p, cache_dtype, s)
