@@ -60,6 +60,37 @@ __device__ __forceinline__ f32x4 four(const void* c, int64_t base, int d) {
   return x;
 }
 
+// Elements of 16 bytes of a cache row, and these widened (unscaled).
+template <typename CT>
+constexpr int kPiece = std::is_same<CT, TF32>::value                                             ? 4
+                       : std::is_same<CT, TF16>::value || std::is_same<CT, TBF16>::value         ? 8
+                       : std::is_same<CT, I4Cache>::value                                        ? 32
+                                                                                                 : 16;
+template <typename CT>
+__device__ __forceinline__ void widen(u32x4 w, float (&x)[kPiece<CT>]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<CT, TF32>::value) {
+      const uint32_t u = w[i];  // (a copy: the cast of a vector's element takes the first one)
+      x[i] = __builtin_bit_cast(float, u);
+    } else if constexpr (std::is_same<CT, Fp8Cache>::value) {
+      x[4 * i] = __builtin_amdgcn_cvt_f32_fp8(w[i], 0);
+      x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(w[i], 1);
+      x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(w[i], 2);
+      x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(w[i], 3);
+    } else if constexpr (std::is_same<CT, I8Cache>::value) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[4 * i + k] = (float)(int8_t)(w[i] >> (8 * k));
+    } else if constexpr (std::is_same<CT, I4Cache>::value) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[8 * i + k] = (float)((int)((w[i] >> (4 * k)) & 15) - 8);
+    } else {
+      x[2 * i] = CT::to_f32((uint16_t)w[i]);
+      x[2 * i + 1] = CT::to_f32((uint16_t)(w[i] >> 16));
+    }
+  }
+}
+
 // One side of a cache, of one kv-head.
 template <typename CT>
 struct Side {
@@ -106,8 +137,8 @@ __device__ __forceinline__ void act_store(void* x, int64_t i, int act, float v) 
 
 template <typename CT, int DP>
 __global__ __launch_bounds__(256) void rows32_kernel(const AttnParams p, int row_blocks, int act) {
-  constexpr int KP = DP + 4, ND = DP / 32;  // pitch of a key's row in LDS
-  __shared__ __attribute__((aligned(16))) float keys[32 * KP], values[32 * DP];
+  constexpr int KP = DP + 4, VP = DP + 8, ND = DP / 32;  // pitches of a key's and a value's row in LDS
+  __shared__ __attribute__((aligned(16))) float keys[32 * KP], values[32 * VP];
   __shared__ int odd, ends[8];
   __shared__ int2 slots[2][32];  // slot and page of a tile's keys, the next tile's beside it
   const int NT = blockDim.x, WAVES = NT >> 6;
@@ -188,15 +219,106 @@ __global__ __launch_bounds__(256) void rows32_kernel(const AttnParams p, int row
     return int2{page * p.block_size + (pos - bi * p.block_size), page};
   };
   const int begin = first & ~31;
-  if (tid < 32 && begin < last) slots[0][tid] = place(begin);
   int buf = 0;
+  // Rows of whole 16 bytes: a thread keeps to row tid % 32 of the tile and takes every NT / 32nd piece of it, R of a round
+  // of keys and of values; the first round of a tile is on its way while the last tile is multiplied, the table's entry a
+  // tile earlier.  Other rows: four elements at a time.
+  constexpr int E = kPiece<CT>, R = DP / E / 2 < 4 ? DP / E / 2 : 4;
+  const int bytes = D * 16 / E, np = bytes / 16, own = tid & 31, piece0 = tid >> 5, stride = NT / 32;
+  const bool pieces = (D * 16) % (16 * E) == 0;
+  u32x4 kr[R], vr[R];
+  float kone = 1.0f, vone = 1.0f;
+  auto place_own = [&](int t0) {
+    const int pos = min(max(t0 + own, first), last - 1), bi = pos / p.block_size;
+    int page = p.block_table[(int64_t)b * p.max_blocks + min(bi, p.max_blocks - 1)];
+    page = min(max(page, 0), (int)p.num_blocks - 1);
+    return int2{page * p.block_size + (pos - bi * p.block_size), page};
+  };
+  auto fetch = [&](int2 at, int r) {
+    const int64_t row = ((int64_t)at.x * p.kv_heads + kh) * bytes;
+    const char *kc = reinterpret_cast<const char*>(p.key_cache) + row, *vc = reinterpret_cast<const char*>(p.value_cache) + row;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      if ((r * R + j) * stride >= np) break;
+      const int piece = min((r * R + j) * stride + piece0, np - 1);
+      __builtin_memcpy(&kr[j], kc + 16 * piece, 16);
+      __builtin_memcpy(&vr[j], vc + 16 * piece, 16);
+    }
+    if (std::is_same<CT, Fp8Cache>::value && r == 0) {
+      kone = p.k_scale[(int64_t)at.y * p.kv_heads + kh];
+      vone = p.v_scale[(int64_t)at.y * p.kv_heads + kh];
+    }
+  };
+  if (kIntCache<CT>) {
+    if (!ks.channel) kone = p.k_scale[0];
+    if (!vs.channel) vone = p.v_scale[0];
+  }
+  auto stash = [&](int r) {  // whether a value is not finite
+    bool strange = false;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const int piece = (r * R + j) * stride + piece0;
+      if (piece >= np) break;
+      float x[E];
+      auto scaled = [&](const Side<CT>& side, float one) {
+        if (kIntCache<CT> && side.channel) {
+#pragma unroll
+          for (int k = 0; k < E; ++k) x[k] *= side.scale[kh * D + piece * E + k];
+        } else if (kIntCache<CT> || std::is_same<CT, Fp8Cache>::value) {
+#pragma unroll
+          for (int k = 0; k < E; ++k) x[k] *= one;
+        }
+      };
+      widen<CT>(kr[j], x);
+      scaled(ks, kone);
+#pragma unroll
+      for (int k = 0; k < E; k += 4)
+        *reinterpret_cast<f32x4*>(&keys[own * KP + piece * E + k]) = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]};
+      widen<CT>(vr[j], x);
+      scaled(vs, vone);
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        if (!(fabsf(x[k]) < -kNegInf)) {
+          strange = true;
+          x[k] = 0.0f;
+        }
+#pragma unroll
+      for (int k = 0; k < E; k += 4)
+        *reinterpret_cast<f32x4*>(&values[own * VP + piece * E + k]) = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]};
+    }
+    return strange;
+  };
+  int2 at{0, 0}, ahead{0, 0};
+  if (pieces) {
+    for (int i = tid; i < 32 * (DP - D); i += NT) {
+      const int kk = i / (DP - D), d = D + i - kk * (DP - D);
+      keys[kk * KP + d] = values[kk * VP + d] = 0.0f;
+    }
+    if (begin < last) {
+      at = place_own(begin);
+      fetch(at, 0);
+      ahead = place_own(begin + 32);
+    }
+  } else if (tid < 32 && begin < last) {
+    slots[0][tid] = place(begin);
+  }
   for (int t0 = begin; t0 < last; t0 += 32, buf ^= 1) {
     if (tid == 0) odd = 0;
     __syncthreads();  // the last tile's readers are done
-    if (tid < 32 && t0 + 32 < last) slots[buf ^ 1][tid] = place(t0 + 32);
     bool strange = false;
-    constexpr int PER = DP / 4, N = 4;  // pieces of a row; of a thread in flight
-    for (int i0 = tid; i0 < 32 * PER; i0 += N * NT) {
+    constexpr int PER = DP / 4, N = 4;  // fours of a row; of a thread in flight
+    if (pieces) {
+      if (tid < 32) slots[buf][tid] = at;
+      strange = stash(0);
+#pragma unroll 1
+      for (int r = 1; r * R * stride < np; ++r) {
+        fetch(at, r);
+        strange |= stash(r);
+      }
+    } else if (tid < 32 && t0 + 32 < last) {
+      slots[buf ^ 1][tid] = place(t0 + 32);
+    }
+    for (int i0 = pieces ? 32 * PER : tid; i0 < 32 * PER; i0 += N * NT) {
       f32x4 kv[N], vv[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) {
@@ -216,11 +338,16 @@ __global__ __launch_bounds__(256) void rows32_kernel(const AttnParams p, int row
             strange = true;
             vv[j][k] = 0.0f;
           }
-        *reinterpret_cast<f32x4*>(&values[kk * DP + d]) = vv[j];
+        *reinterpret_cast<f32x4*>(&values[kk * VP + d]) = vv[j];
       }
     }
     if (strange) odd = 1;
     __syncthreads();
+    if (pieces && t0 + 32 < last) {
+      at = ahead;
+      fetch(at, 0);
+      ahead = place_own(t0 + 64);
+    }
     f32x16 s;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.0f;
@@ -268,7 +395,7 @@ __global__ __launch_bounds__(256) void rows32_kernel(const AttnParams p, int row
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float* row = &values[(8 * (i >> 2) + 4 * h + (i & 3)) * DP + c];
+      const float* row = &values[(8 * (i >> 2) + 4 * h + (i & 3)) * VP + c];
 #pragma unroll
       for (int n = 0; n < ND; ++n) o[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(row[32 * n], s[i], o[n], 0, 0, 0);
     }
