@@ -509,6 +509,8 @@ struct WeighParams {
   int32_t max_keys;  // of any sequence
 };
 hipError_t launch_weigh(const WeighParams& p, pa_dtype act, pa_dtype cache_dtype, hipStream_t s);
+// ... its sums over rows where no scores are held, of other types and heads up to 256 (pa_weigh32.hip)
+hipError_t launch_weigh_columns32(const WeighParams& p, pa_dtype act, pa_dtype cache_dtype, hipStream_t s);
 
 // Rows that move within the pages (pa_upkeep.hip).
 struct RowsParams {  // the caches
@@ -752,8 +754,9 @@ hipError_t launch_axes_append(const AppendParams& p, const AxisParams& ax, pa_dt
                               pa_dtype cache_dtype, hipStream_t s);
 hipError_t launch_attn_generic(const AttnParams& p, pa_dtype act, pa_dtype cache_dtype,
                                hipStream_t s);
-// Drafted trees and weighed rows of heads up to 256 (pa_rows32.hip); partials merged by launch_split_reduce.
+// Drafted trees and weighed rows of heads up to 256 (pa_rows32.hpp); partials merged by launch_split_reduce.
 hipError_t launch_rows32(const AttnParams& p, pa_dtype act, pa_dtype cache_dtype, hipStream_t s);
+hipError_t launch_rows32_coded(const AttnParams& p, pa_dtype act, pa_dtype cache_dtype, hipStream_t s);
 hipError_t launch_decode_mfma(const AttnParams& p, pa_dtype act, pa_dtype cache_dtype,
                               hipStream_t s);
 hipError_t launch_decode_balanced(const AttnParams& p, pa_dtype act, pa_dtype cache_dtype,

@@ -15,26 +15,13 @@
 // softcap, 133 GFLOP of products in 212 us (three transcendental instructions a score; vector and matrix units busy 53
 // and 27 % of the time); without LDS and a tile's lead 467.  The last 32 rows of prompts of 3001 - 5001: 14.
 #include "pa_cache_read.hpp"
-#include "pa_ranged.hpp"
+#include "pa_weigh.hpp"
 
 namespace pa {
 namespace {
 
 constexpr int kWKeys = 64;             // keys of a wavefront
 constexpr int kWBlock = 4 * kWKeys;    // of a workgroup
-
-// Rows of a key: [lo, hi) of its sequence's rows (token * g + head) see it and count.
-struct WRows {
-  int lo, hi;
-};
-__device__ __forceinline__ WRows key_rows(const RangedParams& p, const RSeq& e, int key) {
-  const int g = p.num_heads / p.kv_heads;
-  int lo = p.observed > 0 ? max(e.nq - p.observed, 0) : 0, hi = e.nq;
-  if (p.causal) lo = max(lo, key - e.past);
-  if (p.window > 0) hi = (int)min((int64_t)hi, (int64_t)key - e.past + p.window);
-  if (key >= e.total || lo >= hi) return WRows{INT32_MAX, 0};
-  return WRows{lo * g, hi * g};
-}
 
 // Forms of a score: as it is; under a softcap as a quotient, whose constant the exponent takes along, up to
 // kCapNear, and beyond it by tanh to its own bits -- the attention's own arithmetic (r_softmax), so that what the two
@@ -202,7 +189,7 @@ __global__ __launch_bounds__(256, 2) void weigh_columns_kernel(const WeighParams
   }
 }
 
-// The same for every type and head size: 16 keys in LDS as fp32, 16 rows at a time.  Bound by LDS reads.
+// The same for heads beyond 256, of every type: 16 keys in LDS as fp32, 16 rows at a time.  Bound by LDS reads.
 template <typename TT, typename CT>
 __global__ __launch_bounds__(256) void weigh_columns_valu_kernel(const WeighParams wp) {
   constexpr int KB = 16;
@@ -381,6 +368,8 @@ hipError_t launch_weigh(const WeighParams& p, pa_dtype act, pa_dtype cache_dtype
     hipError_t e;
     if (matrix)
       e = act == PA_DTYPE_FLOAT16 ? launch_matrix<TF16>(p, s) : launch_matrix<TBF16>(p, s);
+    else if (r.head_dim <= 256)
+      e = launch_weigh_columns32(p, act, cache_dtype, s);
     else
       e = act == PA_DTYPE_FLOAT16    ? launch_valu<TF16>(p, cache_dtype, grid, s)
           : act == PA_DTYPE_BFLOAT16 ? launch_valu<TBF16>(p, cache_dtype, grid, s)
