@@ -10,11 +10,12 @@
 //
 // Values that are not finite lie in LDS as zeros and are added for the rows that see them (rare).
 //
-// Bound by the chain of a tile where a sequence has few rows (table, rows into LDS, products: 18 us a tile with one
-// wavefront per SIMD, its products 3.5), by staging and fp32 products, 128 of 64 cycles a tile at head 128, where it has
-// many.  8 sequences of 500 - 6000 keys, 32 heads of 128 and 8 kv-heads, fp8 pages: one token each 244 us (488 on the
-// VALU kernel), trees of 32 nodes 320 (11400); head 80 in bf16 240 (372) and 305 (9400); fp32 at head 64 71 (281) and
-// 189 (6990).
+// Bound, where a sequence has few rows, by the chain of a tile (rows into LDS, products, softmax: 6.8 us at head 128 with one
+// wavefront per SIMD, its products 3.4); where it has many, by the fp32 products, 128 of 64 cycles a tile and wavefront at head
+// 128, which two wavefronts per SIMD keep busy 42 % of the time beside the softmax and the widening of keys.  8 sequences of
+// 500 - 6000 keys, 32 heads of 128 and 8 kv-heads, fp8 pages: one token each 97 us (488 on the VALU kernel; 244 with
+// four elements a load and none ahead), trees of 32 nodes 267 (11400; 339 in one build with the other's registers); head 80 in
+// bf16 91 (372) and 259 (9400); fp32 at head 64 55 (281) and 165 (6990).  Chunks half as long: 112 and 303.
 #pragma once
 
 #include "pa_cache_read.hpp"
@@ -146,8 +147,10 @@ __global__ __launch_bounds__(NT, DP <= 64 || (NT == 256 && DP <= 128) ? 2 : 1) v
   constexpr int WAVES = NT / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
-  const int split = blockIdx.x % p.max_splits, rest = blockIdx.x / p.max_splits;
-  const int blk = rest % row_blocks, z = rest / row_blocks, b = z / p.kv_heads, kh = z - b * p.kv_heads;
+  // chunks of different sequences side by side: 8 or 16 chunks of one would each go to an XCD of their own, the last of
+  // which only the longest sequences have (trees of 32 nodes 282 us for 297 over int8, 259 for 265 at head 80)
+  const int seqs = p.batch * p.kv_heads, rest = blockIdx.x / seqs, z = blockIdx.x - rest * seqs;
+  const int split = rest / row_blocks, blk = rest - split * row_blocks, b = z / p.kv_heads, kh = z - b * p.kv_heads;
   const int g = p.num_heads / p.kv_heads, D = p.head_dim;
   const int cap = (int)min((int64_t)p.max_blocks * p.block_size, (int64_t)(INT32_MAX / 2));
   const int s0 = min(max(p.cum[b], 0), p.num_tokens);

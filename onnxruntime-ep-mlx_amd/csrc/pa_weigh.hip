@@ -13,7 +13,7 @@
 // more in the attention (195 for 162 without) and 11.5 in fold_kernel.  Columns: the exponentials' vector instructions
 // beside the products, at two wavefronts per SIMD that overlap in part: 4095 tokens after 600, 24 heads of 256 under a
 // softcap, 133 GFLOP of products in 212 us (three transcendental instructions a score; vector and matrix units busy 53
-// and 27 % of the time); without LDS and a tile's lead 467.  The last 32 rows of prompts of 3001 - 5001: 14.
+// and 27 % of the time); without LDS and a tile's lead 467.  Other types and heads up to 256: pa_weigh32.hip.  The last 32 rows of prompts of 3001 - 5001: 14.
 #include "pa_cache_read.hpp"
 #include "pa_weigh.hpp"
 
