@@ -41,6 +41,17 @@ def test_coded_pages(kind, scales, dt, D, new, past):
     weigh.compare(st)
 
 
+@pytest.mark.parametrize("dt,D,kind", [(F32, 64, None), (BF16, 80, None), (BF16, 128, torch.float8_e4m3fn), (F16, 256, torch.int8),
+                                       (F32, 300, None)])
+def test_prompts_of_other_types(dt, D, kind):
+    """Rows that fill several chunks of sums, under a window, without causality, few of them observed."""
+    st = make_batch([700, 1, 260], [30, 500, 0], H=4, KV=2, D=D, block=16, dtype=dt, seed=9, cache_dtype=kind)
+    weigh.compare(st)
+    weigh.compare(st, window=90, softcap=20.0)
+    weigh.compare(st, causal=0, observed=600)
+    tree.compare(st, trees(st), window=200)
+
+
 def shifted(x, by=1):
     """The same values `by` elements behind an aligned address."""
     y = torch.empty(x.numel() + by, dtype=x.dtype, device=x.device)[by:].view(x.shape)
