@@ -38,7 +38,8 @@
  * sequence goes on: row path[i] of the new tokens to slot past + i, keys and values of every head.
  * The path begins with row 0 and goes on, while there is one, to the first child of its last node
  * whose token is that node's target (parents, tokens, targets given; path, path_lens and next_tokens
- * are then written), or it is given (parents NULL: rising rows in path, path_lens of them).  Other
+ * are then written), or it is given (parents NULL: rising rows in path, path_lens of them).  A step
+ * without new tokens has empty paths (parents, tokens, targets not NULL; nothing is read there).  Other
  * rows of the new tokens keep what they held or lose it to the path's.  fp8 rows that move to a page
  * of another scale are encoded anew (x / scale as the append does); other rows keep their bytes.
  * The pages of the new tokens must belong to their sequence alone. */

@@ -615,8 +615,9 @@ def accept_drafts(key_cache, value_cache, cum, past, block_table, parents=None, 
         after = draft_tokens.new_empty(B)
     batch = capi.PaBatch(cum.data_ptr(), past.data_ptr(), block_table.data_ptr(), None, B, block_table.shape[1],
                          tokens, max_query_len, 0, 0)
-    drafts = capi.PaDrafts(_ptr(parents), _ptr(draft_tokens), _ptr(target_tokens), _ptr(path), _ptr(path_lens),
-                           _ptr(after), path.shape[1], _ptr(key_weights))
+    # (parents without an address mean a given path; of no tokens any address will do, for nothing is read there)
+    tree = (None,) * 3 if given else [t.data_ptr() or cum.data_ptr() for t in (parents, draft_tokens, target_tokens)]
+    drafts = capi.PaDrafts(*tree, _ptr(path), _ptr(path_lens), _ptr(after), path.shape[1], _ptr(key_weights))
     capi.check(_on_device(dev, capi.load().pa_accept_drafts, C.byref(cache), C.byref(batch), C.byref(drafts)))
     return path, path_lens, after
 
