@@ -622,6 +622,22 @@ Plan make_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dtype 
   return pl;
 }
 
+// Longest context that a call expects: its bound, or the table's capacity.
+int expected_ctx(const pa_cache* c, const pa_batch* b) {
+  const int cap = max_ctx_bound(c, b);
+  return b->max_context_len > 0 ? std::min(b->max_context_len, cap) : cap;
+}
+
+// launch_rows32's plan: as many chunks of the given length as the expected context has, the last of which takes what a
+// sequence beyond it holds (by the table's capacity, 48 sequences of 32 nodes, 32 heads of 128 and at most 1000 keys would
+// take 3.3 GB of partial rows behind tables of 131072 slots).
+Plan rows32_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dtype act, int chunk) {
+  Plan pl = make_plan(c, b, a, act, 3, chunk);
+  pl.max_splits = std::max((expected_ctx(c, b) + pl.chunk - 1) / pl.chunk, 1);
+  pl.part_rows = pl.max_splits > 1 ? (size_t)std::max(b->num_tokens, 0) * a->num_heads * pl.max_splits : 0;
+  return pl;
+}
+
 // Bytes of the partial rows: fp32 elements, except the planned prefill's halves, which are
 // stored as fp16 rows scaled by a power of two (store_rows with half_part).  A short planned prefill
 // (fine) leaves either, as its keys turn out: room for the larger.
@@ -968,8 +984,9 @@ int run_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dty
     return fail(PA_ERR_UNSUPPORTED, "prefill MFMA kernel does not cover this dtype/head_dim");
   if (!(a->softcap >= 0.0f) || !std::isfinite(a->softcap))
     return fail(PA_ERR_INVALID_ARGUMENT, "softcap must be finite and non-negative");
-  Plan pl = make_plan(c, b, a, act, kind, chunk, opts.linear_cap > 0, opts.linear_cap,
-                      plan_images(opts), opts.bias != nullptr, opts.host);
+  Plan pl = opts.rows32 ? rows32_plan(c, b, a, act, chunk)
+                        : make_plan(c, b, a, act, kind, chunk, opts.linear_cap > 0, opts.linear_cap,
+                                    plan_images(opts), opts.bias != nullptr, opts.host);
   if (kind == 2 && pl.kind != 2 && pa::prefill_coded_supported(c->head_dim, act, c->dtype))
     return fail(PA_ERR_UNSUPPORTED,
                 "prefill MFMA kernel: byte-coded pages run on it over operand images only (planned "
@@ -1478,12 +1495,16 @@ int rows32_chunk(const pa_cache* c, const pa_batch* b, const pa_attn* a) {
   const int64_t mq = std::min<int64_t>(b->max_query_len > 0 ? b->max_query_len : T, T);
   const int64_t per = mq * g <= 32 ? 32 : 128, waves = per / 32;
   const int64_t blocks = c->kv_heads * std::max<int64_t>(std::min<int64_t>(b->batch, T), T * g / per);
-  int64_t keys = max_ctx_bound(c, b);
-  if (b->max_context_len > 0) keys = std::min<int64_t>(keys, b->max_context_len);
+  const int64_t keys = expected_ctx(c, b);
   // wavefronts that a CU holds, by LDS (workgroups of one) and registers
   const int64_t held = c->head_dim <= 64 ? 8 : c->head_dim <= 128 ? (waves == 1 ? 4 : 8) : (waves == 1 ? 2 : 4);
   const int64_t splits = std::max<int64_t>(held * device_cus() / std::max<int64_t>(blocks * waves, 1), 1);
   return (int)std::max<int64_t>(((keys + splits - 1) / splits + 31) / 32 * 32, 128);
+}
+
+// Workspace of the attention where the matrix-core kernel does not run: launch_rows32 by chunks, or (0) the VALU kernel.
+size_t other_workspace(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dtype act, int chunk) {
+  return chunk > 0 ? workspace_for(c, b, a, rows32_plan(c, b, a, act, chunk)) : ws_need(c, b, a, act, 3, 0).best;
 }
 
 // ------------------------------------------------------------------------------ drafted trees
@@ -1504,7 +1525,7 @@ TreePlan tree_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dt
   t.bits_bytes = align256((size_t)b->num_tokens * t.words * sizeof(uint32_t));
   t.lag_bytes = align256((size_t)b->num_tokens * sizeof(int32_t));
   t.chunk = t.r.on ? 0 : rows32_chunk(c, b, a);
-  t.attn_bytes = t.r.on ? t.r.bytes() : ws_need(c, b, a, act, 3, t.chunk).best;
+  t.attn_bytes = t.r.on ? t.r.bytes() : other_workspace(c, b, a, act, t.chunk);
   return t;
 }
 
@@ -1524,12 +1545,11 @@ AccountPlan account_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a,
   AccountPlan t;
   const int64_t g = a->num_heads / c->kv_heads, T = b->num_tokens, z = (int64_t)b->batch * c->kv_heads;
   const int64_t mq = std::min<int64_t>(b->max_query_len > 0 ? b->max_query_len : T, T);
-  t.keys = max_ctx_bound(c, b);
-  if (b->max_context_len > 0) t.keys = std::min(t.keys, b->max_context_len);
+  t.keys = expected_ctx(c, b);
   t.ld = ((int64_t)t.keys + 63) / 64 * 64;
   t.r = ranged_plan(c, b, a, nullptr, act);
   t.chunk = t.r.on ? 0 : rows32_chunk(c, b, a);
-  t.attn_bytes = t.r.on ? t.r.bytes() : ws_need(c, b, a, act, 3, t.chunk).best;
+  t.attn_bytes = t.r.on ? t.r.bytes() : other_workspace(c, b, a, act, t.chunk);
   t.stat_bytes = align256((size_t)T * a->num_heads * sizeof(float));
   // Every sequence's rows of a kv-head on a wavefront of their own leave their scores, within a GiB: a step of 48 sequences
   // of up to 8190 keys takes 30 us to write and 12 to read them where its keys take 77 to be read again.
@@ -1782,7 +1802,7 @@ int pa_evict_keys(const pa_cache* c, const pa_batch* b, const pa_eviction* v, pa
     return fail(PA_ERR_INVALID_ARGUMENT, "eviction: key_weights (4-byte aligned), kept and lens_out are required");
   if (v->budget < 1 || v->sinks < 0 || v->recent < 0 || (int64_t)v->sinks + v->recent > v->budget)
     return fail(PA_ERR_INVALID_ARGUMENT, "eviction: sinks + recent must lie within a positive budget");
-  const int cap = max_ctx_bound(c, b), keys = b->max_context_len > 0 ? std::min(b->max_context_len, cap) : cap;
+  const int keys = expected_ctx(c, b);
   if (v->block_table_out) {
     if (v->block_table_out == b->block_table)
       return fail(PA_ERR_INVALID_ARGUMENT, "eviction: block_table_out must name other pages (NULL: in place)");

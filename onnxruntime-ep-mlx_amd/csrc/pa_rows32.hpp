@@ -158,7 +158,8 @@ __global__ __launch_bounds__(NT, DP <= 64 || (NT == 256 && DP <= 128) ? 2 : 1) v
   const int past = min(max(p.past[b], 0), cap - nq), total = past + nq;
   const int64_t start64 = (int64_t)split * p.chunk;
   if (start64 >= total || (int64_t)blk * 32 * WAVES >= (int64_t)nq * g) return;
-  const int start = (int)start64, end = (int)min(start64 + p.chunk, (int64_t)total);
+  // (the last chunk goes to the sequence's end: contexts beyond the call's bound)
+  const int start = (int)start64, end = split == p.max_splits - 1 ? total : (int)min(start64 + p.chunk, (int64_t)total);
   const int r = blk * 32 * WAVES + 32 * wave + c;
   const bool valid = r < nq * g;
   const int qi = valid ? r / g : 0, t = s0 + qi, head = kh * g + (valid ? r - qi * g : 0);
