@@ -428,15 +428,10 @@ hipError_t launch_move_in(const EvictParams& p, hipStream_t s) {
                      dim3(Round<INPLACE>::THREADS), 0, s, p);
   return hipGetLastError();
 }
-template <int U, int W>
-hipError_t launch_move(const EvictParams& p, hipStream_t s) {
-  return p.table_out ? launch_move_in<U, W, false>(p, s) : launch_move_in<U, W, true>(p, s);
-}
 template <int U>
-hipError_t launch_move_u(const EvictParams& p, hipStream_t s) {
-  if constexpr (U == 16)
-    if (p.table_out) return launch_move_in<U, 256, false>(p, s);
-  return launch_move<U, 64>(p, s);  // (odd rows too: bytes, 64 of a row at once)
+hipError_t launch_move(const EvictParams& p, hipStream_t s) {
+  // (odd rows too: bytes, 64 of a row at once)
+  return p.table_out ? launch_move_in<U, U == 16 ? 256 : 64, false>(p, s) : launch_move_in<U, 64, true>(p, s);
 }
 
 // Bytes that rows of both caches allow at once.
@@ -470,7 +465,7 @@ hipError_t launch_evict(const EvictParams& p, hipStream_t s) {
     hipLaunchKernelGGL((evict_select_kernel<32768>), dim3((unsigned)z), dim3(kEThreads), 0, s, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  return u == 16 ? launch_move_u<16>(p, s) : u == 4 ? launch_move_u<4>(p, s) : launch_move_u<1>(p, s);
+  return u == 16 ? launch_move<16>(p, s) : u == 4 ? launch_move<4>(p, s) : launch_move<1>(p, s);
 }
 
 }  // namespace pa
