@@ -10,12 +10,13 @@
 //
 // Values that are not finite lie in LDS as zeros and are added for the rows that see them (rare).
 //
-// Bound, where a sequence has few rows, by the chain of a tile (rows into LDS, products, softmax: 6.8 us at head 128 with one
-// wavefront per SIMD, its products 3.4); where it has many, by the fp32 products, 128 of 64 cycles a tile and wavefront at head
-// 128, which two wavefronts per SIMD keep busy 42 % of the time beside the softmax and the widening of keys.  8 sequences of
-// 500 - 6000 keys, 32 heads of 128 and 8 kv-heads, fp8 pages: one token each 97 us (488 on the VALU kernel; 244 with
-// four elements a load and none ahead), trees of 32 nodes 267 (11400; 339 in one build with the other's registers); head 80 in
-// bf16 91 (372) and 259 (9400); fp32 at head 64 55 (281) and 165 (6990).  Chunks half as long: 112 and 303.
+// Bound, where a sequence has few rows, by the chain of a tile (rows into LDS, products, softmax: 7.6 us at head 128 with
+// one wavefront per SIMD, its products 3.4; matrix units busy 27 % of the time); where it has many, by the fp32 products, 128
+// of 64 cycles a tile and wavefront at head 128, which two wavefronts per SIMD keep busy 42 % of the time beside the softmax
+// and the widening of keys.  8 sequences of 1568 - 5625 keys, 32 heads of 128 and 8 kv-heads, fp8 pages: one token each 103 us
+// a call (about 490 on the VALU kernel; 244 with four elements a load and none ahead), trees of 32 nodes 270 (11400; 339 in one
+// build with the other's registers); head 80 in bf16 96 (372) and 257 (9400); fp32 at head 64 63 (281) and 167 (6990).  Chunks
+// half as long: 112 and 303.  A prompt of 2048 over fp8 pages 520.
 #pragma once
 
 #include "pa_cache_read.hpp"

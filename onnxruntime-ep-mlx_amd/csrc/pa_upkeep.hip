@@ -75,8 +75,9 @@ __device__ __forceinline__ typename Unit<U>::type recode_unit(typename Unit<U>::
 }
 
 // ------------------------------------------------------------------------------------ accepted paths
-// Bound by its chain: metadata, the walk (one LDS read and ballot a node), table, rows: one tree of 26 nodes 6.2 us, 64 of
-// 30 - 64 nodes with 4 heads of 256 15 - 18.
+// Bound by its chain: metadata, the walk (one LDS read and ballot a node), then for eight rows at a time their table entries and the
+// rows: one tree of 26 nodes 6.3 us, 64 of 30 - 64 nodes with 4 heads of 256, a workgroup to each, 18; 64 paths of 8 rows on average, 8
+// heads of 128 13, over fp8 pages, whose codes are encoded anew, 56.
 //
 // The path: from row 0 to the first child whose drafted token is the model's choice at its parent, and so on.  Every
 // workgroup of a sequence walks it for itself, a wavefront over 64 rows at a time; the first writes it down.
@@ -180,7 +181,8 @@ constexpr int kEThreads = 1024, kEWaves = kEThreads / 64, kEBins = 2048;
 // that stay anyway.  Three rounds of counting, 11, 11 and 10 bits of the weights from the top, find the weight of the
 // last one that stays; of those that weigh as much the lowest positions do.  The wavefronts then number what stays in
 // stretches of their own.  HELD weights stay in LDS, more are read again in every round.
-// Bound by latency, 8 us, and its passes over LDS, 0.7 us for 1000 keys (9000 keys of 128 heads 15.7; a weight to a lane at a time 17.2).
+// Bound by latency, 8 us, and its passes over LDS, 0.7 us for 1000 keys (9000 keys of 128 heads 15.7; a weight to a lane at a time 17.2;
+// 32768 of 8 heads 31).  Where the weights do not stay in LDS, by their loads and the tables' in every pass (131072 keys of 8 heads 320).
 template <int HELD>
 __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictParams p) {
   __shared__ __attribute__((aligned(16))) uint32_t held[HELD];
@@ -332,7 +334,8 @@ __global__ __launch_bounds__(kEThreads) void evict_select_kernel(const EvictPara
 // round of 2048 after the other; to other pages one round to a workgroup, of whole rows.
 // Bound by HBM: 2048 of up to 9000 rows of 8 heads of 16 sequences, 268 MB read and written, to other pages in 58 us
 // (4.6 TB/s; a copy of 1 GiB 5.2; in rounds of 64 KB 75 us, with stores that stay in the cache 62).  In place by its rounds:
-// 1, 4 and 16 sequences of 9000 keys 10, 20 and 80 us (in rounds of 256 whole rows the last took 126).
+// 1, 4 and 16 sequences of 9000 keys 8, 18 and 75 us (in rounds of 256 whole rows the last took 126).  fp8 rows, half the bytes, by their
+// encoding: 16 sequences 118 us in place and 160 to other pages.
 template <bool INPLACE>
 struct Round {  // threads, rows in flight of each
   static constexpr int THREADS = INPLACE ? 1024 : 256, DEPTH = INPLACE ? 8 : 4;

@@ -9,11 +9,12 @@
 // workgroups but for the fixed order of the chunks of rows, which fold_kernel adds.  Nothing is atomic: the same
 // call gives the same bits.
 //
-// What bounds it.  Scores: HBM; a step of 48 tokens, 32 heads, over 511 - 8190 keys writes and reads 27 MB of them, 33 us
-// more in the attention (195 for 162 without) and 11.5 in fold_kernel.  Columns: the exponentials' vector instructions
-// beside the products, at two wavefronts per SIMD that overlap in part: 4095 tokens after 600, 24 heads of 256 under a
-// softcap, 133 GFLOP of products in 212 us (three transcendental instructions a score; vector and matrix units busy 53
-// and 27 % of the time); without LDS and a tile's lead 467.  Other types and heads up to 256: pa_weigh32.hip.  The last 32 rows of prompts of 3001 - 5001: 14.
+// What bounds it.  Scores: HBM; a step of 48 tokens, 32 heads, over 511 - 8190 keys writes and reads 27 MB of them, 31 - 33
+// us more in the attention (194 for 162 without; its waits for keys count these stores, too) and 11.5 in fold_kernel.
+// Columns: the exponentials' vector instructions beside the products, at two wavefronts per SIMD that overlap in part: 4095
+// tokens after 600, 24 heads of 256 under a softcap, 133 GFLOP of products in 200 - 212 us (three transcendental
+// instructions a score; vector and matrix units busy 53 and 27 % of the time); without LDS and a tile's lead 467.  Other types
+// and heads up to 256: pa_weigh32.hip.  The last 32 rows of prompts of 3001 - 5001: 14.
 #include "pa_cache_read.hpp"
 #include "pa_weigh.hpp"
 

@@ -4,8 +4,8 @@
 // attention made them (the same products in the same order), so its sum crosses lanes once, at the end.
 //
 // Bound by the fp32 products, 64 of 64 cycles for 32 keys and rows at head 128, and what brings and widens keys for few rows: 32
-// rows each of 8 sequences of 500 - 6000 keys, 32 heads of 128 and 8 kv-heads, fp8 pages 128 us (365 with the keys in LDS and
-// no matrix instructions), fp32 at head 64 81 (283).
+// rows each of 8 sequences of 1568 - 5625 keys, 32 heads of 128 and 8 kv-heads, fp8 pages 119 us, matrix units busy 45 % of the time (365
+// with the keys in LDS and no matrix instructions), fp32 at head 64 75 (283); all rows of a prompt of 2048 over fp8 pages 366.
 #include "pa_rows32.hpp"
 #include "pa_weigh.hpp"
 
