@@ -628,10 +628,10 @@ int expected_ctx(const pa_cache* c, const pa_batch* b) {
   return b->max_context_len > 0 ? std::min(b->max_context_len, cap) : cap;
 }
 
-// launch_rows32's plan: as many chunks of the given length as the expected context has, the last of which takes what a
-// sequence beyond it holds (by the table's capacity, 48 sequences of 32 nodes, 32 heads of 128 and at most 1000 keys would
-// take 3.3 GB of partial rows behind tables of 131072 slots).
-Plan rows32_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dtype act, int chunk) {
+// Plan of trees and accounts on launch_rows32 (chunk > 0) or the VALU kernel: as many chunks as the expected context has, the
+// last of which takes what a sequence beyond it holds (by the table's capacity, 48 sequences of 32 nodes, 32 heads of 128 and
+// at most 1000 keys would take 3.3 GB of partial rows behind tables of 131072 slots).
+Plan upkeep_plan(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dtype act, int chunk) {
   Plan pl = make_plan(c, b, a, act, 3, chunk);
   pl.max_splits = std::max((expected_ctx(c, b) + pl.chunk - 1) / pl.chunk, 1);
   pl.part_rows = pl.max_splits > 1 ? (size_t)std::max(b->num_tokens, 0) * a->num_heads * pl.max_splits : 0;
@@ -984,9 +984,10 @@ int run_attention(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dty
     return fail(PA_ERR_UNSUPPORTED, "prefill MFMA kernel does not cover this dtype/head_dim");
   if (!(a->softcap >= 0.0f) || !std::isfinite(a->softcap))
     return fail(PA_ERR_INVALID_ARGUMENT, "softcap must be finite and non-negative");
-  Plan pl = opts.rows32 ? rows32_plan(c, b, a, act, chunk)
-                        : make_plan(c, b, a, act, kind, chunk, opts.linear_cap > 0, opts.linear_cap,
-                                    plan_images(opts), opts.bias != nullptr, opts.host);
+  Plan pl = opts.tree_bits || opts.row_stats
+                ? upkeep_plan(c, b, a, act, chunk)
+                : make_plan(c, b, a, act, kind, chunk, opts.linear_cap > 0, opts.linear_cap,
+                            plan_images(opts), opts.bias != nullptr, opts.host);
   if (kind == 2 && pl.kind != 2 && pa::prefill_coded_supported(c->head_dim, act, c->dtype))
     return fail(PA_ERR_UNSUPPORTED,
                 "prefill MFMA kernel: byte-coded pages run on it over operand images only (planned "
@@ -1502,9 +1503,9 @@ int rows32_chunk(const pa_cache* c, const pa_batch* b, const pa_attn* a) {
   return (int)std::max<int64_t>(((keys + splits - 1) / splits + 31) / 32 * 32, 128);
 }
 
-// Workspace of the attention where the matrix-core kernel does not run: launch_rows32 by chunks, or (0) the VALU kernel.
+// Workspace of the attention where the matrix-core kernel does not run.
 size_t other_workspace(const pa_cache* c, const pa_batch* b, const pa_attn* a, pa_dtype act, int chunk) {
-  return chunk > 0 ? workspace_for(c, b, a, rows32_plan(c, b, a, act, chunk)) : ws_need(c, b, a, act, 3, 0).best;
+  return workspace_for(c, b, a, upkeep_plan(c, b, a, act, chunk));
 }
 
 // ------------------------------------------------------------------------------ drafted trees

@@ -64,7 +64,8 @@ __global__ __launch_bounds__(64 * NW) void attn_generic_kernel(const AttnParams 
   const int64_t total = seq_keys(p, b, pastb, nq);
   const int64_t start = (int64_t)split * p.chunk;
   if (nq <= 0 || start >= total) return;
-  const int64_t end = min(start + (int64_t)p.chunk, total);
+  // (UPKEEP: the last chunk goes to the sequence's end, contexts beyond the call's bound)
+  const int64_t end = UPKEEP && split == p.max_splits - 1 ? total : min(start + (int64_t)p.chunk, total);
   const int g = p.num_heads / p.kv_heads;
   const int kh = h / g;
   const int64_t rp = pastb + (t - s0);

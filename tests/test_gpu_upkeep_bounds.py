@@ -12,7 +12,7 @@ from upkeep_cases import attention64, causal_seen, trees
 pytestmark = pytest.mark.gpu
 
 BF16, F32, FP8 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
-KINDS = [(F32, 64, None), (BF16, 80, None), (BF16, 128, FP8), (BF16, 256, torch.int8)]
+KINDS = [(F32, 64, None), (BF16, 80, None), (BF16, 128, FP8), (BF16, 256, torch.int8), (BF16, 320, None), (F32, 264, FP8)]
 BATCHES = [([1, 2, 1], [300, 998, 0]), ([32, 7, 0, 30], [70, 993, 64, 400])]
 
 

@@ -11,7 +11,7 @@ FP8 = capi.PA_DTYPE_FP8_E4M3
 # (types of pages and rows, head, tokens of each sequence, sequences, bound)
 STEPS = [(F32, F32, 128, 32, 48, 1000), (F32, F32, 128, 1, 48, 600), (F32, F32, 64, 4000, 1, 4000),
          (FP8, BF16, 128, 32, 48, 1000), (FP8, BF16, 128, 512, 64, 512), (capi.PA_DTYPE_INT8, BF16, 256, 1, 3, 30),
-         (BF16, BF16, 80, 20, 7, 8000)]
+         (BF16, BF16, 80, 20, 7, 8000), (BF16, BF16, 320, 1, 48, 600), (F32, F32, 512, 2, 30, 2000), (FP8, BF16, 640, 40, 8, 300)]
 
 
 @pytest.mark.parametrize("pages,act,head,new,seqs,bound", STEPS)
