@@ -46,7 +46,7 @@
 // TFLOP/s of the two products, 1105 with the second part of the probabilities, the softmax's vector instructions
 // behind them in turn; 64 heads of 64 in 945 us (twice the scores per product), 16 heads of 256 in 767.  64
 // sequences of up to 8192 keys, one token each: 212 us, 5.8 TB/s from HBM.  A tree of 257 nodes after 60001 keys, 32 heads
-// of 128: 427 - 451 us by the card, 592 TFLOP/s at the best (nine blocks of rows of which the last holds four); 16 trees of
+// of 128: 413 - 451 us by the card, 611 TFLOP/s at the best (nine blocks of rows of which the last holds four); 16 trees of
 // 40 - 64 nodes, 28 heads, 84 - 90.  Small calls: 5 us of dependent
 // loads and the scan before the first item, 2 us to its first tile, 3 us per launch.
 #pragma once
